@@ -175,7 +175,8 @@ int ssq_lut_build(const void* q, int32_t q_dtype, int64_t q_sr, int32_t rows, in
  * light-block entries the caller pre-fills with zeros).
  * Contiguous output: codes[b*c_sb + kv*c_sh + s*c_st + blk], pt[b*pt_sb + kv*pt_sh + s*pt_st + slot*bd + d].
  * Paged output (slot_mapping != NULL, [B, S] int64 token slots): slot -> page = slot / page_size,
- *   off = slot % page_size; codes[page*c_sb + kv*c_sh + off*c_st + blk] (pt likewise).
+ *   off = slot % page_size; codes[page*c_sb + kv*c_sh + off*c_st + blk] (pt likewise); a token with a
+ *   negative slot (padding) is not written.
  * Replaces sunshape/codec.py:362-385 and the loop of sunshape/vllm_attn_backend.py:101-123.
  */
 typedef struct ssq_encode_args {
@@ -257,6 +258,82 @@ int ssq_pack_codes(const uint8_t* codes, int64_t c_st, int64_t rows, int32_t n_b
 /* Inverse of ssq_pack_codes. */
 int ssq_unpack_codes(const uint32_t* packed, int64_t p_st, int64_t rows, int32_t n_blocks, int32_t bits,
                      uint8_t* out, int64_t o_st, void* stream);
+
+/*
+ * Position rotation (and, beside it, per-head RMS norm) of rows [B, H, S, D], for ssq_qk_norm_rope and
+ * ssq_append.  Token (b, s) is rotated by row positions[b*p_sb + s*p_ss] of the tables cos / sin
+ * (fp32, row stride ld, max_pos rows of rot_dim / 2 entries): pair i of the first rot_dim dims, (u1, u2) =
+ * dims (i, i + rot_dim / 2), or (2i, 2i + 1) when interleaved, becomes
+ *   (u1 cos_i - u2 sin_i,  u2 cos_i + u1 sin_i),
+ * dims past rot_dim stay.  With a weight w [D] (w_dtype) u = (x * r) * w, r = 1 / sqrt(mean(x^2) + eps)
+ * over the row's D dims (the sum and r in 64 bits, r rounded to 32); else u = x.  Products and sums in fp32,
+ * each rounded, in this order; the result is rounded once to the rows' dtype.  A position outside
+ * [0, max_pos) makes the row's rotated dims NaN.  cos == NULL: no rotation (positions is not read).
+ */
+typedef struct ssq_rope {
+    const float* cos; const float* sin; int64_t ld;
+    int32_t max_pos, rot_dim, interleaved;
+    int32_t w_dtype;
+    const int64_t* positions; int64_t p_sb, p_ss;
+    double eps;
+} ssq_rope;
+
+/* Norm and rotation of queries and keys in one pass (no counterpart in the reference, whose model code
+ * rotates before the cache sees the keys).  q [B, Hq, S, D] -> q_out, k [B, Hk, S, D] -> k_out, of one dtype,
+ * any strides (elements) with D contiguous; in place where out == in with the same strides.  num_k_heads 0:
+ * queries only.  q_weight / k_weight: norm weights or NULL (no norm). */
+typedef struct ssq_rope_args {
+    uint32_t struct_size;
+    int32_t dtype;
+    const void* q; int64_t q_sb, q_sh, q_ss;
+    void* q_out; int64_t qo_sb, qo_sh, qo_ss;
+    const void* k; int64_t k_sb, k_sh, k_ss;
+    void* k_out; int64_t ko_sb, ko_sh, ko_ss;
+    int32_t batch, seq_len, head_dim, num_q_heads, num_k_heads;
+    const void* q_weight; const void* k_weight;
+    ssq_rope rope;
+} ssq_rope_args;
+
+int ssq_qk_norm_rope(const ssq_rope_args* a, void* stream);
+
+/* Append raw keys and values to a paged cache, norm and rotation applied to the keys on the way (no
+ * counterpart in the reference).  enc: as for ssq_encode with a slot_mapping; the keys are normed, rotated and
+ * rounded to k_dtype first, then the codes and passthrough values of ssq_encode are written.  Values
+ * v[b*v_sb + kv*v_sh + s*v_ss + d] (d < value_dim) go to v_pages[page*vp_sb + kv*vp_sh + d*vp_sd + off], converted
+ * to vp_dtype; v NULL: keys only.  num_pages bounds the slots: a token whose slot is negative (padding) or at
+ * least num_pages * page_size is left out.  The slots of a call are distinct.  workspace: see
+ * ssq_append_workspace_size; enc.kernel: 0, or 1 for ssq_encode's exact scan. */
+typedef struct ssq_append_args {
+    uint32_t struct_size;
+    ssq_encode_args enc;
+    int64_t num_pages;
+    const void* k_weight;
+    ssq_rope rope;
+    const void* v; int32_t v_dtype; int64_t v_sb, v_sh, v_ss;
+    int32_t value_dim, vp_dtype;
+    void* v_pages; int64_t vp_sb, vp_sh, vp_sd;
+} ssq_append_args;
+
+size_t ssq_append_workspace_size(const ssq_append_args* a);
+int ssq_append(const ssq_append_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Decode for a batch whose sequences share a prefix: each query row attends the prefix_len[0] (device, at most
+ * prefix_cap) tokens in the pages prefix_table (ceil(prefix_cap / page_size) entries), then its own sequence's
+ * tokens as in ssq_decode: one softmax over both.  The prefix's pages are read once for all sequences' rows.
+ * dec: SSQ_PAGED with v; block_table / seq_lens / seq_len / mask speak of the sequences' own tokens
+ * (seq_len 0: none, block_table may be NULL); scores NULL; kernel 0, or 1 for the path that serves every codec.
+ * A row with nothing to attend (both lengths 0, or a mask of -inf) gives out 0 and lse -inf.
+ * No counterpart in the reference. */
+typedef struct ssq_prefix_args {
+    uint32_t struct_size;
+    ssq_decode_args dec;
+    const int32_t* prefix_table;
+    const int32_t* prefix_len;
+    int32_t prefix_cap;
+} ssq_prefix_args;
+
+size_t ssq_decode_prefix_workspace_size(const ssq_prefix_args* a);
+int ssq_decode_prefix(const ssq_prefix_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
 const char* ssq_last_error(void);
 int ssq_abi_version(void);

@@ -73,3 +73,75 @@ class EncodeArgs(ctypes.Structure):
         self.struct_size = ctypes.sizeof(EncodeArgs)
         for k, v in kw.items():
             setattr(self, k, v)
+
+
+class Rope(ctypes.Structure):
+    """Mirror of ``ssq_rope``."""
+
+    _fields_ = [
+        ("cos", _vp), ("sin", _vp), ("ld", _i64),
+        ("max_pos", _i32), ("rot_dim", _i32), ("interleaved", _i32),
+        ("w_dtype", _i32),
+        ("positions", _vp), ("p_sb", _i64), ("p_ss", _i64),
+        ("eps", ctypes.c_double),
+    ]
+
+
+class RopeArgs(ctypes.Structure):
+    """Mirror of ``ssq_rope_args``."""
+
+    _fields_ = [
+        ("struct_size", _u32), ("dtype", _i32),
+        ("q", _vp), ("q_sb", _i64), ("q_sh", _i64), ("q_ss", _i64),
+        ("q_out", _vp), ("qo_sb", _i64), ("qo_sh", _i64), ("qo_ss", _i64),
+        ("k", _vp), ("k_sb", _i64), ("k_sh", _i64), ("k_ss", _i64),
+        ("k_out", _vp), ("ko_sb", _i64), ("ko_sh", _i64), ("ko_ss", _i64),
+        ("batch", _i32), ("seq_len", _i32), ("head_dim", _i32), ("num_q_heads", _i32), ("num_k_heads", _i32),
+        ("q_weight", _vp), ("k_weight", _vp),
+        ("rope", Rope),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(RopeArgs)
+        for k, v in kw.items():
+            setattr(self, k, v)
+
+
+class AppendArgs(ctypes.Structure):
+    """Mirror of ``ssq_append_args``."""
+
+    _fields_ = [
+        ("struct_size", _u32),
+        ("enc", EncodeArgs),
+        ("num_pages", _i64),
+        ("k_weight", _vp),
+        ("rope", Rope),
+        ("v", _vp), ("v_dtype", _i32), ("v_sb", _i64), ("v_sh", _i64), ("v_ss", _i64),
+        ("value_dim", _i32), ("vp_dtype", _i32),
+        ("v_pages", _vp), ("vp_sb", _i64), ("vp_sh", _i64), ("vp_sd", _i64),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(AppendArgs)
+        self.enc.struct_size = ctypes.sizeof(EncodeArgs)
+        for k, v in kw.items():
+            setattr(self, k, v)
+
+
+class PrefixArgs(ctypes.Structure):
+    """Mirror of ``ssq_prefix_args``."""
+
+    _fields_ = [
+        ("struct_size", _u32),
+        ("dec", DecodeArgs),
+        ("prefix_table", _vp), ("prefix_len", _vp), ("prefix_cap", _i32),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(PrefixArgs)
+        self.dec.struct_size = ctypes.sizeof(DecodeArgs)
+        for k, v in kw.items():
+            setattr(self, k, v)

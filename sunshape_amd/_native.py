@@ -47,11 +47,16 @@ EXPORTED_SYMBOLS = (
     "ssq_transform_rows",
     "ssq_pack_codes",
     "ssq_unpack_codes",
+    "ssq_qk_norm_rope",
+    "ssq_append_workspace_size",
+    "ssq_append",
+    "ssq_decode_prefix_workspace_size",
+    "ssq_decode_prefix",
     "ssq_last_error",
     "ssq_abi_version",
 )
 
-from ._abi import DecodeArgs, EncodeArgs  # noqa: E402  (the structs, torch-free)
+from ._abi import AppendArgs, DecodeArgs, EncodeArgs, PrefixArgs, Rope, RopeArgs  # noqa: E402  (the structs, torch-free)
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -93,6 +98,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ssq_pack_codes.restype = ctypes.c_int
     lib.ssq_unpack_codes.argtypes = [_vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp]
     lib.ssq_unpack_codes.restype = ctypes.c_int
+    lib.ssq_qk_norm_rope.argtypes = [P(RopeArgs), _vp]
+    lib.ssq_qk_norm_rope.restype = ctypes.c_int
+    lib.ssq_append_workspace_size.argtypes = [P(AppendArgs)]
+    lib.ssq_append_workspace_size.restype = ctypes.c_size_t
+    lib.ssq_append.argtypes = [P(AppendArgs), _vp, ctypes.c_size_t, _vp]
+    lib.ssq_append.restype = ctypes.c_int
+    lib.ssq_decode_prefix_workspace_size.argtypes = [P(PrefixArgs)]
+    lib.ssq_decode_prefix_workspace_size.restype = ctypes.c_size_t
+    lib.ssq_decode_prefix.argtypes = [P(PrefixArgs), _vp, ctypes.c_size_t, _vp]
+    lib.ssq_decode_prefix.restype = ctypes.c_int
     lib.ssq_last_error.argtypes = []
     lib.ssq_last_error.restype = ctypes.c_char_p
     lib.ssq_abi_version.argtypes = []

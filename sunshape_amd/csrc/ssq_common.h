@@ -120,6 +120,8 @@ struct SsqKeyMap {
         return (int64_t)b * a.k_sb + (int64_t)kv * a.k_sh + (int64_t)s * a.k_ss;
     }
 };
+// the code row of a padded key (negative slot): nothing is written for it
+constexpr int64_t kNoRow = INT64_MIN;
 // folding applies when a sequence is shorter than one workgroup's keys
 inline bool ssq_encode_fold(const ssq_encode_args* a, int keys_per_wg) {
     return a->seq_len < keys_per_wg && (int64_t)a->batch * a->seq_len <= 0x7fffffff;

@@ -224,10 +224,12 @@ int validate(const ssq_decode_args* a, bool need_v) {
     return SSQ_OK;
 }
 
-int run_generic(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipStream_t st) {
+// partial: leave (o, m, l) of every split in the workspace (at least one split's), merge nothing
+int run_generic(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipStream_t st, bool partial = false) {
     Plan pl;
     int rc = make_plan(*a, pl);
     if (rc) return rc;
+    if (partial) pl.ws_bytes = (size_t)pl.n_splits * a->batch * a->num_q_heads * a->q_len * (a->value_dim + 2) * 4;
     if (a->seq_len == 0) return ssq_fail(SSQ_ERR_INVALID, "seq_len == 0: softmax over an empty context");
     SSQ_REQUIRE(ws_bytes >= pl.ws_bytes, "workspace too small: %zu < %zu bytes", ws_bytes, pl.ws_bytes);
     SSQ_REQUIRE(pl.ws_bytes == 0 || workspace, "workspace is NULL");
@@ -238,6 +240,7 @@ int run_generic(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipS
     dp.R = pl.R;
     dp.split_len = pl.split_len;
     dp.n_splits = pl.n_splits;
+    dp.partial = partial ? 1 : 0;
     dp.cw = ssq_code_width(a->n_centroids);
     const bool aligned = dp.cw == 1 && a->code_bits == 0 && ((uintptr_t)a->codes % 4 == 0) && a->n_blocks % 4 == 0 &&
                          a->c_st % 4 == 0 && a->c_sh % 4 == 0 && a->c_sb % 4 == 0;
@@ -257,7 +260,7 @@ int run_generic(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipS
     }
     if (pl.wide) {
         rc = ssq_decode_wide(dp, pl.RP, pl.n_groups, pl.smem, st);
-        if (rc == SSQ_OK && pl.n_splits > 1) rc = launch_merge(*a, pl.n_splits, dp.ws_o, dp.ws_m, dp.ws_l, st);
+        if (rc == SSQ_OK && pl.n_splits > 1 && !partial) rc = launch_merge(*a, pl.n_splits, dp.ws_o, dp.ws_m, dp.ws_l, st);
         return rc;
     }
     SsqGenericLaunch gl;
@@ -268,7 +271,7 @@ int run_generic(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipS
     gl.has_v = pl.has_v;
     rc = use_w16(*a) ? ssq_generic_w16(dp, gl, st) : launch_generic<false>(dp, gl, st);
     if (rc) return rc;
-    if (pl.has_v && pl.n_splits > 1) {
+    if (pl.has_v && pl.n_splits > 1 && !partial) {
         rc = launch_merge(*a, pl.n_splits, dp.ws_o, dp.ws_m, dp.ws_l, st);
     }
     return rc;
@@ -285,7 +288,8 @@ int ssq_launch_merge(const ssq_decode_args& a, int n_splits, const float* ws_o, 
 int ssq_decode_mfma_supported(const ssq_decode_args* a);
 size_t ssq_decode_mfma_workspace(const ssq_decode_args* a);
 size_t ssq_decode_mfma_workspace_least(const ssq_decode_args* a);
-int ssq_decode_mfma(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipStream_t st);
+int ssq_decode_mfma_splits(const ssq_decode_args* a);
+int ssq_decode_mfma(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipStream_t st, bool partial = false);
 int ssq_decode_contig_supported(const ssq_decode_args* a);
 size_t ssq_decode_contig_workspace(const ssq_decode_args* a);
 int ssq_decode_contig(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipStream_t st);
@@ -319,6 +323,34 @@ extern "C" size_t ssq_decode_workspace_size(const ssq_decode_args* a) { return w
 
 // the smallest workspace ssq_decode accepts: that of one workgroup per (sequence, KV head, split)
 size_t ssq_decode_workspace_least(const ssq_decode_args* a) { return workspace_size(a, true); }
+
+int ssq_decode_validate(const ssq_decode_args* a) { return validate(a, true); }
+
+// Context splits of a paged decode whose partials ssq_decode_partials leaves (0: the problem has no plan;
+// the message says why).  a->num_splits of the later call must be the number returned, which also keeps the
+// batch from being balanced by length (those partials are laid out by share, not by row).
+int ssq_decode_partial_splits(const ssq_decode_args* a) {
+    ssq_decode_args t = *a;
+    for (int k = 0; k < 4; ++k) {  // a plan may round the number of splits: the one that it keeps
+        int n = 0;
+        if (pick_kernel(&t) == 2 && ssq_decode_mfma_supported(&t)) {
+            n = ssq_decode_mfma_splits(&t);
+        } else {
+            Plan pl;
+            n = make_plan(t, pl) == SSQ_OK ? pl.n_splits : 0;
+        }
+        if (n == 0 || n == t.num_splits) return n;
+        t.num_splits = n;
+    }
+    ssq_fail(SSQ_ERR_UNSUPPORTED, "no stable number of context splits");
+    return 0;
+}
+
+// The decode kernels' partials of a paged problem: o [splits, B*Hq*Lq, Dv], then m and l [splits, B*Hq*Lq] in ws.
+int ssq_decode_partials(const ssq_decode_args* a, void* ws, size_t bytes, hipStream_t st) {
+    if (pick_kernel(a) == 2 && ssq_decode_mfma_supported(a)) return ssq_decode_mfma(a, ws, bytes, st, true);
+    return run_generic(a, ws, bytes, st, true);
+}
 
 extern "C" int ssq_decode(const ssq_decode_args* a, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = validate(a, true);

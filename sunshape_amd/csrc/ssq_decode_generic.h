@@ -34,6 +34,7 @@ struct SsqGenericParams {
     int R;          // rows per workgroup
     int split_len;  // tokens per split (multiple of kTile)
     int n_splits;
+    int partial;    // 1: leave (o, m, l) in the workspace also when there is one split
     int word_codes; // 1: code rows are 4-byte aligned with nb % 4 == 0
     int vec_cent;   // 1: codebook 16-byte aligned (per head too), head_dim % 4 == 0, nb*nc % 4 == 0
     int cw;         // code width in bytes (ssq_code_width): > 1 gathers codewords instead of a LUT
@@ -774,7 +775,7 @@ __global__ __launch_bounds__(kThreads) void k_decode_generic(const DecodeParams 
         const int g = row / a.q_len, qi = row - g * a.q_len;
         const int h = kv * p.G + g;
         const int rid = (b * a.num_q_heads + h) * a.q_len + qi;
-        if (p.n_splits == 1) {
+        if (p.n_splits == 1 && !p.partial) {
             ssq_store_elem(a.out, a.v_dtype, (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)qi * a.o_sl + dv, o / l);
             if (a.lse && dv == 0) a.lse[rid] = m + logf(l);
         } else {

@@ -228,10 +228,21 @@ size_t ssq_decode_mfma_workspace_least(const ssq_decode_args* a) {
     return plan(a, pl) ? pl.ws_least : 0;
 }
 
-int ssq_decode_mfma(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipStream_t st) {
+int ssq_decode_mfma_splits(const ssq_decode_args* a) {
+    SsqMfmaPlan pl;
+    return plan(a, pl) ? pl.n_splits : 0;
+}
+
+// partial: leave every split's (o, m, l) in the workspace and merge nothing (a->num_splits is set, so the
+// batch is not balanced by length)
+int ssq_decode_mfma(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipStream_t st, bool partial) {
     SsqMfmaPlan pl;
     if (!plan(a, pl)) return ssq_fail(SSQ_ERR_UNSUPPORTED, "MFMA decode kernel does not support this problem");
     if (a->seq_len == 0) return ssq_fail(SSQ_ERR_INVALID, "seq_len == 0: softmax over an empty context");
+    if (partial) {
+        SSQ_REQUIRE(pl.cut_wg == 0 && a->v, "partials need num_splits and values");
+        pl.ws_bytes = pl.ws_least = (size_t)pl.n_splits * a->batch * a->num_q_heads * a->q_len * (a->value_dim + 2) * 4;
+    }
     if (pl.cut_wg && (ws_bytes < pl.ws_bytes || !workspace)) {  // no room for the shares' partials
         pl.cut_wg = 0;
         pl.ws_bytes = pl.ws_least;
@@ -249,7 +260,8 @@ int ssq_decode_mfma(const ssq_decode_args* a, void* workspace, size_t ws_bytes, 
     mp.rows = mp.G * a->q_len;
     mp.rg = pl.rg;
     mp.split_len = pl.split_len;
-    mp.n_splits = pl.n_splits;
+    mp.n_splits = partial && pl.n_splits == 1 ? 2 : pl.n_splits;  // the kernels write partials unless it is 1
+    const bool merge = pl.n_splits > 1 && !partial;
     const size_t n_rows_all = (size_t)a->batch * a->num_q_heads * a->q_len;
     float* ws = reinterpret_cast<float*>(workspace);
     mp.ws_o = ws;
@@ -270,7 +282,7 @@ int ssq_decode_mfma(const ssq_decode_args* a, void* workspace, size_t ws_bytes, 
     if (pl.q4) {
         rc = ssq_decode_q4_launch(mp, dim3(mp.a.batch * mp.a.num_kv_heads, pl.n_splits, pl.n_groups), st);
         if (rc) return rc;
-        if (pl.n_splits > 1) rc = ssq_launch_merge(*a, pl.n_splits, mp.ws_o, mp.ws_m, mp.ws_l, st);
+        if (merge) rc = ssq_launch_merge(*a, pl.n_splits, mp.ws_o, mp.ws_m, mp.ws_l, st);
         return rc;
     }
     if (pl.ct && !a->v) return ssq_mfma_lut_ct_scores(mp, pl, st);  // scores only: no merge
@@ -282,13 +294,13 @@ int ssq_decode_mfma(const ssq_decode_args* a, void* workspace, size_t ws_bytes, 
         else
             rc = a->v_dtype == SSQ_BF16 ? ssq_mfma_lut_ct_bf16(mp, pl, st) : ssq_mfma_lut_ct_f16(mp, pl, st);
         if (rc) return rc;
-        if (pl.n_splits > 1) rc = ssq_launch_merge(*a, pl.n_splits, mp.ws_o, mp.ws_m, mp.ws_l, st);
+        if (merge) rc = ssq_launch_merge(*a, pl.n_splits, mp.ws_o, mp.ws_m, mp.ws_l, st);
         return rc;
     }
     if (mp.a.n_centroids == 64) {
         rc = ssq_mfma_lut64(mp, pl, st);
         if (rc) return rc;
-        if (pl.n_splits > 1) rc = ssq_launch_merge(*a, pl.n_splits, mp.ws_o, mp.ws_m, mp.ws_l, st);
+        if (merge) rc = ssq_launch_merge(*a, pl.n_splits, mp.ws_o, mp.ws_m, mp.ws_l, st);
         return rc;
     }
     switch (pl.RP) {
@@ -298,6 +310,6 @@ int ssq_decode_mfma(const ssq_decode_args* a, void* workspace, size_t ws_bytes, 
         default: rc = ssq_mfma_lut_rp8_16(mp, pl, st); break;
     }
     if (rc) return rc;
-    if (pl.n_splits > 1) rc = ssq_launch_merge(*a, pl.n_splits, mp.ws_o, mp.ws_m, mp.ws_l, st);
+    if (merge) rc = ssq_launch_merge(*a, pl.n_splits, mp.ws_o, mp.ws_m, mp.ws_l, st);
     return rc;
 }

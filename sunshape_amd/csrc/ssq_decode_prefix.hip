@@ -1,0 +1,238 @@
+// Decode for a batch that shares a prefix (ssq_decode_prefix): every query row attends the prefix's tokens and
+// its own sequence's, one softmax over both.
+//
+//   m = max(m_p, m_o),  l = l_p e^{m_p - m} + l_o e^{m_o - m},  out = (o_p e^{m_p - m} + o_o e^{m_o - m}) / l
+//
+// with (o, m, l) = (sum_t e^{s_t - m} v_t, max_t s_t, sum_t e^{s_t - m}) of a set of tokens.  The prefix is one
+// sequence whose query rows are all sequences' rows of a KV head, so its codes and values are read once for them.
+// Both parts leave fp32 (o, m, l) in the workspace, per context split, and k_merge_prefix joins them.
+#include "ssq_common.h"
+
+#include <math.h>
+
+int ssq_decode_validate(const ssq_decode_args* a);
+int ssq_decode_partial_splits(const ssq_decode_args* a);
+int ssq_decode_partials(const ssq_decode_args* a, void* ws, size_t bytes, hipStream_t st);
+
+namespace {
+
+constexpr int kMergeRows = 4;
+constexpr int kMergeBatch = 8;  // partials in flight per lane
+constexpr int kMergeDims = 4;   // value dims per lane per pass
+
+struct MergeParams {
+    ssq_decode_args a;
+    // The prefix's partials: for each query position and each chunk of `chunk` sequences a block of
+    // n1 (the last chunk n1_last) splits x (num_q_heads * sequences) rows: o, then m, then l.
+    const float* pre;
+    int chunk, n1, n1_last;
+    // the own tokens' partials, n2 splits x (batch * num_q_heads * q_len) rows (0: none)
+    const float* own;
+    int n2;
+};
+
+// One wave per query row; lane j merges value dims j, j + 64, ...
+__global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const MergeParams p) {
+    const ssq_decode_args& a = p.a;
+    const int lane = threadIdx.x & (SSQ_WAVE - 1);
+    const int64_t n_rows = (int64_t)a.batch * a.num_q_heads * a.q_len;
+    const int64_t rid = (int64_t)blockIdx.x * kMergeRows + threadIdx.x / SSQ_WAVE;
+    if (rid >= n_rows) return;  // whole waves
+    const int qi = (int)(rid % a.q_len);
+    const int h = (int)(rid / a.q_len % a.num_q_heads);
+    const int b = (int)(rid / a.q_len / a.num_q_heads);
+    const int Dv = a.value_dim;
+    // this row's prefix block
+    const int c = p.n1 ? b / p.chunk : 0;
+    const int cn = p.n1 ? min(p.chunk, a.batch - c * p.chunk) : 0;
+    const bool last = (int64_t)(c + 1) * p.chunk >= a.batch;
+    const int n1 = p.n1 ? (last ? p.n1_last : p.n1) : 0;
+    const int full = p.n1 ? a.batch / p.chunk : 0;  // whole chunks of a query position
+    const int rest = p.n1 ? a.batch - full * p.chunk : 0;
+    const int64_t per_q = (int64_t)a.num_q_heads * ((int64_t)full * p.chunk * (rest ? p.n1 : 0) +
+                                                    (rest ? (int64_t)rest * p.n1_last
+                                                          : (int64_t)(full - 1) * p.chunk * p.n1 + (int64_t)p.chunk * p.n1_last));
+    const int64_t at0 = (per_q * qi + (int64_t)a.num_q_heads * c * p.chunk * p.n1) * (Dv + 2);
+    const int64_t rows1 = (int64_t)a.num_q_heads * cn, row1 = (int64_t)h * cn + (b - c * p.chunk);
+    const float* pre_o = p.pre + at0;
+    const float* pre_m = pre_o + rows1 * n1 * Dv;
+    const float* pre_l = pre_m + rows1 * n1;
+    const float* own_m = p.own + n_rows * p.n2 * Dv;
+    const float* own_l = own_m + n_rows * p.n2;
+    const int n = n1 + p.n2;
+    float M = -INFINITY, L = 0.f;
+    for (int d0 = 0; d0 < Dv; d0 += kMergeDims * SSQ_WAVE) {
+        float Mr = -INFINITY, Lr = 0.f, o[kMergeDims];
+#pragma unroll
+        for (int k = 0; k < kMergeDims; ++k) o[k] = 0.f;
+        for (int s0 = 0; s0 < n; s0 += kMergeBatch) {
+            float mv[kMergeBatch], lv[kMergeBatch], ov[kMergeBatch][kMergeDims];
+#pragma unroll
+            for (int i = 0; i < kMergeBatch; ++i) {
+                const int s = min(s0 + i, n - 1);  // uniform; a repeated split weighs nothing
+                const bool pre = s < n1;
+                const int64_t at = pre ? (int64_t)s * rows1 + row1 : (int64_t)(s - n1) * n_rows + rid;
+                mv[i] = s0 + i < n ? (pre ? pre_m : own_m)[at] : -INFINITY;
+                lv[i] = (pre ? pre_l : own_l)[at];
+                const float* src = (pre ? pre_o : p.own) + at * Dv;
+#pragma unroll
+                for (int k = 0; k < kMergeDims; ++k)
+                    ov[i][k] = d0 + k * SSQ_WAVE < Dv ? src[min(d0 + k * SSQ_WAVE + lane, Dv - 1)] : 0.f;
+            }
+            float Mc = Mr;
+#pragma unroll
+            for (int i = 0; i < kMergeBatch; ++i) Mc = fmaxf(Mc, mv[i]);
+            const float f = Mr == -INFINITY ? 0.f : __expf(Mr - Mc);
+            Lr *= f;
+#pragma unroll
+            for (int k = 0; k < kMergeDims; ++k) o[k] *= f;
+#pragma unroll
+            for (int i = 0; i < kMergeBatch; ++i) {
+                if (mv[i] == -INFINITY) continue;  // nothing attended in this split
+                const float w = __expf(mv[i] - Mc);
+                Lr += lv[i] * w;
+#pragma unroll
+                for (int k = 0; k < kMergeDims; ++k) o[k] += ov[i][k] * w;
+            }
+            Mr = Mc;
+        }
+#pragma unroll
+        for (int k = 0; k < kMergeDims; ++k) {
+            const int dv = d0 + k * SSQ_WAVE + lane;
+            if (dv < Dv)  // a row with nothing to attend gives 0
+                ssq_store_elem(a.out, a.v_dtype, (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)qi * a.o_sl + dv,
+                               Mr == -INFINITY ? 0.f : o[k] / Lr);
+        }
+        M = Mr;
+        L = Lr;
+    }
+    if (a.lse && lane == 0) a.lse[rid] = M == -INFINITY ? -INFINITY : M + logf(L);
+}
+
+struct PrefixPlan {
+    int chunk, n1, n1_last, n2;
+    size_t pre_bytes, own_bytes;
+};
+
+// sequences [b0, b0 + n) at query position qi as one sequence of n query rows per head, attending the prefix
+ssq_decode_args prefix_part(const ssq_prefix_args& a, int b0, int n, int qi) {
+    ssq_decode_args d = a.dec;
+    const int size = d.q_dtype == SSQ_F32 ? 4 : 2;
+    d.q = reinterpret_cast<const char*>(d.q) + ((int64_t)b0 * d.q_sb + (int64_t)qi * d.q_sl) * size;
+    d.q_sl = d.q_sb;
+    d.q_sb = 0;
+    d.batch = 1;
+    d.q_len = n;
+    d.mask = nullptr;
+    d.lse = nullptr;
+    d.block_table = a.prefix_table;
+    d.bt_sb = 0;
+    d.seq_lens = a.prefix_len;
+    d.seq_len = a.prefix_cap;
+    d.num_splits = 0;
+    return d;
+}
+
+int check(const ssq_prefix_args* a) {
+    if (!a) return ssq_fail(SSQ_ERR_INVALID, "args is NULL");
+    if (a->struct_size != sizeof(ssq_prefix_args))
+        return ssq_fail(SSQ_ERR_ABI, "ssq_prefix_args size %u != library's %zu", a->struct_size, sizeof(ssq_prefix_args));
+    ssq_decode_args d = a->dec;
+    if (d.struct_size != sizeof(ssq_decode_args))
+        return ssq_fail(SSQ_ERR_ABI, "ssq_decode_args size %u != library's %zu", d.struct_size, sizeof(ssq_decode_args));
+    SSQ_REQUIRE(d.layout == SSQ_PAGED, "a shared prefix needs the paged layout");
+    SSQ_REQUIRE(d.scores == nullptr, "decode with a shared prefix writes no raw scores");
+    SSQ_REQUIRE(d.kernel == 0 || d.kernel == 1, "kernel must be 0 or 1");
+    SSQ_REQUIRE(d.num_splits == 0, "num_splits must be 0");
+    SSQ_REQUIRE(a->prefix_cap >= 0, "negative prefix_cap");
+    SSQ_REQUIRE(a->prefix_cap == 0 || (a->prefix_table && a->prefix_len), "a prefix needs prefix_table and prefix_len");
+    SSQ_REQUIRE((int64_t)d.batch * (d.num_q_heads > 0 ? d.num_q_heads : 1) <= (1 << 24) && d.q_len <= 1 << 16 &&
+                    (int64_t)d.batch * d.num_q_heads * d.q_len <= 0x7fffffff,
+                "too many query rows");
+    SSQ_REQUIRE((int64_t)d.batch * (d.num_kv_heads > 0 ? d.num_kv_heads : 1) <= 65535, "batch * num_kv_heads > 65535");
+    if (d.seq_len == 0 || !d.block_table) {  // no own tokens: the rest is checked as the prefix's problem
+        SSQ_REQUIRE(d.seq_len == 0, "paged layout needs block_table and seq_lens");
+        static const int32_t none = 0;
+        d.block_table = &none;
+        d.seq_lens = &none;
+    }
+    return ssq_decode_validate(&d);
+}
+
+int make_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
+    const ssq_decode_args& d = a.dec;
+    pl = PrefixPlan{};
+    pl.chunk = d.batch;
+    if (a.prefix_cap > 0) {
+        // up to 64 query rows of a KV head take the matrix-core decode kernels (16 rows per pass over the
+        // pages); any number the generic one (8 rows per pass)
+        const int G = d.num_q_heads / d.num_kv_heads;
+        if (d.kernel == 0 && (int64_t)G * d.batch > 64) pl.chunk = 64 / G > 0 ? 64 / G : 1;
+        if (pl.chunk > d.batch) pl.chunk = d.batch;
+        const int rest = d.batch % pl.chunk ? d.batch % pl.chunk : pl.chunk;
+        const ssq_decode_args whole = prefix_part(a, 0, pl.chunk, 0), last = prefix_part(a, d.batch - rest, rest, 0);
+        pl.n1 = ssq_decode_partial_splits(&whole);
+        pl.n1_last = ssq_decode_partial_splits(&last);
+        if (pl.n1 == 0 || pl.n1_last == 0) return SSQ_ERR_UNSUPPORTED;
+        const int64_t rows = (int64_t)d.num_q_heads * ((int64_t)(d.batch - rest) * pl.n1 + (int64_t)rest * pl.n1_last);
+        pl.pre_bytes = (size_t)(rows * d.q_len * (d.value_dim + 2) * 4);
+    }
+    if (d.seq_len > 0) {
+        pl.n2 = ssq_decode_partial_splits(&d);
+        if (pl.n2 == 0) return SSQ_ERR_UNSUPPORTED;
+        pl.own_bytes = (size_t)d.batch * d.num_q_heads * d.q_len * pl.n2 * (d.value_dim + 2) * 4;
+    }
+    return SSQ_OK;
+}
+
+}  // namespace
+
+extern "C" size_t ssq_decode_prefix_workspace_size(const ssq_prefix_args* a) {
+    PrefixPlan pl;
+    if (check(a) != SSQ_OK || make_plan(*a, pl) != SSQ_OK) return 0;
+    return pl.pre_bytes + pl.own_bytes;
+}
+
+extern "C" int ssq_decode_prefix(const ssq_prefix_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check(a);
+    if (rc) return rc;
+    const ssq_decode_args& d = a->dec;
+    PrefixPlan pl;
+    rc = make_plan(*a, pl);
+    if (rc) return rc;
+    SSQ_REQUIRE(workspace_bytes >= pl.pre_bytes + pl.own_bytes, "workspace too small: %zu < %zu bytes", workspace_bytes,
+                pl.pre_bytes + pl.own_bytes);
+    SSQ_REQUIRE(workspace || pl.pre_bytes + pl.own_bytes == 0, "workspace is NULL");
+    hipStream_t st = (hipStream_t)stream;
+    MergeParams m{};
+    m.a = d;
+    m.pre = reinterpret_cast<const float*>(workspace);
+    m.chunk = pl.chunk;
+    m.n1 = pl.n1;
+    m.n1_last = pl.n1_last;
+    m.own = reinterpret_cast<const float*>(reinterpret_cast<char*>(workspace) + pl.pre_bytes);
+    m.n2 = pl.n2;
+    if (pl.n1) {
+        char* at = reinterpret_cast<char*>(workspace);
+        for (int qi = 0; qi < d.q_len; ++qi)
+            for (int b0 = 0; b0 < d.batch; b0 += pl.chunk) {
+                const int n = d.batch - b0 < pl.chunk ? d.batch - b0 : pl.chunk;
+                ssq_decode_args part = prefix_part(*a, b0, n, qi);
+                part.num_splits = b0 + pl.chunk >= d.batch ? pl.n1_last : pl.n1;
+                const size_t bytes = (size_t)d.num_q_heads * n * part.num_splits * (d.value_dim + 2) * 4;
+                rc = ssq_decode_partials(&part, at, bytes, st);
+                if (rc) return rc;
+                at += bytes;
+            }
+    }
+    if (pl.n2) {
+        ssq_decode_args own = d;
+        own.num_splits = pl.n2;
+        own.lse = nullptr;
+        rc = ssq_decode_partials(&own, const_cast<float*>(m.own), pl.own_bytes, st);
+        if (rc) return rc;
+    }
+    const int64_t rows = (int64_t)d.batch * d.num_q_heads * d.q_len;
+    hipLaunchKernelGGL(k_merge_prefix, dim3((unsigned)((rows + kMergeRows - 1) / kMergeRows)), dim3(kMergeRows * SSQ_WAVE), 0, st, m);
+    return ssq_check_hip(hipGetLastError(), "k_merge_prefix launch");
+}

@@ -508,7 +508,7 @@ __global__ __launch_bounds__(kWT) void k_decode_wide(const SsqGenericParams p) {
         const int g = row / a.q_len, qi = row - g * a.q_len;
         const int h = kv * p.G + g;
         const int rid = (b * a.num_q_heads + h) * a.q_len + qi;
-        if (p.n_splits == 1) {
+        if (p.n_splits == 1 && !p.partial) {
             ssq_store_elem(a.out, a.v_dtype, (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)qi * a.o_sl + dv, o / l);
             if (a.lse && dv == 0) a.lse[rid] = m + logf(l);
         } else {

@@ -80,6 +80,7 @@ __global__ __launch_bounds__(kScanThreads) void k_encode_scan(const EncodeParams
         for (int d = 0; d < bd; ++d) x[d] = ssq_load_elem(a.keys, a.k_dtype, kbase + perm[blk * bd + d]);
         int64_t crow, prow;
         out_rows(a, b, kv, s, crow, prow);
+        if (crow == kNoRow) continue;
         if (heavy) {
             a.codes[crow + blk] = 0;
             const int slot = a.pt_dense ? blk : heavy_ordinal(a.heavy_mask[0], a.heavy_mask[1], blk);

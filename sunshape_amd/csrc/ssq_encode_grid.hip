@@ -467,6 +467,7 @@ __global__ __launch_bounds__(1024) void k_encode_grid(const GridParams p) {
             const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
             crow_k = page * a.c_sb + (int64_t)kv * a.c_sh + off * a.c_st;
             prow_k = page * a.pt_sb + (int64_t)kv * a.pt_sh + off * a.pt_st;
+            if (slot < 0) crow_k = kNoRow;
         } else {
             crow_k = (int64_t)b * a.c_sb + (int64_t)kv * a.c_sh + (int64_t)ss * a.c_st;
             prow_k = (int64_t)b * a.pt_sb + (int64_t)kv * a.pt_sh + (int64_t)ss * a.pt_st;
@@ -725,6 +726,7 @@ __global__ __launch_bounds__(1024) void k_encode_grid(const GridParams p) {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     const int s_wave = gxi * keys_wg + wave * 64;
+    const bool put = live && crow_k != kNoRow;
     if (p.row_codes) {
         const int pieces = nb >> 4;
         for (int e = lane; e < 64 * pieces; e += 64) {
@@ -734,15 +736,15 @@ __global__ __launch_bounds__(1024) void k_encode_grid(const GridParams p) {
             const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)crow_k, m);
             const uint32_t hi = (uint32_t)__shfl((int)(uint32_t)((uint64_t)crow_k >> 32), m);
             const int64_t crow = (int64_t)(((uint64_t)hi << 32) | lo);
-            if (i < km.n_keys) {
+            if (i < km.n_keys && crow != kNoRow) {
                 const uint32_t* src = reinterpret_cast<const uint32_t*>(cs + m * crb + 16 * q);
                 *reinterpret_cast<uint4*>(a.codes + crow + 16 * q) = make_uint4(src[0], src[1], src[2], src[3]);
             }
         }
-    } else if (live && gridDim.z == 1) {  // every block's code (heavy blocks' 0 included)
+    } else if (put && gridDim.z == 1) {  // every block's code (heavy blocks' 0 included)
         const int64_t crow = crow_k;
         for (int blk = 0; blk < nb; ++blk) a.codes[crow + blk] = cs[lane * crb + blk];
-    } else if (live) {  // one chunk of several: its blocks' codes; chunk 0 also the heavy blocks' 0
+    } else if (put) {  // one chunk of several: its blocks' codes; chunk 0 also the heavy blocks' 0
         const int64_t crow = crow_k;
         for (int li = 0; li < nl; ++li) {
             const int blk = __builtin_amdgcn_readfirstlane(poff[4 * li + 2]);
@@ -752,7 +754,7 @@ __global__ __launch_bounds__(1024) void k_encode_grid(const GridParams p) {
     // chunk 0: the heavy blocks' values as the key holds them, and (with several chunks, whose
     // stores are per block) their code 0.  One pass over the heavy blocks listed in LDS, the
     // stored dtype's branch taken once.
-    if ((hm0 | hm1) && live && blockIdx.z == 0) {
+    if ((hm0 | hm1) && put && blockIdx.z == 0) {
         const int nh = __popcll(hm0) + __popcll(hm1);
         const bool zero_codes = gridDim.z > 1;
         auto heavy_pair = [&](int h, int& blk, int& slot, float& x0, float& x1) {

@@ -56,7 +56,7 @@ __device__ __forceinline__ int heavy_ordinal(uint64_t hm0, uint64_t hm1, int blk
     return __popcll(hm0) + __popcll(hm1 & ((1ull << (blk - 64)) - 1ull));
 }
 
-// output row bases for key (b, kv, s): codes and passthrough
+// output row bases for key (b, kv, s): codes and passthrough; crow is kNoRow for a padded key (negative slot)
 __device__ __forceinline__ void out_rows(const ssq_encode_args& a, int b, int kv, int s, int64_t& crow,
                                          int64_t& prow) {
     if (a.slot_mapping) {
@@ -64,6 +64,7 @@ __device__ __forceinline__ void out_rows(const ssq_encode_args& a, int b, int kv
         const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
         crow = page * a.c_sb + (int64_t)kv * a.c_sh + off * a.c_st;
         prow = page * a.pt_sb + (int64_t)kv * a.pt_sh + off * a.pt_st;
+        if (slot < 0) crow = kNoRow;
     } else {
         crow = (int64_t)b * a.c_sb + (int64_t)kv * a.c_sh + (int64_t)s * a.c_st;
         prow = (int64_t)b * a.pt_sb + (int64_t)kv * a.pt_sh + (int64_t)s * a.pt_st;

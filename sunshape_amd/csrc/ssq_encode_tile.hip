@@ -1039,7 +1039,7 @@ __global__ __launch_bounds__(kTileThreads) void k_encode_tile(const TileParams p
     if (!live) return;
 
     // codes out: whole rows in 16-byte pieces, or element by element; lane and lane + 32 share a key
-    const bool mine = s0 + col < n_keys;
+    const bool mine = s0 + col < n_keys && crow != kNoRow;
     const int cwid = ssq_code_width(nc);
     const u32a* ck = mykeys + col * SD;
     if (p.row_codes) {

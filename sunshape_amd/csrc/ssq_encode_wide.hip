@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kWideThreads) void k_encode_wide(const WideEncodePa
             if (d < bd) x[d] = ssq_load_elem(a.keys, a.k_dtype, kbase + perm[d]);
         out_rows(a, b, kv, s, crow, prow);
         if (heavy) {  // passthrough block: code 0, values copied (sunshape/codec.py:367-372)
-            if (sl == 0) {
+            if (sl == 0 && crow != kNoRow) {
                 store_code(a.codes, cw, crow + blk, 0u);
                 const int slot = a.pt_dense ? blk : heavy_ordinal(a.heavy_mask[0], a.heavy_mask[1], blk);
                 for (int d = 0; d < bd; ++d) ssq_store_elem(a.pt, a.pt_dtype, prow + (int64_t)slot * bd + d, x[d]);
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kWideThreads) void k_encode_wide(const WideEncodePa
             j_best = oj;
         }
     }
-    if (live && sl == 0) store_code(a.codes, cw, crow + blk, j_best);
+    if (live && sl == 0 && crow != kNoRow) store_code(a.codes, cw, crow + blk, j_best);
 }
 
 }  // namespace

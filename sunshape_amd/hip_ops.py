@@ -318,6 +318,111 @@ def decode(q: torch.Tensor, codes: torch.Tensor, v: torch.Tensor, perm: torch.Te
     return tuple(res)
 
 
+def decode_prefix(q: torch.Tensor, codes: torch.Tensor, v: torch.Tensor, perm: torch.Tensor, cent: torch.Tensor, *,
+                  prefix_table: torch.Tensor, prefix_len: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                  scale: Optional[float] = None, mask: Optional[torch.Tensor] = None,
+                  heavy: Optional[Sequence[bool]] = None, pt: Optional[torch.Tensor] = None, pt_dense: bool = False,
+                  return_lse: bool = False, kernel: int = 0, code_bits: int = 0,
+                  rotation: Optional[torch.Tensor] = None):
+    """Decode attention for a batch whose sequences share a prefix, which is read once for all of them.
+
+    Every query row attends the prefix's tokens and its own sequence's, one softmax over both.
+    q [B, Hq, Lq, D], codes, v and pt pages as in decode()'s paged layout (page_size 8 to 256, a
+    divisor of 256).  prefix_table int32 [pages] and prefix_len int32 [1] hold the prefix;
+    block_table int32 [B, max_pages] and seq_lens int32 [B] the sequences' own tokens (a width of 0
+    and lengths of 0 are fine).  All lengths stay on the device.  mask: additive, broadcastable to
+    [B, Hq, Lq, max_pages * page], over the own tokens (the prefix is seen by every row).
+    Returns out [B, Hq, Lq, Dv] in v's dtype, and lse [B, Hq, Lq] (fp32) when requested; a row with
+    nothing to attend gives 0 and -inf.  kernel 1 takes the decode kernels that serve every codec,
+    for comparisons.  No counterpart in the reference.
+    """
+    for name, t in (("query", q), ("codes", codes), ("value", v)):
+        _on_gpu(name, t)
+    if rotation is not None:
+        _require(q.ndim == 4, "Quantized attention expects query/value tensors with shape [batch, heads, seq, dim].")
+        q = transform_rows(q, rotation, scale=scale)
+        scale = None
+        perm = _identity_like(perm)
+    hm0, hm1 = N.mask_words_signed(heavy)
+    try:
+        out, lse = N.torch_ops().decode_prefix(q, codes, v, perm, cent, None if scale is None else float(scale), mask, hm0,
+                                               hm1, pt, bool(pt_dense), prefix_table, prefix_len, block_table, seq_lens,
+                                               bool(return_lse), int(kernel), int(code_bits))
+    except RuntimeError as e:
+        raise N.kernel_error(e) from None
+    return (out, lse) if return_lse else out
+
+
+def rope_table(max_position: int, rot_dim: int, *, base: float = 10000.0,
+               device: Optional[torch.device] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin of position * base^(-2i / rot_dim), fp32 [max_position, rot_dim / 2] from 64-bit
+    angles: the tables of qk_norm_rope and append_kv, made once per model."""
+    _require(rot_dim >= 2 and rot_dim % 2 == 0, f"rot_dim must be even and at least 2, got {rot_dim}")
+    _require(max_position >= 1, "max_position must be at least 1")
+    freq = float(base) ** (-torch.arange(0, rot_dim, 2, device=device, dtype=torch.float64) / rot_dim)
+    ang = torch.arange(max_position, device=device, dtype=torch.float64)[:, None] * freq[None]
+    return ang.cos().float(), ang.sin().float()
+
+
+def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                 positions: Optional[torch.Tensor], *, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Per-head RMS norm and position rotation of queries and keys in one pass.
+
+    q [B, Hq, S, D], k [B, Hkv, S, D] or None, any strides with D contiguous, one dtype (fp32, bf16 or
+    f16).  cos / sin: fp32 [max_position, rot_dim / 2] tables (rope_table), positions int64 [B, S];
+    the first rot_dim dims rotate, in pairs (i, i + rot_dim / 2), or (2i, 2i + 1) when interleaved.
+    None for all three: norm only.  q_weight / k_weight [D]: norm weights of any of the dtypes, shared
+    by the heads; None: no norm.  Computed in fp32 (the norm's sum in 64 bits) and rounded once.
+    Returns new tensors in the inputs' stride order, (q, k) or (q, None).  A position outside the
+    tables makes the row's rotated dims NaN.  No counterpart in the reference, whose model code
+    rotates before the cache sees the keys.
+    """
+    _on_gpu("query", q)
+    try:
+        q_out, k_out = N.torch_ops().qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, float(eps),
+                                                  bool(interleaved))
+    except RuntimeError as e:
+        raise N.kernel_error(e) from None
+    return q_out, None if k is None else k_out
+
+
+def append_kv(keys: torch.Tensor, values: Optional[torch.Tensor], perm: torch.Tensor, cent: torch.Tensor, *,
+              codes_out: torch.Tensor, v_out: Optional[torch.Tensor], slot_mapping: torch.Tensor,
+              cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+              positions: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+              interleaved: bool = False, heavy: Optional[Sequence[bool]] = None, pt_out: Optional[torch.Tensor] = None,
+              pt_dense: bool = False, metric: Optional[torch.Tensor] = None, grid: Optional[torch.Tensor] = None,
+              direct: bool = False, kernel: int = 0, rotation: Optional[torch.Tensor] = None) -> None:
+    """Append raw keys and values to a paged cache, the keys normed and rotated on the way.
+
+    keys [B, Hkv, S, D] (before their norm and rotation), values [B, Hkv, S, Dv] or None; slot_mapping
+    int64 [B, S], distinct slots (page * page_size + offset); a negative slot, or one past the pages, is
+    padding and writes nothing.  The keys are taken through qk_norm_rope's norm (k_weight) and rotation
+    (cos, sin, positions), each left out when None, rounded to their dtype, and encoded as encode()
+    does, into codes_out [P, Hkv, page, nb] and, for heavy blocks, pt_out [P, Hkv, page, slots, bd];
+    values go to v_out [P, Hkv, Dv, page], converted to its dtype.  metric, grid, direct and rotation (the
+    codec's rotated mode, after the position rotation) as in encode(); kernel: 0, or 1 for the exact
+    scan.  No counterpart in the reference.
+    """
+    _on_gpu("key_states", keys)
+    if rotation is not None:
+        _require(keys.ndim == 4, "append_kv expects key_states with shape [batch, kv_heads, seq_len, head_dim].")
+        if cos is not None or k_weight is not None:
+            keys, _ = qk_norm_rope(keys, None, cos, sin, positions, q_weight=k_weight, eps=eps, interleaved=interleaved)
+        cos = sin = positions = k_weight = None
+        keys = transform_rows(keys, rotation)
+        perm = _identity_like(perm)
+    hm0, hm1 = N.mask_words_signed(heavy)
+    try:
+        N.torch_ops().append_kv(keys, values, perm, cent, hm0, hm1, bool(pt_dense), codes_out, pt_out, v_out, slot_mapping,
+                                metric, grid, int(kernel), bool(direct), cos, sin, positions, k_weight, float(eps),
+                                bool(interleaved))
+    except RuntimeError as e:
+        raise N.kernel_error(e) from None
+
+
 def _encode_prepare(keys, perm, cent, heavy, pt_dtype, pt_dense, codes_out, pt_out, slot_mapping, metric, rotation):
     """Validated encode inputs and the outputs to write (allocated unless given): a namespace of
     keys, perm, cent, perm_sh, cent_sh, bd, nb, nc, w0, w1, metric, metric_sh, codes, pt, pt_dtype,

@@ -9,7 +9,12 @@ layout.  This is the caller on the write side of the decode kernel:
 * passthrough [P, Hkv, page, n_heavy, bd] for SunShape-Mixed heavy blocks;
 * value pages [P, Hkv, Dv, page] -- vLLM's dim-major value layout, which the
   MFMA decode kernel reads as B-operand fragments directly;
-* per-sequence block tables and lengths, with a simple free-page allocator.
+* per-sequence block tables and lengths, with a simple free-page allocator;
+* sequences that continue a shared one (``fork``): its pages are held once, and decode reads them once
+  for the whole batch.
+
+``attend`` is one layer's step of a serving loop: norm and rotation of the queries, the append of raw keys
+and values with the same for the keys, and the attention.
 """
 
 from __future__ import annotations
@@ -47,6 +52,7 @@ class PagedSunShapeCache:
         self._free = list(range(num_pages - 1, -1, -1))
         self.block_tables: dict[int, list[int]] = {}
         self.seq_lens: dict[int, int] = {}
+        self.prefix_of: dict[int, int] = {}  # forked sequence -> the sequence it continues
 
     # ------------------------------------------------------------------ pages
     def _ensure_capacity(self, seq_id: int, new_len: int) -> None:
@@ -58,13 +64,42 @@ class PagedSunShapeCache:
             table.append(self._free.pop())
 
     def free(self, seq_id: int) -> None:
+        if seq_id in self.prefix_of.values():
+            raise RuntimeError(f"sequence {seq_id} is the prefix of others; free them first")
+        self.prefix_of.pop(seq_id, None)
         for pg in self.block_tables.pop(seq_id, []):
             self._free.append(pg)
         self.seq_lens.pop(seq_id, None)
 
+    def fork(self, prefix_id: int, seq_ids: list[int]) -> None:
+        """Start empty sequences that continue prefix_id's tokens.  The prefix takes no more tokens while
+        any of them lives."""
+        if prefix_id not in self.seq_lens or prefix_id in self.prefix_of:
+            raise RuntimeError(f"sequence {prefix_id} cannot be a prefix: it holds no tokens or continues another")
+        if len(set(seq_ids)) != len(seq_ids) or any(s == prefix_id or s in self.seq_lens or s in self.prefix_of
+                                                    for s in seq_ids):
+            raise RuntimeError("fork starts new, distinct sequences")
+        for s in seq_ids:
+            self.prefix_of[s] = prefix_id
+
+    def _shared_prefix(self, seq_ids: list[int]) -> Optional[int]:
+        found = {self.prefix_of.get(s) for s in seq_ids}
+        if len(found) > 1:
+            raise RuntimeError("the sequences of one call must continue the same prefix, or none")
+        return found.pop() if found else None
+
+    def positions(self, seq_ids: list[int], num_new: int) -> torch.Tensor:
+        """int64 positions [len(seq_ids), num_new] of the next num_new tokens of (distinct) sequences, their
+        prefix counted."""
+        first = [self.seq_lens.get(s, 0) + self.seq_lens.get(self.prefix_of.get(s), 0) for s in seq_ids]
+        return torch.tensor([[f + i for i in range(num_new)] for f in first], dtype=torch.int64,
+                            device=self.device).view(len(seq_ids), num_new)
+
     def slot_mapping(self, seq_ids: list[int], num_new: int) -> torch.Tensor:
         """Allocate room for num_new tokens per sequence; return int64 slots [len(seq_ids), num_new]."""
         rows = []
+        if any(s in self.prefix_of.values() for s in seq_ids):
+            raise RuntimeError("a sequence that others continue takes no more tokens")
         for sid in seq_ids:
             start = self.seq_lens.get(sid, 0)
             self._ensure_capacity(sid, start + num_new)
@@ -75,11 +110,29 @@ class PagedSunShapeCache:
         return torch.tensor(rows, dtype=torch.int64, device=self.device)
 
     # ------------------------------------------------------------------ append / decode
-    def append(self, seq_ids: list[int], key_states: torch.Tensor, value_states: torch.Tensor) -> torch.Tensor:
-        """Encode keys [B, Hkv, S, D] into the code pages and write values [B, Hkv, S, Dv]; returns the slots."""
+    def append(self, seq_ids: list[int], key_states: torch.Tensor, value_states: torch.Tensor, *,
+               cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+               k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
+        """Encode keys [B, Hkv, S, D] into the code pages and write values [B, Hkv, S, Dv]; returns the slots.
+
+        With cos and sin (tables, hip_ops.rope_table) or k_weight the keys are raw: they are normed and
+        rotated on the way, each token at its position in its sequence (its prefix counted)."""
         B, Hkv, S, _ = key_states.shape
         if Hkv != self.num_kv_heads or value_states.shape[:3] != key_states.shape[:3]:
             raise RuntimeError("key/value shapes do not match the cache")
+        if cos is not None or k_weight is not None:
+            if len(set(seq_ids)) != len(seq_ids):
+                raise RuntimeError("an append with rotation takes each sequence once")
+            positions = self.positions(seq_ids, S) if cos is not None else None
+            slots = self.slot_mapping(seq_ids, S)
+            hip_ops.append_kv(key_states.to(self.device), value_states.to(self.device), self.codec.effective_permutation(),
+                              self.codec.centroids, codes_out=self.code_pages, v_out=self.v_pages, slot_mapping=slots,
+                              cos=cos, sin=sin, positions=positions, k_weight=k_weight, eps=eps, interleaved=interleaved,
+                              heavy=self.heavy, pt_out=self.pt_pages, metric=self.codec.encode_metric(),
+                              grid=self.codec.encode_search_grid(self.codec.centroids),
+                              direct=hip_ops.cdist_direct(S, self.codec.n_centroids),
+                              rotation=self.codec.rotation_matrix())
+            return slots
         slots = self.slot_mapping(seq_ids, S)
         perm = self.codec.effective_permutation()
         # as quantize_key_states: one reference cdist per (sequence, KV head) over its S new keys
@@ -105,10 +158,43 @@ class PagedSunShapeCache:
         return bt.to(self.device), lens.to(self.device)
 
     def decode(self, seq_ids: list[int], query: torch.Tensor, *, scale: Optional[float] = None,
-               return_lse: bool = False):
-        """Fused decode of query [B, Hq, Lq, D] against the cached sequences."""
+               return_lse: bool = False, mask: Optional[torch.Tensor] = None):
+        """Fused decode of query [B, Hq, Lq, D] against the cached sequences; forked ones attend their shared
+        prefix's tokens first.  mask: additive, broadcastable to [B, Hq, Lq, T], T the sequences' own
+        table width times the page size."""
+        prefix = self._shared_prefix(seq_ids)
         bt, lens = self.tables(seq_ids)
-        return hip_ops.decode(query, self.code_pages, self.v_pages, self.codec.effective_permutation(),
-                              self.codec.centroids, scale=scale, heavy=self.heavy, pt=self.pt_pages,
-                              pt_dense=False, block_table=bt, seq_lens=lens, return_lse=return_lse,
-                              rotation=self.codec.rotation_matrix())
+        if prefix is None:
+            return hip_ops.decode(query, self.code_pages, self.v_pages, self.codec.effective_permutation(),
+                                  self.codec.centroids, scale=scale, mask=mask, heavy=self.heavy, pt=self.pt_pages,
+                                  pt_dense=False, block_table=bt, seq_lens=lens, return_lse=return_lse,
+                                  rotation=self.codec.rotation_matrix())
+        ptab, plen = self.tables([prefix])
+        return hip_ops.decode_prefix(query, self.code_pages, self.v_pages, self.codec.effective_permutation(),
+                                     self.codec.centroids, prefix_table=ptab[0], prefix_len=plen, block_table=bt,
+                                     seq_lens=lens, scale=scale, mask=mask, heavy=self.heavy, pt=self.pt_pages,
+                                     return_lse=return_lse, rotation=self.codec.rotation_matrix())
+
+    def attend(self, seq_ids: list[int], query: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor, *,
+               cos: torch.Tensor, sin: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+               k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+               scale: Optional[float] = None) -> torch.Tensor:
+        """One step over raw projections: query [B, Hq, S, D], keys and values [B, Hkv, S, ..] of the S next
+        tokens of each sequence.  Norms and rotates them, appends keys and values, and attends causally;
+        returns [B, Hq, S, Dv]."""
+        B, _, S, _ = query.shape
+        if len(set(seq_ids)) != len(seq_ids):
+            raise RuntimeError("attend takes each sequence once")
+        self._shared_prefix(seq_ids)
+        q, _ = hip_ops.qk_norm_rope(query, None, cos, sin, self.positions(seq_ids, S), q_weight=q_weight, eps=eps,
+                                    interleaved=interleaved)
+        self.append(seq_ids, key_states, value_states, cos=cos, sin=sin, k_weight=k_weight, eps=eps,
+                    interleaved=interleaved)
+        mask = None
+        if S > 1:  # new token i sees its sequence up to itself
+            width = max(len(self.block_tables[s]) for s in seq_ids) * self.page_size
+            last = torch.tensor([self.seq_lens[s] - S for s in seq_ids], device=self.device)[:, None] + \
+                torch.arange(S, device=self.device)[None]
+            mask = torch.zeros(B, 1, S, width, device=self.device)
+            mask.masked_fill_(torch.arange(width, device=self.device) > last[:, None, :, None], float("-inf"))
+        return self.decode(seq_ids, q, scale=scale, mask=mask)

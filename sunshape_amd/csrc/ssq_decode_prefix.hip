@@ -6,7 +6,10 @@
 // with (o, m, l) = (sum_t e^{s_t - m} v_t, max_t s_t, sum_t e^{s_t - m}) of a set of tokens.  The prefix is one
 // sequence whose query rows are all sequences' rows of a KV head, so its codes and values are read once for them.
 // Both parts leave fp32 (o, m, l) in the workspace, per context split, and k_merge_prefix joins them.
-#include "ssq_common.h"
+//
+// Byte-code codecs of head_dim 64 and 128 take the matrix-core kernel (ssq_prefix_mfma.h), one launch for the prefix
+// and the own tokens; every other problem the decode kernels (ssq_decode_partials).
+#include "ssq_prefix_mfma.h"
 
 #include <math.h>
 
@@ -24,36 +27,38 @@ struct MergeParams {
     ssq_decode_args a;
     // The prefix's partials: for each query position and each chunk of `chunk` sequences a block of
     // n1 (the last chunk n1_last) splits x (num_q_heads * sequences) rows: o, then m, then l.
+    // flat: one block of n1 splits x (batch * num_q_heads * q_len) rows instead, as the own tokens'.
     const float* pre;
-    int chunk, n1, n1_last;
+    int chunk, n1, n1_last, flat;
     // the own tokens' partials, n2 splits x (batch * num_q_heads * q_len) rows (0: none)
     const float* own;
     int n2;
 };
 
-// One wave per query row; lane j merges value dims j, j + 64, ...
+// One wave per query row.  A lane takes a split's (m, l), 64 at a time; the splits that hold anything are then
+// joined with lane j on value dims j, j + 64, ...: bytes bound it, and splits without tokens cost no o.
 __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const MergeParams p) {
     const ssq_decode_args& a = p.a;
     const int lane = threadIdx.x & (SSQ_WAVE - 1);
     const int64_t n_rows = (int64_t)a.batch * a.num_q_heads * a.q_len;
-    const int64_t rid = (int64_t)blockIdx.x * kMergeRows + threadIdx.x / SSQ_WAVE;
+    const int64_t rid = (int64_t)blockIdx.x * kMergeRows + __builtin_amdgcn_readfirstlane(threadIdx.x / SSQ_WAVE);
     if (rid >= n_rows) return;  // whole waves
     const int qi = (int)(rid % a.q_len);
     const int h = (int)(rid / a.q_len % a.num_q_heads);
     const int b = (int)(rid / a.q_len / a.num_q_heads);
     const int Dv = a.value_dim;
     // this row's prefix block
-    const int c = p.n1 ? b / p.chunk : 0;
-    const int cn = p.n1 ? min(p.chunk, a.batch - c * p.chunk) : 0;
-    const bool last = (int64_t)(c + 1) * p.chunk >= a.batch;
-    const int n1 = p.n1 ? (last ? p.n1_last : p.n1) : 0;
-    const int full = p.n1 ? a.batch / p.chunk : 0;  // whole chunks of a query position
-    const int rest = p.n1 ? a.batch - full * p.chunk : 0;
-    const int64_t per_q = (int64_t)a.num_q_heads * ((int64_t)full * p.chunk * (rest ? p.n1 : 0) +
-                                                    (rest ? (int64_t)rest * p.n1_last
-                                                          : (int64_t)(full - 1) * p.chunk * p.n1 + (int64_t)p.chunk * p.n1_last));
-    const int64_t at0 = (per_q * qi + (int64_t)a.num_q_heads * c * p.chunk * p.n1) * (Dv + 2);
-    const int64_t rows1 = (int64_t)a.num_q_heads * cn, row1 = (int64_t)h * cn + (b - c * p.chunk);
+    int n1 = p.n1;
+    int64_t at0 = 0, rows1 = n_rows, row1 = rid;
+    if (p.n1 && !p.flat) {
+        const int c = b / p.chunk, cn = min(p.chunk, a.batch - c * p.chunk);
+        if ((int64_t)(c + 1) * p.chunk >= a.batch) n1 = p.n1_last;
+        const int rest = a.batch % p.chunk ? a.batch % p.chunk : p.chunk;
+        const int64_t per_q = (int64_t)a.num_q_heads * ((int64_t)(a.batch - rest) * p.n1 + (int64_t)rest * p.n1_last);
+        at0 = (per_q * qi + (int64_t)a.num_q_heads * c * p.chunk * p.n1) * (Dv + 2);
+        rows1 = (int64_t)a.num_q_heads * cn;
+        row1 = (int64_t)h * cn + (b - c * p.chunk);
+    }
     const float* pre_o = p.pre + at0;
     const float* pre_m = pre_o + rows1 * n1 * Dv;
     const float* pre_l = pre_m + rows1 * n1;
@@ -65,34 +70,39 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
         float Mr = -INFINITY, Lr = 0.f, o[kMergeDims];
 #pragma unroll
         for (int k = 0; k < kMergeDims; ++k) o[k] = 0.f;
-        for (int s0 = 0; s0 < n; s0 += kMergeBatch) {
-            float mv[kMergeBatch], lv[kMergeBatch], ov[kMergeBatch][kMergeDims];
-#pragma unroll
-            for (int i = 0; i < kMergeBatch; ++i) {
-                const int s = min(s0 + i, n - 1);  // uniform; a repeated split weighs nothing
-                const bool pre = s < n1;
-                const int64_t at = pre ? (int64_t)s * rows1 + row1 : (int64_t)(s - n1) * n_rows + rid;
-                mv[i] = s0 + i < n ? (pre ? pre_m : own_m)[at] : -INFINITY;
-                lv[i] = (pre ? pre_l : own_l)[at];
-                const float* src = (pre ? pre_o : p.own) + at * Dv;
-#pragma unroll
-                for (int k = 0; k < kMergeDims; ++k)
-                    ov[i][k] = d0 + k * SSQ_WAVE < Dv ? src[min(d0 + k * SSQ_WAVE + lane, Dv - 1)] : 0.f;
-            }
-            float Mc = Mr;
-#pragma unroll
-            for (int i = 0; i < kMergeBatch; ++i) Mc = fmaxf(Mc, mv[i]);
-            const float f = Mr == -INFINITY ? 0.f : __expf(Mr - Mc);
-            Lr *= f;
+        for (int s0 = 0; s0 < n; s0 += SSQ_WAVE) {
+            const int s = s0 + lane;
+            const bool pre = s < n1;
+            const int64_t at = pre ? (int64_t)s * rows1 + row1 : (int64_t)(s - n1) * n_rows + rid;
+            const float m = s < n ? (pre ? pre_m : own_m)[at] : -INFINITY;
+            const float l = m != -INFINITY ? (pre ? pre_l : own_l)[at] : 0.f;
+            const float Mc = fmaxf(Mr, ssq_wave_max(m));
+            if (Mc == -INFINITY) continue;
+            const float f = Mr == -INFINITY ? 0.f : __expf(Mr - Mc);  // earlier passes, rescaled
+            const float w = m == -INFINITY ? 0.f : __expf(m - Mc);
+            Lr = Lr * f + ssq_wave_sum(l * w);
 #pragma unroll
             for (int k = 0; k < kMergeDims; ++k) o[k] *= f;
+            uint64_t live = __builtin_amdgcn_ballot_w64(m != -INFINITY);
+            while (live) {  // wave-uniform
+                float ov[kMergeBatch][kMergeDims], wv[kMergeBatch];
 #pragma unroll
-            for (int i = 0; i < kMergeBatch; ++i) {
-                if (mv[i] == -INFINITY) continue;  // nothing attended in this split
-                const float w = __expf(mv[i] - Mc);
-                Lr += lv[i] * w;
+                for (int i = 0; i < kMergeBatch; ++i) {
+                    const int src = live ? __builtin_ctzll(live) : 0;
+                    wv[i] = live ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), src)) : 0.f;
+                    const int sp = s0 + src;
+                    const float* ob = live ? (sp < n1 ? pre_o + ((int64_t)sp * rows1 + row1) * Dv
+                                                      : p.own + ((int64_t)(sp - n1) * n_rows + rid) * Dv)
+                                           : nullptr;
 #pragma unroll
-                for (int k = 0; k < kMergeDims; ++k) o[k] += ov[i][k] * w;
+                    for (int k = 0; k < kMergeDims; ++k)
+                        ov[i][k] = ob && d0 + k * SSQ_WAVE < Dv ? ob[min(d0 + k * SSQ_WAVE + lane, Dv - 1)] : 0.f;
+                    live &= live - 1;
+                }
+#pragma unroll
+                for (int i = 0; i < kMergeBatch; ++i)
+#pragma unroll
+                    for (int k = 0; k < kMergeDims; ++k) o[k] += ov[i][k] * wv[i];
             }
             Mr = Mc;
         }
@@ -112,7 +122,85 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
 struct PrefixPlan {
     int chunk, n1, n1_last, n2;
     size_t pre_bytes, own_bytes;
+    bool fast;  // the matrix-core kernel
+    SsqPrefixParams fp;
 };
+
+// Problems of the matrix-core kernel: pages of whole 16-token pieces, byte codes, codewords of 2, 4 or 8 dims.
+bool fast_shape(const ssq_decode_args& d) {
+    if (d.kernel != 0 || (d.head_dim != 64 && d.head_dim != 128) || d.value_dim != d.head_dim) return false;
+    if (d.block_dim != 2 && d.block_dim != 4 && d.block_dim != 8) return false;
+    if (d.n_centroids > 256 || (d.code_bits != 0 && d.code_bits != 8) || d.page_size % 16) return false;
+    if (d.heavy_mask[0] | d.heavy_mask[1]) return false;
+    if (d.v_dtype != SSQ_BF16 && d.v_dtype != SSQ_F16) return false;
+    if ((uintptr_t)d.cent % 16 || d.cent_sh % 4) return false;
+    const int64_t cal = d.n_blocks >= 16 ? 16 : d.n_blocks, unit = d.code_bits ? 4 : 1;  // code rows load in pieces
+    if ((uintptr_t)d.codes % cal || (d.c_sb * unit) % cal || (d.c_sh * unit) % cal || (d.c_st * unit) % cal) return false;
+    if ((uintptr_t)d.v % 16 || d.v_sb % 8 || d.v_sh % 8 || d.v_st % 8) return false;
+    return d.v_st >= 0 && d.v_st <= 1 << 22;  // 32-bit offsets inside a page
+}
+
+// How the prefix and the own tokens are cut into items (ssq_prefix_mfma.h).
+void fast_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
+    const ssq_decode_args& d = a.dec;
+    SsqPrefixParams& f = pl.fp;
+    f = SsqPrefixParams{};
+    f.a = d;
+    if (d.code_bits == 8) {  // 8-bit words are the byte rows
+        f.a.c_sb *= 4; f.a.c_sh *= 4; f.a.c_st *= 4;
+    }
+    f.ptab = a.prefix_table;
+    f.plen = a.prefix_len;
+    f.pcap = a.prefix_cap;
+    f.G = d.num_q_heads / d.num_kv_heads;
+    const int per_b = f.G * d.q_len;
+    f.rows = per_b * d.batch;
+    const int cus = ssq_device_cus();
+    f.n_wg = cus / d.num_kv_heads > 0 ? cus / d.num_kv_heads : 1;
+    while ((16 << f.psh) < d.page_size) ++f.psh;
+    const bool split = !(d.q_dtype == SSQ_BF16 && d.v_dtype == SSQ_BF16) && !(d.q_dtype == SSQ_F16 && d.v_dtype == SSQ_F16);
+    f.pre_nr = split || f.rows <= 32 ? 1 : 2;
+    f.own_nr = split || per_b <= 32 ? 1 : 2;
+    f.n_rg = (f.rows + 32 * f.pre_nr - 1) / (32 * f.pre_nr);
+    f.own_rg = (per_b + 32 * f.own_nr - 1) / (32 * f.own_nr);
+    if (a.prefix_cap > 0) {
+        // Slices of the prefix: the number that takes the fewest rounds of (4 + tiles of a wave) units: an item's
+        // staging and join cost about as much as 4 tiles.
+        const int tiles = (a.prefix_cap + 31) / 32;
+        int64_t best = INT64_MAX;
+        for (int n1 = 1; n1 <= 128 && (n1 == 1 || n1 * 4 <= tiles); ++n1) {
+            const int64_t rounds = ((int64_t)f.n_rg * n1 + f.n_wg - 1) / f.n_wg;
+            const int64_t cost = rounds * (4 + ((tiles + n1 - 1) / n1 + 3) / 4);
+            if (cost < best) {
+                best = cost;
+                f.n1 = n1;
+            }
+        }
+    }
+    if (d.seq_len > 0) {
+        // pieces of 16 tiles (512 tokens), down to 4 where there are fewer items than workgroups; at most 64
+        const int tiles = (d.seq_len + 31) / 32;
+        f.own_tiles = 16;
+        while (f.own_tiles > 4 && (int64_t)d.batch * f.own_rg * ((tiles + f.own_tiles - 1) / f.own_tiles) < 2 * f.n_wg) f.own_tiles /= 2;
+        while ((tiles + f.own_tiles - 1) / f.own_tiles > 64) f.own_tiles *= 2;
+        f.n2 = (tiles + f.own_tiles - 1) / f.own_tiles;
+    }
+    const int64_t rows = (int64_t)d.batch * d.num_q_heads * d.q_len;
+    pl.n1 = pl.n1_last = f.n1;
+    pl.n2 = f.n2;
+    pl.pre_bytes = ((size_t)(rows * f.n1 * (d.value_dim + 2) * 4) + 255) & ~(size_t)255;  // 16-byte stores in both parts
+    pl.own_bytes = (size_t)(rows * f.n2 * (d.value_dim + 2) * 4);
+}
+
+int fast_launch(const PrefixPlan& pl, void* workspace, hipStream_t st) {
+    SsqPrefixParams f = pl.fp;
+    f.pre = reinterpret_cast<float*>(workspace);
+    f.own = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + pl.pre_bytes);
+    const ssq_decode_args& d = f.a;
+    if (d.q_dtype == SSQ_BF16 && d.v_dtype == SSQ_BF16) return ssq_prefix_bf16(f, st);
+    if (d.q_dtype == SSQ_F16 && d.v_dtype == SSQ_F16) return ssq_prefix_f16(f, st);
+    return d.v_dtype == SSQ_BF16 ? ssq_prefix_split_bf16(f, st) : ssq_prefix_split_f16(f, st);
+}
 
 // sequences [b0, b0 + n) at query position qi as one sequence of n query rows per head, attending the prefix
 ssq_decode_args prefix_part(const ssq_prefix_args& a, int b0, int n, int qi) {
@@ -163,6 +251,11 @@ int make_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
     const ssq_decode_args& d = a.dec;
     pl = PrefixPlan{};
     pl.chunk = d.batch;
+    pl.fast = fast_shape(d);
+    if (pl.fast) {
+        fast_plan(a, pl);
+        return SSQ_OK;
+    }
     if (a.prefix_cap > 0) {
         // up to 64 query rows of a KV head take the matrix-core decode kernels (16 rows per pass over the
         // pages); any number the generic one (8 rows per pass)
@@ -212,7 +305,12 @@ extern "C" int ssq_decode_prefix(const ssq_prefix_args* a, void* workspace, size
     m.n1_last = pl.n1_last;
     m.own = reinterpret_cast<const float*>(reinterpret_cast<char*>(workspace) + pl.pre_bytes);
     m.n2 = pl.n2;
-    if (pl.n1) {
+    m.flat = pl.fast ? 1 : 0;
+    if (pl.fast) {
+        if (pl.n1 || pl.n2) rc = fast_launch(pl, workspace, st);
+        if (rc) return rc;
+    }
+    if (pl.n1 && !pl.fast) {
         char* at = reinterpret_cast<char*>(workspace);
         for (int qi = 0; qi < d.q_len; ++qi)
             for (int b0 = 0; b0 < d.batch; b0 += pl.chunk) {
@@ -225,7 +323,7 @@ extern "C" int ssq_decode_prefix(const ssq_prefix_args* a, void* workspace, size
                 at += bytes;
             }
     }
-    if (pl.n2) {
+    if (pl.n2 && !pl.fast) {
         ssq_decode_args own = d;
         own.num_splits = pl.n2;
         own.lse = nullptr;

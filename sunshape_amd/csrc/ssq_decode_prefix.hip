@@ -29,7 +29,11 @@ struct MergeParams {
     // n1 (the last chunk n1_last) splits x (num_q_heads * sequences) rows: o, then m, then l.
     // flat: one block of n1 splits x (batch * num_q_heads * q_len) rows instead, as the own tokens'.
     const float* pre;
+    // (of which those with tokens are read, as the kernel cut them)
     int chunk, n1, n1_last, flat;
+    const int32_t* plen;
+    int pcap;
+    const int* own_per;
     // the own tokens' partials, n2 splits x (batch * num_q_heads * q_len) rows (0: none)
     const float* own;
     int n2;
@@ -59,12 +63,24 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
         rows1 = (int64_t)a.num_q_heads * cn;
         row1 = (int64_t)h * cn + (b - c * p.chunk);
     }
+    const int n1_all = n1;
+    int n2 = p.n2;
+    if (p.flat) {
+        if (n1) {
+            const int len = max(0, min(p.plen[0], p.pcap)), per = ssq_prefix_slice(len, n1);
+            n1 = per ? (ssq_prefix_tiles(len) + per - 1) / per : 0;
+        }
+        if (n2) {
+            const int per = p.own_per[0];
+            n2 = (ssq_prefix_tiles(max(0, min(a.seq_lens[b], a.seq_len))) + per - 1) / per;
+        }
+    }
     const float* pre_o = p.pre + at0;
-    const float* pre_m = pre_o + rows1 * n1 * Dv;
-    const float* pre_l = pre_m + rows1 * n1;
+    const float* pre_m = pre_o + rows1 * n1_all * Dv;
+    const float* pre_l = pre_m + rows1 * n1_all;
     const float* own_m = p.own + n_rows * p.n2 * Dv;
     const float* own_l = own_m + n_rows * p.n2;
-    const int n = n1 + p.n2;
+    const int n = n1 + n2;
     float M = -INFINITY, L = 0.f;
     for (int d0 = 0; d0 < Dv; d0 += kMergeDims * SSQ_WAVE) {
         float Mr = -INFINITY, Lr = 0.f, o[kMergeDims];
@@ -160,9 +176,8 @@ void fast_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
     while ((16 << f.psh) < d.page_size) ++f.psh;
     const bool split = !(d.q_dtype == SSQ_BF16 && d.v_dtype == SSQ_BF16) && !(d.q_dtype == SSQ_F16 && d.v_dtype == SSQ_F16);
     f.pre_nr = split || f.rows <= 32 ? 1 : 2;
-    f.own_nr = split || per_b <= 32 ? 1 : 2;
     f.n_rg = (f.rows + 32 * f.pre_nr - 1) / (32 * f.pre_nr);
-    f.own_rg = (per_b + 32 * f.own_nr - 1) / (32 * f.own_nr);
+    f.own_rg = (per_b + 31) / 32;
     if (a.prefix_cap > 0) {
         // Slices of the prefix: the number that takes the fewest rounds of (4 + tiles of a wave) units: an item's
         // staging and join cost about as much as 4 tiles.
@@ -178,18 +193,26 @@ void fast_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
         }
     }
     if (d.seq_len > 0) {
-        // pieces of 16 tiles (512 tokens), down to 4 where there are fewer items than workgroups; at most 64
-        const int tiles = (d.seq_len + 31) / 32;
-        f.own_tiles = 16;
-        while (f.own_tiles > 4 && (int64_t)d.batch * f.own_rg * ((tiles + f.own_tiles - 1) / f.own_tiles) < 2 * f.n_wg) f.own_tiles /= 2;
-        while ((tiles + f.own_tiles - 1) / f.own_tiles > 64) f.own_tiles *= 2;
-        f.n2 = (tiles + f.own_tiles - 1) / f.own_tiles;
+        // The fewest tiles of a wave's piece: 2 (a piece's own cost is about 5), as many as keep the partials to
+        // 32 per row, and to 16 per wave where every sequence is as long as the tables.
+        const int64_t tiles = ssq_prefix_tiles(d.seq_len), waves = 4 * (int64_t)f.n_wg;
+        int64_t least = 2;
+        if ((tiles + 31) / 32 > least) least = (tiles + 31) / 32;
+        const int64_t all = d.batch * (int64_t)f.own_rg * tiles;
+        if ((all + 16 * waves - 1) / (16 * waves) > least) least = (all + 16 * waves - 1) / (16 * waves);
+        f.own_min = (int)(least < tiles ? least : tiles);
+        f.n2 = (int)((tiles + f.own_min - 1) / f.own_min);
     }
     const int64_t rows = (int64_t)d.batch * d.num_q_heads * d.q_len;
     pl.n1 = pl.n1_last = f.n1;
     pl.n2 = f.n2;
     pl.pre_bytes = ((size_t)(rows * f.n1 * (d.value_dim + 2) * 4) + 255) & ~(size_t)255;  // 16-byte stores in both parts
-    pl.own_bytes = (size_t)(rows * f.n2 * (d.value_dim + 2) * 4);
+    pl.own_bytes = f.n2 ? (size_t)(rows * f.n2 * (d.value_dim + 2) * 4) + 256 : 0;  // and the pieces' size
+}
+
+// where the kernel leaves the pieces' size for the merge: behind the own tokens' partials
+int* own_per_of(const PrefixPlan& pl, void* workspace) {
+    return reinterpret_cast<int*>(reinterpret_cast<char*>(workspace) + pl.pre_bytes + pl.own_bytes - 256);
 }
 
 int fast_launch(const PrefixPlan& pl, void* workspace, hipStream_t st) {
@@ -197,6 +220,7 @@ int fast_launch(const PrefixPlan& pl, void* workspace, hipStream_t st) {
     f.pre = reinterpret_cast<float*>(workspace);
     f.own = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + pl.pre_bytes);
     const ssq_decode_args& d = f.a;
+    if (f.n2) f.own_per = own_per_of(pl, workspace);
     if (d.q_dtype == SSQ_BF16 && d.v_dtype == SSQ_BF16) return ssq_prefix_bf16(f, st);
     if (d.q_dtype == SSQ_F16 && d.v_dtype == SSQ_F16) return ssq_prefix_f16(f, st);
     return d.v_dtype == SSQ_BF16 ? ssq_prefix_split_bf16(f, st) : ssq_prefix_split_f16(f, st);
@@ -307,6 +331,9 @@ extern "C" int ssq_decode_prefix(const ssq_prefix_args* a, void* workspace, size
     m.n2 = pl.n2;
     m.flat = pl.fast ? 1 : 0;
     if (pl.fast) {
+        m.plen = a->prefix_len;
+        m.pcap = a->prefix_cap;
+        if (pl.n2) m.own_per = own_per_of(pl, workspace);
         if (pl.n1 || pl.n2) rc = fast_launch(pl, workspace, st);
         if (rc) return rc;
     }

@@ -13,17 +13,17 @@
 //   which is the V^T operand, loaded straight into registers.
 // K^T's operand is gathered codeword by codeword from the codebook in LDS: no key tile is ever written.  A
 // codeword is stored as two 16-bit parts, c = hi + lo (the rounding of c, and of what that left: 2^-17 of c at most
-// is dropped, 2^-23 with f16 parts), side by side, and the K slots of one MFMA take hi and lo of the same dims
-// against the same query dims twice.  So one gather is one operand without a move, and the logits keep fp32's
-// quality at twice the matrix-core work of 16-bit keys (their third part of all the work).
+// is dropped, 2^-23 with f16 parts), and each 16 dims take one MFMA with the hi parts and one with the lo parts
+// against the same query operand: the logits keep fp32's quality for half as much matrix-core work again.
 // Queries of 16 bits enter exactly (QT bf16 / f16); fp32 ones (rotated codecs) in two bf16 parts.
 // Probabilities are rounded to the values' 16 bits for P.V, as in the other decode kernels; sums stay fp32.
 //
-// A wave holds 32 NR rows (NR 2: 64 rows per gathered operand, which the LDS needs to keep up) and takes every
-// fourth tile of its item's range; the four waves' (o, m, l) join in LDS.  A workgroup (one per CU: the codebook
-// fills the LDS, 128 KiB at head_dim 128) stages its KV head's codebook once and takes items in turn: a group
-// of rows over a slice of the prefix, or a sequence's own rows over a piece of its own tokens.  The work of a
-// tile's softmax (VALU) runs beside the next tile's scores (matrix cores).
+// A workgroup (one per CU: the codebook fills the LDS, 128 KiB at head_dim 128) stages its KV head's codebook once
+// and takes items in turn.  A prefix item is a group of 32 NR rows (NR 2: 64 rows per gathered operand, which the
+// LDS needs to keep up) over a slice of the prefix: each wave takes every fourth tile, and the four waves' (o, m, l)
+// join in LDS.  An own item is one sequence's rows over a piece of its own tokens, by one wave: no barriers, four
+// such latency chains side by side.  The work of a tile's softmax (VALU) runs beside the next tile's scores
+// (matrix cores).
 #pragma once
 
 #include "ssq_common.h"
@@ -36,12 +36,17 @@ struct SsqPrefixParams {
     int G, rows;       // query rows of a KV head: (b, qi, g), g fastest
     int n_wg;          // workgroups per KV head
     int pre_nr, n_rg, n1;    // prefix items: n_rg groups of 32 pre_nr rows x n1 slices (n1 0: none)
-    int own_nr, own_rg, n2;  // own items: sequences x own_rg groups of 32 own_nr rows x n2 pieces (n2 0: none)
-    int own_tiles;     // tiles of a piece
+    int own_rg, n2;    // own items: sequences x own_rg groups of 32 rows x at most n2 pieces (n2 0: none)
+    int own_min;       // the fewest tiles of a piece
     int psh;           // log2(page_size / 16)
     float* pre;        // o [n1][all rows][Dv], then m, l [n1][all rows]
     float* own;        // likewise for n2
+    int* own_per;      // tiles of a piece, chosen by the lengths (written for the merge)
 };
+
+// tiles of a prefix slice, and of a set of tokens
+__host__ __device__ inline int ssq_prefix_tiles(int len) { return (len + 31) / 32; }
+__host__ __device__ inline int ssq_prefix_slice(int len, int n1) { return (ssq_prefix_tiles(len) + n1 - 1) / n1; }
 
 // QT: how queries (and the codebook's parts) enter the matrix cores
 enum { kQtBf16 = 0, kQtF16 = 1, kQtSplit = 2 };
@@ -87,7 +92,8 @@ __device__ __forceinline__ pv16f pf_mfma(const uint4& a, const uint4& b, pv16f c
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pv8bf, a), __builtin_bit_cast(pv8bf, b), c, 0, 0, 0);
 }
 
-// LDS: codebook parts [nb][256][2 bd] | scratch: staged query rows, then the waves' join | m, l [4][64]
+// LDS: the codewords' hi parts [nb][256][bd], their lo parts | scratch: staged query rows, then the waves' join |
+// m, l [4][64] | rows' offsets [2][64] | permutation [D]
 template <int D>
 struct PfLds {
     static constexpr int kBook = D * 256 * 4;
@@ -96,7 +102,8 @@ struct PfLds {
     static constexpr int kQ = 64 * kQRow * 2;                      // 64 rows, or 32 rows in two parts
     static constexpr int kJoin = kPfWaves * 32 * kJoinRow * 4;
     static constexpr int kScratch = kQ > kJoin ? kQ : kJoin;
-    static constexpr int kTotal = kBook + kScratch + 2 * kPfWaves * 64 * 4;
+    static constexpr int kPerm = kBook + kScratch + 2 * kPfWaves * 64 * 4 + 2 * 64 * 8;
+    static constexpr int kTotal = kPerm + 2 * D;
 };
 
 template <int D, int BD, int QT, int VT, int NR>
@@ -115,33 +122,36 @@ struct PfRun {
 
     const SsqPrefixParams& p;
     const unsigned char* book;
-    int lane, half, kv;
+    int lane, half;
     uint4 q[QP][NR][NQ];
     // tokens
     const int32_t* table;
-    int len, last_chunk, tile0, n_tiles, wave;  // this wave's tiles: tile0 + wave + 4 i, i < n_tiles
-    int pg, pgn, batch;                         // table entries of 32 tiles, and of the 32 after them
+    int len, last_chunk, first, step, n_tiles;  // this wave's tiles: first + step i, i < n_tiles
+    // of 32 tiles and the 32 after them (lane: piece lane & 1 of tile lane / 2), element offsets of the pieces' codes
+    // and values
+    int64_t pc, pv, pcn, pvn;
+    int batch;
     const uint8_t* cbase;
     const uint16_t* vbase;
     uint32_t voff, vstep;                       // lane and 32-dim offsets in a page, elements
 
-    __device__ __forceinline__ int entries(int i0) const {  // lane: chunk (lane & 1) of tile i0 + lane / 2
-        const int chunk = min(2 * (tile0 + wave + kPfWaves * (i0 + (lane >> 1))) + (lane & 1), last_chunk);
-        return table[chunk >> p.psh];
+    __device__ __forceinline__ void entries(int i0, int64_t& oc, int64_t& ov) const {
+        const int chunk = min(2 * (first + step * (i0 + (lane >> 1))) + (lane & 1), last_chunk);
+        const int64_t page = table[chunk >> p.psh];
+        const int at = 16 * (chunk & ((1 << p.psh) - 1));
+        oc = page * p.a.c_sb + (int64_t)at * p.a.c_st;
+        ov = page * p.a.v_sb + at;
     }
-    __device__ __forceinline__ int page(int i, int c) const {  // uniform
-        return __builtin_amdgcn_readlane((i >> 5) == batch ? pg : pgn, 2 * (i & 31) + c);
-    }
-    __device__ __forceinline__ int chunk_of(int i, int c) const {
-        return min(2 * (tile0 + wave + kPfWaves * i) + c, last_chunk);
+    __device__ __forceinline__ static int64_t of_lane(int64_t v, int l) {  // uniform
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, l);
+        const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)v >> 32), l);
+        return (int64_t)(((uint64_t)hi << 32) | lo);
     }
     __device__ __forceinline__ void load_codes(int i, Codes& r) const {
-        const int msk = (1 << p.psh) - 1;
-        const int m = lane & 31, c = m >> 4;
-        const int tok = 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3);  // within its 16-token chunk
-        const int pgc = c ? page(i, 1) : page(i, 0);
-        const int at = (c ? (chunk_of(i, 1) & msk) : (chunk_of(i, 0) & msk)) * 16 + tok;
-        const uint8_t* row = cbase + (int64_t)pgc * p.a.c_sb + (int64_t)at * p.a.c_st;
+        const int64_t o = (i >> 5) == batch ? pc : pcn;
+        const int l = 2 * (i & 31);
+        const int64_t o0 = of_lane(o, l), o1 = of_lane(o, l + 1);
+        const uint8_t* row = cbase + (lane & 16 ? o1 : o0);  // cbase: this lane's token of a piece
         if constexpr (NW >= 4) {
 #pragma unroll
             for (int k = 0; k < NW / 4; ++k) {
@@ -153,14 +163,17 @@ struct PfRun {
             r.w[0] = x.x; r.w[1] = x.y;
         }
     }
+    __device__ __forceinline__ const uint16_t* val_row(int i, int c) const {
+        return vbase + of_lane((i >> 5) == batch ? pv : pvn, 2 * (i & 31) + c);
+    }
+    __device__ __forceinline__ uint4 load_val(const uint16_t* row, int dt) const {
+        return *reinterpret_cast<const uint4*>(row + voff + dt * vstep);
+    }
     __device__ __forceinline__ void load_vals(int i, Vals& r) const {
-        const int msk = (1 << p.psh) - 1;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const uint16_t* src = vbase + (int64_t)page(i, c) * p.a.v_sb + (chunk_of(i, c) & msk) * 16;
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) r.v[c][dt] = *reinterpret_cast<const uint4*>(src + voff + dt * vstep);
-        }
+            for (int dt = 0; dt < DT; ++dt) r.v[c][dt] = load_val(val_row(i, c), dt);
     }
     // the K^T operand of step st: dims 16 (st / 2) + 8 half .., the hi parts (st even) or the lo parts
     __device__ __forceinline__ uint4 operand(const Codes& c, int st) const {
@@ -183,22 +196,28 @@ struct PfRun {
             return make_uint4(x[0], x[1], x[2], x[3]);
         }
     }
-    __device__ __forceinline__ void scores(const Codes& c, pv16f (&s)[NR]) const {
-        constexpr int kAhead = 4;
-        uint4 k[kAhead];
+    // kAhead operands are gathered ahead of their MFMAs (the LDS answers random 8-byte reads in 200 cycles or more),
+    // across the end of a tile into the next one's codes
+    static constexpr int kAhead = NST < 8 ? NST : 8;
+    uint4 ring[kAhead];
+    __device__ __forceinline__ void prime(const Codes& c) {
 #pragma unroll
-        for (int st = 0; st < kAhead; ++st) k[st] = operand(c, st);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) s[r] = pv16f{};
+        for (int st = 0; st < kAhead; ++st) ring[st] = operand(c, st);
+    }
+    // beside(st): work for the vector units next to step st's MFMAs.  The barriers keep each step's gathers and
+    // vector work between its MFMAs and the next ones: left alone, the compiler puts one kind after the other.
+    template <class Beside>
+    __device__ __forceinline__ void scores(const Codes& c, const Codes& next, pv16f (&s)[NR], Beside beside) {
 #pragma unroll
         for (int st = 0; st < NST; ++st) {
-            const uint4 kk = k[st % kAhead];
-            if (st + kAhead < NST) k[st % kAhead] = operand(c, st + kAhead);
-            const int qi = st >> 1;
+            const uint4 kk = ring[st % kAhead];
 #pragma unroll
             for (int h = 0; h < QP; ++h)
 #pragma unroll
-                for (int r = 0; r < NR; ++r) s[r] = pf_mfma<kF16>(kk, q[h][r][qi], s[r]);
+                for (int r = 0; r < NR; ++r) s[r] = pf_mfma<kF16>(kk, q[h][r][st >> 1], st || h ? s[r] : pv16f{});
+            ring[st % kAhead] = st + kAhead < NST ? operand(c, st + kAhead) : operand(next, st + kAhead - NST);
+            beside(st);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -206,83 +225,254 @@ struct PfRun {
 // the lane 32 apart
 __device__ __forceinline__ float pf_other(float v) { return __shfl_xor(v, 32); }
 
-// One item: rows [R0, R0 + nr) of the KV head over tiles [t0, t1) of a sequence of `len` tokens; partials go to split
-// `split` of ws.  The whole workgroup calls it.
+// row R of a KV head's rows (b, qi, g): its sequence, query position and query head
+__device__ __forceinline__ void pf_row(const SsqPrefixParams& p, int kv, int R, int& b, int& qi, int& h) {
+    const int per_b = p.a.q_len * p.G;
+    b = R / per_b;
+    const int e = R - b * per_b;
+    qi = e / p.G;
+    h = kv * p.G + (e - qi * p.G);
+}
+__device__ __forceinline__ int64_t pf_rid(const SsqPrefixParams& p, int kv, int R) {
+    int b, qi, h;
+    pf_row(p, kv, R, b, qi, h);
+    return ((int64_t)b * p.a.num_q_heads + h) * p.a.q_len + qi;
+}
+__device__ __forceinline__ int64_t pf_qrow(const SsqPrefixParams& p, int kv, int R) {
+    int b, qi, h;
+    pf_row(p, kv, R, b, qi, h);
+    return (int64_t)b * p.a.q_sb + (int64_t)h * p.a.q_sh + (int64_t)qi * p.a.q_sl;
+}
+
+// element i of the queries, scaled in their dtype (the split form takes any)
+template <int QT>
+__device__ __forceinline__ float pf_query(const ssq_decode_args& a, int64_t i) {
+    if constexpr (QT == kQtSplit) {
+        const float x = ssq_load_elem(a.q, a.q_dtype, i);
+        return a.has_scale ? ssq_round_to(x * a.scale, a.q_dtype) : x;
+    } else {
+        const float x = pf_lo<QT == kQtF16>(reinterpret_cast<const uint16_t*>(a.q)[i]);
+        return a.has_scale ? pf_lo<QT == kQtF16>(pf_pack<QT == kQtF16>(x * a.scale, 0.f)) : x;
+    }
+}
+
+// a wave's tokens: tiles first + step i (i < n) of a sequence of len > 0 tokens
+template <class Run>
+__device__ __forceinline__ void pf_tokens(Run& u, int kv, const int32_t* table, int len, int first, int step, int n) {
+    const ssq_decode_args& a = u.p.a;
+    u.table = table; u.len = len; u.last_chunk = (len - 1) >> 4;
+    u.first = first; u.step = step; u.n_tiles = n;
+    const int m = u.lane & 15;
+    u.cbase = a.codes + (int64_t)kv * a.c_sh + (int64_t)(8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3)) * a.c_st;
+    u.vbase = reinterpret_cast<const uint16_t*>(a.v) + (int64_t)kv * a.v_sh;
+    u.voff = (uint32_t)(u.lane & 31) * (uint32_t)a.v_st + 8 * u.half;
+    u.vstep = 32 * (uint32_t)a.v_st;
+    u.batch = 0;
+    u.entries(0, u.pc, u.pv);
+    u.entries(32, u.pcn, u.pvn);
+}
+
+// Keeps a matrix-core operand in the accumulation registers, which the MFMAs read as well: the compiler otherwise
+// parks what does not fit the 256 others there and copies it back for every use.
+__device__ __forceinline__ void pf_pin(uint4& x) {
+    pv4u v = {x.x, x.y, x.z, x.w};
+    asm("" : "+a"(v));
+    x = make_uint4(v.x, v.y, v.z, v.w);
+}
+
+// max for numbers (an fmaxf would quieten its inputs first)
+__device__ __forceinline__ float pf_max(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+template <int NR>
+__device__ __forceinline__ void pf_top(const pv16f (&s)[NR], float (&top)[NR]) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        float t[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = pf_max(pf_max(s[r][4 * k], s[r][4 * k + 1]), pf_max(s[r][4 * k + 2], s[r][4 * k + 3]));
+        top[r] = pf_max(pf_max(t[0], t[1]), pf_max(t[2], t[3]));
+    }
+}
+
+// The wave's tiles.  mrow[r]: the additive mask's row of this lane's query row (MASK).
+template <bool MASK, int NR, class Run>
+__device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR], float (&m_run)[NR], float (&l_run)[NR],
+                                         pv16f (&o)[NR][Run::DT]) {
+    const int n = u.n_tiles, len = u.len;
+    if (n <= 0) return;  // wave-uniform
+    typename Run::Codes c1, c2, c3;
+    typename Run::Vals val;
+    pv16f s[NR];
+    float top[NR];
+    // tile i's mask, and its end where it holds the sequence's last token
+    auto fix = [&](int i) {
+        const int tile = u.first + u.step * i;
+        const int t_half = kPfTile * tile + 8 * u.half;  // register k: token t_half + 16 (k / 8) + k % 8
+        if constexpr (MASK) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int t = min(t_half + 16 * (k >> 3) + (k & 7), len - 1);
+                    s[r][k] += mrow[r][(int64_t)t * u.p.a.m_st];
+                }
+        }
+        const bool tail = kPfTile * (tile + 1) > len;  // uniform
+        if (tail) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (t_half + 16 * (k >> 3) + (k & 7) >= len) s[r][k] = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {  // values behind the last token are unwritten
+                const int keep = len - (t_half + 16 * c);
+#pragma unroll
+                for (int dt = 0; dt < Run::DT; ++dt) {
+                    uint32_t w[4] = {val.v[c][dt].x, val.v[c][dt].y, val.v[c][dt].z, val.v[c][dt].w};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k >= keep) w[k >> 1] &= (k & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+                    val.v[c][dt] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+        if (MASK || tail) pf_top<NR>(s, top);
+    };
+    u.load_codes(0, c1);
+    u.load_codes(min(1, n - 1), c2);
+    u.load_codes(min(2, n - 1), c3);
+    u.load_vals(0, val);
+    u.prime(c1);
+    u.scores(c1, c2, s, [](int) {});
+    pf_top<NR>(s, top);
+    fix(0);
+    for (int i = 0; i < n; ++i) {
+        // the running maximum moves only when a score passes it by kSoftmaxSlack
+        bool over = false;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) over |= top[r] > m_run[r] + kSoftmaxSlack;
+        if (__builtin_amdgcn_ballot_w64(over) != 0) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const float mn = fmaxf(m_run[r], fmaxf(top[r], pf_other(top[r])));
+                const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[r] - mn) * kLog2e);
+                m_run[r] = mn;
+                l_run[r] *= f;
+#pragma unroll
+                for (int dt = 0; dt < Run::DT; ++dt)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[r][dt][k] *= f;
+            }
+        }
+        // a masked score may be the type's lowest value, which times log2(e) is -inf: m is taken off first
+        if constexpr (MASK) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) s[r][k] -= m_run[r] == -INFINITY ? 0.f : m_run[r];
+        }
+        if ((i & 31) == 31) {  // the next tile starts the next 32 entries (tiles up to i + 3 are asked for)
+            u.batch = (i >> 5) + 1;
+            u.pc = u.pcn;
+            u.pv = u.pvn;
+            u.entries(32 * (u.batch + 1), u.pcn, u.pvn);
+        }
+        c1 = c2;
+        c2 = c3;
+        u.load_codes(min(i + 3, n - 1), c3);
+        // the next tile's scores beside this tile's probabilities
+        pv16f s2[NR];
+        uint32_t pw[NR][8];  // P^T operands
+        float mb[NR], e0[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) mb[r] = MASK || m_run[r] == -INFINITY ? 0.f : m_run[r] * kLog2e;  // -inf: so are its scores
+        __builtin_amdgcn_sched_barrier(0);
+        u.scores(c1, c2, s2, [&](int st) {
+            constexpr int kPer = 16 / Run::NST;
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int x = 0; x < kPer; ++x) {
+                    const int k = st * kPer + x;
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][k], kLog2e, -mb[r]));
+                    l_run[r] += e;
+                    if (k & 1) pw[r][k >> 1] = pf_pack<Run::kVF16>(e0[r], e);
+                    else e0[r] = e;
+                }
+        });
+        // P.V beside the next tile's maxima; a value operand's successor loads once it is used
+        const uint16_t* vsrc[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) vsrc[c] = u.val_row(min(i + 1, n - 1), c);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int dt = 0; dt < Run::DT; ++dt) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+                    o[r][dt] = pf_mfma<Run::kVF16>(val.v[c][dt], make_uint4(pw[r][4 * c], pw[r][4 * c + 1], pw[r][4 * c + 2], pw[r][4 * c + 3]), o[r][dt]);
+                val.v[c][dt] = u.load_val(vsrc[c], dt);
+                constexpr int kPer = 8 / Run::DT;  // score registers per step
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int x = 0; x < kPer; x += 2) {
+                        const int k = (c * Run::DT + dt) * kPer + x;
+                        const float t = pf_max(s2[r][k], s2[r][k + 1]);
+                        top[r] = k ? pf_max(top[r], t) : t;
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) s[r] = s2[r];
+        if (i + 1 < n) fix(i + 1);
+    }
+}
+
+// A prefix item: rows [R0, R0 + nr) of the KV head over tiles [t0, t1) of the prefix (len tokens); partials go to
+// slice `split`.  The whole workgroup calls it.  pj: the query dim of this thread (permuted dim tid % D).
 template <int D, int BD, int QT, int VT, int NR>
-__device__ __forceinline__ void pf_item(const SsqPrefixParams& p, unsigned char* lds, int kv, int R0, int nr,
-                                        const int32_t* table, int len, int t0, int t1, const float* mask, float* ws,
-                                        int n_split, int split) {
+__device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigned char* lds, int kv, int R0, int nr, int64_t pj,
+                                               int len, int t0, int t1, int split) {
     using Run = PfRun<D, BD, QT, VT, NR>;
     using L = PfLds<D>;
     const ssq_decode_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t n_rows = (int64_t)a.batch * a.num_q_heads * a.q_len;
-    float* ws_o = ws + (int64_t)split * n_rows * D;
-    float* ws_m = ws + (int64_t)n_split * n_rows * D + (int64_t)split * n_rows;
-    float* ws_l = ws_m + (int64_t)n_split * n_rows;
-    const int per_b = a.q_len * p.G;
-    auto row_of = [&](int R, int& b, int& qi, int& h) {
-        b = R / per_b;
-        const int e = R - b * per_b;
-        qi = e / p.G;
-        h = kv * p.G + (e - qi * p.G);
-    };
-    auto rid_of = [&](int R) {
-        int b, qi, h;
-        row_of(R, b, qi, h);
-        return ((int64_t)b * a.num_q_heads + h) * a.q_len + qi;
-    };
-    if (t0 >= t1) {  // nothing attended: the merge reads m alone
-        for (int r = tid; r < nr; r += kPfThreads) ws_m[rid_of(R0 + r)] = -INFINITY;
-        return;
-    }
+    float* ws_o = p.pre + (int64_t)split * n_rows * D;
+    float* ws_m = p.pre + (int64_t)p.n1 * n_rows * D + (int64_t)split * n_rows;
+    float* ws_l = ws_m + (int64_t)p.n1 * n_rows;
     unsigned char* scratch = lds + L::kBook;
     float* mL = reinterpret_cast<float*>(scratch + L::kScratch);  // [4][64]
     float* lL = mL + kPfWaves * 64;
-
+    int64_t* rowL = reinterpret_cast<int64_t*>(lL + kPfWaves * 64);  // query rows' offsets, partial rows
     Run u{p, lds};
-    u.lane = lane; u.half = half; u.kv = kv;
-    u.table = table; u.len = len; u.last_chunk = (len - 1) >> 4;
-    u.tile0 = t0; u.wave = wave;
-    u.n_tiles = (t1 - t0 - wave + kPfWaves - 1) / kPfWaves;
-    u.cbase = a.codes + (int64_t)kv * a.c_sh;
-    u.vbase = reinterpret_cast<const uint16_t*>(a.v) + (int64_t)kv * a.v_sh;
-    u.voff = (uint32_t)col * (uint32_t)a.v_st + 8 * half;
-    u.vstep = 32 * (uint32_t)a.v_st;
-    u.batch = 0;
-    u.pg = u.entries(0);
-    u.pgn = u.entries(32);
+    u.lane = lane; u.half = half;
+    pf_tokens(u, kv, p.ptab, len, t0 + wave, kPfWaves, (t1 - t0 - wave + kPfWaves - 1) / kPfWaves);
 
     // ---- query rows: scaled in their dtype, permuted, as 16-bit parts [part][row][D] in LDS
     uint16_t* qL = reinterpret_cast<uint16_t*>(scratch);
-    const int64_t* perm = a.perm + (int64_t)kv * a.perm_sh;
     constexpr int kRows = 32 * NR, kPer = kRows * D / kPfThreads, kBatch = kPer < 16 ? kPer : 16;
-    const int j = tid % D;  // a thread's dim is the same for all its elements
-    const int64_t pj = (int64_t)min((uint64_t)perm[j], (uint64_t)(D - 1));
-#pragma unroll
+    const int j = tid % D;
+    if (tid < kRows) {
+        const int R = R0 + min(tid, nr - 1);
+        rowL[tid] = pf_qrow(p, kv, R);
+        rowL[64 + tid] = pf_rid(p, kv, R);
+    }
+    __syncthreads();
+#pragma unroll 1
     for (int e0 = 0; e0 < kPer; e0 += kBatch) {
-        int64_t at[kBatch];
         float v[kBatch];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int r = (e0 + k) * (kPfThreads / D) + tid / D;
-            int b, qi, h;
-            row_of(R0 + min(r, nr - 1), b, qi, h);
-            at[k] = (int64_t)b * a.q_sb + (int64_t)h * a.q_sh + (int64_t)qi * a.q_sl + pj;
-        }
-        ssq_load_elems<kBatch>(a.q, a.q_dtype, at, v);
+        for (int k = 0; k < kBatch; ++k) v[k] = pf_query<QT>(a, rowL[(e0 + k) * (kPfThreads / D) + tid / D] + pj);
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
             const int r = (e0 + k) * (kPfThreads / D) + tid / D;
-            float x = r < nr ? v[k] : 0.f;
-            if (a.has_scale) x = ssq_round_to(x * a.scale, a.q_dtype);
+            const float x = r < nr ? v[k] : 0.f;
             const uint32_t w = pf_pack<Run::kF16>(x, 0.f);
             qL[r * L::kQRow + j] = (uint16_t)w;
-            if constexpr (Run::QP == 2) {
-                const uint32_t w2 = pf_pack<false>(x - pf_lo<false>(w), 0.f);
-                qL[(kRows + r) * L::kQRow + j] = (uint16_t)w2;
-            }
+            if constexpr (Run::QP == 2) qL[(kRows + r) * L::kQRow + j] = (uint16_t)pf_pack<false>(x - pf_lo<false>(w), 0.f);
         }
     }
     __syncthreads();
@@ -291,23 +481,13 @@ __device__ __forceinline__ void pf_item(const SsqPrefixParams& p, unsigned char*
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-            for (int st = 0; st < Run::NQ; ++st) {
-                const uint16_t* row = qL + (h * kRows + 32 * r + col) * L::kQRow;
-                u.q[h][r][st] = *reinterpret_cast<const uint4*>(row + 16 * st + 8 * half);
+            for (int st = 0; st < Run::NQ; ++st)
+            {
+                u.q[h][r][st] = *reinterpret_cast<const uint4*>(qL + (h * kRows + 32 * r + col) * L::kQRow + 16 * st + 8 * half);
+                if constexpr (NR == 2) pf_pin(u.q[h][r][st]);
             }
 
-    // this lane's mask rows
-    const float* mrow[NR];
-    if (mask) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            int b, qi, h;
-            row_of(R0 + min(32 * r + col, nr - 1), b, qi, h);
-            mrow[r] = mask + (int64_t)b * a.m_sb + (int64_t)h * a.m_sh + (int64_t)qi * a.m_sl;
-        }
-    }
-
-    // ---- tiles
+    const float* mrow[NR] = {};
     float m_run[NR], l_run[NR];
     pv16f o[NR][Run::DT];
 #pragma unroll
@@ -315,116 +495,13 @@ __device__ __forceinline__ void pf_item(const SsqPrefixParams& p, unsigned char*
         m_run[r] = -INFINITY;
         l_run[r] = 0.f;
 #pragma unroll
-        for (int dt = 0; dt < Run::DT; ++dt) o[r][dt] = pv16f{};
-    }
-    const int n = u.n_tiles;
-    if (n > 0) {  // wave-uniform
-        typename Run::Codes c0, c1;
-        typename Run::Vals val;
-        pv16f s[NR], s2[NR];
-        u.load_codes(0, c0);
-        u.load_vals(0, val);
-        u.load_codes(min(1, n - 1), c1);
-        u.scores(c0, s);
-        for (int i = 0; i < n; ++i) {
-            if ((i & 31) == 31) {  // the next tile starts the next 32 entries
-                u.batch = (i >> 5) + 1;
-                u.pg = u.pgn;
-                u.pgn = u.entries(32 * (u.batch + 1));
-            }
-            u.load_codes(min(i + 2, n - 1), c0);
-            const int tile = t0 + wave + kPfWaves * i;
-            const int t_half = kPfTile * tile + 8 * half;  // register k: token t_half + 16 (k / 8) + k % 8
-            const bool tail = kPfTile * (tile + 1) > len;  // uniform
-            if (mask) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const int t = min(t_half + 16 * (k >> 3) + (k & 7), len - 1);
-                        s[r][k] += mrow[r][(int64_t)t * a.m_st];
-                    }
-            }
-            if (tail) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        if (t_half + 16 * (k >> 3) + (k & 7) >= len) s[r][k] = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {  // values behind the last token are unwritten
-                    const int keep = len - (t_half + 16 * c);
-#pragma unroll
-                    for (int dt = 0; dt < Run::DT; ++dt) {
-                        uint32_t w[4] = {val.v[c][dt].x, val.v[c][dt].y, val.v[c][dt].z, val.v[c][dt].w};
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            if (k >= keep) w[k >> 1] &= (k & 1) ? 0x0000FFFFu : 0xFFFF0000u;
-                        val.v[c][dt] = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
-            }
-            // the running maximum moves only when a score passes it by kSoftmaxSlack
-            float top[NR];
-            bool over = false;
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                top[r] = s[r][0];
-#pragma unroll
-                for (int k = 1; k < 16; ++k) top[r] = fmaxf(top[r], s[r][k]);
-                over |= top[r] > m_run[r] + kSoftmaxSlack;
-            }
-            if (__builtin_amdgcn_ballot_w64(over) != 0) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    const float mn = fmaxf(m_run[r], fmaxf(top[r], pf_other(top[r])));
-                    const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[r] - mn) * kLog2e);
-                    m_run[r] = mn;
-                    l_run[r] *= f;
-#pragma unroll
-                    for (int dt = 0; dt < Run::DT; ++dt)
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) o[r][dt][k] *= f;
-                }
-            }
-            // a masked score may be the type's lowest value, which times log2(e) is -inf: m is taken off first
-            if (mask) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) s[r][k] -= m_run[r] == -INFINITY ? 0.f : m_run[r];
-            }
-            // the next tile's scores beside this tile's probabilities
-            u.scores(c1, s2);
-            uint4 pr[NR][2];
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                // -inf while every score seen is (then the probabilities are exp(-inf) = 0)
-                const float mb = mask || m_run[r] == -INFINITY ? 0.f : m_run[r] * kLog2e;
-                float e[16];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][k], kLog2e, -mb));
-                    l_run[r] += e[k];
-                }
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    pr[r][c] = make_uint4(pf_pack<Run::kVF16>(e[8 * c], e[8 * c + 1]), pf_pack<Run::kVF16>(e[8 * c + 2], e[8 * c + 3]),
-                                          pf_pack<Run::kVF16>(e[8 * c + 4], e[8 * c + 5]), pf_pack<Run::kVF16>(e[8 * c + 6], e[8 * c + 7]));
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int dt = 0; dt < Run::DT; ++dt)
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) o[r][dt] = pf_mfma<Run::kVF16>(val.v[c][dt], pr[r][c], o[r][dt]);
-            u.load_vals(min(i + 1, n - 1), val);
-#pragma unroll
-            for (int r = 0; r < NR; ++r) s[r] = s2[r];
-            const typename Run::Codes ct = c0;
-            c1 = ct;
+        for (int dt = 0; dt < Run::DT; ++dt) {
+            o[r][dt] = pv16f{};
+            if constexpr (NR == 2) asm("" : "+a"(o[r][dt]));
         }
     }
+    pf_tiles<false, NR>(u, mrow, m_run, l_run, o);
+
     // ---- the four waves' (m, l), then o, 32 rows x 32 dims at a time
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
@@ -453,7 +530,7 @@ __device__ __forceinline__ void pf_item(const SsqPrefixParams& p, unsigned char*
             const float m = mL[w * 64 + r];
             if (m != -INFINITY) l += lL[w * 64 + r] * __builtin_amdgcn_exp2f((m - M) * kLog2e);
         }
-        const int64_t rid = rid_of(R0 + r);
+        const int64_t rid = rowL[64 + r];
         ws_m[rid] = M;
         ws_l[rid] = l;
     }
@@ -462,7 +539,7 @@ __device__ __forceinline__ void pf_item(const SsqPrefixParams& p, unsigned char*
     for (int r = 0; r < NR; ++r) {
         if (32 * r >= nr) break;  // uniform
         const bool in = 32 * r + jr < nr;
-        const int64_t rid = rid_of(R0 + min(32 * r + jr, nr - 1));
+        float* dst = ws_o + rowL[64 + 32 * r + jr] * D + jd;  // rows past nr repeat the last
 #pragma unroll
         for (int dt = 0; dt < Run::DT; ++dt) {
 #pragma unroll
@@ -478,89 +555,203 @@ __device__ __forceinline__ void pf_item(const SsqPrefixParams& p, unsigned char*
                 const float4 x = *reinterpret_cast<const float4*>(jL + (w * 32 + jr) * L::kJoinRow + jd);
                 t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
             }
-            if (in) *reinterpret_cast<float4*>(ws_o + rid * D + 32 * dt + jd) = t;
+            if (in) *reinterpret_cast<float4*>(dst + 32 * dt) = t;
             __syncthreads();
         }
+    }
+}
+
+// An own item: rows [R0, R0 + nr) (nr <= 32) of one sequence over tiles [t0, t1) of its own tokens, by one wave.
+template <int D, int BD, int QT, int VT, bool MASK>
+__device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsigned char* book, const uint16_t* permL, int kv,
+                                            int R0, int nr, const int32_t* table, int len, int t0, int t1, int split) {
+    using Run = PfRun<D, BD, QT, VT, 1>;
+    const ssq_decode_args& a = p.a;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    Run u{p, book};
+    u.lane = lane; u.half = half;
+    pf_tokens(u, kv, table, len, t0, 1, t1 - t0);
+    // query operands straight from memory: a lane's row, its half of every 16 permuted dims
+    const int R = R0 + min(col, nr - 1);
+    const int64_t qrow = pf_qrow(p, kv, R);
+#pragma unroll
+    for (int st = 0; st < Run::NQ; ++st) {
+        const uint4 pw = *reinterpret_cast<const uint4*>(permL + 16 * st + 8 * half);
+        const uint32_t w[4] = {pw.x, pw.y, pw.z, pw.w};
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = pf_query<QT>(a, qrow + ((w[k >> 1] >> (16 * (k & 1))) & 0xFFFFu));
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float x = col < nr ? v[2 * k] : 0.f, y = col < nr ? v[2 * k + 1] : 0.f;
+            hi[k] = pf_pack<Run::kF16>(x, y);
+            lo[k] = pf_pack<false>(x - pf_lo<false>(hi[k]), y - pf_hi<false>(hi[k]));
+        }
+        u.q[0][0][st] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (Run::QP == 2) u.q[1][0][st] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    const float* mrow[1] = {nullptr};
+    if constexpr (MASK) {
+        int b, qi, h;
+        pf_row(p, kv, R, b, qi, h);
+        mrow[0] = a.mask + (int64_t)b * a.m_sb + (int64_t)h * a.m_sh + (int64_t)qi * a.m_sl;
+    }
+    float m_run[1] = {-INFINITY}, l_run[1] = {0.f};
+    pv16f o[1][Run::DT];
+#pragma unroll
+    for (int dt = 0; dt < Run::DT; ++dt) o[0][dt] = pv16f{};
+    pf_tiles<MASK, 1>(u, mrow, m_run, l_run, o);
+    const float l = l_run[0] + pf_other(l_run[0]);
+    if (col < nr) {
+        const int64_t n_rows = (int64_t)a.batch * a.num_q_heads * a.q_len, rid = pf_rid(p, kv, R);
+        float* ws_m = p.own + (int64_t)p.n2 * n_rows * D + (int64_t)split * n_rows;
+        float* dst = p.own + ((int64_t)split * n_rows + rid) * D + 4 * half;
+#pragma unroll
+        for (int dt = 0; dt < Run::DT; ++dt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<float4*>(dst + 32 * dt + 8 * k) =
+                    make_float4(o[0][dt][4 * k], o[0][dt][4 * k + 1], o[0][dt][4 * k + 2], o[0][dt][4 * k + 3]);
+        if (half == 0) {
+            ws_m[rid] = m_run[0];
+            ws_m[(int64_t)p.n2 * n_rows + rid] = l;
+        }
+    }
+}
+
+// inclusive wave sum: row shifts by 1, 2, 4 and 8, then lane 15 and lane 31 of the rows below
+__device__ __forceinline__ int pf_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
+// The sequences' own tokens, cut by their lengths (which only the device knows): pieces of `per` tiles, the size that
+// gives every wave of the KV head about one, numbered sequence by sequence; wave v takes pieces v, v + n_waves, ...
+// Every number follows from seq_lens, so all waves agree and a call repeats itself bit for bit.
+template <int D, int BD, int QT, int VT>
+__device__ __forceinline__ void pf_own(const SsqPrefixParams& p, const unsigned char* book, const uint16_t* permL, int kv, int v) {
+    const ssq_decode_args& a = p.a;
+    const int lane = threadIdx.x & 63;
+    const int n_waves = p.n_wg * kPfWaves, ns = a.batch * p.own_rg, per_b = a.q_len * p.G;
+    auto tiles_of = [&](int s) {  // of sequence and row group s
+        return s < ns ? ssq_prefix_tiles(max(0, min(a.seq_lens[s / p.own_rg], a.seq_len))) : 0;
+    };
+    const int t_first = tiles_of(lane);
+    auto count = [&](int per) {  // pieces of all sequences
+        int c = __builtin_amdgcn_readlane(pf_scan((t_first + per - 1) / per), 63);
+        for (int s0 = 64; s0 < ns; s0 += 64) c += __builtin_amdgcn_readlane(pf_scan((tiles_of(s0 + lane) + per - 1) / per), 63);
+        return c;
+    };
+    // pieces of the fewest tiles, or larger ones where that is more than a piece a wave
+    int per = p.own_min, n = count(per);
+    if (n > n_waves) {
+        const int total = count(1);
+        per = max(per, (total + n_waves - 1) / n_waves);
+        n = count(per);
+        for (int k = 0; k < 6 && n > n_waves && ns <= n_waves; ++k) {
+            per += (per + 3) / 4;
+            n = count(per);
+        }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.own_per[0] = per;
+    int s0 = 0, base = 0, t = t_first, c = (t_first + per - 1) / per, inc = pf_scan(c);
+    for (int it = v; it < n; it += n_waves) {
+        while (it >= base + __builtin_amdgcn_readlane(inc, 63)) {  // it < n: ends before s0 passes ns
+            base += __builtin_amdgcn_readlane(inc, 63);
+            s0 += 64;
+            t = tiles_of(s0 + lane);
+            c = (t + per - 1) / per;
+            inc = pf_scan(c);
+        }
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + inc > it));
+        const int split = it - base - __builtin_amdgcn_readlane(inc - c, l);
+        const int s = s0 + l, b = s / p.own_rg, r0 = (s - b * p.own_rg) * 32;
+        const int t0 = split * per, t1 = min(t0 + per, __builtin_amdgcn_readlane(t, l));
+        const int len = max(0, min(a.seq_lens[b], a.seq_len));
+        const int32_t* table = a.block_table + (int64_t)b * a.bt_sb;
+        if (a.mask) pf_own_item<D, BD, QT, VT, true>(p, book, permL, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
+        else pf_own_item<D, BD, QT, VT, false>(p, book, permL, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
     }
 }
 
 template <int D, int BD, int QT, int VT>
 __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams p) {
     extern __shared__ __align__(16) unsigned char pf_lds[];
+    using L = PfLds<D>;
     const ssq_decode_args& a = p.a;
     const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kv = blockIdx.x % a.num_kv_heads, w = blockIdx.x / a.num_kv_heads;
-    // ---- the KV head's codebook as 16-bit parts
+    uint16_t* permL = reinterpret_cast<uint16_t*>(pf_lds + L::kPerm);
+    // a permuted dim's source, for this thread's staging and for the waves' own rows
+    const int64_t pj = (int64_t)min((uint64_t)a.perm[(int64_t)kv * a.perm_sh + tid % D], (uint64_t)(D - 1));
+    const int plen = p.n1 ? max(0, min(p.plen[0], p.pcap)) : 0;
+    // ---- the KV head's codebook as 16-bit parts, kIn pieces in flight per thread
     {
         constexpr bool F16 = QT == kQtF16;
+        constexpr int kV = BD < 4 ? BD : 4, kIn = 16;  // floats per piece
         const float* cent = a.cent + (int64_t)kv * a.cent_sh;
-        const int nc = a.n_centroids, total = (D / BD) * nc;
-        constexpr int kV = BD < 4 ? BD : 4;  // floats per load
-        for (int e = tid; e < total * (BD / kV); e += kPfThreads) {
-            const int cw = e / (BD / kV), part = e - cw * (BD / kV);
-            const int blk = cw / nc, c = cw - blk * nc;
-            float x[kV];
-            const float* src = cent + (int64_t)cw * BD + part * kV;
-            if constexpr (kV == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(src);
-                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-            } else {
-                const float2 v = *reinterpret_cast<const float2*>(src);
-                x[0] = v.x; x[1] = v.y;
-            }
-            uint32_t hi[kV / 2], lo[kV / 2];
+        const int nc = a.n_centroids, per = nc * (BD / kV), total = (D / BD) * per;
+        for (int e0 = tid; e0 < total; e0 += kIn * kPfThreads) {
+            float x[kIn][kV];
 #pragma unroll
-            for (int k = 0; k < kV / 2; ++k) {
-                hi[k] = pf_pack<F16>(x[2 * k], x[2 * k + 1]);
-                lo[k] = pf_pack<F16>(x[2 * k] - pf_lo<F16>(hi[k]), x[2 * k + 1] - pf_hi<F16>(hi[k]));
+            for (int i = 0; i < kIn; ++i) {
+                const float* src = cent + (int64_t)min(e0 + i * kPfThreads, total - 1) * kV;
+                if constexpr (kV == 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(src);
+                    x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+                } else {
+                    const float2 v = *reinterpret_cast<const float2*>(src);
+                    x[i][0] = v.x; x[i][1] = v.y;
+                }
             }
-            unsigned char* dst = pf_lds + (blk * 256 + c) * 2 * BD + part * 2 * kV;
-            unsigned char* dlo = dst + PfLds<D>::kBook / 2;
-            if constexpr (BD == 2) {
-                *reinterpret_cast<uint32_t*>(dst) = hi[0];
-                *reinterpret_cast<uint32_t*>(dlo) = lo[0];
-            } else {
-                *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-                *reinterpret_cast<uint2*>(dlo) = make_uint2(lo[0], lo[1]);
+#pragma unroll
+            for (int i = 0; i < kIn; ++i) {
+                const int e = e0 + i * kPfThreads;
+                if (e >= total) break;
+                uint32_t hi[kV / 2], lo[kV / 2];
+#pragma unroll
+                for (int k = 0; k < kV / 2; ++k) {
+                    hi[k] = pf_pack<F16>(x[i][2 * k], x[i][2 * k + 1]);
+                    lo[k] = pf_pack<F16>(x[i][2 * k] - pf_lo<F16>(hi[k]), x[i][2 * k + 1] - pf_hi<F16>(hi[k]));
+                }
+                const int blk = nc == 256 ? e / (256 * (BD / kV)) : e / per;  // a shift where it counts
+                unsigned char* dst = pf_lds + blk * 512 * BD + (e - blk * per) * 2 * kV;
+                unsigned char* dlo = dst + L::kBook / 2;
+                if constexpr (BD == 2) {
+                    *reinterpret_cast<uint32_t*>(dst) = hi[0];
+                    *reinterpret_cast<uint32_t*>(dlo) = lo[0];
+                } else {
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(dlo) = make_uint2(lo[0], lo[1]);
+                }
             }
         }
+        if (tid < D) permL[tid] = (uint16_t)pj;
     }
     __syncthreads();
-    const int n_pre = p.n_rg * p.n1;
-    const int n_items = n_pre + a.batch * p.own_rg * p.n2;
-    for (int it = w; it < n_items; it += p.n_wg) {
-        if (it < n_pre) {
-            const int split = it / p.n_rg, rg = it - split * p.n_rg;  // the groups of one slice side by side
-            const int len = max(0, min(p.plen[0], p.pcap));
-            const int tiles = (len + kPfTile - 1) / kPfTile, per = (tiles + p.n1 - 1) / p.n1;
-            const int R0 = rg * 32 * p.pre_nr, nr = min(32 * p.pre_nr, p.rows - R0);
-            const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
-            if constexpr (QT != kQtSplit) {
-                if (p.pre_nr == 2) {
-                    pf_item<D, BD, QT, VT, 2>(p, pf_lds, kv, R0, nr, p.ptab, len, t0, t1, nullptr, p.pre, p.n1, split);
-                    continue;
-                }
+    // ---- the prefix: slices past its length are not read by the merge either
+    const int tiles = ssq_prefix_tiles(plen), per = p.n1 ? ssq_prefix_slice(plen, p.n1) : 0;
+    const int n_pre = per ? p.n_rg * ((tiles + per - 1) / per) : 0;
+    for (int it = w; it < n_pre; it += p.n_wg) {
+        const int split = it / p.n_rg, rg = it - split * p.n_rg;  // the groups of one slice side by side
+        const int R0 = rg * 32 * p.pre_nr, nr = min(32 * p.pre_nr, p.rows - R0);
+        const int t0 = split * per, t1 = min(t0 + per, tiles);
+        if constexpr (QT != kQtSplit) {
+            if (p.pre_nr == 2) {
+                pf_prefix_item<D, BD, QT, VT, 2>(p, pf_lds, kv, R0, nr, pj, plen, t0, t1, split);
+                continue;
             }
-            pf_item<D, BD, QT, VT, 1>(p, pf_lds, kv, R0, nr, p.ptab, len, t0, t1, nullptr, p.pre, p.n1, split);
-        } else {
-            const int e = it - n_pre;
-            const int split = e % p.n2, br = e / p.n2;
-            const int b = br / p.own_rg, rg = br - b * p.own_rg;
-            const int len = max(0, min(a.seq_lens[b], a.seq_len));
-            const int tiles = (len + kPfTile - 1) / kPfTile;
-            const int per_b = a.q_len * p.G;
-            const int r0 = rg * 32 * p.own_nr, nr = min(32 * p.own_nr, per_b - r0);
-            const int t0 = min(split * p.own_tiles, tiles), t1 = min(t0 + p.own_tiles, tiles);
-            const int32_t* table = a.block_table + (int64_t)b * a.bt_sb;
-            if constexpr (QT != kQtSplit) {
-                if (p.own_nr == 2) {
-                    pf_item<D, BD, QT, VT, 2>(p, pf_lds, kv, b * per_b + r0, nr, table, len, t0, t1, a.mask, p.own, p.n2, split);
-                    continue;
-                }
-            }
-            pf_item<D, BD, QT, VT, 1>(p, pf_lds, kv, b * per_b + r0, nr, table, len, t0, t1, a.mask, p.own, p.n2, split);
         }
+        pf_prefix_item<D, BD, QT, VT, 1>(p, pf_lds, kv, R0, nr, pj, plen, t0, t1, split);
     }
+    if (p.n2) pf_own<D, BD, QT, VT>(p, pf_lds, permL, kv, w * kPfWaves + wave);
 }
 
 template <int D, int BD, int QT, int VT>

@@ -174,6 +174,7 @@ void fast_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
     const int cus = ssq_device_cus();
     f.n_wg = cus / d.num_kv_heads > 0 ? cus / d.num_kv_heads : 1;
     while ((16 << f.psh) < d.page_size) ++f.psh;
+    f.q_vec = d.q_dtype != SSQ_F32 && (uintptr_t)d.q % 16 == 0 && d.q_sb % 8 == 0 && d.q_sh % 8 == 0 && d.q_sl % 8 == 0;
     const bool split = !(d.q_dtype == SSQ_BF16 && d.v_dtype == SSQ_BF16) && !(d.q_dtype == SSQ_F16 && d.v_dtype == SSQ_F16);
     f.pre_nr = split || f.rows <= 32 ? 1 : 2;
     f.n_rg = (f.rows + 32 * f.pre_nr - 1) / (32 * f.pre_nr);

@@ -39,6 +39,7 @@ struct SsqPrefixParams {
     int own_rg, n2;    // own items: sequences x own_rg groups of 32 rows x at most n2 pieces (n2 0: none)
     int own_min;       // the fewest tiles of a piece
     int psh;           // log2(page_size / 16)
+    int q_vec;         // 16-bit query rows load in 16-byte pieces
     float* pre;        // o [n1][all rows][Dv], then m, l [n1][all rows]
     float* own;        // likewise for n2
     int* own_per;      // tiles of a piece, chosen by the lengths (written for the merge)
@@ -70,7 +71,7 @@ typedef unsigned int pv4u __attribute__((ext_vector_type(4)));
 constexpr int kPfThreads = 256;
 constexpr int kPfWaves = 4;
 constexpr int kPfTile = 32;  // tokens
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // two fp32 to 16 bits (RNE), packed
 template <bool F16>
@@ -92,14 +93,14 @@ __device__ __forceinline__ pv16f pf_mfma(const uint4& a, const uint4& b, pv16f c
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pv8bf, a), __builtin_bit_cast(pv8bf, b), c, 0, 0, 0);
 }
 
-// LDS: the codewords' hi parts [nb][256][bd], their lo parts | scratch: staged query rows, then the waves' join |
+// LDS: codebook [nb]: the codewords' hi parts [256][bd], their lo parts | scratch: staged query rows, then the waves' join |
 // m, l [4][64] | rows' offsets [2][64] | permutation [D]
 template <int D>
 struct PfLds {
     static constexpr int kBook = D * 256 * 4;
     static constexpr int kQRow = D + 8;                            // staged query row, 16-bit elements
     static constexpr int kJoinRow = 36;                            // floats: 32 dims, padded
-    static constexpr int kQ = 64 * kQRow * 2;                      // 64 rows, or 32 rows in two parts
+    static constexpr int kQ = 32 * (D + kQRow) * 2;                // 32 rows as they are, and permuted
     static constexpr int kJoin = kPfWaves * 32 * kJoinRow * 4;
     static constexpr int kScratch = kQ > kJoin ? kQ : kJoin;
     static constexpr int kPerm = kBook + kScratch + 2 * kPfWaves * 64 * 4 + 2 * 64 * 8;
@@ -175,30 +176,31 @@ struct PfRun {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) r.v[c][dt] = load_val(val_row(i, c), dt);
     }
-    // the K^T operand of step st: dims 16 (st / 2) + 8 half .., the hi parts (st even) or the lo parts
+    // the K^T operand of step st: dims 16 (st / 2) + 8 half .., the hi parts (st even) or the lo parts.  A gather's
+    // address is code * 2 BD + half's offset, and the step's (a constant, past 64 KiB from a second base).
     __device__ __forceinline__ uint4 operand(const Codes& c, int st) const {
         const int s2 = st >> 1;
-        const unsigned char* part = book + (st & 1) * (L::kBook / 2);
-        if constexpr (BD == 8) {  // block 2 s2 + half
-            const uint32_t code = (c.w[s2 >> 1] >> (16 * (s2 & 1) + 8 * half)) & 0xFFu;
-            return *reinterpret_cast<const uint4*>(part + (2 * s2 + half) * 4096 + code * 16);
-        } else if constexpr (BD == 4) {  // blocks 4 s2 + 2 half, + 1
-            const uint32_t w = c.w[s2] >> (16 * half);
-            const uint2 a = *reinterpret_cast<const uint2*>(part + (4 * s2 + 2 * half) * 2048 + (w & 0xFFu) * 8);
-            const uint2 b = *reinterpret_cast<const uint2*>(part + (4 * s2 + 2 * half + 1) * 2048 + ((w >> 8) & 0xFFu) * 8);
-            return make_uint4(a.x, a.y, b.x, b.y);
-        } else {  // blocks 8 s2 + 4 half ..
+        constexpr int kPerHalf = 8 / BD, kBlk = 1024 * BD;  // blocks of a half's 8 dims; bytes of a block's tables
+        const unsigned char* at0 = book + s2 * 2 * kPerHalf * kBlk + (st & 1) * (kBlk / 2);
+        const uint32_t hb = (uint32_t)half * (kPerHalf * kBlk);
+        if constexpr (BD == 8) {
+            const uint32_t code = __builtin_amdgcn_ubfe(c.w[s2 >> 1], 16 * (s2 & 1) + 8 * half, 8);
+            return *reinterpret_cast<const uint4*>(at0 + (code * 16 + hb));
+        } else if constexpr (BD == 4) {
+            const uint32_t x = __builtin_amdgcn_ubfe(c.w[s2], 16 * half, 8), y = __builtin_amdgcn_ubfe(c.w[s2], 16 * half + 8, 8);
+            const uint2 u = *reinterpret_cast<const uint2*>(at0 + (x * 8 + hb)), v = *reinterpret_cast<const uint2*>(at0 + kBlk + (y * 8 + hb));
+            return make_uint4(u.x, u.y, v.x, v.y);
+        } else {
             const uint32_t w = half ? c.w[2 * s2 + 1] : c.w[2 * s2];
             uint32_t x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                x[k] = *reinterpret_cast<const uint32_t*>(part + (8 * s2 + 4 * half + k) * 1024 + ((w >> (8 * k)) & 0xFFu) * 4);
+            for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint32_t*>(at0 + k * kBlk + (((w >> (8 * k)) & 0xFFu) * 4 + hb));
             return make_uint4(x[0], x[1], x[2], x[3]);
         }
     }
-    // kAhead operands are gathered ahead of their MFMAs (the LDS answers random 8-byte reads in 200 cycles or more),
+    // kAhead operands are gathered ahead of their MFMAs (more would not fit the registers beside 64 rows),
     // across the end of a tile into the next one's codes
-    static constexpr int kAhead = NST < 8 ? NST : 8;
+    static constexpr int kAhead = 4;
     uint4 ring[kAhead];
     __device__ __forceinline__ void prime(const Codes& c) {
 #pragma unroll
@@ -256,6 +258,30 @@ __device__ __forceinline__ float pf_query(const ssq_decode_args& a, int64_t i) {
     }
 }
 
+// eight consecutive dims
+template <int QT>
+__device__ __forceinline__ void pf_query8(const SsqPrefixParams& p, int64_t i, float (&x)[8]) {
+    const ssq_decode_args& a = p.a;
+    constexpr bool F16 = QT == kQtF16;
+    if (QT != kQtSplit && p.q_vec) {  // uniform: rows of 16-byte pieces
+        const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x[2 * k] = pf_lo<F16>(w[k]);
+            x[2 * k + 1] = pf_hi<F16>(w[k]);
+            if (a.has_scale) {
+                const uint32_t y = pf_pack<F16>(x[2 * k] * a.scale, x[2 * k + 1] * a.scale);
+                x[2 * k] = pf_lo<F16>(y);
+                x[2 * k + 1] = pf_hi<F16>(y);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = pf_query<QT>(a, i + k);
+    }
+}
+
 // a wave's tokens: tiles first + step i (i < n) of a sequence of len > 0 tokens
 template <class Run>
 __device__ __forceinline__ void pf_tokens(Run& u, int kv, const int32_t* table, int len, int first, int step, int n) {
@@ -280,20 +306,20 @@ __device__ __forceinline__ void pf_pin(uint4& x) {
     x = make_uint4(v.x, v.y, v.z, v.w);
 }
 
+// likewise an accumulator, where a branch that scales it would have all paths carry it in the others
+__device__ __forceinline__ void pf_pin(pv16f& x) { asm("" : "+a"(x)); }
+
 // max for numbers (an fmaxf would quieten its inputs first)
 __device__ __forceinline__ float pf_max(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
-template <int NR>
-__device__ __forceinline__ void pf_top(const pv16f (&s)[NR], float (&top)[NR]) {
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        float t[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) t[k] = pf_max(pf_max(s[r][4 * k], s[r][4 * k + 1]), pf_max(s[r][4 * k + 2], s[r][4 * k + 3]));
-        top[r] = pf_max(pf_max(t[0], t[1]), pf_max(t[2], t[3]));
-    }
-}
+// Probabilities' sum of a lane's 16 tokens above which the running maximum moves (e^kSoftmaxSlack: each stays below it)
+constexpr float kPfOver = 2980.958f;
 
 // The wave's tiles.  mrow[r]: the additive mask's row of this lane's query row (MASK).
+//
+// One wave a SIMD issues one instruction every 4 cycles at best, so a tile costs its instructions: 48 MFMAs of 32 cycles
+// for 64 rows of 128 dims leave room for about 340 others.  So the codebook is staged times log2(e): a probability is
+// a subtraction and an exp2, and their sum, not a maximum per tile, tells when m has to move.  (With a mask the scores
+// are taken back to natural units, where the type's lowest value stays what it is.)
 template <bool MASK, int NR, class Run>
 __device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR], float (&m_run)[NR], float (&l_run)[NR],
                                          pv16f (&o)[NR][Run::DT]) {
@@ -301,8 +327,10 @@ __device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR],
     if (n <= 0) return;  // wave-uniform
     typename Run::Codes c1, c2, c3;
     typename Run::Vals val;
-    pv16f s[NR];
-    float top[NR];
+    pv16f s[NR];  // scores and m: log2 units, natural ones with a mask
+    float m[NR], mb[NR];  // mb: m, or 0 while that is -inf (as the scores are: their probabilities are 0)
+#pragma unroll
+    for (int r = 0; r < NR; ++r) m[r] = -INFINITY;
     // tile i's mask, and its end where it holds the sequence's last token
     auto fix = [&](int i) {
         const int tile = u.first + u.step * i;
@@ -313,11 +341,10 @@ __device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR],
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     const int t = min(t_half + 16 * (k >> 3) + (k & 7), len - 1);
-                    s[r][k] += mrow[r][(int64_t)t * u.p.a.m_st];
+                    s[r][k] = __builtin_fmaf(s[r][k], kLn2, mrow[r][(int64_t)t * u.p.a.m_st]);
                 }
         }
-        const bool tail = kPfTile * (tile + 1) > len;  // uniform
-        if (tail) {
+        if (kPfTile * (tile + 1) > len) {  // uniform
 #pragma unroll
             for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -336,41 +363,35 @@ __device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR],
                 }
             }
         }
-        if (MASK || tail) pf_top<NR>(s, top);
     };
+    // a probability from its score
+    auto prob = [&](float x, int r) {
+        return __builtin_amdgcn_exp2f(MASK ? (x - mb[r]) * kLog2e : x - mb[r]);
+    };
+    // raises m to the scores' maximum, by[r] >= 0 log2 units
+    auto raise = [&](float (&by)[NR]) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            float top = s[r][0];
+#pragma unroll
+            for (int k = 1; k < 16; ++k) top = pf_max(top, s[r][k]);
+            top = pf_max(top, pf_other(top));
+            const float mn = pf_max(m[r], top);
+            by[r] = mn == -INFINITY ? 0.f : (mn - m[r]) * (MASK ? kLog2e : 1.f);
+            m[r] = mn;
+            mb[r] = mn == -INFINITY ? 0.f : mn;
+        }
+    };
+    float by[NR];
     u.load_codes(0, c1);
     u.load_codes(min(1, n - 1), c2);
     u.load_codes(min(2, n - 1), c3);
     u.load_vals(0, val);
     u.prime(c1);
     u.scores(c1, c2, s, [](int) {});
-    pf_top<NR>(s, top);
     fix(0);
+    raise(by);
     for (int i = 0; i < n; ++i) {
-        // the running maximum moves only when a score passes it by kSoftmaxSlack
-        bool over = false;
-#pragma unroll
-        for (int r = 0; r < NR; ++r) over |= top[r] > m_run[r] + kSoftmaxSlack;
-        if (__builtin_amdgcn_ballot_w64(over) != 0) {
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                const float mn = fmaxf(m_run[r], fmaxf(top[r], pf_other(top[r])));
-                const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[r] - mn) * kLog2e);
-                m_run[r] = mn;
-                l_run[r] *= f;
-#pragma unroll
-                for (int dt = 0; dt < Run::DT; ++dt)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) o[r][dt][k] *= f;
-            }
-        }
-        // a masked score may be the type's lowest value, which times log2(e) is -inf: m is taken off first
-        if constexpr (MASK) {
-#pragma unroll
-            for (int r = 0; r < NR; ++r)
-#pragma unroll
-                for (int k = 0; k < 16; ++k) s[r][k] -= m_run[r] == -INFINITY ? 0.f : m_run[r];
-        }
         if ((i & 31) == 31) {  // the next tile starts the next 32 entries (tiles up to i + 3 are asked for)
             u.batch = (i >> 5) + 1;
             u.pc = u.pcn;
@@ -383,9 +404,9 @@ __device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR],
         // the next tile's scores beside this tile's probabilities
         pv16f s2[NR];
         uint32_t pw[NR][8];  // P^T operands
-        float mb[NR], e0[NR];
+        float e0[NR], lt[NR];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) mb[r] = MASK || m_run[r] == -INFINITY ? 0.f : m_run[r] * kLog2e;  // -inf: so are its scores
+        for (int r = 0; r < NR; ++r) lt[r] = 0.f;
         __builtin_amdgcn_sched_barrier(0);
         u.scores(c1, c2, s2, [&](int st) {
             constexpr int kPer = 16 / Run::NST;
@@ -394,16 +415,46 @@ __device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR],
 #pragma unroll
                 for (int x = 0; x < kPer; ++x) {
                     const int k = st * kPer + x;
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][k], kLog2e, -mb[r]));
-                    l_run[r] += e;
+                    const float e = prob(s[r][k], r);
+                    lt[r] += e;
                     if (k & 1) pw[r][k >> 1] = pf_pack<Run::kVF16>(e0[r], e);
                     else e0[r] = e;
                 }
         });
-        // P.V beside the next tile's maxima; a value operand's successor loads once it is used
+        bool over = false;
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int dt = 0; dt < Run::DT; ++dt) pf_pin(o[r][dt]);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) over |= lt[r] > (m[r] == -INFINITY ? 0.f : kPfOver);
+        if (__builtin_amdgcn_ballot_w64(over) != 0) {  // m moves: once more from the scores
+            raise(by);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const float f = __builtin_amdgcn_exp2f(-by[r]);
+                lt[r] = 0.f;
+                l_run[r] *= f;
+#pragma unroll
+                for (int dt = 0; dt < Run::DT; ++dt) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[r][dt][k] *= f;
+                    pf_pin(o[r][dt]);
+                }
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                    const float x = prob(s[r][k], r), y = prob(s[r][k + 1], r);
+                    pw[r][k >> 1] = pf_pack<Run::kVF16>(x, y);
+                    lt[r] += x + y;
+                }
+            }
+        }
+        // P.V; a value operand's successor loads once it is used
         const uint16_t* vsrc[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) vsrc[c] = u.val_row(min(i + 1, n - 1), c);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) l_run[r] += lt[r];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -412,28 +463,22 @@ __device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR],
                 for (int r = 0; r < NR; ++r)
                     o[r][dt] = pf_mfma<Run::kVF16>(val.v[c][dt], make_uint4(pw[r][4 * c], pw[r][4 * c + 1], pw[r][4 * c + 2], pw[r][4 * c + 3]), o[r][dt]);
                 val.v[c][dt] = u.load_val(vsrc[c], dt);
-                constexpr int kPer = 8 / Run::DT;  // score registers per step
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int x = 0; x < kPer; x += 2) {
-                        const int k = (c * Run::DT + dt) * kPer + x;
-                        const float t = pf_max(s2[r][k], s2[r][k + 1]);
-                        top[r] = k ? pf_max(top[r], t) : t;
-                    }
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
         for (int r = 0; r < NR; ++r) s[r] = s2[r];
         if (i + 1 < n) fix(i + 1);
     }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) m_run[r] = MASK || m[r] == -INFINITY ? m[r] : m[r] * kLn2;
 }
 
 // A prefix item: rows [R0, R0 + nr) of the KV head over tiles [t0, t1) of the prefix (len tokens); partials go to
-// slice `split`.  The whole workgroup calls it.  pj: the query dim of this thread (permuted dim tid % D).
+// slice `split`.  The whole workgroup calls it.  last: the workgroup's last item, after which the codebook's LDS is
+// free for the join.
 template <int D, int BD, int QT, int VT, int NR>
-__device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigned char* lds, int kv, int R0, int nr, int64_t pj,
-                                               int len, int t0, int t1, int split) {
+__device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigned char* lds, int kv, int R0, int nr,
+                                               const uint16_t* permL, int len, int t0, int t1, int split, bool last) {
     using Run = PfRun<D, BD, QT, VT, NR>;
     using L = PfLds<D>;
     const ssq_decode_args& a = p.a;
@@ -451,41 +496,57 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
     u.lane = lane; u.half = half;
     pf_tokens(u, kv, p.ptab, len, t0 + wave, kPfWaves, (t1 - t0 - wave + kPfWaves - 1) / kPfWaves);
 
-    // ---- query rows: scaled in their dtype, permuted, as 16-bit parts [part][row][D] in LDS
-    uint16_t* qL = reinterpret_cast<uint16_t*>(scratch);
-    constexpr int kRows = 32 * NR, kPer = kRows * D / kPfThreads, kBatch = kPer < 16 ? kPer : 16;
-    const int j = tid % D;
-    if (tid < kRows) {
+    // ---- query rows: pieces of 8 dims scaled in their dtype, as 16-bit parts; 32 rows of a part at a time go to
+    // LDS as they are, are permuted there and become operands
+    if (tid < 32 * NR) {
         const int R = R0 + min(tid, nr - 1);
         rowL[tid] = pf_qrow(p, kv, R);
         rowL[64 + tid] = pf_rid(p, kv, R);
     }
     __syncthreads();
-#pragma unroll 1
-    for (int e0 = 0; e0 < kPer; e0 += kBatch) {
-        float v[kBatch];
+    constexpr int kPieces = 32 * D / 8 / kPfThreads;  // of 32 rows, per thread
+    uint4 part[NR][Run::QP][kPieces];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) v[k] = pf_query<QT>(a, rowL[(e0 + k) * (kPfThreads / D) + tid / D] + pj);
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int r = (e0 + k) * (kPfThreads / D) + tid / D;
-            const float x = r < nr ? v[k] : 0.f;
-            const uint32_t w = pf_pack<Run::kF16>(x, 0.f);
-            qL[r * L::kQRow + j] = (uint16_t)w;
-            if constexpr (Run::QP == 2) qL[(kRows + r) * L::kQRow + j] = (uint16_t)pf_pack<false>(x - pf_lo<false>(w), 0.f);
+        for (int k = 0; k < kPieces; ++k) {
+            const int e = tid + k * kPfThreads, row = 32 * r + e / (D / 8), d = e % (D / 8) * 8;
+            float x[8];
+            pf_query8<QT>(p, rowL[row] + d, x);
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (row >= nr) x[2 * i] = x[2 * i + 1] = 0.f;
+                hi[i] = pf_pack<Run::kF16>(x[2 * i], x[2 * i + 1]);
+                lo[i] = pf_pack<false>(x[2 * i] - pf_lo<false>(hi[i]), x[2 * i + 1] - pf_hi<false>(hi[i]));
+            }
+            part[r][0][k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (Run::QP == 2) part[r][1][k] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
-    }
-    __syncthreads();
+    uint16_t* rawL = reinterpret_cast<uint16_t*>(scratch);
+    uint16_t* qL = rawL + 32 * D;
+    const int j2 = tid % (D / 2);
+    const uint32_t s0 = permL[2 * j2], s1 = permL[2 * j2 + 1];
 #pragma unroll
-    for (int h = 0; h < Run::QP; ++h)
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+        for (int h = 0; h < Run::QP; ++h) {
+            if (r || h) __syncthreads();  // the operands before are read
 #pragma unroll
-            for (int st = 0; st < Run::NQ; ++st)
-            {
-                u.q[h][r][st] = *reinterpret_cast<const uint4*>(qL + (h * kRows + 32 * r + col) * L::kQRow + 16 * st + 8 * half);
+            for (int k = 0; k < kPieces; ++k) reinterpret_cast<uint4*>(rawL)[tid + k * kPfThreads] = part[r][h][k];
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 32 * (D / 2) / kPfThreads; ++k) {
+                const int row = tid / (D / 2) + k * (2 * kPfThreads / D);
+                reinterpret_cast<uint32_t*>(qL + row * L::kQRow)[j2] = rawL[row * D + s0] | ((uint32_t)rawL[row * D + s1] << 16);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int st = 0; st < Run::NQ; ++st) {
+                u.q[h][r][st] = *reinterpret_cast<const uint4*>(qL + col * L::kQRow + 16 * st + 8 * half);
                 if constexpr (NR == 2) pf_pin(u.q[h][r][st]);
             }
+        }
 
     const float* mrow[NR] = {};
     float m_run[NR], l_run[NR];
@@ -497,7 +558,7 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
 #pragma unroll
         for (int dt = 0; dt < Run::DT; ++dt) {
             o[r][dt] = pv16f{};
-            if constexpr (NR == 2) asm("" : "+a"(o[r][dt]));
+            pf_pin(o[r][dt]);
         }
     }
     pf_tiles<false, NR>(u, mrow, m_run, l_run, o);
@@ -511,8 +572,7 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
             lL[wave * 64 + 32 * r + col] = l;
         }
     }
-    __syncthreads();  // also: every wave has read its query operands
-    float* jL = reinterpret_cast<float*>(scratch);
+    __syncthreads();  // also: every wave is past its gathers
     float f[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
@@ -535,29 +595,39 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
         ws_l[rid] = l;
     }
     const int jr = tid >> 3, jd = (tid & 7) * 4;  // the row and dims this thread joins
+    constexpr int kTileF = kPfWaves * 32 * L::kJoinRow;  // floats of a (32 rows, 32 dims) tile of every wave
+    float* jL = reinterpret_cast<float*>(last ? lds : scratch);
+    auto join = [&](const float* src, int r, int dt) {
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        if (32 * r >= nr) break;  // uniform
-        const bool in = 32 * r + jr < nr;
-        float* dst = ws_o + rowL[64 + 32 * r + jr] * D + jd;  // rows past nr repeat the last
+        for (int w = 0; w < kPfWaves; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(src + (w * 32 + jr) * L::kJoinRow + jd);
+            t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
+        }
+        if (32 * r + jr < nr) *reinterpret_cast<float4*>(ws_o + rowL[64 + 32 * r + jr] * D + 32 * dt + jd) = t;
+    };
+    static_assert(NR * Run::DT * kTileF * 4 <= L::kBook + L::kScratch, "the last item's join fits the codebook's LDS");
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
         for (int dt = 0; dt < Run::DT; ++dt) {
+            float* dst = jL + (last ? (r * Run::DT + dt) * kTileF : 0);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {  // dims 8 k + 4 half ..
                 float4 x = make_float4(o[r][dt][4 * k] * f[r], o[r][dt][4 * k + 1] * f[r], o[r][dt][4 * k + 2] * f[r], o[r][dt][4 * k + 3] * f[r]);
                 if (f[r] == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
-                *reinterpret_cast<float4*>(jL + (wave * 32 + col) * L::kJoinRow + 8 * k + 4 * half) = x;
+                *reinterpret_cast<float4*>(dst + (wave * 32 + col) * L::kJoinRow + 8 * k + 4 * half) = x;
             }
-            __syncthreads();
-            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kPfWaves; ++w) {
-                const float4 x = *reinterpret_cast<const float4*>(jL + (w * 32 + jr) * L::kJoinRow + jd);
-                t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
+            if (!last) {  // uniform
+                __syncthreads();
+                join(jL, r, dt);
+                __syncthreads();
             }
-            if (in) *reinterpret_cast<float4*>(dst + 32 * dt) = t;
-            __syncthreads();
         }
+    if (last) {
+        __syncthreads();
+#pragma unroll 2
+        for (int t = 0; t < NR * Run::DT; ++t) join(jL + t * kTileF, t / Run::DT, t % Run::DT);
     }
 }
 
@@ -692,17 +762,22 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
     // a permuted dim's source, for this thread's staging and for the waves' own rows
     const int64_t pj = (int64_t)min((uint64_t)a.perm[(int64_t)kv * a.perm_sh + tid % D], (uint64_t)(D - 1));
     const int plen = p.n1 ? max(0, min(p.plen[0], p.pcap)) : 0;
-    // ---- the KV head's codebook as 16-bit parts, kIn pieces in flight per thread
+    // ---- the KV head's codebook times log2(e) as 16-bit parts, kIn pieces in flight per thread; workgroups start at different
+    // pieces, since those of one KV head share an L2
     {
         constexpr bool F16 = QT == kQtF16;
         constexpr int kV = BD < 4 ? BD : 4, kIn = 16;  // floats per piece
         const float* cent = a.cent + (int64_t)kv * a.cent_sh;
         const int nc = a.n_centroids, per = nc * (BD / kV), total = (D / BD) * per;
+        const int shift = (int)((int64_t)total * w / p.n_wg) & ~(kPfThreads - 1);
+#pragma unroll 1
         for (int e0 = tid; e0 < total; e0 += kIn * kPfThreads) {
             float x[kIn][kV];
 #pragma unroll
             for (int i = 0; i < kIn; ++i) {
-                const float* src = cent + (int64_t)min(e0 + i * kPfThreads, total - 1) * kV;
+                int e = min(e0 + i * kPfThreads, total - 1) + shift;
+                e = e < total ? e : e - total;
+                const float* src = cent + (int64_t)e * kV;
                 if constexpr (kV == 4) {
                     const float4 v = *reinterpret_cast<const float4*>(src);
                     x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
@@ -713,29 +788,31 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
             }
 #pragma unroll
             for (int i = 0; i < kIn; ++i) {
-                const int e = e0 + i * kPfThreads;
-                if (e >= total) break;
+                int e = min(e0 + i * kPfThreads, total - 1) + shift;  // past the end: the last piece again
+                e = e < total ? e : e - total;
                 uint32_t hi[kV / 2], lo[kV / 2];
+#pragma unroll
+                for (int k = 0; k < kV; ++k) x[i][k] *= kLog2e;
 #pragma unroll
                 for (int k = 0; k < kV / 2; ++k) {
                     hi[k] = pf_pack<F16>(x[i][2 * k], x[i][2 * k + 1]);
                     lo[k] = pf_pack<F16>(x[i][2 * k] - pf_lo<F16>(hi[k]), x[i][2 * k + 1] - pf_hi<F16>(hi[k]));
                 }
                 const int blk = nc == 256 ? e / (256 * (BD / kV)) : e / per;  // a shift where it counts
-                unsigned char* dst = pf_lds + blk * 512 * BD + (e - blk * per) * 2 * kV;
-                unsigned char* dlo = dst + L::kBook / 2;
+                unsigned char* dst = pf_lds + blk * 1024 * BD + (e - blk * per) * 2 * kV;
                 if constexpr (BD == 2) {
                     *reinterpret_cast<uint32_t*>(dst) = hi[0];
-                    *reinterpret_cast<uint32_t*>(dlo) = lo[0];
+                    *reinterpret_cast<uint32_t*>(dst + 512 * BD) = lo[0];
                 } else {
                     *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-                    *reinterpret_cast<uint2*>(dlo) = make_uint2(lo[0], lo[1]);
+                    *reinterpret_cast<uint2*>(dst + 512 * BD) = make_uint2(lo[0], lo[1]);
                 }
             }
         }
         if (tid < D) permL[tid] = (uint16_t)pj;
     }
     __syncthreads();
+    if (p.n2) pf_own<D, BD, QT, VT>(p, pf_lds, permL, kv, w * kPfWaves + wave);
     // ---- the prefix: slices past its length are not read by the merge either
     const int tiles = ssq_prefix_tiles(plen), per = p.n1 ? ssq_prefix_slice(plen, p.n1) : 0;
     const int n_pre = per ? p.n_rg * ((tiles + per - 1) / per) : 0;
@@ -745,13 +822,12 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
         const int t0 = split * per, t1 = min(t0 + per, tiles);
         if constexpr (QT != kQtSplit) {
             if (p.pre_nr == 2) {
-                pf_prefix_item<D, BD, QT, VT, 2>(p, pf_lds, kv, R0, nr, pj, plen, t0, t1, split);
+                pf_prefix_item<D, BD, QT, VT, 2>(p, pf_lds, kv, R0, nr, permL, plen, t0, t1, split, it + p.n_wg >= n_pre);
                 continue;
             }
         }
-        pf_prefix_item<D, BD, QT, VT, 1>(p, pf_lds, kv, R0, nr, pj, plen, t0, t1, split);
+        pf_prefix_item<D, BD, QT, VT, 1>(p, pf_lds, kv, R0, nr, permL, plen, t0, t1, split, it + p.n_wg >= n_pre);
     }
-    if (p.n2) pf_own<D, BD, QT, VT>(p, pf_lds, permL, kv, w * kPfWaves + wave);
 }
 
 template <int D, int BD, int QT, int VT>

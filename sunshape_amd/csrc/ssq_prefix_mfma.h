@@ -246,16 +246,17 @@ __device__ __forceinline__ int64_t pf_qrow(const SsqPrefixParams& p, int kv, int
     return (int64_t)b * p.a.q_sb + (int64_t)h * p.a.q_sh + (int64_t)qi * p.a.q_sl;
 }
 
-// element i of the queries, scaled in their dtype (the split form takes any)
+// element i of the queries (the split form takes any dtype), and an element scaled in its dtype
 template <int QT>
-__device__ __forceinline__ float pf_query(const ssq_decode_args& a, int64_t i) {
-    if constexpr (QT == kQtSplit) {
-        const float x = ssq_load_elem(a.q, a.q_dtype, i);
-        return a.has_scale ? ssq_round_to(x * a.scale, a.q_dtype) : x;
-    } else {
-        const float x = pf_lo<QT == kQtF16>(reinterpret_cast<const uint16_t*>(a.q)[i]);
-        return a.has_scale ? pf_lo<QT == kQtF16>(pf_pack<QT == kQtF16>(x * a.scale, 0.f)) : x;
-    }
+__device__ __forceinline__ float pf_raw(const ssq_decode_args& a, int64_t i) {
+    if constexpr (QT == kQtSplit) return ssq_load_elem(a.q, a.q_dtype, i);
+    else return pf_lo<QT == kQtF16>(reinterpret_cast<const uint16_t*>(a.q)[i]);
+}
+template <int QT>
+__device__ __forceinline__ float pf_scaled(const ssq_decode_args& a, float x) {
+    if (!a.has_scale) return x;
+    if constexpr (QT == kQtSplit) return ssq_round_to(x * a.scale, a.q_dtype);
+    else return pf_lo<QT == kQtF16>(pf_pack<QT == kQtF16>(x * a.scale, 0.f));
 }
 
 // eight consecutive dims
@@ -278,7 +279,7 @@ __device__ __forceinline__ void pf_query8(const SsqPrefixParams& p, int64_t i, f
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = pf_query<QT>(a, i + k);
+        for (int k = 0; k < 8; ++k) x[k] = pf_scaled<QT>(a, pf_raw<QT>(a, i + k));
     }
 }
 
@@ -295,7 +296,9 @@ __device__ __forceinline__ void pf_tokens(Run& u, int kv, const int32_t* table, 
     u.vstep = 32 * (uint32_t)a.v_st;
     u.batch = 0;
     u.entries(0, u.pc, u.pv);
-    u.entries(32, u.pcn, u.pvn);
+    u.pcn = u.pc;
+    u.pvn = u.pv;
+    if (n > 32) u.entries(32, u.pcn, u.pvn);
 }
 
 // Keeps a matrix-core operand in the accumulation registers, which the MFMAs read as well: the compiler otherwise
@@ -314,6 +317,21 @@ __device__ __forceinline__ float pf_max(float a, float b) { return __builtin_amd
 // Probabilities' sum of a lane's 16 tokens above which the running maximum moves (e^kSoftmaxSlack: each stays below it)
 constexpr float kPfOver = 2980.958f;
 
+// the first tiles' codes and values, asked for before the query rows are
+template <class Run>
+struct PfFirst {
+    typename Run::Codes c1, c2, c3;
+    typename Run::Vals val;
+    __device__ __forceinline__ explicit PfFirst(const Run& u) {
+        if (u.n_tiles > 0) {  // wave-uniform
+            u.load_codes(0, c1);
+            u.load_codes(min(1, u.n_tiles - 1), c2);
+            u.load_codes(min(2, u.n_tiles - 1), c3);
+            u.load_vals(0, val);
+        }
+    }
+};
+
 // The wave's tiles.  mrow[r]: the additive mask's row of this lane's query row (MASK).
 //
 // One wave a SIMD issues one instruction every 4 cycles at best, so a tile costs its instructions: 48 MFMAs of 32 cycles
@@ -321,12 +339,12 @@ constexpr float kPfOver = 2980.958f;
 // a subtraction and an exp2, and their sum, not a maximum per tile, tells when m has to move.  (With a mask the scores
 // are taken back to natural units, where the type's lowest value stays what it is.)
 template <bool MASK, int NR, class Run>
-__device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR], float (&m_run)[NR], float (&l_run)[NR],
-                                         pv16f (&o)[NR][Run::DT]) {
+__device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, const float* const (&mrow)[NR], float (&m_run)[NR],
+                                         float (&l_run)[NR], pv16f (&o)[NR][Run::DT]) {
     const int n = u.n_tiles, len = u.len;
     if (n <= 0) return;  // wave-uniform
-    typename Run::Codes c1, c2, c3;
-    typename Run::Vals val;
+    typename Run::Codes c1 = first.c1, c2 = first.c2, c3 = first.c3;
+    typename Run::Vals val = first.val;
     pv16f s[NR];  // scores and m: log2 units, natural ones with a mask
     float m[NR], mb[NR];  // mb: m, or 0 while that is -inf (as the scores are: their probabilities are 0)
 #pragma unroll
@@ -383,10 +401,6 @@ __device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR],
         }
     };
     float by[NR];
-    u.load_codes(0, c1);
-    u.load_codes(min(1, n - 1), c2);
-    u.load_codes(min(2, n - 1), c3);
-    u.load_vals(0, val);
     u.prime(c1);
     u.scores(c1, c2, s, [](int) {});
     fix(0);
@@ -396,7 +410,7 @@ __device__ __forceinline__ void pf_tiles(Run& u, const float* const (&mrow)[NR],
             u.batch = (i >> 5) + 1;
             u.pc = u.pcn;
             u.pv = u.pvn;
-            u.entries(32 * (u.batch + 1), u.pcn, u.pvn);
+            if (n > 32 * (u.batch + 1)) u.entries(32 * (u.batch + 1), u.pcn, u.pvn);
         }
         c1 = c2;
         c2 = c3;
@@ -495,6 +509,7 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
     Run u{p, lds};
     u.lane = lane; u.half = half;
     pf_tokens(u, kv, p.ptab, len, t0 + wave, kPfWaves, (t1 - t0 - wave + kPfWaves - 1) / kPfWaves);
+    const PfFirst<Run> first(u);
 
     // ---- query rows: pieces of 8 dims scaled in their dtype, as 16-bit parts; 32 rows of a part at a time go to
     // LDS as they are, are permuted there and become operands
@@ -561,7 +576,7 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
             pf_pin(o[r][dt]);
         }
     }
-    pf_tiles<false, NR>(u, mrow, m_run, l_run, o);
+    pf_tiles<false, NR>(u, first, mrow, m_run, l_run, o);
 
     // ---- the four waves' (m, l), then o, 32 rows x 32 dims at a time
 #pragma unroll
@@ -641,22 +656,26 @@ __device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsi
     Run u{p, book};
     u.lane = lane; u.half = half;
     pf_tokens(u, kv, table, len, t0, 1, t1 - t0);
-    // query operands straight from memory: a lane's row, its half of every 16 permuted dims
+    // query operands straight from memory: a lane's row, its half of every 16 permuted dims, all loads in flight
     const int R = R0 + min(col, nr - 1);
     const int64_t qrow = pf_qrow(p, kv, R);
+    float x[Run::NQ][8];
 #pragma unroll
     for (int st = 0; st < Run::NQ; ++st) {
         const uint4 pw = *reinterpret_cast<const uint4*>(permL + 16 * st + 8 * half);
         const uint32_t w[4] = {pw.x, pw.y, pw.z, pw.w};
-        float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = pf_query<QT>(a, qrow + ((w[k >> 1] >> (16 * (k & 1))) & 0xFFFFu));
+        for (int k = 0; k < 8; ++k) x[st][k] = pf_raw<QT>(a, qrow + ((w[k >> 1] >> (16 * (k & 1))) & 0xFFFFu));
+    }
+    const PfFirst<Run> first(u);
+#pragma unroll
+    for (int st = 0; st < Run::NQ; ++st) {
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float x = col < nr ? v[2 * k] : 0.f, y = col < nr ? v[2 * k + 1] : 0.f;
-            hi[k] = pf_pack<Run::kF16>(x, y);
-            lo[k] = pf_pack<false>(x - pf_lo<false>(hi[k]), y - pf_hi<false>(hi[k]));
+            const float y = col < nr ? pf_scaled<QT>(a, x[st][2 * k]) : 0.f, z = col < nr ? pf_scaled<QT>(a, x[st][2 * k + 1]) : 0.f;
+            hi[k] = pf_pack<Run::kF16>(y, z);
+            lo[k] = pf_pack<false>(y - pf_lo<false>(hi[k]), z - pf_hi<false>(hi[k]));
         }
         u.q[0][0][st] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         if constexpr (Run::QP == 2) u.q[1][0][st] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -671,7 +690,7 @@ __device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsi
     pv16f o[1][Run::DT];
 #pragma unroll
     for (int dt = 0; dt < Run::DT; ++dt) o[0][dt] = pv16f{};
-    pf_tiles<MASK, 1>(u, mrow, m_run, l_run, o);
+    pf_tiles<MASK, 1>(u, first, mrow, m_run, l_run, o);
     const float l = l_run[0] + pf_other(l_run[0]);
     if (col < nr) {
         const int64_t n_rows = (int64_t)a.batch * a.num_q_heads * a.q_len, rid = pf_rid(p, kv, R);
@@ -762,57 +781,62 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
     // a permuted dim's source, for this thread's staging and for the waves' own rows
     const int64_t pj = (int64_t)min((uint64_t)a.perm[(int64_t)kv * a.perm_sh + tid % D], (uint64_t)(D - 1));
     const int plen = p.n1 ? max(0, min(p.plen[0], p.pcap)) : 0;
-    // ---- the KV head's codebook times log2(e) as 16-bit parts, kIn pieces in flight per thread; workgroups start at different
-    // pieces, since those of one KV head share an L2
+    // ---- the KV head's codebook times log2(e) as 16-bit parts: a thread takes the same codeword (or half of one, at
+    // 8 dims) of every block, up to kIn of them in flight; workgroups start at different blocks, since those of one
+    // KV head share an L2
     {
         constexpr bool F16 = QT == kQtF16;
-        constexpr int kV = BD < 4 ? BD : 4, kIn = 16;  // floats per piece
+        constexpr int NB = D / BD, kV = BD < 4 ? BD : 4, kParts = BD / kV;  // floats of a piece, pieces of a codeword
+        constexpr int kIn = NB < 32 / kParts ? NB : 32 / kParts;            // blocks in flight
         const float* cent = a.cent + (int64_t)kv * a.cent_sh;
-        const int nc = a.n_centroids, per = nc * (BD / kV), total = (D / BD) * per;
-        const int shift = (int)((int64_t)total * w / p.n_wg) & ~(kPfThreads - 1);
+        const int nc = a.n_centroids;
 #pragma unroll 1
-        for (int e0 = tid; e0 < total; e0 += kIn * kPfThreads) {
-            float x[kIn][kV];
+        for (int i0 = 0; i0 < NB; i0 += kIn) {
+            float x[kIn][kParts][kV];
 #pragma unroll
             for (int i = 0; i < kIn; ++i) {
-                int e = min(e0 + i * kPfThreads, total - 1) + shift;
-                e = e < total ? e : e - total;
-                const float* src = cent + (int64_t)e * kV;
-                if constexpr (kV == 4) {
-                    const float4 v = *reinterpret_cast<const float4*>(src);
-                    x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
-                } else {
-                    const float2 v = *reinterpret_cast<const float2*>(src);
-                    x[i][0] = v.x; x[i][1] = v.y;
+                const float* src = cent + ((i0 + i + w) & (NB - 1)) * nc * BD;  // uniform
+#pragma unroll
+                for (int j = 0; j < kParts; ++j) {
+                    const int e = min(tid + j * kPfThreads, nc * kParts - 1);
+                    if constexpr (kV == 4) {
+                        const float4 v = reinterpret_cast<const float4*>(src)[e];
+                        x[i][j][0] = v.x; x[i][j][1] = v.y; x[i][j][2] = v.z; x[i][j][3] = v.w;
+                    } else {
+                        const float2 v = reinterpret_cast<const float2*>(src)[e];
+                        x[i][j][0] = v.x; x[i][j][1] = v.y;
+                    }
                 }
             }
 #pragma unroll
             for (int i = 0; i < kIn; ++i) {
-                int e = min(e0 + i * kPfThreads, total - 1) + shift;  // past the end: the last piece again
-                e = e < total ? e : e - total;
-                uint32_t hi[kV / 2], lo[kV / 2];
+                unsigned char* blk = pf_lds + ((i0 + i + w) & (NB - 1)) * 1024 * BD;
 #pragma unroll
-                for (int k = 0; k < kV; ++k) x[i][k] *= kLog2e;
+                for (int j = 0; j < kParts; ++j) {
+                    uint32_t hi[kV / 2], lo[kV / 2];
 #pragma unroll
-                for (int k = 0; k < kV / 2; ++k) {
-                    hi[k] = pf_pack<F16>(x[i][2 * k], x[i][2 * k + 1]);
-                    lo[k] = pf_pack<F16>(x[i][2 * k] - pf_lo<F16>(hi[k]), x[i][2 * k + 1] - pf_hi<F16>(hi[k]));
-                }
-                const int blk = nc == 256 ? e / (256 * (BD / kV)) : e / per;  // a shift where it counts
-                unsigned char* dst = pf_lds + blk * 1024 * BD + (e - blk * per) * 2 * kV;
-                if constexpr (BD == 2) {
-                    *reinterpret_cast<uint32_t*>(dst) = hi[0];
-                    *reinterpret_cast<uint32_t*>(dst + 512 * BD) = lo[0];
-                } else {
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-                    *reinterpret_cast<uint2*>(dst + 512 * BD) = make_uint2(lo[0], lo[1]);
+                    for (int k = 0; k < kV / 2; ++k) {
+                        const float u = x[i][j][2 * k] * kLog2e, v = x[i][j][2 * k + 1] * kLog2e;
+                        hi[k] = pf_pack<F16>(u, v);
+                        lo[k] = pf_pack<F16>(u - pf_lo<F16>(hi[k]), v - pf_hi<F16>(hi[k]));
+                    }
+                    // past the last codeword: it again
+                    unsigned char* dst = blk + min(tid + j * kPfThreads, nc * kParts - 1) * 2 * kV;
+                    if constexpr (BD == 2) {
+                        *reinterpret_cast<uint32_t*>(dst) = hi[0];
+                        *reinterpret_cast<uint32_t*>(dst + 512 * BD) = lo[0];
+                    } else {
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2*>(dst + 512 * BD) = make_uint2(lo[0], lo[1]);
+                    }
                 }
             }
         }
         if (tid < D) permL[tid] = (uint16_t)pj;
     }
     __syncthreads();
-    if (p.n2) pf_own<D, BD, QT, VT>(p, pf_lds, permL, kv, w * kPfWaves + wave);
+    // (from the last workgroup down: a small prefix has the first ones)
+    if (p.n2) pf_own<D, BD, QT, VT>(p, pf_lds, permL, kv, (p.n_wg - 1 - w) * kPfWaves + wave);
     // ---- the prefix: slices past its length are not read by the merge either
     const int tiles = ssq_prefix_tiles(plen), per = p.n1 ? ssq_prefix_slice(plen, p.n1) : 0;
     const int n_pre = per ? p.n_rg * ((tiles + per - 1) / per) : 0;

@@ -252,11 +252,18 @@ __device__ __forceinline__ float pf_raw(const ssq_decode_args& a, int64_t i) {
     if constexpr (QT == kQtSplit) return ssq_load_elem(a.q, a.q_dtype, i);
     else return pf_lo<QT == kQtF16>(reinterpret_cast<const uint16_t*>(a.q)[i]);
 }
+// two elements scaled in their dtype, as packed 16-bit parts (a factor of 1 where there is no scale: exact)
 template <int QT>
-__device__ __forceinline__ float pf_scaled(const ssq_decode_args& a, float x) {
-    if (!a.has_scale) return x;
-    if constexpr (QT == kQtSplit) return ssq_round_to(x * a.scale, a.q_dtype);
-    else return pf_lo<QT == kQtF16>(pf_pack<QT == kQtF16>(x * a.scale, 0.f));
+__device__ __forceinline__ void pf_parts(const ssq_decode_args& a, float scale, float x, float y, uint32_t& hi, uint32_t& lo) {
+    if constexpr (QT == kQtSplit) {
+        x = ssq_round_to(x * scale, a.q_dtype);
+        y = ssq_round_to(y * scale, a.q_dtype);
+        hi = pf_pack<false>(x, y);
+        lo = pf_pack<false>(x - pf_lo<false>(hi), y - pf_hi<false>(hi));
+    } else {
+        hi = pf_pack<QT == kQtF16>(x * scale, y * scale);
+        lo = 0;
+    }
 }
 
 // eight consecutive dims
@@ -271,15 +278,10 @@ __device__ __forceinline__ void pf_query8(const SsqPrefixParams& p, int64_t i, f
         for (int k = 0; k < 4; ++k) {
             x[2 * k] = pf_lo<F16>(w[k]);
             x[2 * k + 1] = pf_hi<F16>(w[k]);
-            if (a.has_scale) {
-                const uint32_t y = pf_pack<F16>(x[2 * k] * a.scale, x[2 * k + 1] * a.scale);
-                x[2 * k] = pf_lo<F16>(y);
-                x[2 * k + 1] = pf_hi<F16>(y);
-            }
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = pf_scaled<QT>(a, pf_raw<QT>(a, i + k));
+        for (int k = 0; k < 8; ++k) x[k] = pf_raw<QT>(a, i + k);
     }
 }
 
@@ -519,6 +521,7 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
         rowL[64 + tid] = pf_rid(p, kv, R);
     }
     __syncthreads();
+    const float scale = a.has_scale ? a.scale : 1.f;
     constexpr int kPieces = 32 * D / 8 / kPfThreads;  // of 32 rows, per thread
     uint4 part[NR][Run::QP][kPieces];
 #pragma unroll
@@ -531,9 +534,8 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (row >= nr) x[2 * i] = x[2 * i + 1] = 0.f;
-                hi[i] = pf_pack<Run::kF16>(x[2 * i], x[2 * i + 1]);
-                lo[i] = pf_pack<false>(x[2 * i] - pf_lo<false>(hi[i]), x[2 * i + 1] - pf_hi<false>(hi[i]));
+                pf_parts<QT>(a, scale, x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+                if (row >= nr) hi[i] = lo[i] = 0;
             }
             part[r][0][k] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             if constexpr (Run::QP == 2) part[r][1][k] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -668,14 +670,14 @@ __device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsi
         for (int k = 0; k < 8; ++k) x[st][k] = pf_raw<QT>(a, qrow + ((w[k >> 1] >> (16 * (k & 1))) & 0xFFFFu));
     }
     const PfFirst<Run> first(u);
+    const float scale = a.has_scale ? a.scale : 1.f;
 #pragma unroll
     for (int st = 0; st < Run::NQ; ++st) {
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float y = col < nr ? pf_scaled<QT>(a, x[st][2 * k]) : 0.f, z = col < nr ? pf_scaled<QT>(a, x[st][2 * k + 1]) : 0.f;
-            hi[k] = pf_pack<Run::kF16>(y, z);
-            lo[k] = pf_pack<false>(y - pf_lo<false>(hi[k]), z - pf_hi<false>(hi[k]));
+            pf_parts<QT>(a, scale, x[st][2 * k], x[st][2 * k + 1], hi[k], lo[k]);
+            if (col >= nr) hi[k] = lo[k] = 0;
         }
         u.q[0][0][st] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         if constexpr (Run::QP == 2) u.q[1][0][st] = make_uint4(lo[0], lo[1], lo[2], lo[3]);

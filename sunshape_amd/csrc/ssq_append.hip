@@ -5,10 +5,10 @@
 // Few rows (a decode step): one launch, k_append_few.  A workgroup serves one block of some keys of a KV head:
 // it rotates just that block's dims (and, with a norm, reads the whole row for its sum, from L2 after the first
 // block), keeps the block's codebook in LDS and splits a key's scan over `slices` lanes.  Workgroups past
-// the blocks copy the values.
+// the blocks copy the values.  One chain of loads bounds it, so everything whose address is known is asked for at once.
 //
-// Many rows: k_append_values and the rotation (ssq_rope_run) write the pages' values and the rotated
-// keys, and ssq_encode, which is where the time goes, takes those.
+// Many rows: k_append_prep writes the pages' values and the rotated keys side by side, and ssq_encode, which is
+// where the time goes, takes those.
 #include "ssq_encode_math.h"
 #include "ssq_rope.h"
 
@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kValTok = 64;    // tokens of a value tile
+constexpr int kValTok = 64;    // tokens of a value tile, at most
 constexpr int kValDims = 128;  // dims of a value tile
 constexpr int kStageFloats = 10 * 1024;  // codebook floats (with norms) per LDS stage
 
@@ -34,6 +34,7 @@ struct AppendParams {
     int chunk;     // codewords per LDS stage
     int row_vec;   // key rows load as 16-byte pieces
     int dchunks;   // value dims in chunks of kValDims
+    int vtok;      // tokens of a value tile: 64, or 16 where there are few
     int v_vec;     // value rows load as 16-byte pieces
     int vp_vec;    // pages take 16-byte stores of 8 (16-bit) or 4 (32-bit) tokens
     int64_t* slots_out;  // sanitized slots (many rows) or NULL
@@ -48,20 +49,29 @@ __device__ __forceinline__ int64_t slot_of(const AppendParams& p, int i) {  // -
 // LDS of a value tile: raw elements of the page dtype, one padding dword per row
 __host__ __device__ constexpr int val_row(int size) { return kValDims * size + 4; }
 
-// Tokens [64 tile, +64) (flat over the batch), dims [128 dc, +128) of one KV head: rows in, pages out.  A
+// where a token's values go in its head's pages, and its slot within the page (-1: nowhere)
+struct ValSlots {
+    int64_t base[kValTok];
+    int off[kValTok];
+};
+
+// Tokens [vtok tile, +vtok) (flat over the batch), dims [128 dc, +128) of one KV head: rows in, pages out.  A
 // page holds a dim's tokens side by side, so a run of tokens in consecutive slots of a page that starts on
 // an 8-slot boundary leaves as whole 16-byte pieces; any other token by itself.
-__device__ __forceinline__ void value_tile(const AppendParams& p, unsigned char* lds, int64_t* slotL, int tile, int kv, int dc) {
+__device__ __forceinline__ void value_tile(const AppendParams& p, unsigned char* lds, ValSlots& vs, int tile, int kv, int dc) {
     const ssq_encode_args& a = p.e;
     const int tid = threadIdx.x;
     const int n = a.batch * a.seq_len;
-    const int i0 = tile * kValTok, nt = min(kValTok, n - i0);
+    const int i0 = tile * p.vtok, nt = min(p.vtok, n - i0);
     const int d0 = dc * kValDims, nd = min(kValDims, p.value_dim - d0);
     const int size = p.vp_dtype == SSQ_F32 ? 4 : 2;
     const int row = val_row(size);
+    const int page = a.page_size;
     if (tid < kValTok) {
         const int64_t slot = tid < nt ? slot_of(p, i0 + tid) : -1;
-        slotL[tid] = slot;
+        const int64_t pg = slot / page;
+        vs.off[tid] = slot < 0 ? -1 : (int)(slot - pg * page);
+        vs.base[tid] = slot < 0 ? 0 : pg * p.vp_sb + (int64_t)kv * p.vp_sh + (int64_t)d0 * p.vp_sd + (slot - pg * page);
         if (p.slots_out && kv == 0 && dc == 0 && tid < nt) p.slots_out[i0 + tid] = slot;
     }
     if (!p.v) return;  // the whole workgroup
@@ -91,25 +101,23 @@ __device__ __forceinline__ void value_tile(const AppendParams& p, unsigned char*
     }
     __syncthreads();
     // groups of 8 tokens, cut so that the first token's run meets 8-slot boundaries
-    const int page = a.page_size;
-    const int64_t first = slotL[0];
-    const int lead = first < 0 ? 0 : (int)(first % page) & 7;
-    constexpr int kGroups = kValTok / 8 + 1;
+    const int lead = vs.off[0] < 0 ? 0 : vs.off[0] & 7;
+    const int groups = (nt + lead + 7) >> 3;
     // lanes: the group's parity fastest (both halves of a 16-token page), then dims
-    for (int e = tid; e < kGroups * nd; e += kThreads) {
+    for (int e = tid; e < groups * nd; e += kThreads) {
         const int pair = e / (2 * nd), rest = e - pair * 2 * nd;
-        const bool last = 2 * pair + 1 >= kGroups;  // the odd group out
-        const int g = last ? 2 * pair : 2 * pair + (rest & 1), d = last ? rest : rest >> 1;
+        const bool odd = 2 * pair + 1 >= groups;  // the group without a partner
+        const int g = odd ? 2 * pair : 2 * pair + (rest & 1), d = odd ? rest : rest >> 1;
         const int ta = max(8 * g - lead, 0), tb = min(8 * g - lead + 8, nt);
-        if (ta >= tb) continue;
-        const int64_t s0 = slotL[ta];
-        bool whole = p.vp_vec && tb - ta == 8 && s0 >= 0 && (s0 % page) % 8 == 0;
-        if (whole) {
+        const int64_t dd = (int64_t)d * p.vp_sd;
+        bool whole = p.vp_vec && tb - ta == 8 && vs.off[ta] >= 0 && (vs.off[ta] & 7) == 0;
+        if (whole) {  // one page: its size is a multiple of 8
+            const int64_t b0 = vs.base[ta];
 #pragma unroll
-            for (int k = 1; k < 8; ++k) whole = whole && slotL[ta + k] == s0 + k;
+            for (int k = 1; k < 8; ++k) whole = whole && vs.off[ta + k] == vs.off[ta] + k && vs.base[ta + k] == b0 + k;
         }
         if (whole) {
-            const int64_t at = (s0 / page) * p.vp_sb + (int64_t)kv * p.vp_sh + (int64_t)(d0 + d) * p.vp_sd + s0 % page;
+            const int64_t at = vs.base[ta] + dd;
             if (size == 2) {
                 uint32_t w[4];
 #pragma unroll
@@ -128,20 +136,28 @@ __device__ __forceinline__ void value_tile(const AppendParams& p, unsigned char*
             continue;
         }
         for (int t = ta; t < tb; ++t) {
-            const int64_t slot = slotL[t];
-            if (slot < 0) continue;
-            const int64_t at = (slot / page) * p.vp_sb + (int64_t)kv * p.vp_sh + (int64_t)(d0 + d) * p.vp_sd + slot % page;
+            if (vs.off[t] < 0) continue;
+            const int64_t at = vs.base[t] + dd;
             if (size == 2) reinterpret_cast<uint16_t*>(p.vp)[at] = *reinterpret_cast<const uint16_t*>(lds + t * row + 2 * d);
             else reinterpret_cast<uint32_t*>(p.vp)[at] = *reinterpret_cast<const uint32_t*>(lds + t * row + 4 * d);
         }
     }
 }
 
-// values (and, for kv 0 and the first dims, the sanitized slots) of many rows: x tiles, y KV heads, z dims
-__global__ __launch_bounds__(kThreads) void k_append_values(const AppendParams p) {
-    __shared__ __align__(16) unsigned char lds[kValTok * val_row(4)];
-    __shared__ int64_t slotL[kValTok];
-    value_tile(p, lds, slotL, blockIdx.x, blockIdx.y, blockIdx.z);
+// Many rows: workgroups [0, rope_blocks) rotate the keys, the others write the values (and, for kv 0 and the first
+// dims, the sanitized slots).  They share nothing; one launch lets the values' transposes run beside the rotation.
+template <int DT, bool NORM>
+__global__ __launch_bounds__(kThreads) void k_append_prep(const AppendParams p, const RopeParams rp, int rope_blocks, int tiles) {
+    constexpr int kLds = kValTok * val_row(4) > rope_lds<DT, NORM>() * 4 ? kValTok * val_row(4) : rope_lds<DT, NORM>() * 4;
+    __shared__ __align__(16) unsigned char lds[kLds];
+    __shared__ ValSlots vs;
+    static_assert(kThreads == kRopeThreads, "one block size");
+    if ((int)blockIdx.x < rope_blocks) {
+        rope_units<DT, NORM, 4>(rp, blockIdx.x, reinterpret_cast<float*>(lds));
+        return;
+    }
+    const int e = blockIdx.x - rope_blocks, dk = e / tiles;  // tiles of a KV head side by side
+    value_tile(p, lds, vs, e - dk * tiles, dk % p.e.num_kv_heads, dk / p.e.num_kv_heads);
 }
 
 // BD: the block dim at compile time (1, 2, 4 or 8), or 0 for any other up to 16.  x: keys (or value tiles),
@@ -149,14 +165,14 @@ __global__ __launch_bounds__(kThreads) void k_append_values(const AppendParams p
 template <int BD>
 __global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
     constexpr int kX = BD ? BD : 16;
-    constexpr int kLds = kStageFloats * 4 > kValTok * val_row(4) ? kStageFloats * 4 : kValTok * val_row(4);
-    __shared__ __align__(16) unsigned char lds[kLds];
-    __shared__ int64_t slotL[kValTok];
+    extern __shared__ __align__(16) unsigned char few_lds[];
+    unsigned char* lds = few_lds;
     const ssq_encode_args& a = p.e;
     const int kv = blockIdx.y, blk = blockIdx.z;
     const int n = a.batch * a.seq_len;
     if (blk >= a.n_blocks) {
-        if ((int)blockIdx.x * kValTok < n) value_tile(p, lds, slotL, blockIdx.x, kv, blk - a.n_blocks);
+        __shared__ ValSlots vs;
+        if ((int)blockIdx.x * p.vtok < n) value_tile(p, lds, vs, blockIdx.x, kv, blk - a.n_blocks);
         return;
     }
     const int S = p.slices, sl = threadIdx.x & (S - 1);
@@ -173,9 +189,38 @@ __global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
     const int b = ii / a.seq_len, s = ii - b * a.seq_len;
     const int64_t slot = slot_of(p, ii);
     const int64_t krow = (int64_t)b * a.k_sb + (int64_t)kv * a.k_sh + (int64_t)s * a.k_ss;
-    const bool norm = p.kw != nullptr;
+    // the block's dims, their partners, weights and table entries (dims are the same for the whole workgroup)
+    const bool norm = p.kw != nullptr, turn = p.t.cos != nullptr;
+    const int half = p.t.rot_dim >> 1;
+    bool rot[kX], first[kX];
+    int64_t at[2 * kX], wat[2 * kX];
+    int ti[kX];
+#pragma unroll
+    for (int d = 0; d < kX; ++d) {
+        const int dim = d < bd ? (int)min((uint64_t)perm[d], (uint64_t)(D - 1)) : 0;
+        rot[d] = turn && dim < p.t.rot_dim;
+        first[d] = p.t.interleaved ? !(dim & 1) : dim < half;
+        const int other = !rot[d] ? dim : p.t.interleaved ? dim ^ 1 : first[d] ? dim + half : dim - half;
+        ti[d] = !rot[d] ? 0 : p.t.interleaved ? dim >> 1 : first[d] ? dim : dim - half;
+        at[d] = krow + dim;
+        at[kX + d] = krow + other;
+        wat[d] = dim;
+        wat[kX + d] = other;
+    }
+    float xr[2 * kX], wv[2 * kX], cv[kX], sv[kX];
+    ssq_load_elems<2 * kX>(a.keys, a.k_dtype, at, xr);
+    const int64_t pos = turn ? rope_pos(p.t, b, s) : 0;
+    if (turn) {  // uniform
+        const int64_t trow = (pos < 0 ? 0 : pos) * p.t.ld;
+#pragma unroll
+        for (int d = 0; d < kX; ++d) {
+            cv[d] = p.t.cos[trow + ti[d]];
+            sv[d] = p.t.sin[trow + ti[d]];
+        }
+    }
     float r = 1.f;
     if (norm) {  // the key's S lanes share the row's sum
+        ssq_load_elems<2 * kX>(p.kw, p.t.w_dtype, wat, wv);
         double sum = 0.0;
         if (p.row_vec) {
             const int per = a.k_dtype == SSQ_F32 ? 4 : 8;
@@ -204,17 +249,17 @@ __global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
         for (int o = S >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
         r = rope_rstd(sum, D, p.t.eps);
     }
-    const int64_t pos = p.t.cos ? rope_pos(p.t, b, s) : 0;
-    auto raw = [&](int d) { return ssq_load_elem(a.keys, a.k_dtype, krow + d); };
-    auto wt = [&](int d) { return ssq_load_elem(p.kw, p.t.w_dtype, d); };
     float x[kX];
 #pragma unroll
-    for (int d = 0; d < kX; ++d) {
-        if (d < bd) {
-            const int dim = (int)min((uint64_t)perm[d], (uint64_t)(D - 1));
-            x[d] = rope_dim(p.t, pos, dim, norm, r, raw, wt);
-            if (norm || p.t.cos) x[d] = rope_round(x[d], a.k_dtype);
+    for (int d = 0; d < kX; ++d) {  // as rope_dim
+        float u = norm ? (xr[d] * r) * wv[d] : xr[d];
+        if (rot[d]) {
+            const float v = norm ? (xr[kX + d] * r) * wv[kX + d] : xr[kX + d];
+            const float c = pos < 0 ? __builtin_nanf("") : cv[d], sn = pos < 0 ? __builtin_nanf("") : sv[d];
+            const float y = u * c, z = v * sn;
+            u = first[d] ? y - z : y + z;
         }
+        x[d] = norm || turn ? rope_round(u, a.k_dtype) : u;
     }
     int64_t crow = 0, prow = 0;
     if (slot >= 0) {
@@ -364,12 +409,48 @@ AppendParams params(const ssq_append_args& a) {
     const ssq_encode_args& e = a.enc;
     const int per = e.k_dtype == SSQ_F32 ? 4 : 8;
     p.row_vec = (uintptr_t)e.keys % 16 == 0 && e.head_dim % per == 0 && e.k_sb % per == 0 && e.k_sh % per == 0 && e.k_ss % per == 0;
+    p.vtok = (int64_t)a.enc.batch * a.enc.seq_len > 1024 ? kValTok : 16;
     p.v_vec = a.v && a.v_dtype == a.vp_dtype && a.v_dtype != SSQ_F32 && (uintptr_t)a.v % 16 == 0 && a.value_dim % 8 == 0 &&
               a.v_sb % 8 == 0 && a.v_sh % 8 == 0 && a.v_ss % 8 == 0;
     const int vper = a.vp_dtype == SSQ_F32 ? 4 : 8;
     p.vp_vec = a.v && (uintptr_t)a.v_pages % 16 == 0 && e.page_size % 8 == 0 && a.vp_sb % vper == 0 && a.vp_sh % vper == 0 &&
                a.vp_sd % vper == 0;
     return p;
+}
+
+// the values and the sanitized slots, and the keys' rotation beside them where its unit kernel serves them
+int run_prep(const AppendParams& p, const SsqRopeRows& r, bool turn, unsigned vtiles, hipStream_t st) {
+    RopeParams rp{};
+    rp.r = r;
+    int lpr = 0;
+    int64_t rope_blocks = 0;
+    const bool units = turn && ssq_rope_units_ok(r, lpr);
+    if (units) {
+        rp.lpr = lpr;
+        while ((1 << rp.lpr_log) < lpr) ++rp.lpr_log;
+        rp.groups = (r.heads[0] + 3) / 4;
+        rp.items = (int64_t)r.batch * r.seq_len * rp.groups;
+        rope_blocks = (rp.items * lpr + kThreads - 1) / kThreads;
+    } else if (turn) {
+        int rc = ssq_rope_run(r, st);
+        if (rc) return rc;
+    }
+    const int64_t blocks = rope_blocks + (int64_t)vtiles * p.e.num_kv_heads * (p.dchunks ? p.dchunks : 1);
+    SSQ_UNSUPPORTED(blocks <= 0x7fffffff, "too many rows");
+    const dim3 grid((unsigned)blocks), block(kThreads);
+    const int rb = (int)rope_blocks, vt = (int)vtiles;
+    const bool norm = units && r.w[0];
+    if (!units || r.dtype == SSQ_BF16) {
+        if (norm) hipLaunchKernelGGL((k_append_prep<SSQ_BF16, true>), grid, block, 0, st, p, rp, rb, vt);
+        else hipLaunchKernelGGL((k_append_prep<SSQ_BF16, false>), grid, block, 0, st, p, rp, rb, vt);
+    } else if (r.dtype == SSQ_F16) {
+        if (norm) hipLaunchKernelGGL((k_append_prep<SSQ_F16, true>), grid, block, 0, st, p, rp, rb, vt);
+        else hipLaunchKernelGGL((k_append_prep<SSQ_F16, false>), grid, block, 0, st, p, rp, rb, vt);
+    } else {
+        if (norm) hipLaunchKernelGGL((k_append_prep<SSQ_F32, true>), grid, block, 0, st, p, rp, rb, vt);
+        else hipLaunchKernelGGL((k_append_prep<SSQ_F32, false>), grid, block, 0, st, p, rp, rb, vt);
+    }
+    return ssq_check_hip(hipGetLastError(), "k_append_prep launch");
 }
 
 }  // namespace
@@ -387,7 +468,7 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
     if (n == 0) return SSQ_OK;
     hipStream_t st = (hipStream_t)stream;
     AppendParams p = params(*a);
-    const unsigned vtiles = (unsigned)((n + kValTok - 1) / kValTok);
+    const unsigned vtiles = (unsigned)((n + p.vtok - 1) / p.vtok);
     if (few(*a)) {
         // lanes per key: enough to fill the device, at least 16 codewords each
         const int64_t units = n * e.num_kv_heads * e.n_blocks;
@@ -398,12 +479,15 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
         const int per = kThreads / p.slices;
         const unsigned ktiles = (unsigned)((n + per - 1) / per);
         dim3 grid(ktiles > vtiles ? ktiles : vtiles, e.num_kv_heads, e.n_blocks + p.dchunks);
+        size_t lds = (size_t)p.chunk * (e.block_dim + 1) * 4;
+        const size_t vlds = a->v ? (size_t)p.vtok * val_row(a->vp_dtype == SSQ_F32 ? 4 : 2) : 0;
+        if (vlds > lds) lds = vlds;
         switch (e.block_dim) {
-            case 1: hipLaunchKernelGGL(k_append_few<1>, grid, dim3(kThreads), 0, st, p); break;
-            case 2: hipLaunchKernelGGL(k_append_few<2>, grid, dim3(kThreads), 0, st, p); break;
-            case 4: hipLaunchKernelGGL(k_append_few<4>, grid, dim3(kThreads), 0, st, p); break;
-            case 8: hipLaunchKernelGGL(k_append_few<8>, grid, dim3(kThreads), 0, st, p); break;
-            default: hipLaunchKernelGGL(k_append_few<0>, grid, dim3(kThreads), 0, st, p); break;
+            case 1: hipLaunchKernelGGL(k_append_few<1>, grid, dim3(kThreads), lds, st, p); break;
+            case 2: hipLaunchKernelGGL(k_append_few<2>, grid, dim3(kThreads), lds, st, p); break;
+            case 4: hipLaunchKernelGGL(k_append_few<4>, grid, dim3(kThreads), lds, st, p); break;
+            case 8: hipLaunchKernelGGL(k_append_few<8>, grid, dim3(kThreads), lds, st, p); break;
+            default: hipLaunchKernelGGL(k_append_few<0>, grid, dim3(kThreads), lds, st, p); break;
         }
         return ssq_check_hip(hipGetLastError(), "k_append_few launch");
     }
@@ -412,14 +496,11 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
                 (long long)(rows + n * 8));
     SSQ_REQUIRE((uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");
     p.slots_out = reinterpret_cast<int64_t*>(reinterpret_cast<char*>(workspace) + rows);
-    hipLaunchKernelGGL(k_append_values, dim3(vtiles, e.num_kv_heads, p.dchunks ? p.dchunks : 1), dim3(kThreads), 0, st, p);
-    rc = ssq_check_hip(hipGetLastError(), "k_append_values launch");
-    if (rc) return rc;
     ssq_encode_args enc = e;
     enc.slot_mapping = p.slots_out;
     enc.sm_sb = e.seq_len;
+    SsqRopeRows r{};
     if (turns(*a)) {
-        SsqRopeRows r{};
         r.x[0] = e.keys; r.y[0] = workspace; r.w[0] = a->k_weight; r.heads[0] = e.num_kv_heads;
         r.x_sb[0] = e.k_sb; r.x_sh[0] = e.k_sh; r.x_ss[0] = e.k_ss;
         // token-major, as projections come
@@ -428,10 +509,10 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
         r.y_sb[0] = r.y_ss[0] * e.seq_len;
         r.batch = e.batch; r.seq_len = e.seq_len; r.head_dim = e.head_dim; r.dtype = e.k_dtype;
         r.t = a->rope;
-        rc = ssq_rope_run(r, st);
-        if (rc) return rc;
         enc.keys = workspace;
         enc.k_sb = r.y_sb[0]; enc.k_sh = r.y_sh[0]; enc.k_ss = r.y_ss[0];
     }
+    rc = run_prep(p, r, turns(*a), vtiles, st);
+    if (rc) return rc;
     return ssq_encode(&enc, stream);
 }

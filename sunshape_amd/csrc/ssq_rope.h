@@ -109,7 +109,147 @@ struct SsqRopeRows {
     ssq_rope t;
 };
 
+namespace {
+
+constexpr int kRopeThreads = 256;
+
+struct RopeParams {
+    SsqRopeRows r;
+    int lpr, lpr_log;  // lanes per row, a power of two
+    int groups;        // head groups per token
+    int64_t items;     // tokens * groups
+};
+
+// LDS floats of the weights: two rows of the widest head dim
+template <int DT, bool NORM>
+constexpr int rope_lds() { return NORM ? 4 * RopeVec<DT>::N * SSQ_WAVE : 4; }
+
+// Bytes bound it: every element is read and written once, 7 operations each.  A lane takes a unit of two
+// 16-byte pieces that hold both dims of its pairs ([i, i + V) and [i + rot / 2, ..) of the halves, 2 V
+// consecutive dims when interleaved), so a pair never crosses lanes and only the norm's sum does (within
+// the D / 2V lanes of a row).  A lane keeps its unit for HEADS heads of one token, whose loads are in
+// flight together, with the token's table entries in registers and the weights in LDS.  blk: the workgroup.
+template <int DT, bool NORM, int HEADS>
+__device__ __forceinline__ void rope_units(const RopeParams& p, int64_t blk, float* wl) {
+    constexpr int V = RopeVec<DT>::N, kRow = 2 * V * SSQ_WAVE;
+    const SsqRopeRows& R = p.r;
+    const ssq_rope& t = R.t;
+    const int u = threadIdx.x & (p.lpr - 1);
+    const int64_t item = (blk * kRopeThreads + threadIdx.x) >> p.lpr_log;
+    const bool live = item < p.items;
+    const int64_t it = live ? item : p.items - 1;
+    const int64_t tok = it / p.groups;
+    const int h0 = (int)(it - tok * p.groups) * HEADS;
+    const int b = (int)(tok / R.seq_len), s = (int)(tok - (int64_t)b * R.seq_len);
+    const int H = R.heads[0] + R.heads[1], D = R.head_dim;
+    const int rot = t.cos ? t.rot_dim : 0;
+    // the unit's two pieces
+    const bool turned = u < rot / (2 * V);
+    int o0, o1;
+    if (turned && !t.interleaved) {
+        o0 = u * V;
+        o1 = (rot >> 1) + u * V;
+    } else {  // adjacent pieces: interleaved pairs, or dims past rot (whose units count on from rot's)
+        o0 = 2 * u * V;
+        o1 = o0 + V;
+    }
+    uint4 x0[HEADS], x1[HEADS];
+#pragma unroll
+    for (int k = 0; k < HEADS; ++k) {
+        const int h = min(h0 + k, H - 1);
+        const int j = h >= R.heads[0];
+        const int64_t row = (int64_t)b * R.x_sb[j] + (int64_t)(j ? h - R.heads[0] : h) * R.x_sh[j] + (int64_t)s * R.x_ss[j];
+        const char* src = reinterpret_cast<const char*>(R.x[j]) + row * (16 / V);
+        x0[k] = *reinterpret_cast<const uint4*>(src + o0 * (16 / V));
+        x1[k] = *reinterpret_cast<const uint4*>(src + o1 * (16 / V));
+    }
+    if constexpr (NORM) {
+        for (int i = threadIdx.x; i < 2 * D; i += kRopeThreads) {
+            const int j = i >= D;
+            wl[j * kRow + i - j * D] = R.w[j] ? ssq_load_elem(R.w[j], t.w_dtype, i - j * D) : 0.f;
+        }
+        __syncthreads();
+    }
+    float c[V], sn[V];
+    if (turned) {
+        const int64_t pos = rope_pos(t, b, s);
+        const float* cr = t.cos + (pos < 0 ? 0 : pos) * t.ld + u * V;
+        const float* sr = t.sin + (pos < 0 ? 0 : pos) * t.ld + u * V;
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(cr + i), d = *reinterpret_cast<const float4*>(sr + i);
+            c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
+            sn[i] = d.x; sn[i + 1] = d.y; sn[i + 2] = d.z; sn[i + 3] = d.w;
+        }
+        if (pos < 0) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = sn[i] = __builtin_nanf("");
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < HEADS; ++k) {
+        const int h = min(h0 + k, H - 1);
+        const int j = h >= R.heads[0];
+        float a[V], d[V];
+        rope_unpack<DT>(x0[k], a);
+        rope_unpack<DT>(x1[k], d);
+        if constexpr (NORM) {
+            if (R.w[j]) {  // the same for a whole row, not for a wave: the shuffles stay within a row's lanes
+                double sum = 0.0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    sum = __builtin_fma((double)a[i], (double)a[i], sum);
+                    sum = __builtin_fma((double)d[i], (double)d[i], sum);
+                }
+                for (int o = p.lpr >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+                const float r = rope_rstd(sum, D, t.eps);
+#pragma unroll
+                for (int i = 0; i < V; i += 4) {
+                    const float4 w0 = *reinterpret_cast<const float4*>(&wl[j * kRow + o0 + i]);
+                    const float4 w1 = *reinterpret_cast<const float4*>(&wl[j * kRow + o1 + i]);
+                    a[i] = (a[i] * r) * w0.x; a[i + 1] = (a[i + 1] * r) * w0.y;
+                    a[i + 2] = (a[i + 2] * r) * w0.z; a[i + 3] = (a[i + 3] * r) * w0.w;
+                    d[i] = (d[i] * r) * w1.x; d[i + 1] = (d[i + 1] * r) * w1.y;
+                    d[i + 2] = (d[i + 2] * r) * w1.z; d[i + 3] = (d[i + 3] * r) * w1.w;
+                }
+            }
+        }
+        if (turned) {
+            if (t.interleaved) {
+#pragma unroll
+                for (int i = 0; i < V; i += 2) {
+                    float m = a[i] * c[i >> 1], n = a[i + 1] * sn[i >> 1], q = a[i + 1] * c[i >> 1], e = a[i] * sn[i >> 1];
+                    a[i] = m - n;
+                    a[i + 1] = q + e;
+                    constexpr int W = V / 2;
+                    m = d[i] * c[W + (i >> 1)]; n = d[i + 1] * sn[W + (i >> 1)];
+                    q = d[i + 1] * c[W + (i >> 1)]; e = d[i] * sn[W + (i >> 1)];
+                    d[i] = m - n;
+                    d[i + 1] = q + e;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float m = a[i] * c[i], n = d[i] * sn[i], q = d[i] * c[i], e = a[i] * sn[i];
+                    a[i] = m - n;
+                    d[i] = q + e;
+                }
+            }
+        }
+        if (live && h0 + k < H) {
+            const int64_t row = (int64_t)b * R.y_sb[j] + (int64_t)(j ? h - R.heads[0] : h) * R.y_sh[j] + (int64_t)s * R.y_ss[j];
+            char* dst = reinterpret_cast<char*>(R.y[j]) + row * (16 / V);
+            *reinterpret_cast<uint4*>(dst + o0 * (16 / V)) = rope_packv<DT>(a);
+            *reinterpret_cast<uint4*>(dst + o1 * (16 / V)) = rope_packv<DT>(d);
+        }
+    }
+}
+
+}  // namespace
+
 // argument checks of the rotation (host); the caller has checked head_dim
 int ssq_rope_check(const ssq_rope& t, int head_dim, bool norm);
 // normed and rotated rows, x -> y
 int ssq_rope_run(const SsqRopeRows& r, hipStream_t st);
+// whether the unit kernel serves the rows: whole 16-byte pieces, a power of two of them per row
+bool ssq_rope_units_ok(const SsqRopeRows& r, int& lpr);

@@ -3,9 +3,10 @@
 // rotated keys) and the values' transpose into dim-major pages.
 //
 // Few rows (a decode step): one launch, k_append_few.  A workgroup serves one block of some keys of a KV head:
-// it rotates just that block's dims (and, with a norm, reads the whole row for its sum, from L2 after the first
-// block), keeps the block's codebook in LDS and splits a key's scan over `slices` lanes.  Workgroups past
-// the blocks copy the values.  One chain of loads bounds it, so everything whose address is known is asked for at once.
+// it rotates just that block's dims, keeps the block's codebook in LDS and splits a key's scan over 8 (or 64)
+// lanes.  The first workgroups write the values.  Loads that wait for one another bound it, so the keys' whole
+// rows (which the norm needs anyhow), the codebook, the permutation, slots and positions are all asked for at once,
+// and only the table's and weights' entries after them.
 //
 // Many rows: k_append_prep writes the pages' values and the rotated keys side by side, and ssq_encode, which is
 // where the time goes, takes those.
@@ -30,20 +31,45 @@ struct AppendParams {
     void* vp;
     int64_t v_sb, v_sh, v_ss, vp_sb, vp_sh, vp_sd;
     int v_dtype, vp_dtype, value_dim;
-    int slices;    // lanes per (key, block)
     int chunk;     // codewords per LDS stage
     int row_vec;   // key rows load as 16-byte pieces
     int dchunks;   // value dims in chunks of kValDims
-    int vtok;      // tokens of a value tile: 64, or 16 where there are few
+    int vtok;      // tokens of a value tile
+    int vtiles;    // tiles of tokens
+    int ktiles;    // workgroups per block and KV head (few rows)
+    int krow;      // LDS bytes of a key row (few rows)
+    int page_log;  // log2 of the page size, or -1
+    double inv_d;  // 1 / head_dim
     int v_vec;     // value rows load as 16-byte pieces
     int vp_vec;    // pages take 16-byte stores of 8 (16-bit) or 4 (32-bit) tokens
     int64_t* slots_out;  // sanitized slots (many rows) or NULL
 };
 
-__device__ __forceinline__ int64_t slot_of(const AppendParams& p, int i) {  // -1: nothing is written
-    const int b = i / p.e.seq_len, s = i - b * p.e.seq_len;
+__device__ __forceinline__ int64_t slot_of(const AppendParams& p, int b, int s) {  // -1: nothing is written
     const int64_t slot = p.e.slot_mapping[(int64_t)b * p.e.sm_sb + s];
     return slot >= 0 && slot < p.n_slots ? slot : -1;
+}
+
+// slot = page * page_size + off
+__device__ __forceinline__ void split_slot(const AppendParams& p, int64_t slot, int64_t& page, int& off) {
+    const int size = p.e.page_size;
+    if (p.page_log >= 0) {
+        page = slot >> p.page_log;
+        off = (int)slot & (size - 1);
+    } else if ((uint64_t)slot >> 32 == 0) {
+        const uint32_t q = (uint32_t)slot / (uint32_t)size;
+        page = q;
+        off = (int)((uint32_t)slot - q * (uint32_t)size);
+    } else {
+        page = slot / size;
+        off = (int)(slot - page * size);
+    }
+}
+
+// token i of the batch, [B, S] flat
+__device__ __forceinline__ void split_token(const AppendParams& p, int i, int& b, int& s) {
+    b = p.e.seq_len == 1 ? i : i / p.e.seq_len;
+    s = i - b * p.e.seq_len;
 }
 
 // LDS of a value tile: raw elements of the page dtype, one padding dword per row
@@ -66,17 +92,21 @@ __device__ __forceinline__ void value_tile(const AppendParams& p, unsigned char*
     const int d0 = dc * kValDims, nd = min(kValDims, p.value_dim - d0);
     const int size = p.vp_dtype == SSQ_F32 ? 4 : 2;
     const int row = val_row(size);
-    const int page = a.page_size;
     if (tid < kValTok) {
-        const int64_t slot = tid < nt ? slot_of(p, i0 + tid) : -1;
-        const int64_t pg = slot / page;
-        vs.off[tid] = slot < 0 ? -1 : (int)(slot - pg * page);
-        vs.base[tid] = slot < 0 ? 0 : pg * p.vp_sb + (int64_t)kv * p.vp_sh + (int64_t)d0 * p.vp_sd + (slot - pg * page);
+        int b, s;
+        split_token(p, min(i0 + tid, n - 1), b, s);
+        const int64_t slot = tid < nt ? slot_of(p, b, s) : -1;
+        int64_t pg;
+        int off;
+        split_slot(p, slot < 0 ? 0 : slot, pg, off);
+        vs.off[tid] = slot < 0 ? -1 : off;
+        vs.base[tid] = slot < 0 ? 0 : pg * p.vp_sb + (int64_t)kv * p.vp_sh + (int64_t)d0 * p.vp_sd + off;
         if (p.slots_out && kv == 0 && dc == 0 && tid < nt) p.slots_out[i0 + tid] = slot;
     }
     if (!p.v) return;  // the whole workgroup
     auto vrow = [&](int t) {
-        const int i = i0 + t, b = i / a.seq_len, s = i - b * a.seq_len;
+        int b, s;
+        split_token(p, i0 + t, b, s);
         return (int64_t)b * p.v_sb + (int64_t)kv * p.v_sh + (int64_t)s * p.v_ss + d0;
     };
     if (p.v_vec) {  // same 16-bit dtype: pieces of 8
@@ -160,110 +190,259 @@ __global__ __launch_bounds__(kThreads) void k_append_prep(const AppendParams p, 
     value_tile(p, lds, vs, e - dk * tiles, dk % p.e.num_kv_heads, dk / p.e.num_kv_heads);
 }
 
-// BD: the block dim at compile time (1, 2, 4 or 8), or 0 for any other up to 16.  x: keys (or value tiles),
-// y: KV heads, z: blocks, then value dims.
-template <int BD>
-__global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
-    constexpr int kX = BD ? BD : 16;
-    extern __shared__ __align__(16) unsigned char few_lds[];
-    unsigned char* lds = few_lds;
+// Tokens [4 tile, +4) one by one: where a sequence brings few tokens, no two share a page's 16-byte piece.
+constexpr int kOneTok = 4;
+__device__ __forceinline__ void value_rows(const AppendParams& p, int tile, int kv, int dc) {
     const ssq_encode_args& a = p.e;
-    const int kv = blockIdx.y, blk = blockIdx.z;
+    const int d0 = dc * kValDims, nd = min(kValDims, p.value_dim - d0), d = threadIdx.x & (kValDims - 1);
     const int n = a.batch * a.seq_len;
-    if (blk >= a.n_blocks) {
+    constexpr int kStep = kThreads / kValDims, kSteps = kOneTok / kStep;
+    static_assert(kThreads % kValDims == 0 && kOneTok % kStep == 0, "rows per step");
+    uint32_t w[kSteps];
+    int64_t slot[kSteps];
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        const int i = tile * kOneTok + k * kStep + (int)(threadIdx.x / kValDims);
+        slot[k] = -1;
+        if (i < n && d < nd) {
+            int b, s;
+            split_token(p, i, b, s);
+            slot[k] = slot_of(p, b, s);
+            w[k] = ssq_load_bits(p.v, p.v_dtype, (int64_t)b * p.v_sb + (int64_t)kv * p.v_sh + (int64_t)s * p.v_ss + d0 + d);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        if (slot[k] < 0) continue;
+        int64_t pg;
+        int off;
+        split_slot(p, slot[k], pg, off);
+        const int64_t at = pg * p.vp_sb + (int64_t)kv * p.vp_sh + (int64_t)(d0 + d) * p.vp_sd + off;
+        if (p.v_dtype != p.vp_dtype) rope_store(p.vp, p.vp_dtype, at, ssq_bits_to_f32(w[k], p.v_dtype));
+        else if (p.v_dtype == SSQ_F32) reinterpret_cast<uint32_t*>(p.vp)[at] = w[k];
+        else reinterpret_cast<uint16_t*>(p.vp)[at] = (uint16_t)w[k];
+    }
+}
+
+constexpr int kScan = 16;  // codewords of a lane whose distances are held at once
+
+// Clamped pre-sqrt values v[u] >= 0 of codewords j0 + u stride against the least distance so far: the first codeword
+// with the smallest correctly rounded sqrt wins.  The square roots of all are not taken: the smallest v has the
+// smallest one, and equal ones come from values less than 2^-21 apart relatively (below 2^-126, a few units of the
+// smallest subnormal), so only where a second value lies that close are they compared.  Four operations a
+// codeword, where keeping the first minimum as it goes takes its exact branch at almost every step of
+// so short a scan, in one lane or another.
+__device__ __forceinline__ void first_least(const float (&v)[kScan], uint32_t j0, uint32_t stride, float& f_best, uint32_t& j_best) {
+    float least = v[0];
+#pragma unroll
+    for (int u = 1; u < kScan; ++u) least = __builtin_fminf(least, v[u]);
+    const float f = __builtin_sqrtf(least);
+    if (!(f < f_best)) return;
+    const float near = least * 0x1.00001p+0f + 0x1.0p-146f;
+    int at = 0, n = 0;
+#pragma unroll
+    for (int u = kScan - 1; u >= 0; --u) {
+        const bool c = v[u] <= near;
+        at = c ? u : at;
+        n += c ? 1 : 0;
+    }
+    if (n > 1) {
+#pragma unroll
+        for (int u = kScan - 1; u >= 0; --u)
+            if (v[u] <= near && __builtin_sqrtf(v[u]) == f) at = u;
+    }
+    f_best = f;
+    j_best = j0 + (uint32_t)at * stride;
+}
+
+// A key's row into LDS by its S lanes, and, if asked, its lane's share of the sum of squares.
+template <int DT, int S>
+__device__ __forceinline__ double stage_row(const AppendParams& p, int64_t at, unsigned char* dst, int sl) {
+    constexpr int V = RopeVec<DT>::N, kAhead = 4;
+    const int D = p.e.head_dim;
+    const bool norm = p.kw != nullptr;
+    double sum = 0.0;
+    if (p.row_vec) {
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p.e.keys) + at * (16 / V));
+        const int units = D / V;
+        for (int q0 = sl; q0 < units; q0 += kAhead * S) {
+            uint4 w[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (q0 + k * S < units) w[k] = src[q0 + k * S];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (q0 + k * S >= units) continue;
+                *reinterpret_cast<uint4*>(dst + 16 * (q0 + k * S)) = w[k];
+                if (!norm) continue;
+                float x[V];
+                rope_unpack<DT>(w[k], x);
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum = __builtin_fma((double)x[i], (double)x[i], sum);
+            }
+        }
+    } else {
+        for (int q = sl; q < D; q += S) {
+            const uint32_t w = ssq_load_bits(p.e.keys, DT, at + q);
+            if constexpr (DT == SSQ_F32) reinterpret_cast<uint32_t*>(dst)[q] = w;
+            else reinterpret_cast<uint16_t*>(dst)[q] = (uint16_t)w;
+            const double x = (double)ssq_bits_to_f32(w, DT);
+            sum = __builtin_fma(x, x, sum);
+        }
+    }
+    return sum;
+}
+
+// The dims of one block of a key, normed, rotated and rounded as rope_dim does it, from its row in LDS.
+template <int DT, int N>
+__device__ __forceinline__ void block_dims(const unsigned char* row, const int (&dim)[N], const int (&other)[N],
+                                           const bool (&rot)[N], const bool (&first)[N], bool norm, bool turn, float r,
+                                           const float (&w0)[N], const float (&w1)[N], const float (&cv)[N], const float (&sv)[N],
+                                           float (&x)[N]) {
+    auto elem = [&](int i) {
+        if constexpr (DT == SSQ_F32) return reinterpret_cast<const float*>(row)[i];
+        else return ssq_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[i], DT);
+    };
+#pragma unroll
+    for (int d = 0; d < N; ++d) x[d] = elem(dim[d]);
+    if (norm) {
+#pragma unroll
+        for (int d = 0; d < N; ++d) x[d] = (x[d] * r) * w0[d];
+    }
+    if (turn) {
+#pragma unroll
+        for (int d = 0; d < N; ++d) {
+            float v = elem(other[d]);
+            if (norm) v = (v * r) * w1[d];
+            const float y = x[d] * cv[d], z = v * sv[d], t = first[d] ? y - z : y + z;
+            x[d] = rot[d] ? t : x[d];
+        }
+    }
+    if (norm || turn) {
+#pragma unroll
+        for (int d = 0; d < N; ++d) x[d] = rope_round(x[d], DT);
+    }
+}
+
+// BD: the block dim at compile time (1, 2, 4 or 8), or 0 for any other up to 16; S: lanes of a key.  x: value
+// tiles, then blocks and their tiles of keys; y: KV heads.
+template <int BD, int S>
+__global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
+    constexpr int kX = BD ? BD : 16, kPer = kThreads / S;
+    extern __shared__ __align__(16) unsigned char few_lds[];
+    const ssq_encode_args& a = p.e;
+    const int kv = blockIdx.y, n = a.batch * a.seq_len;
+    int kt = blockIdx.x;
+    if (kt < p.vtiles * p.dchunks) {
         __shared__ ValSlots vs;
-        if ((int)blockIdx.x * p.vtok < n) value_tile(p, lds, vs, blockIdx.x, kv, blk - a.n_blocks);
+        const int dc = kt / p.vtiles, tile = kt - dc * p.vtiles;
+        if (p.vtok == kOneTok) value_rows(p, tile, kv, dc);
+        else value_tile(p, few_lds, vs, tile, kv, dc);
         return;
     }
-    const int S = p.slices, sl = threadIdx.x & (S - 1);
-    const int k0 = blockIdx.x * (kThreads / S);
-    if (k0 >= n) return;  // the whole workgroup
-    const int i = k0 + (int)(threadIdx.x / S);
+    kt -= p.vtiles * p.dchunks;
+    const int blk = kt / p.ktiles;
+    kt -= blk * p.ktiles;
+    const int sl = threadIdx.x & (S - 1), local = (int)threadIdx.x / S, i = kt * kPer + local;
     const bool live = i < n;
     const int bd = BD ? BD : a.block_dim, nc = a.n_centroids, D = a.head_dim;
     const int cw = ssq_code_width(nc);
     const bool heavy = ssq_is_heavy(a.heavy_mask[0], a.heavy_mask[1], blk);
     const float* met = a.metric ? a.metric + (int64_t)kv * a.metric_sh + (int64_t)blk * bd * D + blk * bd : nullptr;
-    const int64_t* perm = a.perm + (int64_t)kv * a.perm_sh + (int64_t)blk * bd;
-    const int ii = live ? i : n - 1;
-    const int b = ii / a.seq_len, s = ii - b * a.seq_len;
-    const int64_t slot = slot_of(p, ii);
-    const int64_t krow = (int64_t)b * a.k_sb + (int64_t)kv * a.k_sh + (int64_t)s * a.k_ss;
-    // the block's dims, their partners, weights and table entries (dims are the same for the whole workgroup)
+    int b, s;
+    split_token(p, live ? i : n - 1, b, s);
     const bool norm = p.kw != nullptr, turn = p.t.cos != nullptr;
+    // LDS: the codebook's stage [chunk][bd] and norms [chunk], then the key rows
+    float* cb = reinterpret_cast<float*>(few_lds);
+    float* cn = cb + (size_t)p.chunk * bd;
+    unsigned char* row = few_lds + (((size_t)p.chunk * (bd + 1) * 4 + 15) & ~(size_t)15) + (size_t)local * p.krow;
+
+    // everything whose address is known
+    const int64_t slot = slot_of(p, b, s);
+    const int64_t pos = turn ? rope_pos(p.t, b, s) : 0;
+    const float* cent = a.cent + (int64_t)kv * a.cent_sh + (int64_t)blk * nc * bd;
+    float c0[kX];
+    const bool mine0 = (int)threadIdx.x < min(p.chunk, nc);
+    if (mine0) {
+#pragma unroll
+        for (int d = 0; d < kX; ++d)
+            if (d < bd) c0[d] = cent[threadIdx.x * bd + d];
+    }
+    const int64_t* perm = a.perm + (int64_t)kv * a.perm_sh + (int64_t)blk * bd;
+    int dim[kX];
+#pragma unroll
+    for (int d = 0; d < kX; ++d) dim[d] = d < bd ? (int)min((uint64_t)perm[d], (uint64_t)(D - 1)) : 0;
+    const int64_t at = (int64_t)b * a.k_sb + (int64_t)kv * a.k_sh + (int64_t)s * a.k_ss;
+    double sum = a.k_dtype == SSQ_BF16  ? stage_row<SSQ_BF16, S>(p, at, row, sl)
+                 : a.k_dtype == SSQ_F16 ? stage_row<SSQ_F16, S>(p, at, row, sl)
+                                        : stage_row<SSQ_F32, S>(p, at, row, sl);
+    // the block's dims, their partners and table entries
     const int half = p.t.rot_dim >> 1;
+    int other[kX];
     bool rot[kX], first[kX];
-    int64_t at[2 * kX], wat[2 * kX];
-    int ti[kX];
+    float cv[kX], sv[kX], w0[kX], w1[kX];
 #pragma unroll
     for (int d = 0; d < kX; ++d) {
-        const int dim = d < bd ? (int)min((uint64_t)perm[d], (uint64_t)(D - 1)) : 0;
-        rot[d] = turn && dim < p.t.rot_dim;
-        first[d] = p.t.interleaved ? !(dim & 1) : dim < half;
-        const int other = !rot[d] ? dim : p.t.interleaved ? dim ^ 1 : first[d] ? dim + half : dim - half;
-        ti[d] = !rot[d] ? 0 : p.t.interleaved ? dim >> 1 : first[d] ? dim : dim - half;
-        at[d] = krow + dim;
-        at[kX + d] = krow + other;
-        wat[d] = dim;
-        wat[kX + d] = other;
+        const int m = dim[d];
+        rot[d] = turn && m < p.t.rot_dim;
+        first[d] = p.t.interleaved ? !(m & 1) : m < half;
+        other[d] = !rot[d] ? m : p.t.interleaved ? m ^ 1 : first[d] ? m + half : m - half;
     }
-    float xr[2 * kX], wv[2 * kX], cv[kX], sv[kX];
-    ssq_load_elems<2 * kX>(a.keys, a.k_dtype, at, xr);
-    const int64_t pos = turn ? rope_pos(p.t, b, s) : 0;
-    if (turn) {  // uniform
-        const int64_t trow = (pos < 0 ? 0 : pos) * p.t.ld;
+    if (turn) {
+        const float* cr = p.t.cos + (pos < 0 ? 0 : pos) * p.t.ld;
+        const float* sr = p.t.sin + (pos < 0 ? 0 : pos) * p.t.ld;
 #pragma unroll
         for (int d = 0; d < kX; ++d) {
-            cv[d] = p.t.cos[trow + ti[d]];
-            sv[d] = p.t.sin[trow + ti[d]];
+            const int ti = !rot[d] ? 0 : p.t.interleaved ? dim[d] >> 1 : min(dim[d], other[d]);
+            cv[d] = cr[ti];
+            sv[d] = sr[ti];
         }
     }
-    float r = 1.f;
-    if (norm) {  // the key's S lanes share the row's sum
-        ssq_load_elems<2 * kX>(p.kw, p.t.w_dtype, wat, wv);
-        double sum = 0.0;
-        if (p.row_vec) {
-            const int per = a.k_dtype == SSQ_F32 ? 4 : 8;
-            const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(a.keys) + krow * (16 / per));
-            for (int q = sl; q < D / per; q += S) {
-                const uint4 w = src[q];
-                if (a.k_dtype == SSQ_F32) {
-                    float x[4];
-                    rope_unpack<SSQ_F32>(w, x);
+    if (norm) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) sum = __builtin_fma((double)x[k], (double)x[k], sum);
-                } else {
-                    float x[8];
-                    if (a.k_dtype == SSQ_BF16) rope_unpack<SSQ_BF16>(w, x);
-                    else rope_unpack<SSQ_F16>(w, x);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) sum = __builtin_fma((double)x[k], (double)x[k], sum);
-                }
-            }
-        } else {
-            for (int q = sl; q < D; q += S) {
-                const double x = (double)ssq_load_elem(a.keys, a.k_dtype, krow + q);
-                sum = __builtin_fma(x, x, sum);
-            }
+        for (int d = 0; d < kX; ++d) {
+            w0[d] = ssq_load_elem(p.kw, p.t.w_dtype, dim[d]);
+            w1[d] = ssq_load_elem(p.kw, p.t.w_dtype, other[d]);
         }
+    }
+    auto map = [&](float (&c)[kX]) {  // into the metric space
+        float y[kX];
+#pragma unroll
+        for (int k = 0; k < kX; ++k)
+            if (k < bd) y[k] = metric_row(met + (int64_t)k * D, c, bd);
+#pragma unroll
+        for (int k = 0; k < kX; ++k)
+            if (k < bd) c[k] = y[k];
+    };
+    auto stage = [&](float (&c)[kX], int e) {
+        if (met) map(c);
+#pragma unroll
+        for (int d = 0; d < kX; ++d)
+            if (d < bd) cb[e * bd + d] = c[d];
+        cn[e] = sq_norm(c, bd);
+    };
+    if (mine0) stage(c0, threadIdx.x);
+    __syncthreads();
+
+    float r = 1.f;
+    if (norm) {  // the key's lanes' shares
+#pragma unroll
         for (int o = S >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        r = rope_rstd(sum, D, p.t.eps);
+        r = rope_rstd(sum, p.inv_d, p.t.eps);
+    }
+    if (turn && pos < 0) {  // a position outside the tables
+#pragma unroll
+        for (int d = 0; d < kX; ++d) cv[d] = sv[d] = __builtin_nanf("");
     }
     float x[kX];
-#pragma unroll
-    for (int d = 0; d < kX; ++d) {  // as rope_dim
-        float u = norm ? (xr[d] * r) * wv[d] : xr[d];
-        if (rot[d]) {
-            const float v = norm ? (xr[kX + d] * r) * wv[kX + d] : xr[kX + d];
-            const float c = pos < 0 ? __builtin_nanf("") : cv[d], sn = pos < 0 ? __builtin_nanf("") : sv[d];
-            const float y = u * c, z = v * sn;
-            u = first[d] ? y - z : y + z;
-        }
-        x[d] = norm || turn ? rope_round(u, a.k_dtype) : u;
-    }
+    if (a.k_dtype == SSQ_BF16) block_dims<SSQ_BF16>(row, dim, other, rot, first, norm, turn, r, w0, w1, cv, sv, x);
+    else if (a.k_dtype == SSQ_F16) block_dims<SSQ_F16>(row, dim, other, rot, first, norm, turn, r, w0, w1, cv, sv, x);
+    else block_dims<SSQ_F32>(row, dim, other, rot, first, norm, turn, r, w0, w1, cv, sv, x);
     int64_t crow = 0, prow = 0;
     if (slot >= 0) {
-        const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
+        int64_t page;
+        int off;
+        split_slot(p, slot, page, off);
         crow = page * a.c_sb + (int64_t)kv * a.c_sh + off * a.c_st;
         prow = page * a.pt_sb + (int64_t)kv * a.pt_sh + off * a.pt_st;
     }
@@ -278,54 +457,46 @@ __global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
         }
         return;
     }
-    auto map = [&](float (&c)[kX]) {  // into the metric space
-        float y[kX];
-#pragma unroll
-        for (int k = 0; k < kX; ++k)
-            if (k < bd) y[k] = metric_row(met + (int64_t)k * D, c, bd);
-#pragma unroll
-        for (int k = 0; k < kX; ++k)
-            if (k < bd) c[k] = y[k];
-    };
     if (met) map(x);
     const float xn = sq_norm(x, bd);
     const bool direct = a.direct_dist != 0;
-    float* cb = reinterpret_cast<float*>(lds);  // [chunk][bd]
-    float* cn = cb + (size_t)p.chunk * bd;      // [chunk]
-    const float* cent = a.cent + (int64_t)kv * a.cent_sh + (int64_t)blk * nc * bd;
-    float e_min = INFINITY;
+    float f_best = INFINITY;
     uint32_t j_best = 0;
     for (int j0 = 0; j0 < nc; j0 += p.chunk) {
         const int m = min(p.chunk, nc - j0);
-        __syncthreads();  // the previous stage's reads are done
-        for (int e = threadIdx.x; e < m; e += kThreads) {
+        // codewords past the first kThreads, and past the first stage
+        if (j0) __syncthreads();  // the previous stage's reads are done
+        for (int e = threadIdx.x + (j0 ? 0 : kThreads); e < m; e += kThreads) {
             float c[kX];
 #pragma unroll
             for (int d = 0; d < kX; ++d)
                 if (d < bd) c[d] = cent[(int64_t)(j0 + e) * bd + d];
-            if (met) map(c);
-#pragma unroll
-            for (int d = 0; d < kX; ++d)
-                if (d < bd) cb[(size_t)e * bd + d] = c[d];
-            cn[e] = sq_norm(c, bd);
+            stage(c, e);
         }
-        __syncthreads();
-        if (direct) {
-            for (int j = sl; j < m; j += S) take_min(direct_dist2(x, cb + (size_t)j * bd, bd), (uint32_t)(j0 + j), e_min, j_best);
-        } else {
-            int j = sl;
-            for (; j + 3 * S < m; j += 4 * S) {  // four codewords' LDS reads in flight
-                float v[4];
+        if (j0 || m > kThreads) __syncthreads();
+        for (int g = 0; g < m; g += kScan * S) {  // the next kScan codewords of each lane
+            float v[kScan];
+            if (!direct && g + kScan * S <= m) {
+                const float* c = cb + (g + sl) * bd;
+                const float* q = cn + g + sl;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = mm_dist2(x, xn, cb + (size_t)(j + u * S) * bd, cn[j + u * S], bd);
+                for (int u = 0; u < kScan; ++u) v[u] = __builtin_fmaxf(mm_dist2(x, xn, c + u * S * bd, q[u * S], bd), 0.f);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < kScan; ++u) {
+                    const int j = g + sl + u * S, jj = min(j, m - 1);
+                    const float* c = cb + jj * bd;
+                    const float y = direct ? direct_dist2(x, c, bd) : mm_dist2(x, xn, c, cn[jj], bd);
+                    // NaN: 0, as clamp_min's
 #pragma unroll
-                for (int u = 0; u < 4; ++u) take_min(v[u], (uint32_t)(j0 + j + u * S), e_min, j_best);
+                    for (int k = 0; k < kScan; ++k) v[k] = k != u ? v[k] : j < m ? __builtin_fmaxf(y, 0.f) : INFINITY;
+                }
             }
-            for (; j < m; j += S) take_min(mm_dist2(x, xn, cb + (size_t)j * bd, cn[j], bd), (uint32_t)(j0 + j), e_min, j_best);
+            first_least(v, (uint32_t)(j0 + g + sl), (uint32_t)S, f_best, j_best);
         }
     }
     // the key's lanes: the smaller distance, then the smaller index
-    float f_best = __builtin_sqrtf(e_min);
+#pragma unroll
     for (int o = S >> 1; o > 0; o >>= 1) {
         const float of = __shfl_xor(f_best, o);
         const uint32_t oj = (uint32_t)__shfl_xor((int)j_best, o);
@@ -395,21 +566,26 @@ int64_t rows_bytes(const ssq_append_args& a) {
 
 AppendParams params(const ssq_append_args& a) {
     AppendParams p{};
-    p.e = a.enc;
+    const ssq_encode_args& e = a.enc;
+    p.e = e;
     p.t = a.rope;
     if (!p.t.cos) p.t.rot_dim = 0;
     p.kw = a.k_weight;
     p.n_slots = a.num_pages * a.enc.page_size;
+    p.page_log = -1;
+    for (int l = 0; l < 31; ++l)
+        if (e.page_size == 1 << l) p.page_log = l;
+    p.inv_d = 1.0 / (double)e.head_dim;
     p.v = a.v;
     p.vp = a.v_pages;
     p.v_sb = a.v_sb; p.v_sh = a.v_sh; p.v_ss = a.v_ss;
     p.vp_sb = a.vp_sb; p.vp_sh = a.vp_sh; p.vp_sd = a.vp_sd;
     p.v_dtype = a.v_dtype; p.vp_dtype = a.vp_dtype; p.value_dim = a.v ? a.value_dim : 0;
     p.dchunks = (p.value_dim + kValDims - 1) / kValDims;
-    const ssq_encode_args& e = a.enc;
     const int per = e.k_dtype == SSQ_F32 ? 4 : 8;
     p.row_vec = (uintptr_t)e.keys % 16 == 0 && e.head_dim % per == 0 && e.k_sb % per == 0 && e.k_sh % per == 0 && e.k_ss % per == 0;
-    p.vtok = (int64_t)a.enc.batch * a.enc.seq_len > 1024 ? kValTok : 16;
+    p.vtok = !few(a) ? kValTok : e.seq_len < 8 ? kOneTok : 16;
+    p.vtiles = (int)(((int64_t)e.batch * e.seq_len + p.vtok - 1) / p.vtok);
     p.v_vec = a.v && a.v_dtype == a.vp_dtype && a.v_dtype != SSQ_F32 && (uintptr_t)a.v % 16 == 0 && a.value_dim % 8 == 0 &&
               a.v_sb % 8 == 0 && a.v_sh % 8 == 0 && a.v_ss % 8 == 0;
     const int vper = a.vp_dtype == SSQ_F32 ? 4 : 8;
@@ -419,7 +595,7 @@ AppendParams params(const ssq_append_args& a) {
 }
 
 // the values and the sanitized slots, and the keys' rotation beside them where its unit kernel serves them
-int run_prep(const AppendParams& p, const SsqRopeRows& r, bool turn, unsigned vtiles, hipStream_t st) {
+int run_prep(const AppendParams& p, const SsqRopeRows& r, bool turn, hipStream_t st) {
     RopeParams rp{};
     rp.r = r;
     int lpr = 0;
@@ -435,10 +611,10 @@ int run_prep(const AppendParams& p, const SsqRopeRows& r, bool turn, unsigned vt
         int rc = ssq_rope_run(r, st);
         if (rc) return rc;
     }
-    const int64_t blocks = rope_blocks + (int64_t)vtiles * p.e.num_kv_heads * (p.dchunks ? p.dchunks : 1);
+    const int64_t blocks = rope_blocks + (int64_t)p.vtiles * p.e.num_kv_heads * (p.dchunks ? p.dchunks : 1);
     SSQ_UNSUPPORTED(blocks <= 0x7fffffff, "too many rows");
     const dim3 grid((unsigned)blocks), block(kThreads);
-    const int rb = (int)rope_blocks, vt = (int)vtiles;
+    const int rb = (int)rope_blocks, vt = p.vtiles;
     const bool norm = units && r.w[0];
     if (!units || r.dtype == SSQ_BF16) {
         if (norm) hipLaunchKernelGGL((k_append_prep<SSQ_BF16, true>), grid, block, 0, st, p, rp, rb, vt);
@@ -451,6 +627,18 @@ int run_prep(const AppendParams& p, const SsqRopeRows& r, bool turn, unsigned vt
         else hipLaunchKernelGGL((k_append_prep<SSQ_F32, false>), grid, block, 0, st, p, rp, rb, vt);
     }
     return ssq_check_hip(hipGetLastError(), "k_append_prep launch");
+}
+
+template <int S>
+int launch_few(const AppendParams& p, dim3 grid, size_t lds, hipStream_t st) {
+    switch (p.e.block_dim) {
+        case 1: hipLaunchKernelGGL((k_append_few<1, S>), grid, dim3(kThreads), lds, st, p); break;
+        case 2: hipLaunchKernelGGL((k_append_few<2, S>), grid, dim3(kThreads), lds, st, p); break;
+        case 4: hipLaunchKernelGGL((k_append_few<4, S>), grid, dim3(kThreads), lds, st, p); break;
+        case 8: hipLaunchKernelGGL((k_append_few<8, S>), grid, dim3(kThreads), lds, st, p); break;
+        default: hipLaunchKernelGGL((k_append_few<0, S>), grid, dim3(kThreads), lds, st, p); break;
+    }
+    return ssq_check_hip(hipGetLastError(), "k_append_few launch");
 }
 
 }  // namespace
@@ -468,28 +656,25 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
     if (n == 0) return SSQ_OK;
     hipStream_t st = (hipStream_t)stream;
     AppendParams p = params(*a);
-    const unsigned vtiles = (unsigned)((n + p.vtok - 1) / p.vtok);
     if (few(*a)) {
-        // lanes per key: enough to fill the device, at least 16 codewords each
+        // 8 lanes a key; a whole wave where the keys are too few for the device and a lane's share of the scan is
+        // long, or 32 rows too large for LDS
         const int64_t units = n * e.num_kv_heads * e.n_blocks;
-        p.slices = 8;
-        while (p.slices < 64 && units * p.slices < (int64_t)ssq_device_cus() * 1024 && p.slices * 16 <= e.n_centroids) p.slices *= 2;
+        const int row = e.head_dim * (e.k_dtype == SSQ_F32 ? 4 : 2);
+        p.krow = ((row + 15) & ~15) + 16;  // rows on other LDS banks
+        const bool wide = (units * 8 < (int64_t)ssq_device_cus() * 256 && e.n_centroids >= 1024) ||
+                          kThreads / 8 * p.krow > 20 * 1024;
         const int stage = kStageFloats / (e.block_dim + 1);
         p.chunk = e.n_centroids < stage ? e.n_centroids : stage;
-        const int per = kThreads / p.slices;
-        const unsigned ktiles = (unsigned)((n + per - 1) / per);
-        dim3 grid(ktiles > vtiles ? ktiles : vtiles, e.num_kv_heads, e.n_blocks + p.dchunks);
-        size_t lds = (size_t)p.chunk * (e.block_dim + 1) * 4;
-        const size_t vlds = a->v ? (size_t)p.vtok * val_row(a->vp_dtype == SSQ_F32 ? 4 : 2) : 0;
+        const int per = kThreads / (wide ? SSQ_WAVE : 8);
+        p.ktiles = (int)((n + per - 1) / per);
+        const int64_t xs = (int64_t)p.vtiles * p.dchunks + (int64_t)p.ktiles * e.n_blocks;
+        SSQ_UNSUPPORTED(xs <= 0x7fffffff, "too many rows");
+        dim3 grid((unsigned)xs, e.num_kv_heads);
+        size_t lds = (((size_t)p.chunk * (e.block_dim + 1) * 4 + 15) & ~(size_t)15) + (size_t)per * p.krow;
+        const size_t vlds = a->v && p.vtok != kOneTok ? (size_t)p.vtok * val_row(a->vp_dtype == SSQ_F32 ? 4 : 2) : 0;
         if (vlds > lds) lds = vlds;
-        switch (e.block_dim) {
-            case 1: hipLaunchKernelGGL(k_append_few<1>, grid, dim3(kThreads), lds, st, p); break;
-            case 2: hipLaunchKernelGGL(k_append_few<2>, grid, dim3(kThreads), lds, st, p); break;
-            case 4: hipLaunchKernelGGL(k_append_few<4>, grid, dim3(kThreads), lds, st, p); break;
-            case 8: hipLaunchKernelGGL(k_append_few<8>, grid, dim3(kThreads), lds, st, p); break;
-            default: hipLaunchKernelGGL(k_append_few<0>, grid, dim3(kThreads), lds, st, p); break;
-        }
-        return ssq_check_hip(hipGetLastError(), "k_append_few launch");
+        return wide ? launch_few<SSQ_WAVE>(p, grid, lds, st) : launch_few<8>(p, grid, lds, st);
     }
     const int64_t rows = rows_bytes(*a);
     SSQ_REQUIRE(workspace && workspace_bytes >= (size_t)(rows + n * 8), "workspace too small: %zu < %lld bytes", workspace_bytes,
@@ -512,7 +697,7 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
         enc.keys = workspace;
         enc.k_sb = r.y_sb[0]; enc.k_sh = r.y_sh[0]; enc.k_ss = r.y_ss[0];
     }
-    rc = run_prep(p, r, turns(*a), vtiles, st);
+    rc = run_prep(p, r, turns(*a), st);
     if (rc) return rc;
     return ssq_encode(&enc, stream);
 }

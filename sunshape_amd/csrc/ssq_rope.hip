@@ -35,7 +35,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_any(const RopeParams p) {
             sum = __builtin_fma(x, x, sum);
         }
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        r = rope_rstd(sum, D, t.eps);
+        r = rope_rstd(sum, 1.0 / (double)D, t.eps);
     }
     const int rot = t.cos ? t.rot_dim : 0;
     const int64_t pos = rot ? rope_pos(t, b, s) : 0;

@@ -18,7 +18,8 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kValTok = 64;    // tokens of a value tile, at most
+constexpr int kValTok = 16;    // tokens of a value tile
+constexpr int kOneTok = 4;     // tokens of a workgroup where they go one by one
 constexpr int kValDims = 128;  // dims of a value tile
 constexpr int kStageFloats = 10 * 1024;  // codebook floats (with norms) per LDS stage
 
@@ -34,8 +35,9 @@ struct AppendParams {
     int chunk;     // codewords per LDS stage
     int row_vec;   // key rows load as 16-byte pieces
     int dchunks;   // value dims in chunks of kValDims
-    int vtok;      // tokens of a value tile
-    int vtiles;    // tiles of tokens
+    int vone;      // value tokens one by one
+    int vseq;      // value tiles per sequence
+    int vtiles;    // value tiles
     int ktiles;    // workgroups per block and KV head (few rows)
     int krow;      // LDS bytes of a key row (few rows)
     int page_log;  // log2 of the page size, or -1
@@ -72,8 +74,10 @@ __device__ __forceinline__ void split_token(const AppendParams& p, int i, int& b
     s = i - b * p.e.seq_len;
 }
 
-// LDS of a value tile: raw elements of the page dtype, one padding dword per row
-__host__ __device__ constexpr int val_row(int size) { return kValDims * size + 4; }
+// LDS row of a value tile: raw elements of the page dtype and 16 bytes, which puts the two groups of 8 tokens on
+// other banks
+__host__ __device__ constexpr int val_row(int size) { return kValDims * size + 16; }
+constexpr int kValLds = kValTok * val_row(4);
 
 // where a token's values go in its head's pages, and its slot within the page (-1: nowhere)
 struct ValSlots {
@@ -81,64 +85,57 @@ struct ValSlots {
     int off[kValTok];
 };
 
-// Tokens [vtok tile, +vtok) (flat over the batch), dims [128 dc, +128) of one KV head: rows in, pages out.  A
-// page holds a dim's tokens side by side, so a run of tokens in consecutive slots of a page that starts on
-// an 8-slot boundary leaves as whole 16-byte pieces; any other token by itself.
+// Up to 16 tokens of a sequence, dims [128 dc, +128) of one KV head: rows in, pages out.  A page holds a dim's tokens
+// side by side, so 8 tokens in consecutive slots of a page from an 8-slot boundary leave as one 16-byte piece, any
+// other token by itself.  Tiles begin where the sequence's first slot, counted on, is a multiple of 16:
+// a prompt into whole pages then has pieces only, and two lanes fill a 16-token page's 32 bytes of a dim.
+// One load and one store a lane: 8,192 tokens of 8 heads of 128 dims took 14.4 us by tiles of 64, which leave
+// the device four workgroups a CU that load together and store together.
 __device__ __forceinline__ void value_tile(const AppendParams& p, unsigned char* lds, ValSlots& vs, int tile, int kv, int dc) {
     const ssq_encode_args& a = p.e;
     const int tid = threadIdx.x;
-    const int n = a.batch * a.seq_len;
-    const int i0 = tile * p.vtok, nt = min(p.vtok, n - i0);
+    const int b = tile / p.vseq, end = (tile - b * p.vseq + 1) * kValTok;
+    const int64_t first = slot_of(p, b, 0);
+    const int s1 = end - (first < 0 ? 0 : (int)first & (kValTok - 1)), s0 = max(s1 - kValTok, 0);
+    const int nt = min(s1, a.seq_len) - s0;
+    if (nt <= 0) return;  // the whole workgroup
     const int d0 = dc * kValDims, nd = min(kValDims, p.value_dim - d0);
     const int size = p.vp_dtype == SSQ_F32 ? 4 : 2;
     const int row = val_row(size);
-    if (tid < kValTok) {
-        int b, s;
-        split_token(p, min(i0 + tid, n - 1), b, s);
-        const int64_t slot = tid < nt ? slot_of(p, b, s) : -1;
+    if (tid < nt) {
+        const int64_t slot = slot_of(p, b, s0 + tid);
         int64_t pg;
         int off;
         split_slot(p, slot < 0 ? 0 : slot, pg, off);
         vs.off[tid] = slot < 0 ? -1 : off;
         vs.base[tid] = slot < 0 ? 0 : pg * p.vp_sb + (int64_t)kv * p.vp_sh + (int64_t)d0 * p.vp_sd + off;
-        if (p.slots_out && kv == 0 && dc == 0 && tid < nt) p.slots_out[i0 + tid] = slot;
+        if (p.slots_out && kv == 0 && dc == 0) p.slots_out[(int64_t)b * a.seq_len + s0 + tid] = slot;
     }
     if (!p.v) return;  // the whole workgroup
-    auto vrow = [&](int t) {
-        int b, s;
-        split_token(p, i0 + t, b, s);
-        return (int64_t)b * p.v_sb + (int64_t)kv * p.v_sh + (int64_t)s * p.v_ss + d0;
-    };
+    const int64_t vrow = (int64_t)b * p.v_sb + (int64_t)kv * p.v_sh + (int64_t)s0 * p.v_ss + d0;
     if (p.v_vec) {  // same 16-bit dtype: pieces of 8
         const int pieces = nd >> 3;
         for (int e = tid; e < nt * pieces; e += kThreads) {
             const int t = e / pieces, q = e - t * pieces;
-            const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.v) + vrow(t) + 8 * q);
-            uint32_t* dst = reinterpret_cast<uint32_t*>(lds + t * row + 16 * q);  // rows are 4-byte aligned
-            dst[0] = w.x; dst[1] = w.y; dst[2] = w.z; dst[3] = w.w;
+            *reinterpret_cast<uint4*>(lds + t * row + 16 * q) =
+                *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.v) + vrow + (int64_t)t * p.v_ss + 8 * q);
         }
     } else {
         for (int e = tid; e < nt * nd; e += kThreads) {
             const int t = e / nd, d = e - t * nd;
+            const int64_t at = vrow + (int64_t)t * p.v_ss + d;
             unsigned char* dst = lds + t * row + d * size;
-            if (p.v_dtype == p.vp_dtype) {
-                if (size == 4) *reinterpret_cast<uint32_t*>(dst) = reinterpret_cast<const uint32_t*>(p.v)[vrow(t) + d];
-                else *reinterpret_cast<uint16_t*>(dst) = reinterpret_cast<const uint16_t*>(p.v)[vrow(t) + d];
-            } else {
-                rope_store(dst, p.vp_dtype, 0, ssq_load_elem(p.v, p.v_dtype, vrow(t) + d));
-            }
+            if (p.v_dtype != p.vp_dtype) rope_store(dst, p.vp_dtype, 0, ssq_load_elem(p.v, p.v_dtype, at));
+            else if (size == 4) *reinterpret_cast<uint32_t*>(dst) = reinterpret_cast<const uint32_t*>(p.v)[at];
+            else *reinterpret_cast<uint16_t*>(dst) = reinterpret_cast<const uint16_t*>(p.v)[at];
         }
     }
     __syncthreads();
-    // groups of 8 tokens, cut so that the first token's run meets 8-slot boundaries
-    const int lead = vs.off[0] < 0 ? 0 : vs.off[0] & 7;
-    const int groups = (nt + lead + 7) >> 3;
-    // lanes: the group's parity fastest (both halves of a 16-token page), then dims
-    for (int e = tid; e < groups * nd; e += kThreads) {
-        const int pair = e / (2 * nd), rest = e - pair * 2 * nd;
-        const bool odd = 2 * pair + 1 >= groups;  // the group without a partner
-        const int g = odd ? 2 * pair : 2 * pair + (rest & 1), d = odd ? rest : rest >> 1;
-        const int ta = max(8 * g - lead, 0), tb = min(8 * g - lead + 8, nt);
+    // both groups of 8 tokens of a dim side by side; a sequence's first tile lacks its first cut tokens
+    const int cut = s0 - (s1 - kValTok);
+    for (int e = tid; e < 2 * nd; e += kThreads) {
+        const int g = e & 1, d = e >> 1;
+        const int ta = max(8 * g - cut, 0), tb = min(8 * g - cut + 8, nt);
         const int64_t dd = (int64_t)d * p.vp_sd;
         bool whole = p.vp_vec && tb - ta == 8 && vs.off[ta] >= 0 && (vs.off[ta] & 7) == 0;
         if (whole) {  // one page: its size is a multiple of 8
@@ -174,24 +171,7 @@ __device__ __forceinline__ void value_tile(const AppendParams& p, unsigned char*
     }
 }
 
-// Many rows: workgroups [0, rope_blocks) rotate the keys, the others write the values (and, for kv 0 and the first
-// dims, the sanitized slots).  They share nothing; one launch lets the values' transposes run beside the rotation.
-template <int DT, bool NORM>
-__global__ __launch_bounds__(kThreads) void k_append_prep(const AppendParams p, const RopeParams rp, int rope_blocks, int tiles) {
-    constexpr int kLds = kValTok * val_row(4) > rope_lds<DT, NORM>() * 4 ? kValTok * val_row(4) : rope_lds<DT, NORM>() * 4;
-    __shared__ __align__(16) unsigned char lds[kLds];
-    __shared__ ValSlots vs;
-    static_assert(kThreads == kRopeThreads, "one block size");
-    if ((int)blockIdx.x < rope_blocks) {
-        rope_units<DT, NORM, 4>(rp, blockIdx.x, reinterpret_cast<float*>(lds));
-        return;
-    }
-    const int e = blockIdx.x - rope_blocks, dk = e / tiles;  // tiles of a KV head side by side
-    value_tile(p, lds, vs, e - dk * tiles, dk % p.e.num_kv_heads, dk / p.e.num_kv_heads);
-}
-
-// Tokens [4 tile, +4) one by one: where a sequence brings few tokens, no two share a page's 16-byte piece.
-constexpr int kOneTok = 4;
+// Tokens [4 tile, +4) one by one: where a sequence brings few tokens, few share a page's 16-byte piece.
 __device__ __forceinline__ void value_rows(const AppendParams& p, int tile, int kv, int dc) {
     const ssq_encode_args& a = p.e;
     const int d0 = dc * kValDims, nd = min(kValDims, p.value_dim - d0), d = threadIdx.x & (kValDims - 1);
@@ -204,11 +184,13 @@ __device__ __forceinline__ void value_rows(const AppendParams& p, int tile, int 
     for (int k = 0; k < kSteps; ++k) {
         const int i = tile * kOneTok + k * kStep + (int)(threadIdx.x / kValDims);
         slot[k] = -1;
-        if (i < n && d < nd) {
+        if (i < n) {
             int b, s;
             split_token(p, i, b, s);
             slot[k] = slot_of(p, b, s);
-            w[k] = ssq_load_bits(p.v, p.v_dtype, (int64_t)b * p.v_sb + (int64_t)kv * p.v_sh + (int64_t)s * p.v_ss + d0 + d);
+            if (p.slots_out && kv == 0 && dc == 0 && d == 0) p.slots_out[i] = slot[k];
+            if (d >= nd || !p.v) slot[k] = -1;
+            else w[k] = ssq_load_bits(p.v, p.v_dtype, (int64_t)b * p.v_sb + (int64_t)kv * p.v_sh + (int64_t)s * p.v_ss + d0 + d);
         }
     }
 #pragma unroll
@@ -222,6 +204,24 @@ __device__ __forceinline__ void value_rows(const AppendParams& p, int tile, int 
         else if (p.v_dtype == SSQ_F32) reinterpret_cast<uint32_t*>(p.vp)[at] = w[k];
         else reinterpret_cast<uint16_t*>(p.vp)[at] = (uint16_t)w[k];
     }
+}
+
+// Many rows: workgroups [0, rope_blocks) rotate the keys, the others write the values (and, for kv 0 and the first
+// dims, the sanitized slots).  They share nothing; one launch lets the values' transposes run beside the rotation.
+template <int DT, bool NORM>
+__global__ __launch_bounds__(kThreads) void k_append_prep(const AppendParams p, const RopeParams rp, int rope_blocks, int tiles) {
+    constexpr int kLds = kValLds > rope_lds<DT, NORM>() * 4 ? kValLds : rope_lds<DT, NORM>() * 4;
+    __shared__ __align__(16) unsigned char lds[kLds];
+    __shared__ ValSlots vs;
+    static_assert(kThreads == kRopeThreads, "one block size");
+    if ((int)blockIdx.x < rope_blocks) {
+        rope_units<DT, NORM, 4>(rp, blockIdx.x, reinterpret_cast<float*>(lds));
+        return;
+    }
+    const int e = blockIdx.x - rope_blocks, dk = e / tiles;  // tiles of a KV head side by side
+    const int dc = dk / p.e.num_kv_heads, kv = dk - dc * p.e.num_kv_heads;
+    if (p.vone) value_rows(p, e - dk * tiles, kv, dc);
+    else value_tile(p, lds, vs, e - dk * tiles, kv, dc);
 }
 
 constexpr int kScan = 16;  // codewords of a lane whose distances are held at once
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
     if (kt < p.vtiles * p.dchunks) {
         __shared__ ValSlots vs;
         const int dc = kt / p.vtiles, tile = kt - dc * p.vtiles;
-        if (p.vtok == kOneTok) value_rows(p, tile, kv, dc);
+        if (p.vone) value_rows(p, tile, kv, dc);
         else value_tile(p, few_lds, vs, tile, kv, dc);
         return;
     }
@@ -547,13 +547,21 @@ int check(const ssq_append_args* a) {
     return SSQ_OK;
 }
 
-// One launch up to about 2^26 (key, block, codeword) triples.
-constexpr int64_t kFewWork = (int64_t)1 << 26;
+// One launch or three?  The few kernel stages a codebook per 32 keys, the others spread it over many; measured, calls
+// in a row, 8 heads of 128 dims, us in one launch and in three:
+//   256 codewords of dim 4: 64 tokens 8.8 and 18.8, 256 17.8 and 20.2, 512 28 and 22.5;  of dim 2: 128 tokens 14.7 and
+//   21.2, 256 23.5 and 21.7;  of dim 8: 256 tokens 16.8 and 22.1, 512 27.4 and 24.7;  4,096 of dim 4: 4 tokens 11.9
+//   and 23.2, 16 29.1 and 31.4, 64 44 and 26
+// -- about 2^24 (key, block, codeword) triples.  Codebooks that ssq_encode serves by its exact scan, whose workgroups
+// take more keys than such calls have, stay to 2^26 and 2^20 rows: 64 codewords of dim 2, 2,048 tokens 254 and 591;
+// 128 of dim 8, 4,096 tokens 137 and 2,147; 16 of dim 4, 4,096 tokens 283 and 253, 2,048 143 and 247.
 bool few(const ssq_append_args& a) {
     const ssq_encode_args& e = a.enc;
     if (e.kernel != 0) return false;
+    const bool scan = e.n_centroids < 256 || e.direct_dist || (e.n_centroids == 256 && e.block_dim > 10);
     const int64_t rows = (int64_t)e.batch * e.seq_len * e.num_kv_heads * e.n_blocks;
-    return rows <= kFewWork && rows * e.n_centroids <= kFewWork;
+    return scan && e.n_centroids <= 256 ? rows <= 1 << 20 && rows * e.n_centroids <= 1 << 26
+                                        : rows <= 1 << 24 && rows * e.n_centroids <= 1 << 24;
 }
 
 bool turns(const ssq_append_args& a) { return a.k_weight || a.rope.cos; }
@@ -584,8 +592,9 @@ AppendParams params(const ssq_append_args& a) {
     p.dchunks = (p.value_dim + kValDims - 1) / kValDims;
     const int per = e.k_dtype == SSQ_F32 ? 4 : 8;
     p.row_vec = (uintptr_t)e.keys % 16 == 0 && e.head_dim % per == 0 && e.k_sb % per == 0 && e.k_sh % per == 0 && e.k_ss % per == 0;
-    p.vtok = !few(a) ? kValTok : e.seq_len < 8 ? kOneTok : 16;
-    p.vtiles = (int)(((int64_t)e.batch * e.seq_len + p.vtok - 1) / p.vtok);
+    p.vone = e.seq_len < 8;
+    p.vseq = (e.seq_len + 2 * (kValTok - 1)) / kValTok;  // a first tile of one token, at worst
+    p.vtiles = p.vone ? (int)(((int64_t)e.batch * e.seq_len + kOneTok - 1) / kOneTok) : e.batch * p.vseq;
     p.v_vec = a.v && a.v_dtype == a.vp_dtype && a.v_dtype != SSQ_F32 && (uintptr_t)a.v % 16 == 0 && a.value_dim % 8 == 0 &&
               a.v_sb % 8 == 0 && a.v_sh % 8 == 0 && a.v_ss % 8 == 0;
     const int vper = a.vp_dtype == SSQ_F32 ? 4 : 8;
@@ -658,7 +667,8 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
     AppendParams p = params(*a);
     if (few(*a)) {
         // 8 lanes a key; a whole wave where the keys are too few for the device and a lane's share of the scan is
-        // long, or 32 rows too large for LDS
+        // long (4,096 codewords, 4 tokens: 11.9 us against 32; 16 tokens 29 and 34, 64 79 and 44; at 256 codewords
+        // 11.8 against 7.4 for one token), or 32 rows too large for LDS
         const int64_t units = n * e.num_kv_heads * e.n_blocks;
         const int row = e.head_dim * (e.k_dtype == SSQ_F32 ? 4 : 2);
         p.krow = ((row + 15) & ~15) + 16;  // rows on other LDS banks
@@ -672,7 +682,7 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
         SSQ_UNSUPPORTED(xs <= 0x7fffffff, "too many rows");
         dim3 grid((unsigned)xs, e.num_kv_heads);
         size_t lds = (((size_t)p.chunk * (e.block_dim + 1) * 4 + 15) & ~(size_t)15) + (size_t)per * p.krow;
-        const size_t vlds = a->v && p.vtok != kOneTok ? (size_t)p.vtok * val_row(a->vp_dtype == SSQ_F32 ? 4 : 2) : 0;
+        const size_t vlds = a->v && !p.vone ? (size_t)kValTok * val_row(a->vp_dtype == SSQ_F32 ? 4 : 2) : 0;
         if (vlds > lds) lds = vlds;
         return wide ? launch_few<SSQ_WAVE>(p, grid, lds, st) : launch_few<8>(p, grid, lds, st);
     }

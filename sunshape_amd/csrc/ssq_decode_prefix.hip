@@ -142,12 +142,20 @@ struct PrefixPlan {
     SsqPrefixParams fp;
 };
 
-// Problems of the matrix-core kernel: pages of whole 16-token pieces, byte codes, codewords of 2, 4 or 8 dims.
+int kept_dims(const ssq_decode_args& d) {
+    return (__builtin_popcountll(d.heavy_mask[0]) + __builtin_popcountll(d.heavy_mask[1])) * d.block_dim;
+}
+
+// Problems of the matrix-core kernel: pages of whole 16-token pieces, byte codes, codewords of 2, 4 or 8 dims, at most
+// half of the dims kept.
 bool fast_shape(const ssq_decode_args& d) {
     if (d.kernel != 0 || (d.head_dim != 64 && d.head_dim != 128) || d.value_dim != d.head_dim) return false;
     if (d.block_dim != 2 && d.block_dim != 4 && d.block_dim != 8) return false;
     if (d.n_centroids > 256 || (d.code_bits != 0 && d.code_bits != 8) || d.page_size % 16) return false;
-    if (d.heavy_mask[0] | d.heavy_mask[1]) return false;
+    if (const int kept = kept_dims(d)) {  // compact rows of whole 16-byte pieces in the values' dtype
+        if (kept > d.head_dim / 2 || kept % 8 || d.pt_dense || d.pt_dtype != d.v_dtype) return false;
+        if ((uintptr_t)d.pt % 16 || d.pt_sb % 8 || d.pt_sh % 8 || d.pt_st % 8) return false;
+    }
     if (d.v_dtype != SSQ_BF16 && d.v_dtype != SSQ_F16) return false;
     if ((uintptr_t)d.cent % 16 || d.cent_sh % 4) return false;
     const int64_t cal = d.n_blocks >= 16 ? 16 : d.n_blocks, unit = d.code_bits ? 4 : 1;  // code rows load in pieces
@@ -176,7 +184,8 @@ void fast_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
     while ((16 << f.psh) < d.page_size) ++f.psh;
     f.q_vec = d.q_dtype != SSQ_F32 && (uintptr_t)d.q % 16 == 0 && d.q_sb % 8 == 0 && d.q_sh % 8 == 0 && d.q_sl % 8 == 0;
     const bool split = !(d.q_dtype == SSQ_BF16 && d.v_dtype == SSQ_BF16) && !(d.q_dtype == SSQ_F16 && d.v_dtype == SSQ_F16);
-    f.pre_nr = split || f.rows <= 32 ? 1 : 2;
+    f.kept = kept_dims(d);
+    f.pre_nr = split || f.kept || f.rows <= 32 ? 1 : 2;  // the others' registers have no room for 64 rows
     f.n_rg = (f.rows + 32 * f.pre_nr - 1) / (32 * f.pre_nr);
     f.own_rg = (per_b + 31) / 32;
     if (a.prefix_cap > 0) {
@@ -222,9 +231,13 @@ int fast_launch(const PrefixPlan& pl, void* workspace, hipStream_t st) {
     f.own = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + pl.pre_bytes);
     const ssq_decode_args& d = f.a;
     if (f.n2) f.own_per = own_per_of(pl, workspace);
-    if (d.q_dtype == SSQ_BF16 && d.v_dtype == SSQ_BF16) return ssq_prefix_bf16(f, st);
-    if (d.q_dtype == SSQ_F16 && d.v_dtype == SSQ_F16) return ssq_prefix_f16(f, st);
-    return d.v_dtype == SSQ_BF16 ? ssq_prefix_split_bf16(f, st) : ssq_prefix_split_f16(f, st);
+    const bool bf = d.v_dtype == SSQ_BF16;
+    if (d.q_dtype != d.v_dtype) {
+        if (f.kept) return bf ? ssq_prefix_split_bf16_mixed(f, st) : ssq_prefix_split_f16_mixed(f, st);
+        return bf ? ssq_prefix_split_bf16(f, st) : ssq_prefix_split_f16(f, st);
+    }
+    if (f.kept) return bf ? ssq_prefix_bf16_mixed(f, st) : ssq_prefix_f16_mixed(f, st);
+    return bf ? ssq_prefix_bf16(f, st) : ssq_prefix_f16(f, st);
 }
 
 // sequences [b0, b0 + n) at query position qi as one sequence of n query rows per head, attending the prefix

@@ -15,6 +15,8 @@
 // codeword is stored as two 16-bit parts, c = hi + lo (the rounding of c, and of what that left: 2^-17 of c at most
 // is dropped, 2^-23 with f16 parts), and each 16 dims take one MFMA with the hi parts and one with the lo parts
 // against the same query operand: the logits keep fp32's quality for half as much matrix-core work again.
+// Kept (passthrough) dims of a SunShape-Mixed codec, up to half of the head's, take a step per 16 more: their codewords are
+// staged as zeros, and a token's kept values, one 16-byte piece a lane and step, are split into parts on the way.
 // Queries of 16 bits enter exactly (QT bf16 / f16); fp32 ones (rotated codecs) in two bf16 parts.
 // Probabilities are rounded to the values' 16 bits for P.V, as in the other decode kernels; sums stay fp32.
 //
@@ -28,6 +30,8 @@
 
 #include "ssq_common.h"
 
+#include <type_traits>
+
 struct SsqPrefixParams {
     ssq_decode_args a;  // own tokens' tables, lengths and mask; everything shared
     const int32_t* ptab;
@@ -40,6 +44,7 @@ struct SsqPrefixParams {
     int own_min;       // the fewest tiles of a piece
     int psh;           // log2(page_size / 16)
     int q_vec;         // 16-bit query rows load in 16-byte pieces
+    int kept;          // dims of the kept blocks, a multiple of 8, at most head_dim / 2
     float* pre;        // o [n1][all rows][Dv], then m, l [n1][all rows]
     float* own;        // likewise for n2
     int* own_per;      // tiles of a piece, chosen by the lengths (written for the merge)
@@ -57,6 +62,10 @@ SSQ_PREFIX_UNIT(ssq_prefix_bf16);        // bf16 queries, bf16 values
 SSQ_PREFIX_UNIT(ssq_prefix_f16);         // f16, f16
 SSQ_PREFIX_UNIT(ssq_prefix_split_bf16);  // fp32 or other queries, bf16 values
 SSQ_PREFIX_UNIT(ssq_prefix_split_f16);
+SSQ_PREFIX_UNIT(ssq_prefix_bf16_mixed);  // with kept blocks
+SSQ_PREFIX_UNIT(ssq_prefix_f16_mixed);
+SSQ_PREFIX_UNIT(ssq_prefix_split_bf16_mixed);
+SSQ_PREFIX_UNIT(ssq_prefix_split_f16_mixed);
 
 namespace {
 
@@ -85,6 +94,15 @@ __device__ __forceinline__ float pf_lo(uint32_t w) { return F16 ? ssq_f16_to_f32
 template <bool F16>
 __device__ __forceinline__ float pf_hi(uint32_t w) { return F16 ? ssq_f16_to_f32(w >> 16) : __uint_as_float(w & 0xFFFF0000u); }
 
+// two fp32 values as packed parts; f16's reach to twice its largest value (log2(e) times a key's largest)
+template <bool F16>
+__device__ __forceinline__ void pf_split(float u, float v, uint32_t& hi, uint32_t& lo) {
+    constexpr float kTop = 65504.f;
+    if constexpr (F16) hi = pf_pack<true>(__builtin_amdgcn_fmed3f(u, -kTop, kTop), __builtin_amdgcn_fmed3f(v, -kTop, kTop));
+    else hi = pf_pack<false>(u, v);
+    lo = pf_pack<F16>(u - pf_lo<F16>(hi), v - pf_hi<F16>(hi));
+}
+
 template <bool F16>
 __device__ __forceinline__ pv16f pf_mfma(const uint4& a, const uint4& b, pv16f c) {
     if constexpr (F16)
@@ -94,7 +112,7 @@ __device__ __forceinline__ pv16f pf_mfma(const uint4& a, const uint4& b, pv16f c
 }
 
 // LDS: codebook [nb]: the codewords' hi parts [256][bd], their lo parts | scratch: staged query rows, then the waves' join |
-// m, l [4][64] | rows' offsets [2][64] | permutation [D]
+// m, l [4][64] | rows' offsets [2][64] | permutation [D] | kept dims' places in it [D / 2]
 template <int D>
 struct PfLds {
     static constexpr int kBook = D * 256 * 4;
@@ -104,11 +122,15 @@ struct PfLds {
     static constexpr int kJoin = kPfWaves * 32 * kJoinRow * 4;
     static constexpr int kScratch = kQ > kJoin ? kQ : kJoin;
     static constexpr int kPerm = kBook + kScratch + 2 * kPfWaves * 64 * 4 + 2 * 64 * 8;
-    static constexpr int kTotal = kPerm + 2 * D;
+    static constexpr int kKept = kPerm + 2 * D;
+    static constexpr int kKeptMax = D / 2;                         // a multiple of 32
+    static constexpr int kTotal = kKept + 2 * kKeptMax;
 };
 
-template <int D, int BD, int QT, int VT, int NR>
+// HV: the codec keeps blocks
+template <int D, int BD, int QT, int VT, int NR, bool HV>
 struct PfRun {
+    using L = PfLds<D>;
     static constexpr bool kF16 = QT == kQtF16;    // parts of the codebook and queries
     static constexpr bool kVF16 = VT == SSQ_F16;  // probabilities and values
     static constexpr int NB = D / BD, NW = NB / 4;
@@ -116,10 +138,18 @@ struct PfRun {
     static constexpr int NQ = D / 16;                    // query operands: 16 dims each
     static constexpr int DT = D / 32;
     static constexpr int QP = QT == kQtSplit ? 2 : 1;
-    using L = PfLds<D>;
+    static constexpr int NK = HV ? L::kKeptMax / 16 : 0;  // steps of kept dims, at most
+    static constexpr bool kKept = HV;
 
     struct Codes { uint32_t w[NW]; };
     struct Vals { uint4 v[2][DT]; };
+    template <int N>
+    struct KeptOf {  // kept dims: queries, and the next tile's values
+        uint4 q[QP][NR][N], v[N];
+        int64_t o, on;  // as pc and pcn
+        const uint16_t* base;
+    };
+    struct None {};
 
     const SsqPrefixParams& p;
     const unsigned char* book;
@@ -135,13 +165,28 @@ struct PfRun {
     const uint8_t* cbase;
     const uint16_t* vbase;
     uint32_t voff, vstep;                       // lane and 32-dim offsets in a page, elements
+    std::conditional_t<HV, KeptOf<NK>, None> kept;
 
-    __device__ __forceinline__ void entries(int i0, int64_t& oc, int64_t& ov) const {
+    __device__ __forceinline__ void entries(int i0, int64_t& oc, int64_t& ov, int64_t& ok) const {
         const int chunk = min(2 * (first + step * (i0 + (lane >> 1))) + (lane & 1), last_chunk);
         const int64_t page = table[chunk >> p.psh];
         const int at = 16 * (chunk & ((1 << p.psh) - 1));
         oc = page * p.a.c_sb + (int64_t)at * p.a.c_st;
         ov = page * p.a.v_sb + at;
+        if constexpr (HV) ok = page * p.a.pt_sb + (int64_t)at * p.a.pt_st;
+    }
+    // this and the next 32 tiles' entries
+    __device__ __forceinline__ void entries_now(int i0) {
+        int64_t ok = 0;
+        entries(i0, pc, pv, ok);
+        pcn = pc;
+        pvn = pv;
+        if constexpr (HV) kept.o = kept.on = ok;
+    }
+    __device__ __forceinline__ void entries_next(int i0) {
+        int64_t ok = 0;
+        entries(i0, pcn, pvn, ok);
+        if constexpr (HV) kept.on = ok;
     }
     __device__ __forceinline__ static int64_t of_lane(int64_t v, int l) {  // uniform
         const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, l);
@@ -162,6 +207,19 @@ struct PfRun {
         } else {
             const uint2 x = *reinterpret_cast<const uint2*>(row);
             r.w[0] = x.x; r.w[1] = x.y;
+        }
+    }
+    __device__ __forceinline__ void load_kept(int i) {
+        if constexpr (HV) {
+            const int64_t o = (i >> 5) == batch ? kept.o : kept.on;
+            const int l = 2 * (i & 31);
+            const int64_t o0 = of_lane(o, l), o1 = of_lane(o, l + 1);
+            const uint16_t* row = kept.base + (lane & 16 ? o1 : o0);
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {  // dims past the last: others, against zeros in q
+                const int d = 16 * k + 8 * half;
+                kept.v[k] = *reinterpret_cast<const uint4*>(row + (d < p.kept ? d : 0));
+            }
         }
     }
     __device__ __forceinline__ const uint16_t* val_row(int i, int c) const {
@@ -208,8 +266,9 @@ struct PfRun {
     }
     // beside(st): work for the vector units next to step st's MFMAs.  The barriers keep each step's gathers and
     // vector work between its MFMAs and the next ones: left alone, the compiler puts one kind after the other.
+    // kept dims: the values asked for before, then those of tile i_kept are.
     template <class Beside>
-    __device__ __forceinline__ void scores(const Codes& c, const Codes& next, pv16f (&s)[NR], Beside beside) {
+    __device__ __forceinline__ void scores(const Codes& c, const Codes& next, int i_kept, pv16f (&s)[NR], Beside beside) {
 #pragma unroll
         for (int st = 0; st < NST; ++st) {
             const uint4 kk = ring[st % kAhead];
@@ -220,6 +279,24 @@ struct PfRun {
             ring[st % kAhead] = st + kAhead < NST ? operand(c, st + kAhead) : operand(next, st + kAhead - NST);
             beside(st);
             __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (HV) {
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                if (16 * k >= p.kept) continue;  // uniform
+                const uint32_t w[4] = {kept.v[k].x, kept.v[k].y, kept.v[k].z, kept.v[k].w};
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pf_split<kF16>(pf_lo<kVF16>(w[e]) * kLog2e, pf_hi<kVF16>(w[e]) * kLog2e, hi[e], lo[e]);
+#pragma unroll
+                for (int h = 0; h < QP; ++h)
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        s[r] = pf_mfma<kF16>(make_uint4(hi[0], hi[1], hi[2], hi[3]), kept.q[h][r][k], s[r]);
+                        s[r] = pf_mfma<kF16>(make_uint4(lo[0], lo[1], lo[2], lo[3]), kept.q[h][r][k], s[r]);
+                    }
+            }
+            load_kept(i_kept);
         }
     }
 };
@@ -297,10 +374,11 @@ __device__ __forceinline__ void pf_tokens(Run& u, int kv, const int32_t* table, 
     u.voff = (uint32_t)(u.lane & 31) * (uint32_t)a.v_st + 8 * u.half;
     u.vstep = 32 * (uint32_t)a.v_st;
     u.batch = 0;
-    u.entries(0, u.pc, u.pv);
-    u.pcn = u.pc;
-    u.pvn = u.pv;
-    if (n > 32) u.entries(32, u.pcn, u.pvn);
+    if constexpr (Run::kKept)
+        u.kept.base = reinterpret_cast<const uint16_t*>(a.pt) + (int64_t)kv * a.pt_sh +
+                      (int64_t)(8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3)) * a.pt_st;
+    u.entries_now(0);
+    if (n > 32) u.entries_next(32);
 }
 
 // Keeps a matrix-core operand in the accumulation registers, which the MFMAs read as well: the compiler otherwise
@@ -324,12 +402,13 @@ template <class Run>
 struct PfFirst {
     typename Run::Codes c1, c2, c3;
     typename Run::Vals val;
-    __device__ __forceinline__ explicit PfFirst(const Run& u) {
+    __device__ __forceinline__ explicit PfFirst(Run& u) {
         if (u.n_tiles > 0) {  // wave-uniform
             u.load_codes(0, c1);
             u.load_codes(min(1, u.n_tiles - 1), c2);
             u.load_codes(min(2, u.n_tiles - 1), c3);
             u.load_vals(0, val);
+            u.load_kept(0);
         }
     }
 };
@@ -404,7 +483,7 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
     };
     float by[NR];
     u.prime(c1);
-    u.scores(c1, c2, s, [](int) {});
+    u.scores(c1, c2, min(1, n - 1), s, [](int) {});
     fix(0);
     raise(by);
     for (int i = 0; i < n; ++i) {
@@ -412,7 +491,8 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
             u.batch = (i >> 5) + 1;
             u.pc = u.pcn;
             u.pv = u.pvn;
-            if (n > 32 * (u.batch + 1)) u.entries(32 * (u.batch + 1), u.pcn, u.pvn);
+            if constexpr (Run::kKept) u.kept.o = u.kept.on;
+            if (n > 32 * (u.batch + 1)) u.entries_next(32 * (u.batch + 1));
         }
         c1 = c2;
         c2 = c3;
@@ -424,7 +504,7 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
 #pragma unroll
         for (int r = 0; r < NR; ++r) lt[r] = 0.f;
         __builtin_amdgcn_sched_barrier(0);
-        u.scores(c1, c2, s2, [&](int st) {
+        u.scores(c1, c2, min(i + 2, n - 1), s2, [&](int st) {
             constexpr int kPer = 16 / Run::NST;
 #pragma unroll
             for (int r = 0; r < NR; ++r)
@@ -492,10 +572,10 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
 // A prefix item: rows [R0, R0 + nr) of the KV head over tiles [t0, t1) of the prefix (len tokens); partials go to
 // slice `split`.  The whole workgroup calls it.  last: the workgroup's last item, after which the codebook's LDS is
 // free for the join.
-template <int D, int BD, int QT, int VT, int NR>
+template <int D, int BD, int QT, int VT, int NR, bool HV>
 __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigned char* lds, int kv, int R0, int nr,
                                                const uint16_t* permL, int len, int t0, int t1, int split, bool last) {
-    using Run = PfRun<D, BD, QT, VT, NR>;
+    using Run = PfRun<D, BD, QT, VT, NR, HV>;
     using L = PfLds<D>;
     const ssq_decode_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
@@ -562,6 +642,19 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
             for (int st = 0; st < Run::NQ; ++st) {
                 u.q[h][r][st] = *reinterpret_cast<const uint4*>(qL + col * L::kQRow + 16 * st + 8 * half);
                 if constexpr (NR == 2) pf_pin(u.q[h][r][st]);
+            }
+            if constexpr (HV) {
+                const uint16_t* keptL = reinterpret_cast<const uint16_t*>(lds + L::kKept);
+#pragma unroll
+                for (int k = 0; k < Run::NK; ++k) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t x = keptL[16 * k + 8 * half + 2 * e], y = keptL[16 * k + 8 * half + 2 * e + 1];
+                        w[e] = (x < D ? qL[col * L::kQRow + x] : 0u) | (y < D ? (uint32_t)qL[col * L::kQRow + y] << 16 : 0u);
+                    }
+                    u.kept.q[h][r][k] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
             }
         }
 
@@ -649,10 +742,10 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
 }
 
 // An own item: rows [R0, R0 + nr) (nr <= 32) of one sequence over tiles [t0, t1) of its own tokens, by one wave.
-template <int D, int BD, int QT, int VT, bool MASK>
+template <int D, int BD, int QT, int VT, bool MASK, bool HV>
 __device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsigned char* book, const uint16_t* permL, int kv,
                                             int R0, int nr, const int32_t* table, int len, int t0, int t1, int split) {
-    using Run = PfRun<D, BD, QT, VT, 1>;
+    using Run = PfRun<D, BD, QT, VT, 1, HV>;
     const ssq_decode_args& a = p.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     Run u{p, book};
@@ -661,7 +754,7 @@ __device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsi
     // query operands straight from memory: a lane's row, its half of every 16 permuted dims, all loads in flight
     const int R = R0 + min(col, nr - 1);
     const int64_t qrow = pf_qrow(p, kv, R);
-    float x[Run::NQ][8];
+    float x[Run::NQ + Run::NK][8];
 #pragma unroll
     for (int st = 0; st < Run::NQ; ++st) {
         const uint4 pw = *reinterpret_cast<const uint4*>(permL + 16 * st + 8 * half);
@@ -669,18 +762,37 @@ __device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsi
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[st][k] = pf_raw<QT>(a, qrow + ((w[k >> 1] >> (16 * (k & 1))) & 0xFFFFu));
     }
+    if constexpr (HV) {
+        const uint16_t* keptL = reinterpret_cast<const uint16_t*>(book + PfLds<D>::kKept);
+#pragma unroll
+        for (int st = 0; st < Run::NK; ++st)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t at = keptL[16 * st + 8 * half + k];
+                x[Run::NQ + st][k] = at < D ? pf_raw<QT>(a, qrow + permL[at]) : 0.f;
+            }
+    }
     const PfFirst<Run> first(u);
     const float scale = a.has_scale ? a.scale : 1.f;
 #pragma unroll
-    for (int st = 0; st < Run::NQ; ++st) {
+    for (int st = 0; st < Run::NQ + Run::NK; ++st) {
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             pf_parts<QT>(a, scale, x[st][2 * k], x[st][2 * k + 1], hi[k], lo[k]);
             if (col >= nr) hi[k] = lo[k] = 0;
         }
-        u.q[0][0][st] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (Run::QP == 2) u.q[1][0][st] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        const uint4 part[2] = {make_uint4(hi[0], hi[1], hi[2], hi[3]), make_uint4(lo[0], lo[1], lo[2], lo[3])};
+#pragma unroll
+        for (int h = 0; h < Run::QP; ++h) {
+            if constexpr (HV) {
+                if (st >= Run::NQ) {
+                    u.kept.q[h][0][st - Run::NQ] = part[h];
+                    continue;
+                }
+            }
+            u.q[h][0][st] = part[h];
+        }
     }
     const float* mrow[1] = {nullptr};
     if constexpr (MASK) {
@@ -725,7 +837,7 @@ __device__ __forceinline__ int pf_scan(int v) {
 // The sequences' own tokens, cut by their lengths (which only the device knows): pieces of `per` tiles, the size that
 // gives every wave of the KV head about one, numbered sequence by sequence; wave v takes pieces v, v + n_waves, ...
 // Every number follows from seq_lens, so all waves agree and a call repeats itself bit for bit.
-template <int D, int BD, int QT, int VT>
+template <int D, int BD, int QT, int VT, bool HV>
 __device__ __forceinline__ void pf_own(const SsqPrefixParams& p, const unsigned char* book, const uint16_t* permL, int kv, int v) {
     const ssq_decode_args& a = p.a;
     const int lane = threadIdx.x & 63;
@@ -766,12 +878,12 @@ __device__ __forceinline__ void pf_own(const SsqPrefixParams& p, const unsigned 
         const int t0 = split * per, t1 = min(t0 + per, __builtin_amdgcn_readlane(t, l));
         const int len = max(0, min(a.seq_lens[b], a.seq_len));
         const int32_t* table = a.block_table + (int64_t)b * a.bt_sb;
-        if (a.mask) pf_own_item<D, BD, QT, VT, true>(p, book, permL, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
-        else pf_own_item<D, BD, QT, VT, false>(p, book, permL, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
+        if (a.mask) pf_own_item<D, BD, QT, VT, true, HV>(p, book, permL, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
+        else pf_own_item<D, BD, QT, VT, false, HV>(p, book, permL, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
     }
 }
 
-template <int D, int BD, int QT, int VT>
+template <int D, int BD, int QT, int VT, bool HV>
 __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams p) {
     extern __shared__ __align__(16) unsigned char pf_lds[];
     using L = PfLds<D>;
@@ -812,15 +924,16 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
             }
 #pragma unroll
             for (int i = 0; i < kIn; ++i) {
-                unsigned char* blk = pf_lds + ((i0 + i + w) & (NB - 1)) * 1024 * BD;
+                const int at = (i0 + i + w) & (NB - 1);
+                const bool zero = HV && ssq_is_heavy(a.heavy_mask[0], a.heavy_mask[1], at);
+                unsigned char* blk = pf_lds + at * 1024 * BD;
 #pragma unroll
                 for (int j = 0; j < kParts; ++j) {
                     uint32_t hi[kV / 2], lo[kV / 2];
 #pragma unroll
                     for (int k = 0; k < kV / 2; ++k) {
-                        const float u = x[i][j][2 * k] * kLog2e, v = x[i][j][2 * k + 1] * kLog2e;
-                        hi[k] = pf_pack<F16>(u, v);
-                        lo[k] = pf_pack<F16>(u - pf_lo<F16>(hi[k]), v - pf_hi<F16>(hi[k]));
+                        pf_split<F16>(x[i][j][2 * k] * kLog2e, x[i][j][2 * k + 1] * kLog2e, hi[k], lo[k]);
+                        if (zero) hi[k] = lo[k] = 0;
                     }
                     // past the last codeword: it again
                     unsigned char* dst = blk + min(tid + j * kPfThreads, nc * kParts - 1) * 2 * kV;
@@ -835,10 +948,18 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
             }
         }
         if (tid < D) permL[tid] = (uint16_t)pj;
+        if constexpr (HV) {  // where kept dim tid is
+            if (tid < L::kKeptMax) {
+                int at = 0xFFFF, left = tid / BD;
+                for (int blk = 0; blk < NB; ++blk)
+                    if (ssq_is_heavy(a.heavy_mask[0], a.heavy_mask[1], blk) && left-- == 0) at = blk * BD + tid % BD;
+                reinterpret_cast<uint16_t*>(pf_lds + L::kKept)[tid] = (uint16_t)at;
+            }
+        }
     }
     __syncthreads();
     // (from the last workgroup down: a small prefix has the first ones)
-    if (p.n2) pf_own<D, BD, QT, VT>(p, pf_lds, permL, kv, (p.n_wg - 1 - w) * kPfWaves + wave);
+    if (p.n2) pf_own<D, BD, QT, VT, HV>(p, pf_lds, permL, kv, (p.n_wg - 1 - w) * kPfWaves + wave);
     // ---- the prefix: slices past its length are not read by the merge either
     const int tiles = ssq_prefix_tiles(plen), per = p.n1 ? ssq_prefix_slice(plen, p.n1) : 0;
     const int n_pre = per ? p.n_rg * ((tiles + per - 1) / per) : 0;
@@ -846,38 +967,38 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
         const int split = it / p.n_rg, rg = it - split * p.n_rg;  // the groups of one slice side by side
         const int R0 = rg * 32 * p.pre_nr, nr = min(32 * p.pre_nr, p.rows - R0);
         const int t0 = split * per, t1 = min(t0 + per, tiles);
-        if constexpr (QT != kQtSplit) {
+        if constexpr (QT != kQtSplit && !HV) {
             if (p.pre_nr == 2) {
-                pf_prefix_item<D, BD, QT, VT, 2>(p, pf_lds, kv, R0, nr, permL, plen, t0, t1, split, it + p.n_wg >= n_pre);
+                pf_prefix_item<D, BD, QT, VT, 2, HV>(p, pf_lds, kv, R0, nr, permL, plen, t0, t1, split, it + p.n_wg >= n_pre);
                 continue;
             }
         }
-        pf_prefix_item<D, BD, QT, VT, 1>(p, pf_lds, kv, R0, nr, permL, plen, t0, t1, split, it + p.n_wg >= n_pre);
+        pf_prefix_item<D, BD, QT, VT, 1, HV>(p, pf_lds, kv, R0, nr, permL, plen, t0, t1, split, it + p.n_wg >= n_pre);
     }
 }
 
-template <int D, int BD, int QT, int VT>
+template <int D, int BD, int QT, int VT, bool HV>
 int launch_prefix(const SsqPrefixParams& p, hipStream_t st) {
-    auto kern = k_prefix<D, BD, QT, VT>;
+    auto kern = k_prefix<D, BD, QT, VT, HV>;
     int rc = ssq_allow_lds((const void*)kern, PfLds<D>::kTotal, "hipFuncSetAttribute(k_prefix)");
     if (rc) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)(p.n_wg * p.a.num_kv_heads)), dim3(kPfThreads), PfLds<D>::kTotal, st, p);
     return ssq_check_hip(hipGetLastError(), "k_prefix launch");
 }
 
-template <int QT, int VT>
+template <int QT, int VT, bool HV>
 int launch_prefix_qv(const SsqPrefixParams& p, hipStream_t st) {
     if (p.a.head_dim == 64) {
         switch (p.a.block_dim) {
-            case 2: return launch_prefix<64, 2, QT, VT>(p, st);
-            case 4: return launch_prefix<64, 4, QT, VT>(p, st);
-            default: return launch_prefix<64, 8, QT, VT>(p, st);
+            case 2: return launch_prefix<64, 2, QT, VT, HV>(p, st);
+            case 4: return launch_prefix<64, 4, QT, VT, HV>(p, st);
+            default: return launch_prefix<64, 8, QT, VT, HV>(p, st);
         }
     }
     switch (p.a.block_dim) {
-        case 2: return launch_prefix<128, 2, QT, VT>(p, st);
-        case 4: return launch_prefix<128, 4, QT, VT>(p, st);
-        default: return launch_prefix<128, 8, QT, VT>(p, st);
+        case 2: return launch_prefix<128, 2, QT, VT, HV>(p, st);
+        case 4: return launch_prefix<128, 4, QT, VT, HV>(p, st);
+        default: return launch_prefix<128, 8, QT, VT, HV>(p, st);
     }
 }
 

@@ -1,3 +1,3 @@
 #include "ssq_prefix_mfma.h"
 
-SSQ_PREFIX_UNIT(ssq_prefix_bf16) { return launch_prefix_qv<kQtBf16, SSQ_BF16>(p, st); }
+SSQ_PREFIX_UNIT(ssq_prefix_bf16) { return launch_prefix_qv<kQtBf16, SSQ_BF16, false>(p, st); }

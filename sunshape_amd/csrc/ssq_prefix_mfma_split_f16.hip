@@ -1,3 +1,3 @@
 #include "ssq_prefix_mfma.h"
 
-SSQ_PREFIX_UNIT(ssq_prefix_split_f16) { return launch_prefix_qv<kQtSplit, SSQ_F16>(p, st); }
+SSQ_PREFIX_UNIT(ssq_prefix_split_f16) { return launch_prefix_qv<kQtSplit, SSQ_F16, false>(p, st); }

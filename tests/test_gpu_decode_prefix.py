@@ -97,6 +97,17 @@ CASES = {
     "shared_codec": dict(B=6, Hq=8, Hkv=4, Lq=1, D=64, Dv=64, bd=4, nc=256, T=100, lens=[20] * 6, per_head=False),
     "mixed": dict(B=6, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=256, T=150, lens=[20] * 6, heavy=(0, 3, 9)),
     "mixed_many": dict(B=3, Hq=4, Hkv=2, Lq=1, D=128, Dv=128, bd=4, nc=256, T=80, lens=[9] * 3, heavy=tuple(range(0, 30, 3))),
+    "mixed_64_8": dict(B=9, Hq=14, Hkv=2, Lq=1, D=64, Dv=64, bd=2, nc=256, T=517, lens=[20, 0, 1, 33] + [64] * 5, heavy=(0, 31, 7, 8)),
+    "mixed_64_16": dict(B=5, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=8, nc=256, T=333, lens=[20, 0, 1, 33, 40], heavy=(1, 6)),
+    "mixed_128_16": dict(B=21, Hq=8, Hkv=2, Lq=1, D=128, Dv=128, bd=4, nc=256, T=1100, lens=[7 * i for i in range(21)], heavy=(0, 5, 6, 31)),
+    "mixed_128_24": dict(B=5, Hq=8, Hkv=2, Lq=1, D=128, Dv=128, bd=8, nc=256, T=130, lens=[20, 0, 1, 33, 40], heavy=(15, 2, 3)),
+    "mixed_128_32": dict(B=5, Hq=32, Hkv=2, Lq=2, D=128, Dv=128, bd=2, nc=64, T=200, lens=[20, 2, 3, 33, 40],
+                         heavy=tuple(range(0, 64, 4)), own_mask="causal"),
+    "mixed_128_40": dict(B=21, Hq=8, Hkv=2, Lq=1, D=128, Dv=128, bd=4, nc=256, T=300, lens=[7 * i for i in range(21)], heavy=tuple(range(1, 31, 3))),
+    "mixed_128_64": dict(B=3, Hq=8, Hkv=2, Lq=1, D=128, Dv=128, bd=8, nc=256, T=130, lens=[20, 0, 101], heavy=tuple(range(8))),
+    "mixed_64_32": dict(B=3, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=256, T=130, lens=[20, 0, 101], heavy=tuple(range(1, 16, 2)), qdt=F16, vdt=F16),
+    "mixed_f16": dict(B=6, Hq=8, Hkv=2, Lq=1, D=128, Dv=128, bd=4, nc=256, T=260, lens=[40] * 6, qdt=F16, vdt=F16, heavy=(3, 4, 30, 31)),
+    "mixed_long": dict(B=2, Hq=4, Hkv=1, Lq=1, D=64, Dv=64, bd=4, nc=256, T=9000, lens=[2500, 3], heavy=(3, 4, 9, 11, 12, 15)),
     "wide": dict(B=4, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=4096, T=300, lens=[33, 2, 0, 70]),
     "wide_32bit": dict(B=2, Hq=2, Hkv=1, Lq=1, D=64, Dv=64, bd=16, nc=65536, T=40, lens=[9, 2]),
     "page8": dict(B=4, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=256, T=77, lens=[11, 8, 0, 9], page=8),
@@ -177,6 +188,47 @@ def test_large_logits():
         p["q"] = p["q"] * f
         out, lse = _call(p)
         _check(p, out, lse, f"queries times {f}")
+
+
+@pytest.mark.parametrize("qdt", [BF, F32])
+def test_kept_blocks_codewords_and_unwritten_tokens(qdt):
+    """A kept block's codewords are not read into the sum, nor what lies behind the lengths in the passthrough."""
+    log(f"decode_prefix: kept blocks, {qdt}")
+    p = _problem(B=6, Hq=8, Hkv=2, Lq=1, D=128, Dv=128, bd=4, nc=256, T=400, lens=[100] * 6, heavy=(2, 9, 17, 18, 30, 31))
+    p["plen"] = torch.tensor([133], dtype=torch.int32)
+    p["lens"] = torch.tensor([0, 1, 15, 16, 17, 99], dtype=torch.int32)
+    used = torch.zeros(p["codes"].shape[0], 16, dtype=torch.bool)
+    for t in range(133):
+        used[p["ptable"][t // 16], t % 16] = True
+    for b in range(6):
+        for t in range(int(p["lens"][b])):
+            used[p["table"][b, t // 16], t % 16] = True
+    p["q"] = p["q"].to(qdt)
+    pt, cent = p["pt"].clone(), p["cent"].clone()
+    pt.permute(0, 2, 1, 3, 4)[~used] = float("nan")
+    cent[:, list(p["heavy"])] = float("nan")
+    for kernel in (0, 1):
+        out, lse = _call(dict(p, pt=pt, cent=cent), kernel=kernel)
+        _check(p, out, lse, f"kept blocks, kernel {kernel}")
+
+
+def test_keys_near_the_largest_f16():
+    """log2(e) times a codeword or a kept value passes what f16 holds from 45,401 on."""
+    log("decode_prefix: large f16 keys")
+    p = _problem(B=5, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=256, T=300, lens=[40, 1, 0, 5, 33], qdt=F16, vdt=F16, heavy=(1, 5))
+    rng = np.random.default_rng(5)
+    p["cent"][:, 3] = torch.from_numpy(rng.choice([-65504.0, 65504.0, 50000.0, -46000.0], p["cent"][:, 3].shape)).float()
+    p["pt"][:, :, :, 0] = torch.from_numpy(rng.choice([-65504.0, 65504.0, 50000.0], tuple(p["pt"][:, :, :, 0].shape))).to(F16)
+    p["q"] = p["q"] * 2.0 ** -12
+    out, lse = _call(p)
+    # past f16's largest value the two parts leave 2^-12 of what the second one holds, less than half as much as the first
+    ref, rlse, mag, pv = prefix_attention64(p["q"], p["scale"], p["perm"], p["cent"], p["codes"], p["v"], p["ptable"],
+                                            int(p["plen"]), p["table"], p["lens"], None, p["pt"], p["mask"])
+    dx = 2.0 ** -13 * mag + 1e-5
+    assert ((lse.cpu().double() - rlse).abs() <= dx).all()
+    half = torch.finfo(F16).eps / 2
+    bound = half * ref.abs() + (2 * dx[..., None] + half + 1e-5) * pv + 2.0 ** -24 * (1 + pv)
+    assert ((out.cpu().double() - ref).abs() <= bound).all()
 
 
 def test_repeats_itself_and_streams():

@@ -152,9 +152,9 @@ bool fast_shape(const ssq_decode_args& d) {
     if (d.kernel != 0 || (d.head_dim != 64 && d.head_dim != 128) || d.value_dim != d.head_dim) return false;
     if (d.block_dim != 2 && d.block_dim != 4 && d.block_dim != 8) return false;
     if (d.n_centroids > 256 || (d.code_bits != 0 && d.code_bits != 8) || d.page_size % 16) return false;
-    if (const int kept = kept_dims(d)) {  // compact rows of whole 16-byte pieces in the values' dtype
-        if (kept > d.head_dim / 2 || kept % 8 || d.pt_dense || d.pt_dtype != d.v_dtype) return false;
-        if ((uintptr_t)d.pt % 16 || d.pt_sb % 8 || d.pt_sh % 8 || d.pt_st % 8) return false;
+    if (const int kept = kept_dims(d)) {  // compact rows of whole 8-byte pieces in the values' dtype
+        if (kept > d.head_dim / 2 || kept % 4 || d.pt_dense || d.pt_dtype != d.v_dtype) return false;
+        if ((uintptr_t)d.pt % 8 || d.pt_sb % 4 || d.pt_sh % 4 || d.pt_st % 4) return false;
     }
     if (d.v_dtype != SSQ_BF16 && d.v_dtype != SSQ_F16) return false;
     if ((uintptr_t)d.cent % 16 || d.cent_sh % 4) return false;

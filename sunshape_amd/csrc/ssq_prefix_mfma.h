@@ -16,7 +16,7 @@
 // is dropped, 2^-23 with f16 parts), and each 16 dims take one MFMA with the hi parts and one with the lo parts
 // against the same query operand: the logits keep fp32's quality for half as much matrix-core work again.
 // Kept (passthrough) dims of a SunShape-Mixed codec, up to half of the head's, take a step per 16 more: their codewords are
-// staged as zeros, and a token's kept values, one 16-byte piece a lane and step, are split into parts on the way.
+// staged as zeros, and a token's kept values, two 8-byte pieces a lane and step, are split into parts on the way.
 // Queries of 16 bits enter exactly (QT bf16 / f16); fp32 ones (rotated codecs) in two bf16 parts.
 // Probabilities are rounded to the values' 16 bits for P.V, as in the other decode kernels; sums stay fp32.
 //
@@ -44,7 +44,7 @@ struct SsqPrefixParams {
     int own_min;       // the fewest tiles of a piece
     int psh;           // log2(page_size / 16)
     int q_vec;         // 16-bit query rows load in 16-byte pieces
-    int kept;          // dims of the kept blocks, a multiple of 8, at most head_dim / 2
+    int kept;          // dims of the kept blocks, a multiple of 4, at most head_dim / 2
     float* pre;        // o [n1][all rows][Dv], then m, l [n1][all rows]
     float* own;        // likewise for n2
     int* own_per;      // tiles of a piece, chosen by the lengths (written for the merge)
@@ -218,7 +218,9 @@ struct PfRun {
 #pragma unroll
             for (int k = 0; k < NK; ++k) {  // dims past the last: others, against zeros in q
                 const int d = 16 * k + 8 * half;
-                kept.v[k] = *reinterpret_cast<const uint4*>(row + (d < p.kept ? d : 0));
+                const uint2 x = *reinterpret_cast<const uint2*>(row + (d < p.kept ? d : 0));
+                const uint2 y = *reinterpret_cast<const uint2*>(row + (d + 4 < p.kept ? d + 4 : 0));
+                kept.v[k] = make_uint4(x.x, x.y, y.x, y.y);
             }
         }
     }

@@ -106,6 +106,8 @@ CASES = {
     "mixed_128_40": dict(B=21, Hq=8, Hkv=2, Lq=1, D=128, Dv=128, bd=4, nc=256, T=300, lens=[7 * i for i in range(21)], heavy=tuple(range(1, 31, 3))),
     "mixed_128_64": dict(B=3, Hq=8, Hkv=2, Lq=1, D=128, Dv=128, bd=8, nc=256, T=130, lens=[20, 0, 101], heavy=tuple(range(8))),
     "mixed_64_32": dict(B=3, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=256, T=130, lens=[20, 0, 101], heavy=tuple(range(1, 16, 2)), qdt=F16, vdt=F16),
+    "mixed_64_4": dict(B=3, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=2, nc=256, T=130, lens=[20, 0, 101], heavy=(4, 30)),
+    "mixed_64_6": dict(B=3, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=2, nc=256, T=130, lens=[20, 0, 101], heavy=(4, 30, 31)),
     "mixed_f16": dict(B=6, Hq=8, Hkv=2, Lq=1, D=128, Dv=128, bd=4, nc=256, T=260, lens=[40] * 6, qdt=F16, vdt=F16, heavy=(3, 4, 30, 31)),
     "mixed_long": dict(B=2, Hq=4, Hkv=1, Lq=1, D=64, Dv=64, bd=4, nc=256, T=9000, lens=[2500, 3], heavy=(3, 4, 9, 11, 12, 15)),
     "wide": dict(B=4, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=4096, T=300, lens=[33, 2, 0, 70]),

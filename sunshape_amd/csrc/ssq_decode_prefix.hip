@@ -5,7 +5,7 @@
 //
 // with (o, m, l) = (sum_t e^{s_t - m} v_t, max_t s_t, sum_t e^{s_t - m}) of a set of tokens.  The prefix is one
 // sequence whose query rows are all sequences' rows of a KV head, so its codes and values are read once for them.
-// Both parts leave fp32 (o, m, l) in the workspace, per context split, and k_merge_prefix joins them.
+// Both parts leave fp32 (o, m, l) in the workspace, per context split, and a merge joins them.
 //
 // Byte-code codecs of head_dim 64 and 128 take the matrix-core kernel (ssq_prefix_mfma.h), one launch for the prefix
 // and the own tokens; every other problem the decode kernels (ssq_decode_partials).
@@ -27,13 +27,8 @@ struct MergeParams {
     ssq_decode_args a;
     // The prefix's partials: for each query position and each chunk of `chunk` sequences a block of
     // n1 (the last chunk n1_last) splits x (num_q_heads * sequences) rows: o, then m, then l.
-    // flat: one block of n1 splits x (batch * num_q_heads * q_len) rows instead, as the own tokens'.
     const float* pre;
-    // (of which those with tokens are read, as the kernel cut them)
-    int chunk, n1, n1_last, flat;
-    const int32_t* plen;
-    int pcap;
-    const int* own_per;
+    int chunk, n1, n1_last;
     // the own tokens' partials, n2 splits x (batch * num_q_heads * q_len) rows (0: none)
     const float* own;
     int n2;
@@ -54,7 +49,7 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
     // this row's prefix block
     int n1 = p.n1;
     int64_t at0 = 0, rows1 = n_rows, row1 = rid;
-    if (p.n1 && !p.flat) {
+    if (p.n1) {
         const int c = b / p.chunk, cn = min(p.chunk, a.batch - c * p.chunk);
         if ((int64_t)(c + 1) * p.chunk >= a.batch) n1 = p.n1_last;
         const int rest = a.batch % p.chunk ? a.batch % p.chunk : p.chunk;
@@ -64,17 +59,7 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
         row1 = (int64_t)h * cn + (b - c * p.chunk);
     }
     const int n1_all = n1;
-    int n2 = p.n2;
-    if (p.flat) {
-        if (n1) {
-            const int len = max(0, min(p.plen[0], p.pcap)), per = ssq_prefix_slice(len, n1);
-            n1 = per ? (ssq_prefix_tiles(len) + per - 1) / per : 0;
-        }
-        if (n2) {
-            const int per = p.own_per[0];
-            n2 = (ssq_prefix_tiles(max(0, min(a.seq_lens[b], a.seq_len))) + per - 1) / per;
-        }
-    }
+    const int n2 = p.n2;
     const float* pre_o = p.pre + at0;
     const float* pre_m = pre_o + rows1 * n1_all * Dv;
     const float* pre_l = pre_m + rows1 * n1_all;
@@ -131,6 +116,127 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
         }
         M = Mr;
         L = Lr;
+    }
+    if (a.lse && lane == 0) a.lse[rid] = M == -INFINITY ? -INFINITY : M + logf(L);
+}
+
+// The same for the matrix-core kernel's partials, n1 prefix slices and n2 own pieces x (batch * num_q_heads * q_len)
+// rows, of which those with tokens are written.  Loads that wait for one another bound it (partials come from
+// other XCDs), so the lengths, every (m, l) and the first few o of both kinds are asked for at once, and what
+// the lengths rule out is dropped after.  Lane j has dims D / 64 j ...
+struct MergeFlat {
+    ssq_decode_args a;
+    const float* pre;
+    const float* own;
+    int n1, n2, pcap;
+    int pair;  // pairs of output dims store as one word
+    const int32_t* plen;
+    const int* own_per;
+};
+
+template <int D>
+__global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_flat(const MergeFlat p) {
+    constexpr int E = D / SSQ_WAVE, kMl = 3;      // n1 <= 128, n2 <= 32
+    constexpr int kAhead = 8, kAheadOwn = 2;      // most sequences have one or two pieces; unwritten ones cost their bytes
+    const ssq_decode_args& a = p.a;
+    const int lane = threadIdx.x & (SSQ_WAVE - 1);
+    const int64_t n_rows = (int64_t)a.batch * a.num_q_heads * a.q_len;
+    const int64_t at_row = (int64_t)blockIdx.x * kMergeRows + __builtin_amdgcn_readfirstlane(threadIdx.x / SSQ_WAVE);
+    if (at_row >= n_rows) return;  // whole waves
+    const int rid = (int)at_row;
+    const int bh = rid / a.q_len, qi = rid - bh * a.q_len, b = bh / a.num_q_heads, h = bh - b * a.num_q_heads;
+    auto o_of = [&](const float* part, int i, float (&o)[E]) {
+        const float* src = part + ((int64_t)i * n_rows + rid) * D + lane * E;
+        if constexpr (E == 2) {
+            const float2 x = *reinterpret_cast<const float2*>(src);
+            o[0] = x.x; o[1] = x.y;
+        } else {
+            o[0] = src[0];
+        }
+    };
+    float m[kMl], l[kMl], o1[kAhead][E], o2[kAheadOwn][E];
+#pragma unroll
+    for (int i = 0; i < kMl; ++i) {
+        const int s = i * SSQ_WAVE + lane, n = s < p.n1 ? p.n1 : p.n2;
+        const float* part = s < p.n1 ? p.pre : p.own;
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+        if (s < p.n1 + p.n2) {
+            const float* src = part + (int64_t)n * n_rows * D + (int64_t)(s < p.n1 ? s : s - p.n1) * n_rows + rid;
+            m[i] = src[0];
+            l[i] = src[(int64_t)n * n_rows];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (i < p.n1) o_of(p.pre, i, o1[i]);  // uniform
+#pragma unroll
+    for (int i = 0; i < kAheadOwn; ++i)
+        if (i < p.n2) o_of(p.own, i, o2[i]);
+    int n1 = 0, n2 = 0;  // those with tokens, as the kernel cut them
+    if (p.n1) {
+        const int len = max(0, min(p.plen[0], p.pcap)), per = ssq_prefix_slice(len, p.n1);
+        n1 = per ? (ssq_prefix_tiles(len) + per - 1) / per : 0;
+    }
+    if (p.n2) {
+        const int per = p.own_per[0];
+        n2 = (ssq_prefix_tiles(max(0, min(a.seq_lens[b], a.seq_len))) + per - 1) / per;
+    }
+    float M = -INFINITY, L = 0.f, w[kMl];
+#pragma unroll
+    for (int i = 0; i < kMl; ++i) {
+        const int s = i * SSQ_WAVE + lane;
+        if (s < p.n1 ? s >= n1 : s - p.n1 >= n2) m[i] = -INFINITY;
+        M = fmaxf(M, m[i]);
+    }
+    M = ssq_wave_max(M);
+#pragma unroll
+    for (int i = 0; i < kMl; ++i) {
+        w[i] = m[i] == -INFINITY ? 0.f : __expf(m[i] - M);
+        L += m[i] == -INFINITY ? 0.f : l[i] * w[i];
+    }
+    L = ssq_wave_sum(L);
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    auto weight = [&](int s) {
+        const float x = s < SSQ_WAVE ? w[0] : s < 2 * SSQ_WAVE ? w[1] : w[2];  // uniform
+        return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), s & (SSQ_WAVE - 1)));
+    };
+    auto add = [&](const float* part, int first, int n, const auto& ahead) {
+        constexpr int kHave = sizeof(ahead) / sizeof(ahead[0]);
+#pragma unroll
+        for (int i = 0; i < kHave; ++i) {
+            const float f = i < n ? weight(first + i) : 0.f;
+            if (f == 0.f) continue;  // uniform
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += ahead[i][e] * f;
+        }
+        for (int i0 = kHave; i0 < n; i0 += kAhead) {
+            float x[kAhead][E];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (i0 + i < n) o_of(part, i0 + i, x[i]);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const float f = i0 + i < n ? weight(first + i0 + i) : 0.f;
+                if (f == 0.f) continue;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] += x[i][e] * f;
+            }
+        }
+    };
+    add(p.pre, 0, n1, o1);
+    add(p.own, p.n1, n2, o2);
+    const int64_t at = (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)qi * a.o_sl + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = M == -INFINITY ? 0.f : o[e] / L;  // a row with nothing to attend gives 0
+    if (E == 2 && p.pair) {
+        const uint32_t x = a.v_dtype == SSQ_BF16 ? pf_pack<false>(o[0], o[E - 1]) : pf_pack<true>(o[0], o[E - 1]);
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + at) = x;
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) ssq_store_elem(a.out, a.v_dtype, at + e, o[e]);
     }
     if (a.lse && lane == 0) a.lse[rid] = M == -INFINITY ? -INFINITY : M + logf(L);
 }
@@ -335,23 +441,34 @@ extern "C" int ssq_decode_prefix(const ssq_prefix_args* a, void* workspace, size
                 pl.pre_bytes + pl.own_bytes);
     SSQ_REQUIRE(workspace || pl.pre_bytes + pl.own_bytes == 0, "workspace is NULL");
     hipStream_t st = (hipStream_t)stream;
+    const float* pre = reinterpret_cast<const float*>(workspace);
+    const float* own = reinterpret_cast<const float*>(reinterpret_cast<char*>(workspace) + pl.pre_bytes);
+    const int64_t rows = (int64_t)d.batch * d.num_q_heads * d.q_len;
+    const dim3 grid((unsigned)((rows + kMergeRows - 1) / kMergeRows)), block(kMergeRows * SSQ_WAVE);
+    if (pl.fast) {
+        if (pl.n1 || pl.n2) rc = fast_launch(pl, workspace, st);
+        if (rc) return rc;
+        MergeFlat m{};
+        m.a = d;
+        m.pre = pre; m.own = own;
+        m.n1 = pl.n1; m.n2 = pl.n2;
+        m.plen = a->prefix_len;
+        m.pcap = a->prefix_cap;
+        m.pair = (uintptr_t)d.out % 4 == 0 && d.o_sb % 2 == 0 && d.o_sh % 2 == 0 && d.o_sl % 2 == 0;
+        if (pl.n2) m.own_per = own_per_of(pl, workspace);
+        if (d.head_dim == 64) hipLaunchKernelGGL(k_merge_flat<64>, grid, block, 0, st, m);
+        else hipLaunchKernelGGL(k_merge_flat<128>, grid, block, 0, st, m);
+        return ssq_check_hip(hipGetLastError(), "k_merge_flat launch");
+    }
     MergeParams m{};
     m.a = d;
-    m.pre = reinterpret_cast<const float*>(workspace);
+    m.pre = pre;
     m.chunk = pl.chunk;
     m.n1 = pl.n1;
     m.n1_last = pl.n1_last;
-    m.own = reinterpret_cast<const float*>(reinterpret_cast<char*>(workspace) + pl.pre_bytes);
+    m.own = own;
     m.n2 = pl.n2;
-    m.flat = pl.fast ? 1 : 0;
-    if (pl.fast) {
-        m.plen = a->prefix_len;
-        m.pcap = a->prefix_cap;
-        if (pl.n2) m.own_per = own_per_of(pl, workspace);
-        if (pl.n1 || pl.n2) rc = fast_launch(pl, workspace, st);
-        if (rc) return rc;
-    }
-    if (pl.n1 && !pl.fast) {
+    if (pl.n1) {
         char* at = reinterpret_cast<char*>(workspace);
         for (int qi = 0; qi < d.q_len; ++qi)
             for (int b0 = 0; b0 < d.batch; b0 += pl.chunk) {
@@ -364,14 +481,13 @@ extern "C" int ssq_decode_prefix(const ssq_prefix_args* a, void* workspace, size
                 at += bytes;
             }
     }
-    if (pl.n2 && !pl.fast) {
+    if (pl.n2) {
         ssq_decode_args own = d;
         own.num_splits = pl.n2;
         own.lse = nullptr;
         rc = ssq_decode_partials(&own, const_cast<float*>(m.own), pl.own_bytes, st);
         if (rc) return rc;
     }
-    const int64_t rows = (int64_t)d.batch * d.num_q_heads * d.q_len;
-    hipLaunchKernelGGL(k_merge_prefix, dim3((unsigned)((rows + kMergeRows - 1) / kMergeRows)), dim3(kMergeRows * SSQ_WAVE), 0, st, m);
+    hipLaunchKernelGGL(k_merge_prefix, grid, block, 0, st, m);
     return ssq_check_hip(hipGetLastError(), "k_merge_prefix launch");
 }

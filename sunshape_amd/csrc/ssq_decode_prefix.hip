@@ -291,20 +291,33 @@ void fast_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
     f.q_vec = d.q_dtype != SSQ_F32 && (uintptr_t)d.q % 16 == 0 && d.q_sb % 8 == 0 && d.q_sh % 8 == 0 && d.q_sl % 8 == 0;
     const bool split = !(d.q_dtype == SSQ_BF16 && d.v_dtype == SSQ_BF16) && !(d.q_dtype == SSQ_F16 && d.v_dtype == SSQ_F16);
     f.kept = kept_dims(d);
-    f.pre_nr = split || f.kept || f.rows <= 32 ? 1 : 2;  // the others' registers have no room for 64 rows
-    f.n_rg = (f.rows + 32 * f.pre_nr - 1) / (32 * f.pre_nr);
     f.own_rg = (per_b + 31) / 32;
+    f.pre_nr = 1;
     if (a.prefix_cap > 0) {
-        // Slices of the prefix: the number that takes the fewest rounds of (4 + tiles of a wave) units: an item's
-        // staging and join cost about as much as 4 tiles.
-        const int tiles = (a.prefix_cap + 31) / 32;
+        // Rows of an item and slices of the prefix: the fewest hundredths of a microsecond by what items measured: 10 us
+        // and 1.35 per tile of a wave with 64 rows, 3 and 0.98 with 32 (twice the gathers, but fewer queries to move
+        // through LDS); and 6 where the prefix's items leave a KV head too few workgroups for its own items, which then
+        // wait for one another.  8 heads of 128 dims, 4 query heads each, 64 own tokens, us with 32 and with 64 rows:
+        // 16 sequences on 4,096 tokens 19.9 and 22.9, on 65,536 55.8 and 49.9; 48 sequences 26.4 and 27.1, 129 and 97.
+        // Workgroups left for the own items or not: 8 sequences on 4,096 tokens 18.6 and 26.0, 48 on 1,000 19.8
+        // and 26.1.  Split queries and kept dims leave no registers for 64 rows.
+        const int most = split || f.kept || f.rows <= 32 ? 1 : 2, tiles = (a.prefix_cap + 31) / 32;
+        const int64_t own_items = d.seq_len > 0 ? (int64_t)d.batch * f.own_rg : 0;
+        const int64_t room = f.n_wg - (own_items + 3) / 4;
         int64_t best = INT64_MAX;
-        for (int n1 = 1; n1 <= 128 && (n1 == 1 || n1 * 4 <= tiles); ++n1) {
-            const int64_t rounds = ((int64_t)f.n_rg * n1 + f.n_wg - 1) / f.n_wg;
-            const int64_t cost = rounds * (4 + ((tiles + n1 - 1) / n1 + 3) / 4);
-            if (cost < best) {
-                best = cost;
-                f.n1 = n1;
+        for (int nr = 1; nr <= most; ++nr) {
+            const int n_rg = (f.rows + 32 * nr - 1) / (32 * nr);
+            for (int n1 = 1; n1 <= 128 && (n1 == 1 || n1 * 4 <= tiles); ++n1) {
+                const int64_t items = (int64_t)n_rg * n1, rounds = (items + f.n_wg - 1) / f.n_wg;
+                const int64_t wave = ((tiles + n1 - 1) / n1 + 3) / 4;
+                const int64_t cost = rounds * (nr == 1 ? 300 + 98 * wave : 1000 + 135 * wave) +
+                                     (own_items && items > room ? 600 : 0);
+                if (cost < best) {
+                    best = cost;
+                    f.pre_nr = nr;
+                    f.n_rg = n_rg;
+                    f.n1 = n1;
+                }
             }
         }
     }

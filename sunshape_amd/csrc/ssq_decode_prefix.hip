@@ -302,7 +302,8 @@ void fast_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
         // Workgroups left for the own items or not: 8 sequences on 4,096 tokens 18.6 and 26.0, 48 on 1,000 19.8
         // and 26.1.  Split queries and kept dims leave no registers for 64 rows.
         const int most = split || f.kept || f.rows <= 32 ? 1 : 2, tiles = (a.prefix_cap + 31) / 32;
-        const int64_t own_items = d.seq_len > 0 ? (int64_t)d.batch * f.own_rg : 0;
+        // pieces of two tiles, of sequences taken to fill half of their tables
+        const int64_t own_items = d.seq_len > 0 ? (int64_t)d.batch * f.own_rg * ((d.seq_len + 127) / 128) : 0;
         const int64_t room = f.n_wg - (own_items + 3) / 4;
         int64_t best = INT64_MAX;
         for (int nr = 1; nr <= most; ++nr) {

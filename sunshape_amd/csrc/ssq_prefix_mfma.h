@@ -26,6 +26,14 @@
 // join in LDS.  An own item is one sequence's rows over a piece of its own tokens, by one wave: no barriers, four
 // such latency chains side by side.  The work of a tile's softmax (VALU) runs beside the next tile's scores
 // (matrix cores).
+//
+// Measured, one MI355X, whole calls with the merge: 128 sequences of 64 query heads (8 KV heads of 128 dims, byte codes of
+// dim 4) on a prefix of 65,536 tokens with up to 1,024 own ones 412 us, 64 sequences of 32 on 32,768 76; attending every
+// sequence's copy of the prefix by itself, 64 on 8,192: 122 against 55.  A tile of 32 tokens and 64 rows takes a wave
+// 1.35 us, where the rate of a large library product (1.39 PFLOP/s) would take 1.16 for its 48 MFMAs, and the MFMAs
+// alone, in this loop, 1.0: the matrix cores bound long prefixes, at 86 % of the rate that they reach.  Of a short one's
+// 50 us, 3 to 4 are the codebook's staging, 3 the queries', 2.5 the first loads, 4 the join, 9 the own
+// items, 8 the merge (a launch of its own).
 #pragma once
 
 #include "ssq_common.h"

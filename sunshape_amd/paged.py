@@ -121,18 +121,12 @@ class PagedSunShapeCache:
         if Hkv != self.num_kv_heads or value_states.shape[:3] != key_states.shape[:3]:
             raise RuntimeError("key/value shapes do not match the cache")
         if cos is not None or k_weight is not None:
+            if len(seq_ids) != B:
+                raise RuntimeError(f"{B} rows of keys for {len(seq_ids)} sequences")
             if len(set(seq_ids)) != len(seq_ids):
                 raise RuntimeError("an append with rotation takes each sequence once")
-            positions = self.positions(seq_ids, S) if cos is not None else None
-            slots = self.slot_mapping(seq_ids, S)
-            hip_ops.append_kv(key_states.to(self.device), value_states.to(self.device), self.codec.effective_permutation(),
-                              self.codec.centroids, codes_out=self.code_pages, v_out=self.v_pages, slot_mapping=slots,
-                              cos=cos, sin=sin, positions=positions, k_weight=k_weight, eps=eps, interleaved=interleaved,
-                              heavy=self.heavy, pt_out=self.pt_pages, metric=self.codec.encode_metric(),
-                              grid=self.codec.encode_search_grid(self.codec.centroids),
-                              direct=hip_ops.cdist_direct(S, self.codec.n_centroids),
-                              rotation=self.codec.rotation_matrix())
-            return slots
+            return self._append_raw(seq_ids, key_states, value_states, self.positions(seq_ids, S) if cos is not None else None,
+                                    cos=cos, sin=sin, k_weight=k_weight, eps=eps, interleaved=interleaved)
         slots = self.slot_mapping(seq_ids, S)
         perm = self.codec.effective_permutation()
         # as quantize_key_states: one reference cdist per (sequence, KV head) over its S new keys
@@ -145,6 +139,17 @@ class PagedSunShapeCache:
         page, off = flat // self.page_size, flat % self.page_size
         vals = value_states.to(self.device, self.v_pages.dtype).permute(0, 2, 1, 3).reshape(B * S, Hkv, self.value_dim)
         self.v_pages[page, :, :, off] = vals
+        return slots
+
+    def _append_raw(self, seq_ids, key_states, value_states, positions, **turn) -> torch.Tensor:
+        S = key_states.shape[2]
+        slots = self.slot_mapping(seq_ids, S)
+        hip_ops.append_kv(key_states.to(self.device), value_states.to(self.device), self.codec.effective_permutation(),
+                          self.codec.centroids, codes_out=self.code_pages, v_out=self.v_pages, slot_mapping=slots,
+                          positions=positions, heavy=self.heavy, pt_out=self.pt_pages, metric=self.codec.encode_metric(),
+                          grid=self.codec.encode_search_grid(self.codec.centroids),
+                          direct=hip_ops.cdist_direct(S, self.codec.n_centroids),
+                          rotation=self.codec.rotation_matrix(), **turn)
         return slots
 
     def tables(self, seq_ids: list[int]) -> tuple[torch.Tensor, torch.Tensor]:
@@ -185,11 +190,15 @@ class PagedSunShapeCache:
         B, _, S, _ = query.shape
         if len(set(seq_ids)) != len(seq_ids):
             raise RuntimeError("attend takes each sequence once")
+        if len(seq_ids) != B or key_states.shape[0] != B or key_states.shape[2] != S:
+            raise RuntimeError("query, keys and values must hold the same new tokens of each sequence")
+        if key_states.shape[1] != self.num_kv_heads or value_states.shape[:3] != key_states.shape[:3]:
+            raise RuntimeError("key/value shapes do not match the cache")
         self._shared_prefix(seq_ids)
-        q, _ = hip_ops.qk_norm_rope(query, None, cos, sin, self.positions(seq_ids, S), q_weight=q_weight, eps=eps,
-                                    interleaved=interleaved)
-        self.append(seq_ids, key_states, value_states, cos=cos, sin=sin, k_weight=k_weight, eps=eps,
-                    interleaved=interleaved)
+        positions = self.positions(seq_ids, S)
+        q, _ = hip_ops.qk_norm_rope(query, None, cos, sin, positions, q_weight=q_weight, eps=eps, interleaved=interleaved)
+        self._append_raw(seq_ids, key_states, value_states, positions, cos=cos, sin=sin, k_weight=k_weight, eps=eps,
+                         interleaved=interleaved)
         mask = None
         if S > 1:  # new token i sees its sequence up to itself
             width = max(len(self.block_tables[s]) for s in seq_ids) * self.page_size

@@ -319,3 +319,78 @@ def test_graph_replays(B, S):
         torch.cuda.synchronize()
         for c, vp in bufs:
             assert torch.equal(c, want[0]) and torch.equal(vp, want[1]), step
+
+
+def _codes_of_append(k, perm, cent, direct, S=1):
+    """Codes [n, nb] of rows k [n, D] appended as they are, by the form that appends take of themselves."""
+    n, D = k.shape
+    nb = cent.shape[1]
+    pages = (n + 15) // 16
+    c = torch.zeros(pages, 1, 16, nb, dtype=hip_ops.index_dtype(cent.shape[2]), device=DEV)
+    hip_ops.append_kv(k.view(n // S, S, 1, D).transpose(1, 2), None, perm, cent, codes_out=c, v_out=None,
+                      slot_mapping=torch.arange(n, device=DEV).view(n // S, S), direct=direct)
+    return c.permute(0, 2, 1, 3).reshape(pages * 16, nb)[:n]
+
+
+@pytest.mark.parametrize("direct", [False, True])
+@pytest.mark.parametrize("bd, nc", [(1, 256), (2, 64), (2, 256), (4, 17), (4, 256), (8, 256), (3, 100), (4, 4096), (16, 1500)])
+def test_ties_and_extremes(bd, nc, direct):
+    """Codewords twice, codewords a step of fp32 apart, distances of zero, subnormal ones, infinities and NaN: the
+    codes are those of the exact scan."""
+    log(f"append_kv ties bd {bd} nc {nc} direct {direct}")
+    rng = np.random.default_rng(bd * 1000 + nc)
+    D = 48 if bd == 3 else 64
+    nb = D // bd
+    base = rng.standard_normal((1, nb, nc, bd)).astype(np.float32)
+    half = nc // 2
+    base[:, :, half:2 * half] = base[:, :, rng.permutation(half)]             # twice
+    base[:, : nb // 2, half:2 * half] *= np.float32(1 + 2.0 ** -23)            # or a step apart
+    cent = torch.from_numpy(base)
+    pick = cent[0][torch.arange(nb), torch.from_numpy(rng.integers(0, nc, (24, nb)))].reshape(24, D)  # on codewords
+    far = torch.from_numpy(rng.standard_normal((24, D)).astype(np.float32)) * 1e4
+    odd = torch.from_numpy(rng.standard_normal((16, D)).astype(np.float32))
+    odd[0], odd[1], odd[2, ::3], odd[3, ::5] = math.nan, math.inf, -math.inf, math.nan
+    odd[4], odd[5] = 0.0, 3e38
+    keys = torch.cat((pick, far, odd))
+    perm = torch.from_numpy(rng.permutation(D))
+    for scale in (1.0, 1e-19, 1e-22):
+        dk, dc, dp = (keys * scale).to(DEV), (cent * scale).to(DEV), perm.to(DEV)
+        want, _ = hip_ops.encode(dk.view(len(keys), 1, 1, D), dp, dc, kernel=1, direct=direct)
+        want = want.view(len(keys), nb)
+        for S in (1, 8):
+            got = _codes_of_append(dk, dp, dc, direct, S)
+            assert torch.equal(got, want), f"scale {scale}, {S} a sequence"
+        half_keys = dk.to(BF)
+        want, _ = hip_ops.encode(half_keys.view(len(keys), 1, 1, D), dp, dc, kernel=1, direct=direct)
+        assert torch.equal(_codes_of_append(half_keys, dp, dc, direct), want.view(len(keys), nb)), f"bf16, scale {scale}"
+
+
+@pytest.mark.parametrize("S, first", [(8, 0), (8, 7), (9, 15), (16, 1), (31, 8), (40, 3), (64, 0), (300, 13)])
+@pytest.mark.parametrize("kernel", [0, 1])
+def test_values_from_any_slot(S, first, kernel):
+    """Runs of slots that begin anywhere in a page, with holes, over pages of 8, 16, 24 and 64 tokens."""
+    log(f"append_kv values, {S} tokens from slot {first}")
+    for page in (8, 16, 24, 64):
+        rng = np.random.default_rng(S + page)
+        B, Hkv, D, Dv = 3, 2, 64, 72
+        per = (S + first) // page + 1
+        table = rng.permutation(B * per + 2)[:B * per].reshape(B, per)
+        at = first + np.arange(S)[None] + np.zeros((B, 1), np.int64)
+        slots = np.take_along_axis(table, at // page, 1) * page + at % page
+        slots[1, 0] = -1
+        slots[2, S // 2] = -1
+        g = torch.Generator().manual_seed(S)
+        k, v = torch.randn(B, S, Hkv, D, generator=g).to(BF), torch.randn(B, S, Hkv, Dv, generator=g).to(BF)
+        perm, cent, _, _ = codec_arrays(rng, Hkv, D, 4, 256)
+        pages = B * per + 2
+        v0 = torch.randn(pages, Hkv, Dv, page, generator=g).to(BF)
+        vp = v0.to(DEV)
+        c = torch.zeros(pages, Hkv, page, 16, dtype=torch.uint8, device=DEV)
+        hip_ops.append_kv(k.to(DEV).transpose(1, 2), v.to(DEV).transpose(1, 2), perm.to(DEV), cent.to(DEV), codes_out=c,
+                          v_out=vp, slot_mapping=torch.from_numpy(slots).to(DEV), kernel=kernel)
+        want = v0.clone()
+        for b in range(B):
+            for s in range(S):
+                if slots[b, s] >= 0:
+                    want[slots[b, s] // page, :, :, slots[b, s] % page] = v[b, s]
+        assert torch.equal(vp.cpu(), want), f"page {page}"

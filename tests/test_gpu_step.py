@@ -151,3 +151,20 @@ def test_fork_rules():
     cache.append([0], k, k)
     cache.free(0)
     assert len(cache._free) == cache.num_pages - 1
+
+
+def test_attend_refusals_leave_the_cache_as_it_was():
+    log("attend: refusals")
+    D, Hq, Hkv = 64, 4, 2
+    cache, _ = _cache(D, Hkv)
+    cos, sin = (t.to(DEV) for t in hip_ops.rope_table(64, D))
+    q, k = torch.randn(2, Hq, 1, D, device=DEV).bfloat16(), torch.randn(2, Hkv, 1, D, device=DEV).bfloat16()
+    before = (list(cache._free), dict(cache.seq_lens))
+    for ids, args in (([1], (q, k, k)), ([1, 1], (q, k, k)), ([1, 2], (q[:1], k, k)), ([1, 2], (q, k[:1], k[:1])),
+                      ([1, 2], (q, k[:, :1], k[:, :1])), ([1, 2], (q, k, k[:1]))):
+        with pytest.raises(RuntimeError):
+            cache.attend(ids, *args, cos=cos, sin=sin)
+    with pytest.raises(RuntimeError):
+        cache.append([1], k, k, cos=cos, sin=sin)
+    assert (list(cache._free), dict(cache.seq_lens)) == before
+    assert torch.isfinite(cache.attend([1, 2], q, k, k, cos=cos, sin=sin).float()).all()

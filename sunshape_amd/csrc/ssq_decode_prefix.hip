@@ -364,7 +364,7 @@ int fast_launch(const PrefixPlan& pl, void* workspace, hipStream_t st) {
 ssq_decode_args prefix_part(const ssq_prefix_args& a, int b0, int n, int qi) {
     ssq_decode_args d = a.dec;
     const int size = d.q_dtype == SSQ_F32 ? 4 : 2;
-    d.q = reinterpret_cast<const char*>(d.q) + ((int64_t)b0 * d.q_sb + (int64_t)qi * d.q_sl) * size;
+    d.q = reinterpret_cast<const void*>((uintptr_t)d.q + (uintptr_t)(((int64_t)b0 * d.q_sb + (int64_t)qi * d.q_sl) * size));
     d.q_sl = d.q_sb;
     d.q_sb = 0;
     d.batch = 1;
@@ -390,7 +390,8 @@ int check(const ssq_prefix_args* a) {
     SSQ_REQUIRE(d.scores == nullptr, "decode with a shared prefix writes no raw scores");
     SSQ_REQUIRE(d.kernel == 0 || d.kernel == 1, "kernel must be 0 or 1");
     SSQ_REQUIRE(d.num_splits == 0, "num_splits must be 0");
-    SSQ_REQUIRE(a->prefix_cap >= 0, "negative prefix_cap");
+    SSQ_REQUIRE(a->prefix_cap >= 0 && a->prefix_cap <= 1 << 30, "prefix_cap must be in [0, 2^30]");
+    SSQ_REQUIRE(d.seq_len <= 1 << 30, "seq_len must be at most 2^30");
     SSQ_REQUIRE(a->prefix_cap == 0 || (a->prefix_table && a->prefix_len), "a prefix needs prefix_table and prefix_len");
     SSQ_REQUIRE((int64_t)d.batch * (d.num_q_heads > 0 ? d.num_q_heads : 1) <= (1 << 24) && d.q_len <= 1 << 16 &&
                     (int64_t)d.batch * d.num_q_heads * d.q_len <= 0x7fffffff,

@@ -131,6 +131,7 @@ extern "C" int ssq_qk_norm_rope(const ssq_rope_args* a, void* stream) {
         return ssq_fail(SSQ_ERR_ABI, "ssq_rope_args size %u != library's %zu", a->struct_size, sizeof(ssq_rope_args));
     SSQ_REQUIRE(a->dtype >= SSQ_F32 && a->dtype <= SSQ_F16, "bad dtype");
     SSQ_REQUIRE(a->batch >= 0 && a->seq_len >= 0 && a->head_dim >= 1 && a->head_dim <= 1024, "bad batch/seq_len/head_dim");
+    SSQ_REQUIRE((int64_t)a->batch * a->seq_len <= 0x7fffffff, "too many tokens");
     SSQ_REQUIRE(a->num_q_heads >= 1 && a->num_k_heads >= 0 && a->num_q_heads + (int64_t)a->num_k_heads <= 1 << 20,
                 "bad head counts");
     SSQ_REQUIRE(a->q && a->q_out, "q and q_out must be non-NULL");

@@ -84,6 +84,7 @@ typedef __bf16 pv2bf __attribute__((ext_vector_type(2)));
 typedef _Float16 pv2h __attribute__((ext_vector_type(2)));
 typedef float pv2f __attribute__((ext_vector_type(2)));
 typedef unsigned int pv4u __attribute__((ext_vector_type(4)));
+typedef unsigned int pv2u __attribute__((ext_vector_type(2)));
 
 constexpr int kPfThreads = 256;
 constexpr int kPfWaves = 4;
@@ -160,8 +161,8 @@ struct PfRun {
     struct None {};
 
     const SsqPrefixParams& p;
-    const unsigned char* book;
     int lane, half;
+    uint32_t lds[2];
     uint4 q[QP][NR][NQ];
     // tokens
     const int32_t* table;
@@ -245,29 +246,40 @@ struct PfRun {
             for (int dt = 0; dt < DT; ++dt) r.v[c][dt] = load_val(val_row(i, c), dt);
     }
     // the K^T operand of step st: dims 16 (st / 2) + 8 half .., the hi parts (st even) or the lo parts.  A gather's
-    // address is code * 2 BD + half's offset, and the step's (a constant, past 64 KiB from a second base).
+    // address is code * 2 BD + a base, and the step's place in the instruction's 16-bit offset: lds[0] is the
+    // codebook and this half's offset, lds[1] 64 KiB further.
+    static constexpr int kPerHalf = 8 / BD, kBlk = 1024 * BD;  // blocks of a half's 8 dims; bytes of a block's tables
+    template <class T>
+    __device__ __forceinline__ T gather(uint32_t code, int at) const {  // at: a constant
+        typedef const __attribute__((address_space(3))) T* Lds;
+        return *(Lds)(code * (2 * BD) + lds[at >> 16] + (at & 0xFFFF));
+    }
+    __device__ __forceinline__ void set_book(const unsigned char* book) {
+        lds[0] = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)book + half * (kPerHalf * kBlk);
+        asm("" : "+v"(lds[0]));  // or the LDS's address is added again for every gather
+        lds[1] = lds[0] + 65536;
+        asm("" : "+v"(lds[1]));
+    }
     __device__ __forceinline__ uint4 operand(const Codes& c, int st) const {
-        const int s2 = st >> 1;
-        constexpr int kPerHalf = 8 / BD, kBlk = 1024 * BD;  // blocks of a half's 8 dims; bytes of a block's tables
-        const unsigned char* at0 = book + s2 * 2 * kPerHalf * kBlk + (st & 1) * (kBlk / 2);
-        const uint32_t hb = (uint32_t)half * (kPerHalf * kBlk);
+        const int s2 = st >> 1, at = s2 * 2 * kPerHalf * kBlk + (st & 1) * (kBlk / 2);
         if constexpr (BD == 8) {
-            const uint32_t code = __builtin_amdgcn_ubfe(c.w[s2 >> 1], 16 * (s2 & 1) + 8 * half, 8);
-            return *reinterpret_cast<const uint4*>(at0 + (code * 16 + hb));
+            const pv4u x = gather<pv4u>(__builtin_amdgcn_ubfe(c.w[s2 >> 1], 16 * (s2 & 1) + 8 * half, 8), at);
+            return make_uint4(x.x, x.y, x.z, x.w);
         } else if constexpr (BD == 4) {
             const uint32_t x = __builtin_amdgcn_ubfe(c.w[s2], 16 * half, 8), y = __builtin_amdgcn_ubfe(c.w[s2], 16 * half + 8, 8);
-            const uint2 u = *reinterpret_cast<const uint2*>(at0 + (x * 8 + hb)), v = *reinterpret_cast<const uint2*>(at0 + kBlk + (y * 8 + hb));
+            const pv2u u = gather<pv2u>(x, at), v = gather<pv2u>(y, at + kBlk);
             return make_uint4(u.x, u.y, v.x, v.y);
         } else {
             const uint32_t w = half ? c.w[2 * s2 + 1] : c.w[2 * s2];
             uint32_t x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint32_t*>(at0 + k * kBlk + (((w >> (8 * k)) & 0xFFu) * 4 + hb));
+            for (int k = 0; k < 4; ++k) x[k] = gather<uint32_t>((w >> (8 * k)) & 0xFFu, at + k * kBlk);
             return make_uint4(x[0], x[1], x[2], x[3]);
         }
     }
-    // kAhead operands are gathered ahead of their MFMAs (more would not fit the registers beside 64 rows),
-    // across the end of a tile into the next one's codes
+    // kAhead operands are gathered ahead of their MFMAs, across the end of a tile into the next one's codes: more do
+    // not fit the registers beside 64 rows, and with 32 rows 8 of them cost more copies than they hide (64 sequences on
+    // 32,768 tokens 81 us for 76)
     static constexpr int kAhead = 4;
     uint4 ring[kAhead];
     __device__ __forceinline__ void prime(const Codes& c) {
@@ -598,8 +610,9 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
     float* mL = reinterpret_cast<float*>(scratch + L::kScratch);  // [4][64]
     float* lL = mL + kPfWaves * 64;
     int64_t* rowL = reinterpret_cast<int64_t*>(lL + kPfWaves * 64);  // query rows' offsets, partial rows
-    Run u{p, lds};
+    Run u{p};
     u.lane = lane; u.half = half;
+    u.set_book(lds);
     pf_tokens(u, kv, p.ptab, len, t0 + wave, kPfWaves, (t1 - t0 - wave + kPfWaves - 1) / kPfWaves);
     const PfFirst<Run> first(u);
 
@@ -758,8 +771,9 @@ __device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsi
     using Run = PfRun<D, BD, QT, VT, 1, HV>;
     const ssq_decode_args& a = p.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
-    Run u{p, book};
+    Run u{p};
     u.lane = lane; u.half = half;
+    u.set_book(book);
     pf_tokens(u, kv, table, len, t0, 1, t1 - t0);
     // query operands straight from memory: a lane's row, its half of every 16 permuted dims, all loads in flight
     const int R = R0 + min(col, nr - 1);
@@ -911,7 +925,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
     {
         constexpr bool F16 = QT == kQtF16;
         constexpr int NB = D / BD, kV = BD < 4 ? BD : 4, kParts = BD / kV;  // floats of a piece, pieces of a codeword
-        constexpr int kIn = NB < 32 / kParts ? NB : 32 / kParts;            // blocks in flight
+        constexpr int kIn = NB < 128 / BD ? NB : 128 / BD;                  // blocks in flight: 128 floats a lane
         const float* cent = a.cent + (int64_t)kv * a.cent_sh;
         const int nc = a.n_centroids;
 #pragma unroll 1

@@ -611,6 +611,7 @@ AppendParams params(const ssq_append_args& a) {
 int run_prep(const AppendParams& p, const SsqRopeRows& r, bool turn, hipStream_t st) {
     RopeParams rp{};
     rp.r = r;
+    rp.inv_d = p.inv_d;
     int lpr = 0;
     int64_t rope_blocks = 0;
     const bool units = turn && ssq_rope_units_ok(r, lpr);

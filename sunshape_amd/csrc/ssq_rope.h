@@ -124,6 +124,7 @@ struct RopeParams {
     int lpr, lpr_log;  // lanes per row, a power of two
     int groups;        // head groups per token
     int64_t items;     // tokens * groups
+    double inv_d;      // 1 / head_dim
 };
 
 // LDS floats of the weights: two rows of the widest head dim
@@ -176,7 +177,6 @@ __device__ __forceinline__ void rope_units(const RopeParams& p, int64_t blk, flo
         }
         __syncthreads();
     }
-    const double inv_d = 1.0 / (double)D;
     float c[V], sn[V];
     if (turned) {
         const int64_t pos = rope_pos(t, b, s);
@@ -209,7 +209,7 @@ __device__ __forceinline__ void rope_units(const RopeParams& p, int64_t blk, flo
                     sum = __builtin_fma((double)d[i], (double)d[i], sum);
                 }
                 for (int o = p.lpr >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-                const float r = rope_rstd(sum, inv_d, t.eps);
+                const float r = rope_rstd(sum, p.inv_d, t.eps);
 #pragma unroll
                 for (int i = 0; i < V; i += 4) {
                     const float4 w0 = *reinterpret_cast<const float4*>(&wl[j * kRow + o0 + i]);

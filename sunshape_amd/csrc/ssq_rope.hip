@@ -35,7 +35,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_any(const RopeParams p) {
             sum = __builtin_fma(x, x, sum);
         }
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        r = rope_rstd(sum, 1.0 / (double)D, t.eps);
+        r = rope_rstd(sum, p.inv_d, t.eps);
     }
     const int rot = t.cos ? t.rot_dim : 0;
     const int64_t pos = rot ? rope_pos(t, b, s) : 0;
@@ -101,6 +101,7 @@ int ssq_rope_check(const ssq_rope& t, int head_dim, bool norm) {
 int ssq_rope_run(const SsqRopeRows& r, hipStream_t st) {
     RopeParams p{};
     p.r = r;
+    p.inv_d = 1.0 / (double)r.head_dim;
     const int64_t tokens = (int64_t)r.batch * r.seq_len;
     const int H = r.heads[0] + r.heads[1];
     if (tokens == 0 || H == 0) return SSQ_OK;
@@ -113,8 +114,10 @@ int ssq_rope_run(const SsqRopeRows& r, hipStream_t st) {
     }
     p.lpr = lpr;
     while ((1 << p.lpr_log) < lpr) ++p.lpr_log;
-    // one head per lane while the rows leave lanes idle (latency is what counts there), else four
-    const bool many = tokens * H * lpr >= (int64_t)ssq_device_cus() * 2048;
+    // One head per lane while the rows leave lanes idle (latency is what counts there), else four, which read a token's
+    // table entries once: 40 heads of 128 dims in bf16, us with one and with four: 64 tokens 3.6 and 6.0, 2,048 11.3
+    // and 11.9, 4,096 19.9 and 20.1, 8,192 35.2 and 33.6; fp32, 512 6.3 and 7.5, 2,048 18.3 and 16.4
+    const bool many = tokens * H * lpr >= (int64_t)ssq_device_cus() * 4096;
     p.groups = many ? (H + 3) / 4 : H;
     p.items = tokens * p.groups;
     const int64_t blocks = (p.items * lpr + kRopeThreads - 1) / kRopeThreads;

@@ -193,3 +193,24 @@ def test_graph_replays_and_side_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("dt, D, rot, inter, norm", [(BF, 128, 128, False, True), (BF, 64, 32, True, False), (F16, 128, 64, True, True),
+                                                     (F32, 128, 128, False, True), (BF, 256, 256, False, True)])
+def test_many_rows_are_the_rows_by_themselves(dt, D, rot, inter, norm):
+    """Many rows (four heads a lane, head counts that four does not divide) and the same tokens a few at a time."""
+    log(f"rope, many rows {dt} {D} {rot} {inter} {norm}")
+    Hq, Hkv = 11, 3
+    lanes = D // (8 if dt == F32 else 16)
+    S = -(-256 * 4096 // ((Hq + Hkv) * lanes)) + 5  # past 4,096 lanes a CU
+    g = torch.Generator(device=DEV).manual_seed(D + rot)
+    q = torch.randn(1, S, Hq, D, generator=g, device=DEV).to(dt).transpose(1, 2)
+    k = torch.randn(1, S, Hkv, D, generator=g, device=DEV).to(dt).transpose(1, 2)
+    qw, kw = ((1 + 0.2 * torch.randn(D, generator=g, device=DEV)).to(dt) if norm else None for _ in range(2))
+    cos, sin = (t.to(DEV) for t in hip_ops.rope_table(S, rot))
+    pos = torch.randperm(S, generator=g, device=DEV)[None]
+    a, b = hip_ops.qk_norm_rope(q, k, cos, sin, pos, q_weight=qw, k_weight=kw, interleaved=inter)
+    for s0 in list(range(0, S, S // 5)) + [S - 3]:
+        s1 = min(s0 + 97, S)
+        x, y = hip_ops.qk_norm_rope(q[:, :, s0:s1], k[:, :, s0:s1], cos, sin, pos[:, s0:s1], q_weight=qw, k_weight=kw, interleaved=inter)
+        assert torch.equal(a[:, :, s0:s1], x) and torch.equal(b[:, :, s0:s1], y), s0

@@ -319,7 +319,8 @@ int ssq_append(const ssq_append_args* a, void* workspace, size_t workspace_bytes
 
 /* Decode for a batch whose sequences share a prefix: each query row attends the prefix_len[0] (device, at most
  * prefix_cap) tokens in the pages prefix_table (ceil(prefix_cap / page_size) entries), then its own sequence's
- * tokens as in ssq_decode: one softmax over both.  The prefix's pages are read once for all sequences' rows.
+ * tokens as in ssq_decode: one softmax over both.  The prefix is held once, and read for 32 or 64 rows
+ * of a KV head at a time, whichever sequences they belong to.
  * dec: SSQ_PAGED with v; block_table / seq_lens / seq_len / mask speak of the sequences' own tokens
  * (seq_len 0: none, block_table may be NULL); scores NULL; kernel 0, or 1 for the path that serves every codec.
  * A row with nothing to attend (both lengths 0, or a mask of -inf) gives out 0 and lse -inf.

@@ -308,10 +308,11 @@ void fast_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
         int64_t best = INT64_MAX;
         for (int nr = 1; nr <= most; ++nr) {
             const int n_rg = (f.rows + 32 * nr - 1) / (32 * nr);
-            for (int n1 = 1; n1 <= 128 && (n1 == 1 || n1 * 4 <= tiles); ++n1) {
-                const int64_t items = (int64_t)n_rg * n1, rounds = (items + f.n_wg - 1) / f.n_wg;
-                const int64_t wave = ((tiles + n1 - 1) / n1 + 3) / 4;
-                const int64_t cost = rounds * (nr == 1 ? 300 + 98 * wave : 1000 + 135 * wave) +
+            const int n1_most = 4 * f.n_wg / n_rg;  // about four rounds
+            for (int n1 = 1; n1 <= 128 && (n1 == 1 || (n1 * 4 <= tiles && n1 <= n1_most)); ++n1) {
+                const int items = n_rg * n1, rounds = (items + f.n_wg - 1) / f.n_wg;
+                const int wave = ((tiles + n1 - 1) / n1 + 3) / 4;
+                const int64_t cost = (int64_t)rounds * (nr == 1 ? 300 + 98 * (int64_t)wave : 1000 + 135 * (int64_t)wave) +
                                      (own_items && items > room ? 600 : 0);
                 if (cost < best) {
                     best = cost;

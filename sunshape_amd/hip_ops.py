@@ -336,8 +336,9 @@ def decode_prefix(q: torch.Tensor, codes: torch.Tensor, v: torch.Tensor, perm: t
     nothing to attend gives 0 and -inf.  kernel 1 takes the decode kernels that serve every codec,
     for comparisons.  No counterpart in the reference.
     """
-    for name, t in (("query", q), ("codes", codes), ("value", v)):
-        _on_gpu(name, t)
+    if not (q.is_cuda and codes.is_cuda and v.is_cuda):
+        for name, t in (("query", q), ("codes", codes), ("value", v)):
+            _on_gpu(name, t)
     if rotation is not None:
         _require(q.ndim == 4, "Quantized attention expects query/value tensors with shape [batch, heads, seq, dim].")
         q = transform_rows(q, rotation, scale=scale)
@@ -379,7 +380,8 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: Optional[torch
     tables makes the row's rotated dims NaN.  No counterpart in the reference, whose model code
     rotates before the cache sees the keys.
     """
-    _on_gpu("query", q)
+    if not q.is_cuda:
+        _on_gpu("query", q)
     try:
         q_out, k_out = N.torch_ops().qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, float(eps),
                                                   bool(interleaved))
@@ -406,7 +408,8 @@ def append_kv(keys: torch.Tensor, values: Optional[torch.Tensor], perm: torch.Te
     codec's rotated mode, after the position rotation) as in encode(); kernel: 0, or 1 for the exact
     scan.  No counterpart in the reference.
     """
-    _on_gpu("key_states", keys)
+    if not keys.is_cuda:
+        _on_gpu("key_states", keys)
     if rotation is not None:
         _require(keys.ndim == 4, "append_kv expects key_states with shape [batch, kv_heads, seq_len, head_dim].")
         if cos is not None or k_weight is not None:

@@ -3,7 +3,7 @@
 // rotated keys) and the values' transpose into dim-major pages.
 //
 // Few rows (a decode step): one launch, k_append_few.  A workgroup serves one block of some keys of a KV head:
-// it rotates just that block's dims, keeps the block's codebook in LDS and splits a key's scan over 8 (or 64)
+// it rotates just that block's dims, keeps the block's codebook in LDS and splits a key's scan over 4 to 64
 // lanes.  The first workgroups write the values.  Loads that wait for one another bound it, so the keys' whole
 // rows (which the norm needs anyhow), the codebook, the permutation, slots and positions are all asked for at once,
 // and only the table's and weights' entries after them.  64 sequences' step (8 heads of 128 dims, 256 codewords of dim
@@ -485,13 +485,18 @@ __global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
                 const float* q = cn + g + sl;
 #pragma unroll
                 for (int u = 0; u < kScan; ++u) v[u] = __builtin_fmaxf(mm_dist2(x, xn, c + u * S * bd, q[u * S], bd), 0.f);
-            } else {
-#pragma unroll 1
+            } else if (!direct) {
+#pragma unroll
                 for (int u = 0; u < kScan; ++u) {
                     const int j = g + sl + u * S, jj = min(j, m - 1);
-                    const float* c = cb + jj * bd;
-                    const float y = direct ? direct_dist2(x, c, bd) : mm_dist2(x, xn, c, cn[jj], bd);
-                    // NaN: 0, as clamp_min's
+                    const float y = mm_dist2(x, xn, cb + jj * bd, cn[jj], bd);
+                    v[u] = j < m ? __builtin_fmaxf(y, 0.f) : INFINITY;  // NaN: 0, as clamp_min's
+                }
+            } else {  // at most 25 codewords and keys: small code counts
+#pragma unroll 1
+                for (int u = 0; u < kScan; ++u) {
+                    const int j = g + sl + u * S;
+                    const float y = direct_dist2(x, cb + min(j, m - 1) * bd, bd);
 #pragma unroll
                     for (int k = 0; k < kScan; ++k) v[k] = k != u ? v[k] : j < m ? __builtin_fmaxf(y, 0.f) : INFINITY;
                 }
@@ -551,21 +556,21 @@ int check(const ssq_append_args* a) {
     return SSQ_OK;
 }
 
-// One launch or three?  The few kernel stages a codebook per 32 keys, the others spread it over many; measured, calls
-// in a row, 8 heads of 128 dims, us in one launch and in three:
-//   256 codewords of dim 4: 64 tokens 8.8 and 18.8, 256 17.8 and 20.2, 512 28 and 22.5;  of dim 2: 128 tokens 14.7 and
-//   21.2, 256 23.5 and 21.7;  of dim 8: 256 tokens 16.8 and 22.1, 512 27.4 and 24.7;  4,096 of dim 4: 4 tokens 11.9
-//   and 23.2, 16 29.1 and 31.4, 64 44 and 26
-// -- about 2^24 (key, block, codeword) triples.  Codebooks that ssq_encode serves by its exact scan, whose workgroups
-// take more keys than such calls have, stay to 2^26 and 2^20 rows: 64 codewords of dim 2, 2,048 tokens 254 and 591;
-// 128 of dim 8, 4,096 tokens 137 and 2,147; 16 of dim 4, 4,096 tokens 283 and 253, 2,048 143 and 247.
+// One launch or two and the encode's?  The few kernel stages a codebook per 4 to 64 keys, the encode's screen spreads it
+// over 512; measured, calls in a row, 8 heads of 128 dims, us in one launch and through the encode:
+//   256 codewords of dim 4: 64 tokens 8.5 and 18.8, 256 14.2 and 20.2, 512 22.8 and 18.5;  of dim 2: 128 tokens 12.1 and
+//   21.2, 256 20.0 and 17.5;  of dim 8: 512 tokens 20.3 and 24.7, 1,024 33.5 and 22.1;  4,096 of dim 4: 4 tokens 11.4
+//   and 23.2, 16 28.2 and 31.4, 64 42 and 22
+// -- about 2^24 (key, block, codeword) triples.  Codebooks of at most 256 codewords that ssq_encode serves by its exact
+// scan, whose workgroups take more keys than most calls have, stay: 16 of dim 4, 4,096 tokens 90 and 253, 8,192 167 and
+// 427; 128 of dim 8, 8,192 tokens 165 and 2,157; up to as many workgroups as one launch holds with ease.
 bool few(const ssq_append_args& a) {
     const ssq_encode_args& e = a.enc;
     if (e.kernel != 0) return false;
-    const bool scan = e.n_centroids < 256 || e.direct_dist || (e.n_centroids == 256 && e.block_dim > 10);
+    const bool grid = e.grid && !e.direct_dist && ssq_encode_grid_supported(&e);
+    const bool scan = !grid && (e.n_centroids < 256 || (e.n_centroids == 256 && (e.direct_dist || e.block_dim > 10)));
     const int64_t rows = (int64_t)e.batch * e.seq_len * e.num_kv_heads * e.n_blocks;
-    return scan && e.n_centroids <= 256 ? rows <= 1 << 20 && rows * e.n_centroids <= 1 << 26
-                                        : rows <= 1 << 24 && rows * e.n_centroids <= 1 << 24;
+    return scan ? rows <= 1 << 26 : rows <= 1 << 24 && rows * e.n_centroids <= 1 << 24;
 }
 
 bool turns(const ssq_append_args& a) { return a.k_weight || a.rope.cos; }
@@ -671,17 +676,21 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
     hipStream_t st = (hipStream_t)stream;
     AppendParams p = params(*a);
     if (few(*a)) {
-        // 8 lanes a key; a whole wave where the keys are too few for the device and a lane's share of the scan is
-        // long (4,096 codewords, 4 tokens: 11.9 us against 32; 16 tokens 29 and 34, 64 79 and 44; at 256 codewords
-        // 11.8 against 7.4 for one token), or 32 rows too large for LDS
+        // Lanes of a key, by (key, block) pairs: more where pairs are few (the chain of loads and a lane's scan bound the
+        // call), fewer where they are many (what every lane does besides its scan does), us with 16, 8 and 4, 256
+        // codewords of dim 4: 8,192 pairs 7.4, 7.5, 9.1; 16,384 9.4, 8.6, 9.4; 65,536 23, 17.2, 14.3; 4 for at most 64
+        // codewords, a scan of 16 each: 512 pairs 8.4, 8.2, 5.2.  A whole wave where the scan is long and the keys
+        // too few for the device (4,096 codewords, 4 tokens: 11.9 with 64, 32 with 8; 64 tokens 79 and 44).  A
+        // workgroup's key rows fit 20 KiB of LDS.
         const int64_t units = n * e.num_kv_heads * e.n_blocks;
         const int row = e.head_dim * (e.k_dtype == SSQ_F32 ? 4 : 2);
         p.krow = ((row + 15) & ~15) + 16;  // rows on other LDS banks
-        const bool wide = (units * 8 < (int64_t)ssq_device_cus() * 256 && e.n_centroids >= 1024) ||
-                          kThreads / 8 * p.krow > 20 * 1024;
+        int S = e.n_centroids <= 64 || units >= 32768 ? 4 : units <= 8192 ? 16 : 8;
+        if (units * 8 < (int64_t)ssq_device_cus() * 256 && e.n_centroids >= 1024) S = SSQ_WAVE;
+        while (S < SSQ_WAVE && kThreads / S * p.krow > 20 * 1024) S = S == 16 ? SSQ_WAVE : 2 * S;
         const int stage = kStageFloats / (e.block_dim + 1);
         p.chunk = e.n_centroids < stage ? e.n_centroids : stage;
-        const int per = kThreads / (wide ? SSQ_WAVE : 8);
+        const int per = kThreads / S;
         p.ktiles = (int)((n + per - 1) / per);
         const int64_t xs = (int64_t)p.vtiles * p.dchunks + (int64_t)p.ktiles * e.n_blocks;
         SSQ_UNSUPPORTED(xs <= 0x7fffffff, "too many rows");
@@ -689,7 +698,12 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
         size_t lds = (((size_t)p.chunk * (e.block_dim + 1) * 4 + 15) & ~(size_t)15) + (size_t)per * p.krow;
         const size_t vlds = a->v && !p.vone ? (size_t)kValTok * val_row(a->vp_dtype == SSQ_F32 ? 4 : 2) : 0;
         if (vlds > lds) lds = vlds;
-        return wide ? launch_few<SSQ_WAVE>(p, grid, lds, st) : launch_few<8>(p, grid, lds, st);
+        switch (S) {
+            case 4: return launch_few<4>(p, grid, lds, st);
+            case 8: return launch_few<8>(p, grid, lds, st);
+            case 16: return launch_few<16>(p, grid, lds, st);
+            default: return launch_few<SSQ_WAVE>(p, grid, lds, st);
+        }
     }
     const int64_t rows = rows_bytes(*a);
     SSQ_REQUIRE(workspace && workspace_bytes >= (size_t)(rows + n * 8), "workspace too small: %zu < %lld bytes", workspace_bytes,

@@ -394,3 +394,29 @@ def test_values_from_any_slot(S, first, kernel):
                 if slots[b, s] >= 0:
                     want[slots[b, s] // page, :, :, slots[b, s] % page] = v[b, s]
         assert torch.equal(vp.cpu(), want), f"page {page}"
+
+
+@pytest.mark.parametrize("bd, nc, D, Hkv, S", [(2, 64, 64, 2, 9000), (4, 16, 128, 4, 3000), (8, 128, 128, 4, 3000), (16, 200, 64, 1, 2000)])
+def test_many_rows_of_small_codebooks(bd, nc, D, Hkv, S):
+    """Codebooks that the encode serves by its exact scan keep to one launch: the same codes, with a search grid too
+    where there is one."""
+    log(f"append_kv small codebooks bd {bd} nc {nc} S {S}")
+    rng = np.random.default_rng(nc)
+    g = torch.Generator(device=DEV).manual_seed(nc)
+    perm, cent, _, sigma = codec_arrays(rng, Hkv, D, bd, nc)
+    perm, cent = perm.to(DEV), cent.to(DEV)
+    k = (torch.randn(1, S, Hkv, D, generator=g, device=DEV) * torch.from_numpy(sigma).to(DEV).float()).to(BF).transpose(1, 2)
+    v = torch.randn(1, S, Hkv, D, generator=g, device=DEV).to(BF).transpose(1, 2)
+    pages = S // 16 + 2
+    slots = 7 + torch.arange(S, device=DEV)[None]
+    grids = [None] + ([hip_ops.encode_grid(cent, Hkv)] if bd == 2 else [])
+    for grid in grids:
+        got = []
+        for kernel in (0, 1):
+            c = torch.zeros(pages, Hkv, 16, D // bd, dtype=torch.uint8, device=DEV)
+            vp = torch.zeros(pages, Hkv, D, 16, dtype=BF, device=DEV)
+            hip_ops.append_kv(k, v, perm, cent, codes_out=c, v_out=vp, slot_mapping=slots, kernel=kernel, grid=grid)
+            got.append((c, vp))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+        flat = got[0][1].permute(0, 3, 1, 2).reshape(pages * 16, Hkv, D)[7:7 + S]
+        assert torch.equal(flat, v[0].transpose(0, 1))

@@ -2,7 +2,7 @@
 // ssq_rope.h).
 //
 // Measured, one MI355X: 32,768 tokens of 32 + 8 heads of 128 dims, bf16 with norm: 131-134 us for 688 MB, 5.1-5.2 TB/s,
-// a copy's rate; a step of 64 tokens 4.2 us, 8.3 with the call (latency of one chain: position, table, row).
+// a copy's rate; a step of 64 tokens 4.2 us, 7.5 with the call (latency of one chain: position, table, row).
 #include "ssq_rope.h"
 
 namespace {

@@ -539,13 +539,15 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
                     else e0[r] = e;
                 }
         });
+        // While a row has met hidden tokens only (m -inf), its probabilities, taken against 0, may underflow whatever
+        // the scores are: these decide, not the sum.
         bool over = false;
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
             for (int dt = 0; dt < Run::DT; ++dt) pf_pin(o[r][dt]);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) over |= lt[r] > (m[r] == -INFINITY ? 0.f : kPfOver);
+        for (int r = 0; r < NR; ++r) over |= lt[r] > (m[r] == -INFINITY ? -1.f : kPfOver);
         if (__builtin_amdgcn_ballot_w64(over) != 0) {  // m moves: once more from the scores
             raise(by);
 #pragma unroll

@@ -288,7 +288,7 @@ int ssq_launch_merge(const ssq_decode_args& a, int n_splits, const float* ws_o, 
 int ssq_decode_mfma_supported(const ssq_decode_args* a);
 size_t ssq_decode_mfma_workspace(const ssq_decode_args* a);
 size_t ssq_decode_mfma_workspace_least(const ssq_decode_args* a);
-int ssq_decode_mfma_splits(const ssq_decode_args* a);
+int ssq_decode_mfma_splits(const ssq_decode_args* a, int& split_len);
 int ssq_decode_mfma(const ssq_decode_args* a, void* workspace, size_t ws_bytes, hipStream_t st, bool partial = false);
 int ssq_decode_contig_supported(const ssq_decode_args* a);
 size_t ssq_decode_contig_workspace(const ssq_decode_args* a);
@@ -328,16 +328,18 @@ int ssq_decode_validate(const ssq_decode_args* a) { return validate(a, true); }
 
 // Context splits of a paged decode whose partials ssq_decode_partials leaves (0: the problem has no plan;
 // the message says why).  a->num_splits of the later call must be the number returned, which also keeps the
-// batch from being balanced by length (those partials are laid out by share, not by row).
-int ssq_decode_partial_splits(const ssq_decode_args* a) {
+// batch from being balanced by length (those partials are laid out by share, not by row).  Split s holds the
+// tokens [s split_len, (s + 1) split_len) of each sequence.
+int ssq_decode_partial_splits(const ssq_decode_args* a, int& split_len) {
     ssq_decode_args t = *a;
     for (int k = 0; k < 4; ++k) {  // a plan may round the number of splits: the one that it keeps
         int n = 0;
         if (pick_kernel(&t) == 2 && ssq_decode_mfma_supported(&t)) {
-            n = ssq_decode_mfma_splits(&t);
+            n = ssq_decode_mfma_splits(&t, split_len);
         } else {
-            Plan pl;
+            Plan pl{};
             n = make_plan(t, pl) == SSQ_OK ? pl.n_splits : 0;
+            split_len = pl.split_len;
         }
         if (n == 0 || n == t.num_splits) return n;
         t.num_splits = n;

@@ -228,9 +228,11 @@ size_t ssq_decode_mfma_workspace_least(const ssq_decode_args* a) {
     return plan(a, pl) ? pl.ws_least : 0;
 }
 
-int ssq_decode_mfma_splits(const ssq_decode_args* a) {
+int ssq_decode_mfma_splits(const ssq_decode_args* a, int& split_len) {
     SsqMfmaPlan pl;
-    return plan(a, pl) ? pl.n_splits : 0;
+    if (!plan(a, pl)) return 0;
+    split_len = pl.split_len;
+    return pl.n_splits;
 }
 
 // partial: leave every split's (o, m, l) in the workspace and merge nothing (a->num_splits is set, so the

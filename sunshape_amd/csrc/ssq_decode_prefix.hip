@@ -14,7 +14,7 @@
 #include <math.h>
 
 int ssq_decode_validate(const ssq_decode_args* a);
-int ssq_decode_partial_splits(const ssq_decode_args* a);
+int ssq_decode_partial_splits(const ssq_decode_args* a, int& split_len);
 int ssq_decode_partials(const ssq_decode_args* a, void* ws, size_t bytes, hipStream_t st);
 
 namespace {
@@ -32,10 +32,13 @@ struct MergeParams {
     // the own tokens' partials, n2 splits x (batch * num_q_heads * q_len) rows (0: none)
     const float* own;
     int n2;
+    int len1, len1_last, len2;  // tokens of a split
+    const int32_t* plen;
 };
 
-// One wave per query row.  A lane takes a split's (m, l), 64 at a time; the splits that hold anything are then
-// joined with lane j on value dims j, j + 64, ...: bytes bound it, and splits without tokens cost no o.
+// One wave per query row.  A lane takes a split's (m, l), 64 at a time; the splits that hold tokens are then
+// joined with lane j on value dims j, j + 64, ...: bytes bound it, and splits without tokens cost no o.  Those
+// with tokens count also at weight 0: 0 times an infinite or NaN value is NaN, as in one pass over all tokens.
 __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const MergeParams p) {
     const ssq_decode_args& a = p.a;
     const int lane = threadIdx.x & (SSQ_WAVE - 1);
@@ -47,11 +50,14 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
     const int b = (int)(rid / a.q_len / a.num_q_heads);
     const int Dv = a.value_dim;
     // this row's prefix block
-    int n1 = p.n1;
+    int n1 = p.n1, len1 = p.len1;
     int64_t at0 = 0, rows1 = n_rows, row1 = rid;
     if (p.n1) {
         const int c = b / p.chunk, cn = min(p.chunk, a.batch - c * p.chunk);
-        if ((int64_t)(c + 1) * p.chunk >= a.batch) n1 = p.n1_last;
+        if ((int64_t)(c + 1) * p.chunk >= a.batch) {
+            n1 = p.n1_last;
+            len1 = p.len1_last;
+        }
         const int rest = a.batch % p.chunk ? a.batch % p.chunk : p.chunk;
         const int64_t per_q = (int64_t)a.num_q_heads * ((int64_t)(a.batch - rest) * p.n1 + (int64_t)rest * p.n1_last);
         at0 = (per_q * qi + (int64_t)a.num_q_heads * c * p.chunk * p.n1) * (Dv + 2);
@@ -66,6 +72,7 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
     const float* own_m = p.own + n_rows * p.n2 * Dv;
     const float* own_l = own_m + n_rows * p.n2;
     const int n = n1 + n2;
+    const int t1 = n1 ? p.plen[0] : 0, t2 = n2 ? a.seq_lens[b] : 0;
     float M = -INFINITY, L = 0.f;
     for (int d0 = 0; d0 < Dv; d0 += kMergeDims * SSQ_WAVE) {
         float Mr = -INFINITY, Lr = 0.f, o[kMergeDims];
@@ -78,13 +85,13 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
             const float m = s < n ? (pre ? pre_m : own_m)[at] : -INFINITY;
             const float l = m != -INFINITY ? (pre ? pre_l : own_l)[at] : 0.f;
             const float Mc = fmaxf(Mr, ssq_wave_max(m));
-            if (Mc == -INFINITY) continue;
             const float f = Mr == -INFINITY ? 0.f : __expf(Mr - Mc);  // earlier passes, rescaled
             const float w = m == -INFINITY ? 0.f : __expf(m - Mc);
             Lr = Lr * f + ssq_wave_sum(l * w);
 #pragma unroll
             for (int k = 0; k < kMergeDims; ++k) o[k] *= f;
-            uint64_t live = __builtin_amdgcn_ballot_w64(m != -INFINITY);
+            const bool holds = pre ? (int64_t)s * len1 < t1 : s < n && (int64_t)(s - n1) * p.len2 < t2;
+            uint64_t live = __builtin_amdgcn_ballot_w64(holds);
             while (live) {  // wave-uniform
                 float ov[kMergeBatch][kMergeDims], wv[kMergeBatch];
 #pragma unroll
@@ -203,12 +210,13 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_flat(const Merg
         const float x = s < SSQ_WAVE ? w[0] : s < 2 * SSQ_WAVE ? w[1] : w[2];  // uniform
         return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), s & (SSQ_WAVE - 1)));
     };
+    // at weight 0 too: an infinite or NaN value counts as in one pass over all tokens
     auto add = [&](const float* part, int first, int n, const auto& ahead) {
         constexpr int kHave = sizeof(ahead) / sizeof(ahead[0]);
 #pragma unroll
         for (int i = 0; i < kHave; ++i) {
-            const float f = i < n ? weight(first + i) : 0.f;
-            if (f == 0.f) continue;  // uniform
+            if (i >= n) continue;  // uniform
+            const float f = weight(first + i);
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] += ahead[i][e] * f;
         }
@@ -219,8 +227,8 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_flat(const Merg
                 if (i0 + i < n) o_of(part, i0 + i, x[i]);
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                const float f = i0 + i < n ? weight(first + i0 + i) : 0.f;
-                if (f == 0.f) continue;
+                if (i0 + i >= n) continue;
+                const float f = weight(first + i0 + i);
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[e] += x[i][e] * f;
             }
@@ -243,6 +251,7 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_flat(const Merg
 
 struct PrefixPlan {
     int chunk, n1, n1_last, n2;
+    int len1, len1_last, len2;  // tokens of a split
     size_t pre_bytes, own_bytes;
     bool fast;  // the matrix-core kernel
     SsqPrefixParams fp;
@@ -424,14 +433,14 @@ int make_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
         if (pl.chunk > d.batch) pl.chunk = d.batch;
         const int rest = d.batch % pl.chunk ? d.batch % pl.chunk : pl.chunk;
         const ssq_decode_args whole = prefix_part(a, 0, pl.chunk, 0), last = prefix_part(a, d.batch - rest, rest, 0);
-        pl.n1 = ssq_decode_partial_splits(&whole);
-        pl.n1_last = ssq_decode_partial_splits(&last);
+        pl.n1 = ssq_decode_partial_splits(&whole, pl.len1);
+        pl.n1_last = ssq_decode_partial_splits(&last, pl.len1_last);
         if (pl.n1 == 0 || pl.n1_last == 0) return SSQ_ERR_UNSUPPORTED;
         const int64_t rows = (int64_t)d.num_q_heads * ((int64_t)(d.batch - rest) * pl.n1 + (int64_t)rest * pl.n1_last);
         pl.pre_bytes = (size_t)(rows * d.q_len * (d.value_dim + 2) * 4);
     }
     if (d.seq_len > 0) {
-        pl.n2 = ssq_decode_partial_splits(&d);
+        pl.n2 = ssq_decode_partial_splits(&d, pl.len2);
         if (pl.n2 == 0) return SSQ_ERR_UNSUPPORTED;
         pl.own_bytes = (size_t)d.batch * d.num_q_heads * d.q_len * pl.n2 * (d.value_dim + 2) * 4;
     }
@@ -484,6 +493,10 @@ extern "C" int ssq_decode_prefix(const ssq_prefix_args* a, void* workspace, size
     m.n1_last = pl.n1_last;
     m.own = own;
     m.n2 = pl.n2;
+    m.len1 = pl.len1;
+    m.len1_last = pl.len1_last;
+    m.len2 = pl.len2;
+    m.plen = a->prefix_len;
     if (pl.n1) {
         char* at = reinterpret_cast<char*>(workspace);
         for (int qi = 0; qi < d.q_len; ++qi)

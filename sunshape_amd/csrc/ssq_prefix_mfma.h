@@ -698,7 +698,8 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
     }
     pf_tiles<false, NR>(u, first, mrow, m_run, l_run, o);
 
-    // ---- the four waves' (m, l), then o, 32 rows x 32 dims at a time
+    // ---- the four waves' (m, l), then o, 32 rows x 32 dims at a time (at weight 0 too: an infinite or NaN value
+    // counts as in one pass; a wave without tiles has zeros)
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
         const float l = l_run[r] + pf_other(l_run[r]);
@@ -749,8 +750,7 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
             float* dst = jL + (last ? (r * Run::DT + dt) * kTileF : 0);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {  // dims 8 k + 4 half ..
-                float4 x = make_float4(o[r][dt][4 * k] * f[r], o[r][dt][4 * k + 1] * f[r], o[r][dt][4 * k + 2] * f[r], o[r][dt][4 * k + 3] * f[r]);
-                if (f[r] == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 x = make_float4(o[r][dt][4 * k] * f[r], o[r][dt][4 * k + 1] * f[r], o[r][dt][4 * k + 2] * f[r], o[r][dt][4 * k + 3] * f[r]);
                 *reinterpret_cast<float4*>(dst + (wave * 32 + col) * L::kJoinRow + 8 * k + 4 * half) = x;
             }
             if (!last) {  // uniform

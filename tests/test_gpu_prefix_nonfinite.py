@@ -1,0 +1,72 @@
+"""Infinities and NaN that decode_prefix meets.  What one pass over all
+tokens gives (0 times infinity is NaN) does not depend on where the tokens are cut."""
+
+import math
+
+import pytest
+import torch
+
+from _util import log
+from test_gpu_decode_prefix import _call, _problem
+
+pytestmark = pytest.mark.gpu
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _spike(p, at, logit):
+    """Prefix token `at` beats all others by `logit`: a codeword of its own in block 0, along a query dim that is 1
+    after the scale."""
+    G = p["q"].shape[1] // p["cent"].shape[0]
+    p["codes"][..., 0] = p["codes"][..., 0].clamp(min=1)
+    for h in range(p["cent"].shape[0]):
+        p["q"][:, h * G:(h + 1) * G, :, int(p["perm"][h, 0])] = math.sqrt(p["q"].shape[-1])
+        p["cent"][h, 0, :, 0] = 0.0
+        p["cent"][h, 0, 0, 0] = logit
+    p["codes"][p["ptable"][at // 16].long(), :, at % 16, 0] = 0
+    return p
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("T, at, where", [
+    (64, 3, 40),      # another tile: another wave of the same workgroup
+    (64, 3, 20),      # the same tile
+    (2000, 3, 1500),  # another slice of the prefix
+    (2000, 1900, 4),
+    (2000, 700, 731),
+    (300, 7, -1),     # an own token
+])
+def test_values_under_probabilities_that_underflow(T, at, where, bad):
+    log(f"decode_prefix: a value of {bad} at {where}, the logit at {at} 400 above, prefix of {T}")
+    p = _spike(_problem(B=3, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=256, T=T, lens=[70, 5, 0]), at, 400.0)
+    clean = _call(p)
+    v = p["v"].clone()
+    if where >= 0:
+        v[p["ptable"][where // 16].long(), :, 5, where % 16] = bad
+        hit = torch.ones(3, dtype=torch.bool)
+    else:
+        v[p["table"][0, 3].long(), :, 5, 9] = bad
+        hit = torch.tensor([True, False, False])
+    for kernel in (0, 1):
+        out, lse = _call(dict(p, v=v), kernel=kernel)
+        assert torch.isnan(out[hit][..., 5]).all(), f"kernel {kernel}"
+        assert torch.isfinite(out[~hit]).all() and torch.isfinite(out[..., :5]).all() and torch.isfinite(out[..., 6:]).all()
+        assert torch.isfinite(lse).all()
+        if kernel == 0:
+            assert torch.equal(out[..., 6:], clean[0][..., 6:]) and torch.equal(lse, clean[1])
+
+
+@pytest.mark.parametrize("where", [20, 40, 100])
+def test_values_of_hidden_tokens(where):
+    """A token at a mask of -inf has probability 0, and 0 times an infinite value is NaN: in the piece with the visible
+    tokens and in one that is hidden whole, wherever the sequence is cut."""
+    log(f"decode_prefix: an infinite value at hidden token {where}")
+    p = _problem(B=2, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=256, T=20, lens=[200, 150])
+    v = p["v"].clone()
+    v[p["table"][0, where // 16].long(), :, 5, where % 16] = math.inf
+    m = torch.zeros(2, 1, 1, p["table"].shape[1] * 16)
+    m[..., :128] = -math.inf
+    p["own_mask"] = m
+    for kernel in (0, 1):
+        out, lse = _call(dict(p, v=v), kernel=kernel)
+        assert torch.isnan(out[0, ..., 5]).all(), f"kernel {kernel}"
+        assert torch.isfinite(out[1]).all() and torch.isfinite(out[..., :5]).all() and torch.isfinite(lse).all()

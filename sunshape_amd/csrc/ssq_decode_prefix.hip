@@ -36,6 +36,17 @@ struct MergeParams {
     const int32_t* plen;
 };
 
+// Whether a query row holds a NaN (a wave's question).
+__device__ __forceinline__ bool nan_query(const ssq_decode_args& a, int b, int h, int qi, int lane) {
+    const int64_t at = (int64_t)b * a.q_sb + (int64_t)h * a.q_sh + (int64_t)qi * a.q_sl;
+    bool is = false;
+    for (int d = lane; d < a.head_dim; d += SSQ_WAVE) {
+        const float x = ssq_load_elem(a.q, a.q_dtype, at + d);
+        is |= x != x;
+    }
+    return __builtin_amdgcn_ballot_w64(is) != 0;
+}
+
 // One wave per query row.  A lane takes a split's (m, l), 64 at a time; the splits that hold tokens are then
 // joined with lane j on value dims j, j + 64, ...: bytes bound it, and splits without tokens cost no o.  Those
 // with tokens count also at weight 0: 0 times an infinite or NaN value is NaN, as in one pass over all tokens.
@@ -114,6 +125,8 @@ __global__ __launch_bounds__(kMergeRows * SSQ_WAVE) void k_merge_prefix(const Me
             }
             Mr = Mc;
         }
+        // the decode kernels leave a row of NaN scores as one without tokens
+        if (Mr == -INFINITY && nan_query(a, b, h, qi, lane)) Mr = Lr = __builtin_nanf("");
 #pragma unroll
         for (int k = 0; k < kMergeDims; ++k) {
             const int dv = d0 + k * SSQ_WAVE + lane;

@@ -435,7 +435,8 @@ struct PfFirst {
     }
 };
 
-// The wave's tiles.  mrow[r]: the additive mask's row of this lane's query row (MASK).
+// The wave's tiles: a row's (m, l, o) over them, l over both halves.  mrow[r]: the additive mask's row of this lane's
+// query row (MASK).
 //
 // One wave a SIMD issues one instruction every 4 cycles at best, so a tile costs its instructions: 48 MFMAs of 32 cycles
 // for 64 rows of 128 dims leave room for about 340 others.  So the codebook is staged times log2(e): a probability is
@@ -590,7 +591,11 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
         if (i + 1 < n) fix(i + 1);
     }
 #pragma unroll
-    for (int r = 0; r < NR; ++r) m_run[r] = MASK || m[r] == -INFINITY ? m[r] : m[r] * kLn2;
+    for (int r = 0; r < NR; ++r) {
+        l_run[r] += pf_other(l_run[r]);  // both halves' tokens
+        m_run[r] = MASK || m[r] == -INFINITY ? m[r] : m[r] * kLn2;
+        if (l_run[r] != l_run[r]) m_run[r] = 0.f;  // NaN scores: the maxima pass them over, the sum does not
+    }
 }
 
 // A prefix item: rows [R0, R0 + nr) of the KV head over tiles [t0, t1) of the prefix (len tokens); partials go to
@@ -702,10 +707,9 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
     // counts as in one pass; a wave without tiles has zeros)
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-        const float l = l_run[r] + pf_other(l_run[r]);
         if (half == 0) {
             mL[wave * 64 + 32 * r + col] = m_run[r];
-            lL[wave * 64 + 32 * r + col] = l;
+            lL[wave * 64 + 32 * r + col] = l_run[r];
         }
     }
     __syncthreads();  // also: every wave is past its gathers
@@ -831,7 +835,6 @@ __device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsi
 #pragma unroll
     for (int dt = 0; dt < Run::DT; ++dt) o[0][dt] = pv16f{};
     pf_tiles<MASK, 1>(u, first, mrow, m_run, l_run, o);
-    const float l = l_run[0] + pf_other(l_run[0]);
     if (col < nr) {
         const int64_t n_rows = (int64_t)a.batch * a.num_q_heads * a.q_len, rid = pf_rid(p, kv, R);
         float* ws_m = p.own + (int64_t)p.n2 * n_rows * D + (int64_t)split * n_rows;
@@ -844,7 +847,7 @@ __device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsi
                     make_float4(o[0][dt][4 * k], o[0][dt][4 * k + 1], o[0][dt][4 * k + 2], o[0][dt][4 * k + 3]);
         if (half == 0) {
             ws_m[rid] = m_run[0];
-            ws_m[(int64_t)p.n2 * n_rows + rid] = l;
+            ws_m[(int64_t)p.n2 * n_rows + rid] = l_run[0];
         }
     }
 }

@@ -70,3 +70,31 @@ def test_values_of_hidden_tokens(where):
         out, lse = _call(dict(p, v=v), kernel=kernel)
         assert torch.isnan(out[0, ..., 5]).all(), f"kernel {kernel}"
         assert torch.isfinite(out[1]).all() and torch.isfinite(out[..., :5]).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("T, lens", [(300, [70, 5, 0]), (0, [70, 5, 40]), (2000, [0, 0, 0])])
+@pytest.mark.parametrize("qdt, vdt", [(BF, BF), (F16, F16), (F32, BF)])
+def test_queries_of_nan(T, lens, qdt, vdt):
+    """A row whose query holds a NaN is NaN, and no other row."""
+    log(f"decode_prefix: a NaN query, {qdt}, prefix {T}")
+    p = _problem(B=3, Hq=8, Hkv=2, Lq=1, D=64, Dv=64, bd=4, nc=256, T=T, lens=lens, qdt=qdt, vdt=vdt)
+    p["q"][1, 6, 0, 11] = math.nan
+    for kernel in (0, 1):
+        out, lse = _call(p, kernel=kernel)
+        bad = torch.zeros(3, 8, 1, dtype=torch.bool, device=out.device)
+        bad[1, 6] = True
+        assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all(), f"kernel {kernel}"
+        assert torch.isfinite(out[~bad]).all() and torch.isfinite(lse[~bad]).all(), f"kernel {kernel}"
+
+
+@pytest.mark.parametrize("kw", [dict(D=64, Dv=64, bd=4, nc=4096), dict(D=256, Dv=256, bd=4, nc=256), dict(D=64, Dv=64, bd=4, nc=256, vdt=F32),
+                                dict(D=64, Dv=128, bd=4, nc=256), dict(D=128, Dv=128, bd=4, nc=256, heavy=tuple(range(20)))])
+def test_queries_of_nan_under_other_codecs(kw):
+    log(f"decode_prefix: a NaN query, {kw}")
+    p = _problem(B=3, Hq=8, Hkv=2, Lq=2, T=300, lens=[70, 5, 0], **kw)
+    p["q"][1, 6, 1, 11] = math.nan
+    out, lse = _call(p)
+    bad = torch.zeros(3, 8, 2, dtype=torch.bool, device=out.device)
+    bad[1, 6, 1] = True
+    assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
+    assert torch.isfinite(out[~bad]).all() and torch.isfinite(lse[~bad]).all()

@@ -12,11 +12,11 @@
 //   token 16 (i / 8) + 8 h + i % 8: the 8 consecutive tokens of one 16-byte piece of a dim-major value page,
 //   which is the V^T operand, loaded straight into registers.
 // K^T's operand is gathered codeword by codeword from the codebook in LDS: no key tile is ever written.  A
-// codeword is stored as two 16-bit parts, c = hi + lo (the rounding of c, and of what that left: 2^-17 of c at most
-// is dropped, 2^-23 with f16 parts), and each 16 dims take one MFMA with the hi parts and one with the lo parts
-// against the same query operand: the logits keep fp32's quality for half as much matrix-core work again.
+// codeword is stored as two 16-bit parts, c = hi + lo (the rounding of c, and of what that left), and each 16 dims take
+// one MFMA with the hi parts and one with the lo parts against the same query operand, half as much matrix-core work
+// again.  Dropped is at most 2^-17 of a codeword with bf16 parts (one part would drop 2^-9), 2^-23 with f16 parts.
 // Kept (passthrough) dims of a SunShape-Mixed codec, up to half of the head's, take a step per 16 more: their codewords are
-// staged as zeros, and a token's kept values, two 8-byte pieces a lane and step, are split into parts on the way.
+// staged as zeros, and a token's kept values, two 8-byte pieces a lane and step, enter exactly, into sums of their own.
 // Queries of 16 bits enter exactly (QT bf16 / f16); fp32 ones (rotated codecs) in two bf16 parts.
 // Probabilities are rounded to the values' 16 bits for P.V, as in the other decode kernels; sums stay fp32.
 //
@@ -148,6 +148,7 @@ struct PfRun {
     static constexpr int DT = D / 32;
     static constexpr int QP = QT == kQtSplit ? 2 : 1;
     static constexpr int NK = HV ? L::kKeptMax / 16 : 0;  // steps of kept dims, at most
+    static constexpr int KP = QT == kQtSplit && kVF16 ? 2 : 1;  // parts of a kept value: exact in its own type, or in two
     static constexpr bool kKept = HV;
 
     struct Codes { uint32_t w[NW]; };
@@ -225,7 +226,7 @@ struct PfRun {
             const int64_t o0 = of_lane(o, l), o1 = of_lane(o, l + 1);
             const uint16_t* row = kept.base + (lane & 16 ? o1 : o0);
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {  // dims past the last: others, against zeros in q
+            for (int k = 0; k < NK; ++k) {  // dims past the last: others, left out where they are used
                 const int d = 16 * k + 8 * half;
                 const uint2 x = *reinterpret_cast<const uint2*>(row + (d < p.kept ? d : 0));
                 const uint2 y = *reinterpret_cast<const uint2*>(row + (d + 4 < p.kept ? d + 4 : 0));
@@ -302,22 +303,39 @@ struct PfRun {
             beside(st);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (HV) {
+        if constexpr (HV) {  // in sums of their own, natural units
+            pv16f t[NR];
+#pragma unroll
+            for (int r = 0; r < NR; ++r) t[r] = pv16f{};
 #pragma unroll
             for (int k = 0; k < NK; ++k) {
                 if (16 * k >= p.kept) continue;  // uniform
-                const uint32_t w[4] = {kept.v[k].x, kept.v[k].y, kept.v[k].z, kept.v[k].w};
-                uint32_t hi[4], lo[4];
+                const int d = 16 * k + 8 * half;
+                uint4 x = kept.v[k];
+                if (d >= p.kept) x.x = x.y = 0u;
+                if (d + 4 >= p.kept) x.z = x.w = 0u;
+                uint4 part[KP];
+                if constexpr (KP == 2) {
+                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) pf_split<kF16>(pf_lo<kVF16>(w[e]) * kLog2e, pf_hi<kVF16>(w[e]) * kLog2e, hi[e], lo[e]);
+                    for (int e = 0; e < 4; ++e) pf_split<kF16>(pf_lo<kVF16>(w[e]), pf_hi<kVF16>(w[e]), hi[e], lo[e]);
+                    part[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    part[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                } else {
+                    part[0] = x;
+                }
 #pragma unroll
                 for (int h = 0; h < QP; ++h)
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        s[r] = pf_mfma<kF16>(make_uint4(hi[0], hi[1], hi[2], hi[3]), kept.q[h][r][k], s[r]);
-                        s[r] = pf_mfma<kF16>(make_uint4(lo[0], lo[1], lo[2], lo[3]), kept.q[h][r][k], s[r]);
-                    }
+                    for (int r = 0; r < NR; ++r)
+#pragma unroll
+                        for (int j = 0; j < KP; ++j) t[r] = pf_mfma<kF16>(part[j], kept.q[h][r][k], t[r]);
             }
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) s[r][k] = __builtin_fmaf(t[r][k], kLog2e, s[r][k]);
             load_kept(i_kept);
         }
     }
@@ -924,55 +942,51 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
     // a permuted dim's source, for this thread's staging and for the waves' own rows
     const int64_t pj = (int64_t)min((uint64_t)a.perm[(int64_t)kv * a.perm_sh + tid % D], (uint64_t)(D - 1));
     const int plen = p.n1 ? max(0, min(p.plen[0], p.pcap)) : 0;
-    // ---- the KV head's codebook times log2(e) as 16-bit parts: a thread takes the same codeword (or half of one, at
-    // 8 dims) of every block, up to kIn of them in flight; workgroups start at different blocks, since those of one
-    // KV head share an L2
+    // ---- the KV head's codebook times log2(e) as 16-bit parts: a thread takes the
+    // same codeword (or half of one, at 8 dims) of every block, all of them in flight; workgroups start at different
+    // blocks, since those of one KV head share an L2
     {
         constexpr bool F16 = QT == kQtF16;
         constexpr int NB = D / BD, kV = BD < 4 ? BD : 4, kParts = BD / kV;  // floats of a piece, pieces of a codeword
-        constexpr int kIn = NB < 128 / BD ? NB : 128 / BD;                  // blocks in flight: 128 floats a lane
         const float* cent = a.cent + (int64_t)kv * a.cent_sh;
         const int nc = a.n_centroids;
-#pragma unroll 1
-        for (int i0 = 0; i0 < NB; i0 += kIn) {
-            float x[kIn][kParts][kV];
+        auto block = [&](int i) { return (i + w) & (NB - 1); };
+        auto zero = [&](int i) { return HV && ssq_is_heavy(a.heavy_mask[0], a.heavy_mask[1], block(i)); };
+        float x[NB][kParts][kV];  // at most 128 floats a lane
 #pragma unroll
-            for (int i = 0; i < kIn; ++i) {
-                const float* src = cent + ((i0 + i + w) & (NB - 1)) * nc * BD;  // uniform
+        for (int i = 0; i < NB; ++i) {
+            const float* src = cent + block(i) * nc * BD;  // uniform
 #pragma unroll
-                for (int j = 0; j < kParts; ++j) {
-                    const int e = min(tid + j * kPfThreads, nc * kParts - 1);
-                    if constexpr (kV == 4) {
-                        const float4 v = reinterpret_cast<const float4*>(src)[e];
-                        x[i][j][0] = v.x; x[i][j][1] = v.y; x[i][j][2] = v.z; x[i][j][3] = v.w;
-                    } else {
-                        const float2 v = reinterpret_cast<const float2*>(src)[e];
-                        x[i][j][0] = v.x; x[i][j][1] = v.y;
-                    }
+            for (int j = 0; j < kParts; ++j) {
+                const int e = min(tid + j * kPfThreads, nc * kParts - 1);
+                if constexpr (kV == 4) {
+                    const float4 v = reinterpret_cast<const float4*>(src)[e];
+                    x[i][j][0] = v.x; x[i][j][1] = v.y; x[i][j][2] = v.z; x[i][j][3] = v.w;
+                } else {
+                    const float2 v = reinterpret_cast<const float2*>(src)[e];
+                    x[i][j][0] = v.x; x[i][j][1] = v.y;
                 }
             }
+        }
 #pragma unroll
-            for (int i = 0; i < kIn; ++i) {
-                const int at = (i0 + i + w) & (NB - 1);
-                const bool zero = HV && ssq_is_heavy(a.heavy_mask[0], a.heavy_mask[1], at);
-                unsigned char* blk = pf_lds + at * 1024 * BD;
+        for (int i = 0; i < NB; ++i) {
+            unsigned char* blk = pf_lds + block(i) * 1024 * BD;
 #pragma unroll
-                for (int j = 0; j < kParts; ++j) {
-                    uint32_t hi[kV / 2], lo[kV / 2];
+            for (int j = 0; j < kParts; ++j) {
+                uint32_t hi[kV / 2], lo[kV / 2];
 #pragma unroll
-                    for (int k = 0; k < kV / 2; ++k) {
-                        pf_split<F16>(x[i][j][2 * k] * kLog2e, x[i][j][2 * k + 1] * kLog2e, hi[k], lo[k]);
-                        if (zero) hi[k] = lo[k] = 0;
-                    }
-                    // past the last codeword: it again
-                    unsigned char* dst = blk + min(tid + j * kPfThreads, nc * kParts - 1) * 2 * kV;
-                    if constexpr (BD == 2) {
-                        *reinterpret_cast<uint32_t*>(dst) = hi[0];
-                        *reinterpret_cast<uint32_t*>(dst + 512 * BD) = lo[0];
-                    } else {
-                        *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2*>(dst + 512 * BD) = make_uint2(lo[0], lo[1]);
-                    }
+                for (int k = 0; k < kV / 2; ++k) {
+                    pf_split<F16>(x[i][j][2 * k] * kLog2e, x[i][j][2 * k + 1] * kLog2e, hi[k], lo[k]);
+                    if (zero(i)) hi[k] = lo[k] = 0;
+                }
+                // past the last codeword: it again
+                unsigned char* dst = blk + min(tid + j * kPfThreads, nc * kParts - 1) * 2 * kV;
+                if constexpr (BD == 2) {
+                    *reinterpret_cast<uint32_t*>(dst) = hi[0];
+                    *reinterpret_cast<uint32_t*>(dst + 512 * BD) = lo[0];
+                } else {
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(dst + 512 * BD) = make_uint2(lo[0], lo[1]);
                 }
             }
         }

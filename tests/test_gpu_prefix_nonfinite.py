@@ -98,3 +98,25 @@ def test_queries_of_nan_under_other_codecs(kw):
     bad[1, 6, 1] = True
     assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
     assert torch.isfinite(out[~bad]).all() and torch.isfinite(lse[~bad]).all()
+
+
+@pytest.mark.parametrize("heavy, bd, D", [((1,), 4, 64), ((0, 5, 6), 4, 128), ((2,), 8, 64), ((3, 8), 8, 128), ((4, 9), 2, 64)])
+@pytest.mark.parametrize("dt", [BF, F16])
+def test_infinite_kept_dims(heavy, bd, D, dt):
+    """A kept key dim of infinity against a query dim of the other sign is a logit of -inf: a token that counts for
+    nothing, as one of -30,000 does."""
+    log(f"decode_prefix: infinite kept dims, heavy {heavy} of dims {bd}, head_dim {D}, {dt}")
+    p = _problem(B=3, Hq=8, Hkv=2, Lq=1, D=D, Dv=D, bd=bd, nc=256, T=150, lens=[70, 5, 0], heavy=heavy, qdt=dt, vdt=dt)
+    for h in range(2):  # the first kept dim's queries are 1
+        p["q"][:, h * 4:(h + 1) * 4, :, int(p["perm"][h, min(heavy) * bd])] = 1.0
+
+    def at(x):
+        pt = p["pt"].clone()
+        for t in (0, 33, 149):
+            pt[p["ptable"][t // 16].long(), :, t % 16, 0, 0] = x
+        pt[p["table"][0, 1].long(), :, 7, 0, 0] = x
+        return dict(p, pt=pt)
+
+    for kernel in (0, 1):
+        want, out = _call(at(-30000.0), kernel=kernel), _call(at(-math.inf), kernel=kernel)
+        assert torch.isfinite(want[0]).all() and torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), f"kernel {kernel}"

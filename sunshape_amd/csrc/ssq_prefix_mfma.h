@@ -14,7 +14,8 @@
 // K^T's operand is gathered codeword by codeword from the codebook in LDS: no key tile is ever written.  A
 // codeword is stored as two 16-bit parts, c = hi + lo (the rounding of c, and of what that left), and each 16 dims take
 // one MFMA with the hi parts and one with the lo parts against the same query operand, half as much matrix-core work
-// again.  Dropped is at most 2^-17 of a codeword with bf16 parts (one part would drop 2^-9), 2^-23 with f16 parts.
+// again.  Dropped is at most 2^-17 of a codeword with bf16 parts (one part would drop 2^-9); with f16 parts, which a
+// power of two per KV head keeps off the subnormals, 2^-22 of it or 2^-38 of the head's largest one.
 // Kept (passthrough) dims of a SunShape-Mixed codec, up to half of the head's, take a step per 16 more: their codewords are
 // staged as zeros, and a token's kept values, two 8-byte pieces a lane and step, enter exactly, into sums of their own.
 // Queries of 16 bits enter exactly (QT bf16 / f16); fp32 ones (rotated codecs) in two bf16 parts.
@@ -103,12 +104,10 @@ __device__ __forceinline__ float pf_lo(uint32_t w) { return F16 ? ssq_f16_to_f32
 template <bool F16>
 __device__ __forceinline__ float pf_hi(uint32_t w) { return F16 ? ssq_f16_to_f32(w >> 16) : __uint_as_float(w & 0xFFFF0000u); }
 
-// two fp32 values as packed parts; f16's reach to twice its largest value (log2(e) times a key's largest)
+// two fp32 values as packed parts
 template <bool F16>
 __device__ __forceinline__ void pf_split(float u, float v, uint32_t& hi, uint32_t& lo) {
-    constexpr float kTop = 65504.f;
-    if constexpr (F16) hi = pf_pack<true>(__builtin_amdgcn_fmed3f(u, -kTop, kTop), __builtin_amdgcn_fmed3f(v, -kTop, kTop));
-    else hi = pf_pack<false>(u, v);
+    hi = pf_pack<F16>(u, v);
     lo = pf_pack<F16>(u - pf_lo<F16>(hi), v - pf_hi<F16>(hi));
 }
 
@@ -150,6 +149,7 @@ struct PfRun {
     static constexpr int NK = HV ? L::kKeptMax / 16 : 0;  // steps of kept dims, at most
     static constexpr int KP = QT == kQtSplit && kVF16 ? 2 : 1;  // parts of a kept value: exact in its own type, or in two
     static constexpr bool kKept = HV;
+    static constexpr bool kScaled = kF16 && !HV;  // scores come times the codebook's scale
 
     struct Codes { uint32_t w[NW]; };
     struct Vals { uint4 v[2][DT]; };
@@ -163,6 +163,7 @@ struct PfRun {
 
     const SsqPrefixParams& p;
     int lane, half;
+    float inv;  // f16 parts: 1 / the codebook's scale
     uint32_t lds[2];
     uint4 q[QP][NR][NQ];
     // tokens
@@ -335,7 +336,7 @@ struct PfRun {
 #pragma unroll
             for (int r = 0; r < NR; ++r)
 #pragma unroll
-                for (int k = 0; k < 16; ++k) s[r][k] = __builtin_fmaf(t[r][k], kLog2e, s[r][k]);
+                for (int k = 0; k < 16; ++k) s[r][k] = __builtin_fmaf(t[r][k], kLog2e, kF16 ? s[r][k] * inv : s[r][k]);
             load_kept(i_kept);
         }
     }
@@ -467,7 +468,7 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
     if (n <= 0) return;  // wave-uniform
     typename Run::Codes c1 = first.c1, c2 = first.c2, c3 = first.c3;
     typename Run::Vals val = first.val;
-    pv16f s[NR];  // scores and m: log2 units, natural ones with a mask
+    pv16f s[NR];  // scores and m: log2 units (scores times the codebook's scale), natural ones with a mask
     float m[NR], mb[NR];  // mb: m, or 0 while that is -inf (as the scores are: their probabilities are 0)
 #pragma unroll
     for (int r = 0; r < NR; ++r) m[r] = -INFINITY;
@@ -481,7 +482,7 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     const int t = min(t_half + 16 * (k >> 3) + (k & 7), len - 1);
-                    s[r][k] = __builtin_fmaf(s[r][k], kLn2, mrow[r][(int64_t)t * u.p.a.m_st]);
+                    s[r][k] = __builtin_fmaf(s[r][k], Run::kScaled ? kLn2 * u.inv : kLn2, mrow[r][(int64_t)t * u.p.a.m_st]);
                 }
         }
         if (kPfTile * (tile + 1) > len) {  // uniform
@@ -506,7 +507,7 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
     };
     // a probability from its score
     auto prob = [&](float x, int r) {
-        return __builtin_amdgcn_exp2f(MASK ? (x - mb[r]) * kLog2e : x - mb[r]);
+        return __builtin_amdgcn_exp2f(MASK ? (x - mb[r]) * kLog2e : Run::kScaled ? __builtin_fmaf(x, u.inv, -mb[r]) : x - mb[r]);
     };
     // raises m to the scores' maximum, by[r] >= 0 log2 units
     auto raise = [&](float (&by)[NR]) {
@@ -516,6 +517,7 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
 #pragma unroll
             for (int k = 1; k < 16; ++k) top = pf_max(top, s[r][k]);
             top = pf_max(top, pf_other(top));
+            if (Run::kScaled && !MASK) top *= u.inv;
             const float mn = pf_max(m[r], top);
             by[r] = mn == -INFINITY ? 0.f : (mn - m[r]) * (MASK ? kLog2e : 1.f);
             m[r] = mn;
@@ -621,7 +623,7 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
 // free for the join.
 template <int D, int BD, int QT, int VT, int NR, bool HV>
 __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigned char* lds, int kv, int R0, int nr,
-                                               const uint16_t* permL, int len, int t0, int t1, int split, bool last) {
+                                               const uint16_t* permL, float inv, int len, int t0, int t1, int split, bool last) {
     using Run = PfRun<D, BD, QT, VT, NR, HV>;
     using L = PfLds<D>;
     const ssq_decode_args& a = p.a;
@@ -636,7 +638,7 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
     float* lL = mL + kPfWaves * 64;
     int64_t* rowL = reinterpret_cast<int64_t*>(lL + kPfWaves * 64);  // query rows' offsets, partial rows
     Run u{p};
-    u.lane = lane; u.half = half;
+    u.lane = lane; u.half = half; u.inv = inv;
     u.set_book(lds);
     pf_tokens(u, kv, p.ptab, len, t0 + wave, kPfWaves, (t1 - t0 - wave + kPfWaves - 1) / kPfWaves);
     const PfFirst<Run> first(u);
@@ -790,13 +792,13 @@ __device__ __forceinline__ void pf_prefix_item(const SsqPrefixParams& p, unsigne
 
 // An own item: rows [R0, R0 + nr) (nr <= 32) of one sequence over tiles [t0, t1) of its own tokens, by one wave.
 template <int D, int BD, int QT, int VT, bool MASK, bool HV>
-__device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsigned char* book, const uint16_t* permL, int kv,
-                                            int R0, int nr, const int32_t* table, int len, int t0, int t1, int split) {
+__device__ __forceinline__ void pf_own_item(const SsqPrefixParams& p, const unsigned char* book, const uint16_t* permL, float inv,
+                                            int kv, int R0, int nr, const int32_t* table, int len, int t0, int t1, int split) {
     using Run = PfRun<D, BD, QT, VT, 1, HV>;
     const ssq_decode_args& a = p.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     Run u{p};
-    u.lane = lane; u.half = half;
+    u.lane = lane; u.half = half; u.inv = inv;
     u.set_book(book);
     pf_tokens(u, kv, table, len, t0, 1, t1 - t0);
     // query operands straight from memory: a lane's row, its half of every 16 permuted dims, all loads in flight
@@ -885,7 +887,7 @@ __device__ __forceinline__ int pf_scan(int v) {
 // gives every wave of the KV head about one, numbered sequence by sequence; wave v takes pieces v, v + n_waves, ...
 // Every number follows from seq_lens, so all waves agree and a call repeats itself bit for bit.
 template <int D, int BD, int QT, int VT, bool HV>
-__device__ __forceinline__ void pf_own(const SsqPrefixParams& p, const unsigned char* book, const uint16_t* permL, int kv, int v) {
+__device__ __forceinline__ void pf_own(const SsqPrefixParams& p, const unsigned char* book, const uint16_t* permL, float inv, int kv, int v) {
     const ssq_decode_args& a = p.a;
     const int lane = threadIdx.x & 63;
     const int n_waves = p.n_wg * kPfWaves, ns = a.batch * p.own_rg, per_b = a.q_len * p.G;
@@ -925,8 +927,8 @@ __device__ __forceinline__ void pf_own(const SsqPrefixParams& p, const unsigned 
         const int t0 = split * per, t1 = min(t0 + per, __builtin_amdgcn_readlane(t, l));
         const int len = max(0, min(a.seq_lens[b], a.seq_len));
         const int32_t* table = a.block_table + (int64_t)b * a.bt_sb;
-        if (a.mask) pf_own_item<D, BD, QT, VT, true, HV>(p, book, permL, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
-        else pf_own_item<D, BD, QT, VT, false, HV>(p, book, permL, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
+        if (a.mask) pf_own_item<D, BD, QT, VT, true, HV>(p, book, permL, inv, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
+        else pf_own_item<D, BD, QT, VT, false, HV>(p, book, permL, inv, kv, b * per_b + r0, min(32, per_b - r0), table, len, t0, t1, split);
     }
 }
 
@@ -942,7 +944,8 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
     // a permuted dim's source, for this thread's staging and for the waves' own rows
     const int64_t pj = (int64_t)min((uint64_t)a.perm[(int64_t)kv * a.perm_sh + tid % D], (uint64_t)(D - 1));
     const int plen = p.n1 ? max(0, min(p.plen[0], p.pcap)) : 0;
-    // ---- the KV head's codebook times log2(e) as 16-bit parts: a thread takes the
+    float inv = 1.f;
+    // ---- the KV head's codebook times log2(e) (and, in f16 parts, a power of two) as 16-bit parts: a thread takes the
     // same codeword (or half of one, at 8 dims) of every block, all of them in flight; workgroups start at different
     // blocks, since those of one KV head share an L2
     {
@@ -968,6 +971,38 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
                 }
             }
         }
+        float unit = kLog2e;
+        if constexpr (F16) {
+            // The power of two takes the head's largest codeword to [2^13, 2^14): what the low parts drop, half a step of
+            // f16's subnormals (2^-25) where they are small, is then at most 2^-38 of it, whatever the keys' size.
+            // Scores are scaled back where the maximum is subtracted.  A codeword without a finite value does not count.
+            auto largest = [&](bool all) {
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    float t = 0.f;
+#pragma unroll
+                    for (int j = 0; j < kParts; ++j)
+#pragma unroll
+                        for (int k = 0; k < kV; ++k) {
+                            const float y = __builtin_fabsf(x[i][j][k]);
+                            t = pf_max(t, all || y < INFINITY ? y : 0.f);
+                        }
+                    top = pf_max(top, zero(i) ? 0.f : t);
+                }
+                return ssq_wave_max(top);
+            };
+            float top = largest(true);
+            if (!(top < INFINITY)) top = largest(false);  // uniform
+            float* topL = reinterpret_cast<float*>(pf_lds + L::kBook);
+            if ((tid & 63) == 0) topL[wave] = top;
+            __syncthreads();
+            top = fmaxf(fmaxf(topL[0], topL[1]), fmaxf(topL[2], topL[3]));
+            const int up = top > 0.f ? max(-100, min(100, 14 - __builtin_amdgcn_frexp_expf(top))) : 0;
+            unit = kLog2e * __uint_as_float((uint32_t)(127 + up) << 23);
+            inv = __uint_as_float((uint32_t)(127 - up) << 23);
+            inv = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(inv)));
+        }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             unsigned char* blk = pf_lds + block(i) * 1024 * BD;
@@ -976,7 +1011,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
                 uint32_t hi[kV / 2], lo[kV / 2];
 #pragma unroll
                 for (int k = 0; k < kV / 2; ++k) {
-                    pf_split<F16>(x[i][j][2 * k] * kLog2e, x[i][j][2 * k + 1] * kLog2e, hi[k], lo[k]);
+                    pf_split<F16>(x[i][j][2 * k] * unit, x[i][j][2 * k + 1] * unit, hi[k], lo[k]);
                     if (zero(i)) hi[k] = lo[k] = 0;
                 }
                 // past the last codeword: it again
@@ -1002,7 +1037,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
     }
     __syncthreads();
     // (from the last workgroup down: a small prefix has the first ones)
-    if (p.n2) pf_own<D, BD, QT, VT, HV>(p, pf_lds, permL, kv, (p.n_wg - 1 - w) * kPfWaves + wave);
+    if (p.n2) pf_own<D, BD, QT, VT, HV>(p, pf_lds, permL, inv, kv, (p.n_wg - 1 - w) * kPfWaves + wave);
     // ---- the prefix: slices past its length are not read by the merge either
     const int tiles = ssq_prefix_tiles(plen), per = p.n1 ? ssq_prefix_slice(plen, p.n1) : 0;
     const int n_pre = per ? p.n_rg * ((tiles + per - 1) / per) : 0;
@@ -1012,11 +1047,11 @@ __global__ __launch_bounds__(kPfThreads, 1) void k_prefix(const SsqPrefixParams 
         const int t0 = split * per, t1 = min(t0 + per, tiles);
         if constexpr (QT != kQtSplit && !HV) {
             if (p.pre_nr == 2) {
-                pf_prefix_item<D, BD, QT, VT, 2, HV>(p, pf_lds, kv, R0, nr, permL, plen, t0, t1, split, it + p.n_wg >= n_pre);
+                pf_prefix_item<D, BD, QT, VT, 2, HV>(p, pf_lds, kv, R0, nr, permL, inv, plen, t0, t1, split, it + p.n_wg >= n_pre);
                 continue;
             }
         }
-        pf_prefix_item<D, BD, QT, VT, 1, HV>(p, pf_lds, kv, R0, nr, permL, plen, t0, t1, split, it + p.n_wg >= n_pre);
+        pf_prefix_item<D, BD, QT, VT, 1, HV>(p, pf_lds, kv, R0, nr, permL, inv, plen, t0, t1, split, it + p.n_wg >= n_pre);
     }
 }
 

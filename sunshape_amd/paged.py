@@ -19,6 +19,7 @@ and values with the same for the keys, and the attention.
 
 from __future__ import annotations
 
+import contextlib
 from typing import Optional
 
 import torch
@@ -55,13 +56,28 @@ class PagedSunShapeCache:
         self.prefix_of: dict[int, int] = {}  # forked sequence -> the sequence it continues
 
     # ------------------------------------------------------------------ pages
-    def _ensure_capacity(self, seq_id: int, new_len: int) -> None:
-        table = self.block_tables.setdefault(seq_id, [])
-        need = (new_len + self.page_size - 1) // self.page_size
-        while len(table) < need:
-            if not self._free:
-                raise RuntimeError("PagedSunShapeCache is out of pages")
-            table.append(self._free.pop())
+    def _pages(self, length: int) -> int:
+        return (length + self.page_size - 1) // self.page_size
+
+    @contextlib.contextmanager
+    def _undone_if_refused(self, seq_ids: list[int]):
+        """Gives the sequences' new pages and tokens back if the body raises: a refused step leaves no unwritten
+        tokens behind."""
+        before = {s: (self.seq_lens.get(s), len(self.block_tables.get(s, ()))) for s in seq_ids}
+        try:
+            yield
+        except BaseException:
+            for s, (length, pages) in reversed(before.items()):
+                table = self.block_tables.get(s, [])
+                while len(table) > pages:
+                    self._free.append(table.pop())
+                if length is None:
+                    self.seq_lens.pop(s, None)
+                    if not pages:
+                        self.block_tables.pop(s, None)
+                else:
+                    self.seq_lens[s] = length
+            raise
 
     def free(self, seq_id: int) -> None:
         if seq_id in self.prefix_of.values():
@@ -96,14 +112,23 @@ class PagedSunShapeCache:
                             device=self.device).view(len(seq_ids), num_new)
 
     def slot_mapping(self, seq_ids: list[int], num_new: int) -> torch.Tensor:
-        """Allocate room for num_new tokens per sequence; return int64 slots [len(seq_ids), num_new]."""
-        rows = []
-        if any(s in self.prefix_of.values() for s in seq_ids):
+        """Allocate room for num_new tokens per sequence, for all or for none; return int64 slots
+        [len(seq_ids), num_new]."""
+        shared = set(self.prefix_of.values())
+        if any(s in shared for s in seq_ids):
             raise RuntimeError("a sequence that others continue takes no more tokens")
+        lengths: dict[int, int] = {}
+        for sid in seq_ids:
+            lengths[sid] = lengths.get(sid, self.seq_lens.get(sid, 0)) + num_new
+        missing = sum(max(0, self._pages(n) - len(self.block_tables.get(sid, ()))) for sid, n in lengths.items())
+        if missing > len(self._free):
+            raise RuntimeError("PagedSunShapeCache is out of pages")
+        rows = []
         for sid in seq_ids:
             start = self.seq_lens.get(sid, 0)
-            self._ensure_capacity(sid, start + num_new)
-            table = self.block_tables[sid]
+            table = self.block_tables.setdefault(sid, [])
+            while len(table) < self._pages(start + num_new):
+                table.append(self._free.pop())
             rows.append([table[(start + i) // self.page_size] * self.page_size + (start + i) % self.page_size
                          for i in range(num_new)])
             self.seq_lens[sid] = start + num_new
@@ -127,29 +152,31 @@ class PagedSunShapeCache:
                 raise RuntimeError("an append with rotation takes each sequence once")
             return self._append_raw(seq_ids, key_states, value_states, self.positions(seq_ids, S) if cos is not None else None,
                                     cos=cos, sin=sin, k_weight=k_weight, eps=eps, interleaved=interleaved)
-        slots = self.slot_mapping(seq_ids, S)
-        perm = self.codec.effective_permutation()
-        # as quantize_key_states: one reference cdist per (sequence, KV head) over its S new keys
-        hip_ops.encode(key_states.to(self.device), perm, self.codec.centroids, heavy=self.heavy,
-                       codes_out=self.code_pages, pt_out=self.pt_pages, slot_mapping=slots,
-                       metric=self.codec.encode_metric(), grid=self.codec.encode_search_grid(self.codec.centroids),
-                       direct=hip_ops.cdist_direct(S, self.codec.n_centroids),
-                       rotation=self.codec.rotation_matrix())
-        flat = slots.reshape(-1)
-        page, off = flat // self.page_size, flat % self.page_size
-        vals = value_states.to(self.device, self.v_pages.dtype).permute(0, 2, 1, 3).reshape(B * S, Hkv, self.value_dim)
-        self.v_pages[page, :, :, off] = vals
+        with self._undone_if_refused(seq_ids):
+            slots = self.slot_mapping(seq_ids, S)
+            perm = self.codec.effective_permutation()
+            # as quantize_key_states: one reference cdist per (sequence, KV head) over its S new keys
+            hip_ops.encode(key_states.to(self.device), perm, self.codec.centroids, heavy=self.heavy,
+                           codes_out=self.code_pages, pt_out=self.pt_pages, slot_mapping=slots,
+                           metric=self.codec.encode_metric(), grid=self.codec.encode_search_grid(self.codec.centroids),
+                           direct=hip_ops.cdist_direct(S, self.codec.n_centroids),
+                           rotation=self.codec.rotation_matrix())
+            flat = slots.reshape(-1)
+            page, off = flat // self.page_size, flat % self.page_size
+            vals = value_states.to(self.device, self.v_pages.dtype).permute(0, 2, 1, 3).reshape(B * S, Hkv, self.value_dim)
+            self.v_pages[page, :, :, off] = vals
         return slots
 
     def _append_raw(self, seq_ids, key_states, value_states, positions, **turn) -> torch.Tensor:
         S = key_states.shape[2]
-        slots = self.slot_mapping(seq_ids, S)
-        hip_ops.append_kv(key_states.to(self.device), value_states.to(self.device), self.codec.effective_permutation(),
-                          self.codec.centroids, codes_out=self.code_pages, v_out=self.v_pages, slot_mapping=slots,
-                          positions=positions, heavy=self.heavy, pt_out=self.pt_pages, metric=self.codec.encode_metric(),
-                          grid=self.codec.encode_search_grid(self.codec.centroids),
-                          direct=hip_ops.cdist_direct(S, self.codec.n_centroids),
-                          rotation=self.codec.rotation_matrix(), **turn)
+        with self._undone_if_refused(seq_ids):
+            slots = self.slot_mapping(seq_ids, S)
+            hip_ops.append_kv(key_states.to(self.device), value_states.to(self.device), self.codec.effective_permutation(),
+                              self.codec.centroids, codes_out=self.code_pages, v_out=self.v_pages, slot_mapping=slots,
+                              positions=positions, heavy=self.heavy, pt_out=self.pt_pages, metric=self.codec.encode_metric(),
+                              grid=self.codec.encode_search_grid(self.codec.centroids),
+                              direct=hip_ops.cdist_direct(S, self.codec.n_centroids),
+                              rotation=self.codec.rotation_matrix(), **turn)
         return slots
 
     def tables(self, seq_ids: list[int]) -> tuple[torch.Tensor, torch.Tensor]:
@@ -186,7 +213,7 @@ class PagedSunShapeCache:
                scale: Optional[float] = None) -> torch.Tensor:
         """One step over raw projections: query [B, Hq, S, D], keys and values [B, Hkv, S, ..] of the S next
         tokens of each sequence.  Norms and rotates them, appends keys and values, and attends causally;
-        returns [B, Hq, S, Dv]."""
+        returns [B, Hq, S, Dv].  A step that is refused leaves the sequences as they were."""
         B, _, S, _ = query.shape
         if len(set(seq_ids)) != len(seq_ids):
             raise RuntimeError("attend takes each sequence once")
@@ -197,13 +224,14 @@ class PagedSunShapeCache:
         self._shared_prefix(seq_ids)
         positions = self.positions(seq_ids, S)
         q, _ = hip_ops.qk_norm_rope(query, None, cos, sin, positions, q_weight=q_weight, eps=eps, interleaved=interleaved)
-        self._append_raw(seq_ids, key_states, value_states, positions, cos=cos, sin=sin, k_weight=k_weight, eps=eps,
-                         interleaved=interleaved)
-        mask = None
-        if S > 1:  # new token i sees its sequence up to itself
-            width = max(len(self.block_tables[s]) for s in seq_ids) * self.page_size
-            last = torch.tensor([self.seq_lens[s] - S for s in seq_ids], device=self.device)[:, None] + \
-                torch.arange(S, device=self.device)[None]
-            mask = torch.zeros(B, 1, S, width, device=self.device)
-            mask.masked_fill_(torch.arange(width, device=self.device) > last[:, None, :, None], float("-inf"))
-        return self.decode(seq_ids, q, scale=scale, mask=mask)
+        with self._undone_if_refused(seq_ids):
+            self._append_raw(seq_ids, key_states, value_states, positions, cos=cos, sin=sin, k_weight=k_weight, eps=eps,
+                             interleaved=interleaved)
+            mask = None
+            if S > 1:  # new token i sees its sequence up to itself
+                width = max(len(self.block_tables[s]) for s in seq_ids) * self.page_size
+                last = torch.tensor([self.seq_lens[s] - S for s in seq_ids], device=self.device)[:, None] + \
+                    torch.arange(S, device=self.device)[None]
+                mask = torch.zeros(B, 1, S, width, device=self.device)
+                mask.masked_fill_(torch.arange(width, device=self.device) > last[:, None, :, None], float("-inf"))
+            return self.decode(seq_ids, q, scale=scale, mask=mask)

@@ -111,6 +111,13 @@ class PagedSunShapeCache:
         return torch.tensor([[f + i for i in range(num_new)] for f in first], dtype=torch.int64,
                             device=self.device).view(len(seq_ids), num_new)
 
+    def _within(self, seq_ids: list[int], num_new: int, cos: torch.Tensor) -> None:
+        """The next tokens' positions lie inside the rotation's tables (past them a key would be NaN, and its codes
+        those of some other key)."""
+        end = max((self.seq_lens.get(s, 0) + self.seq_lens.get(self.prefix_of.get(s), 0) for s in seq_ids), default=0) + num_new
+        if num_new and cos.dim() == 2 and end > cos.shape[0]:
+            raise RuntimeError(f"position {end - 1} is outside the rotation's tables ({cos.shape[0]} rows)")
+
     def slot_mapping(self, seq_ids: list[int], num_new: int) -> torch.Tensor:
         """Allocate room for num_new tokens per sequence, for all or for none; return int64 slots
         [len(seq_ids), num_new]."""
@@ -141,7 +148,8 @@ class PagedSunShapeCache:
         """Encode keys [B, Hkv, S, D] into the code pages and write values [B, Hkv, S, Dv]; returns the slots.
 
         With cos and sin (tables, hip_ops.rope_table) or k_weight the keys are raw: they are normed and
-        rotated on the way, each token at its position in its sequence (its prefix counted)."""
+        rotated on the way, each token at its position in its sequence (its prefix counted), which the tables
+        have to reach."""
         B, Hkv, S, _ = key_states.shape
         if Hkv != self.num_kv_heads or value_states.shape[:3] != key_states.shape[:3]:
             raise RuntimeError("key/value shapes do not match the cache")
@@ -150,6 +158,8 @@ class PagedSunShapeCache:
                 raise RuntimeError(f"{B} rows of keys for {len(seq_ids)} sequences")
             if len(set(seq_ids)) != len(seq_ids):
                 raise RuntimeError("an append with rotation takes each sequence once")
+            if cos is not None:
+                self._within(seq_ids, S, cos)
             return self._append_raw(seq_ids, key_states, value_states, self.positions(seq_ids, S) if cos is not None else None,
                                     cos=cos, sin=sin, k_weight=k_weight, eps=eps, interleaved=interleaved)
         with self._undone_if_refused(seq_ids):
@@ -222,6 +232,7 @@ class PagedSunShapeCache:
         if key_states.shape[1] != self.num_kv_heads or value_states.shape[:3] != key_states.shape[:3]:
             raise RuntimeError("key/value shapes do not match the cache")
         self._shared_prefix(seq_ids)
+        self._within(seq_ids, S, cos)
         positions = self.positions(seq_ids, S)
         q, _ = hip_ops.qk_norm_rope(query, None, cos, sin, positions, q_weight=q_weight, eps=eps, interleaved=interleaved)
         with self._undone_if_refused(seq_ids):

@@ -105,3 +105,21 @@ def test_an_append_without_rotation_that_is_refused():
         with pytest.raises(RuntimeError):
             cache.append([1, 2], _rows(2, 3), _rows(2, 3), **kw)
         assert _state(cache) == before
+
+
+def test_positions_past_the_tables(stand_ins):
+    cache = _cache(num_pages=8)
+    cos, sin = hip_ops.rope_table(24, 64)
+    cache.attend([7], _rows(1, 20, 4), _rows(1, 20), _rows(1, 20), cos=cos, sin=sin)
+    cache.fork(7, [1])
+    before = _state(cache)
+    for ids, S in (([1], 5), ([2], 25)):
+        with pytest.raises(RuntimeError, match=r"outside the rotation's tables \(24 rows\)"):
+            cache.attend(ids, _rows(1, S, 4), _rows(1, S), _rows(1, S), cos=cos, sin=sin)
+        with pytest.raises(RuntimeError, match="outside the rotation's tables"):
+            cache.append(ids, _rows(1, S), _rows(1, S), cos=cos, sin=sin)
+        assert _state(cache) == before
+    cache.attend([1], _rows(1, 4, 4), _rows(1, 4), _rows(1, 4), cos=cos, sin=sin)  # up to the last row
+    cache.append([2], _rows(1, 24), _rows(1, 24), cos=cos, sin=sin)
+    cache.append([3], _rows(1, 30), _rows(1, 30), k_weight=torch.ones(64))  # no rotation, no end
+    cache.append([2], _rows(1, 0), _rows(1, 0), cos=cos, sin=sin)  # nothing new

@@ -153,6 +153,8 @@ class PagedSunShapeCache:
         B, Hkv, S, _ = key_states.shape
         if Hkv != self.num_kv_heads or value_states.shape[:3] != key_states.shape[:3]:
             raise RuntimeError("key/value shapes do not match the cache")
+        if (cos is None) != (sin is None):
+            raise RuntimeError("cos and sin come together")
         if cos is not None or k_weight is not None:
             if len(seq_ids) != B:
                 raise RuntimeError(f"{B} rows of keys for {len(seq_ids)} sequences")

@@ -123,3 +123,13 @@ def test_positions_past_the_tables(stand_ins):
     cache.append([2], _rows(1, 24), _rows(1, 24), cos=cos, sin=sin)
     cache.append([3], _rows(1, 30), _rows(1, 30), k_weight=torch.ones(64))  # no rotation, no end
     cache.append([2], _rows(1, 0), _rows(1, 0), cos=cos, sin=sin)  # nothing new
+
+
+def test_a_sine_without_its_cosine():
+    """append takes both tables or neither: one alone is refused, not left aside."""
+    cache = _cache()
+    _, sin = hip_ops.rope_table(24, 64)
+    before = _state(cache)
+    with pytest.raises(RuntimeError, match="cos and sin"):
+        cache.append([1], _rows(1, 3), _rows(1, 3), sin=sin)
+    assert _state(cache) == before

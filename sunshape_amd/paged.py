@@ -90,7 +90,7 @@ class PagedSunShapeCache:
     def fork(self, prefix_id: int, seq_ids: list[int]) -> None:
         """Start empty sequences that continue prefix_id's tokens.  The prefix takes no more tokens while
         any of them lives."""
-        if prefix_id not in self.seq_lens or prefix_id in self.prefix_of:
+        if not self.seq_lens.get(prefix_id) or prefix_id in self.prefix_of:
             raise RuntimeError(f"sequence {prefix_id} cannot be a prefix: it holds no tokens or continues another")
         if len(set(seq_ids)) != len(seq_ids) or any(s == prefix_id or s in self.seq_lens or s in self.prefix_of
                                                     for s in seq_ids):

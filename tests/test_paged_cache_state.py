@@ -133,3 +133,14 @@ def test_a_sine_without_its_cosine():
     with pytest.raises(RuntimeError, match="cos and sin"):
         cache.append([1], _rows(1, 3), _rows(1, 3), sin=sin)
     assert _state(cache) == before
+
+
+def test_fork_of_a_sequence_without_tokens(stand_ins):
+    cache = _cache()
+    cache.append([1], _rows(1, 0), _rows(1, 0))
+    for prefix in (1, 9):
+        with pytest.raises(RuntimeError, match="holds no tokens"):
+            cache.fork(prefix, [2])
+    assert cache.prefix_of == {}
+    cache.append([1], _rows(1, 1), _rows(1, 1), k_weight=torch.ones(64))
+    cache.fork(1, [2])

@@ -176,8 +176,9 @@ def mask_words_signed(mask) -> tuple[int, int]:
     """heavy_mask_words as two signed int64 (the operators' int arguments), cached per mask tuple."""
     key = None
     if mask is not None:
-        seq = mask.tolist() if hasattr(mask, "tolist") else mask
-        key = tuple(seq) if set(map(type, seq)) == {bool} else tuple(bool(x) for x in seq)
+        key = tuple(mask.tolist() if hasattr(mask, "tolist") else mask)
+        if set(map(type, key)) != {bool}:
+            key = tuple(bool(x) for x in key)
     hit = _WORDS.get(key)
     if hit is None:
         w0, w1 = heavy_mask_words(key)

@@ -517,6 +517,10 @@ __global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
     if (put) store_code(a.codes, cw, crow + blk, j_best);
 }
 
+bool uses_grid(const ssq_encode_args& e) {  // as ssq_encode chooses
+    return e.kernel == 0 && e.grid && !e.direct_dist && ssq_encode_grid_supported(&e);
+}
+
 int check(const ssq_append_args* a) {
     if (!a) return ssq_fail(SSQ_ERR_INVALID, "args is NULL");
     if (a->struct_size != sizeof(ssq_append_args))
@@ -545,6 +549,12 @@ int check(const ssq_append_args* a) {
     SSQ_REQUIRE(e.direct_dist == 0 || e.direct_dist == 1, "direct_dist must be 0 or 1");
     // 2 and 3 serve some codebooks only; a refusal by ssq_encode would come after the values are written
     SSQ_UNSUPPORTED(e.kernel == 0 || e.kernel == 1, "append takes kernel 0, or 1 for the exact scan, not %d", e.kernel);
+    if (uses_grid(e)) {  // likewise
+        const uint64_t need = ssq_encode_grid_bytes(&e);
+        SSQ_REQUIRE((uintptr_t)e.grid % 16 == 0, "the grid must be 16-byte aligned");
+        SSQ_REQUIRE(e.grid_bytes >= need, "grid too small for this codebook (%llu < %llu bytes)",
+                    (unsigned long long)e.grid_bytes, (unsigned long long)need);
+    }
     int rc = ssq_rope_check(a->rope, e.head_dim, a->k_weight != nullptr);
     if (rc) return rc;
     if (a->v) {
@@ -567,8 +577,7 @@ int check(const ssq_append_args* a) {
 bool few(const ssq_append_args& a) {
     const ssq_encode_args& e = a.enc;
     if (e.kernel != 0) return false;
-    const bool grid = e.grid && !e.direct_dist && ssq_encode_grid_supported(&e);
-    const bool scan = !grid && (e.n_centroids < 256 || (e.n_centroids == 256 && (e.direct_dist || e.block_dim > 10)));
+    const bool scan = !uses_grid(e) && (e.n_centroids < 256 || (e.n_centroids == 256 && (e.direct_dist || e.block_dim > 10)));
     const int64_t rows = (int64_t)e.batch * e.seq_len * e.num_kv_heads * e.n_blocks;
     return scan ? rows <= 1 << 26 : rows <= 1 << 24 && rows * e.n_centroids <= 1 << 24;
 }

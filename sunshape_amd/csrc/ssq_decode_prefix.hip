@@ -462,6 +462,19 @@ int make_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
 
 }  // namespace
 
+// A call's plan, for tests that mean to reach a form of the matrix-core kernel (zeros where it does not serve the
+// call): rows of a prefix item / 32, row groups, slices, workgroups per KV head, own pieces at most, their fewest tiles.
+int ssq_decode_prefix_plan(const ssq_prefix_args* a, int32_t* out) {
+    PrefixPlan pl;
+    int rc = check(a);
+    if (rc == SSQ_OK) rc = make_plan(*a, pl);
+    if (rc) return rc;
+    const SsqPrefixParams f = pl.fast ? pl.fp : SsqPrefixParams{};
+    const int32_t v[6] = {f.n1 ? f.pre_nr : 0, f.n_rg, f.n1, f.n_wg, f.n2, f.own_min};
+    for (int i = 0; i < 6; ++i) out[i] = v[i];
+    return SSQ_OK;
+}
+
 extern "C" size_t ssq_decode_prefix_workspace_size(const ssq_prefix_args* a) {
     PrefixPlan pl;
     if (check(a) != SSQ_OK || make_plan(*a, pl) != SSQ_OK) return 0;

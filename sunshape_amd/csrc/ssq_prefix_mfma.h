@@ -509,14 +509,17 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
     auto prob = [&](float x, int r) {
         return __builtin_amdgcn_exp2f(MASK ? (x - mb[r]) * kLog2e : Run::kScaled ? __builtin_fmaf(x, u.inv, -mb[r]) : x - mb[r]);
     };
+    auto top_of = [&](int r) {
+        float top = s[r][0];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) top = pf_max(top, s[r][k]);
+        return pf_max(top, pf_other(top));
+    };
     // raises m to the scores' maximum, by[r] >= 0 log2 units
     auto raise = [&](float (&by)[NR]) {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            float top = s[r][0];
-#pragma unroll
-            for (int k = 1; k < 16; ++k) top = pf_max(top, s[r][k]);
-            top = pf_max(top, pf_other(top));
+            float top = top_of(r);
             if (Run::kScaled && !MASK) top *= u.inv;
             const float mn = pf_max(m[r], top);
             by[r] = mn == -INFINITY ? 0.f : (mn - m[r]) * (MASK ? kLog2e : 1.f);
@@ -560,15 +563,19 @@ __device__ __forceinline__ void pf_tiles(Run& u, const PfFirst<Run>& first, cons
                     else e0[r] = e;
                 }
         });
-        // While a row has met hidden tokens only (m -inf), its probabilities, taken against 0, may underflow whatever
-        // the scores are: these decide, not the sum.
         bool over = false;
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
             for (int dt = 0; dt < Run::DT; ++dt) pf_pin(o[r][dt]);
+        // While a row has met hidden tokens only (m -inf), its probabilities, taken against 0, may underflow whatever
+        // the scores are: these decide, not the sum.
 #pragma unroll
-        for (int r = 0; r < NR; ++r) over |= lt[r] > (m[r] == -INFINITY ? -1.f : kPfOver);
+        for (int r = 0; r < NR; ++r) {
+            const bool none = m[r] == -INFINITY;
+            over |= lt[r] > (none && !MASK ? -1.f : kPfOver);
+            if (MASK && __builtin_amdgcn_ballot_w64(none) != 0) over |= none && top_of(r) > -INFINITY;
+        }
         if (__builtin_amdgcn_ballot_w64(over) != 0) {  // m moves: once more from the scores
             raise(by);
 #pragma unroll

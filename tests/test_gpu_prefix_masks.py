@@ -115,3 +115,15 @@ def test_graph_replays_with_hidden_tiles():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want[0]) and torch.equal(lse, want[1]), first
+
+
+@pytest.mark.parametrize("kw", [dict(nc=4096), dict(D=256, Dv=256), dict(nc=64, bd=2, vdt=F32), dict(D=128, Dv=64), dict(bd=1, nc=16),
+                                dict(D=128, Dv=128, heavy=tuple(range(20))), dict(page=8)])
+def test_hidden_tiles_under_other_codecs(kw):
+    """The forms that take the decode kernels by chunks of rows."""
+    log(f"decode_prefix: hidden tiles, {kw}")
+    for T in (0, 45):
+        p = _problem(T=T, **{**BASE, "Hq": 8, **kw})
+        _low(p, -95.0 * math.sqrt(p["q"].shape[-1]) / 8)
+        out, lse = _call(_hide(p, [32, 96, 0, 64]))
+        _check(p, out, lse, "other codecs")

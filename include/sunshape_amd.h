@@ -323,7 +323,8 @@ int ssq_append(const ssq_append_args* a, void* workspace, size_t workspace_bytes
  * of a KV head at a time, whichever sequences they belong to.
  * dec: SSQ_PAGED with v; block_table / seq_lens / seq_len / mask speak of the sequences' own tokens
  * (seq_len 0: none, block_table may be NULL); scores NULL; kernel 0, or 1 for the path that serves every codec.
- * A row with nothing to attend (both lengths 0, or a mask of -inf) gives out 0 and lse -inf.
+ * A row with nothing to attend (both lengths 0, or a mask of -inf) gives out 0 and lse -inf; one whose query
+ * holds a NaN gives NaN.
  * No counterpart in the reference. */
 typedef struct ssq_prefix_args {
     uint32_t struct_size;

@@ -7,11 +7,11 @@
 // lanes.  The first workgroups write the values.  Loads that wait for one another bound it, so the keys' whole
 // rows (which the norm needs anyhow), the codebook, the permutation, slots and positions are all asked for at once,
 // and only the table's and weights' entries after them.  64 sequences' step (8 heads of 128 dims, 256 codewords of dim
-// 4, norm and rotation, values): 9.1 us, of which 1.0 the values, 1.1 the norm, 0.9 the rotation, 2 the scan's
-// vector instructions and about 4 the launch and the first loads.
+// 4, norm and rotation, values): 9.3 us in a trace (8.2 a call among others, whose launches overlap), of which 1.0 the
+// values, 1.1 the norm, 0.9 the rotation, 2 the scan's vector instructions and about 4 the launch and the first loads.
 //
 // Many rows: k_append_prep writes the pages' values and the rotated keys side by side, and ssq_encode, which is
-// where the time goes, takes those.  8,192 tokens of the same layer: 20.0 us for 67 MB (3.4 TB/s) and 62 us.
+// where the time goes, takes those.  8,192 tokens of the same layer: 19.8 us for 67 MB (3.4 TB/s) and 61.5 us.
 #include "ssq_encode_math.h"
 #include "ssq_rope.h"
 

@@ -320,7 +320,9 @@ void fast_plan(const ssq_prefix_args& a, PrefixPlan& pl) {
         // and 1.35 per tile of a wave with 64 rows, 3 and 0.98 with 32 (twice the gathers, but fewer queries to move
         // through LDS); and 6 where the prefix's items leave a KV head too few workgroups for its own items, which then
         // wait for one another.  8 heads of 128 dims, 4 query heads each, 64 own tokens, us with 32 and with 64 rows:
-        // 16 sequences on 4,096 tokens 19.9 and 22.9, on 65,536 55.8 and 49.9; 48 sequences 26.4 and 27.1, 129 and 97.
+        // 16 sequences on 4,096 tokens 19.7 and 21.6, on 65,536 53.4 and 49.2; 48 sequences 25.9 and 25.8, 122 and 95.6.
+        // The costs are those of 128 dims; at 64 the choice is the same but for close calls: 14.6 and 15.8, 41.6 and
+        // 37.4; 20.2 and 19.9, 94.2 and 74.9; of 2 heads with 7 each, 128 sequences on 8,192 28.8, the choice, and 26.2.
         // Workgroups left for the own items or not: 8 sequences on 4,096 tokens 18.6 and 26.0, 48 on 1,000 19.8
         // and 26.1.  Split queries and kept dims leave no registers for 64 rows.
         const int most = split || f.kept || f.rows <= 32 ? 1 : 2, tiles = (a.prefix_cap + 31) / 32;

@@ -18,8 +18,10 @@
 // power of two per KV head keeps off the subnormals, 2^-22 of it or 2^-38 of the head's largest one.
 // Kept (passthrough) dims of a SunShape-Mixed codec, up to half of the head's, take a step per 16 more: their codewords are
 // staged as zeros, and a token's kept values, two 8-byte pieces a lane and step, enter exactly, into sums of their own.
-// Queries of 16 bits enter exactly (QT bf16 / f16); fp32 ones (rotated codecs) in two bf16 parts.
-// Probabilities are rounded to the values' 16 bits for P.V, as in the other decode kernels; sums stay fp32.
+// Queries of 16 bits enter exactly (QT bf16 / f16); fp32 ones (rotated codecs) in two bf16 parts (2^-17 of a query dim
+// is dropped; an infinite kept dim against a part of 0 gives NaN there).
+// Probabilities are rounded to the values' 16 bits for P.V, as in the other decode kernels (two parts would take those
+// products twice); sums stay fp32.
 //
 // A workgroup (one per CU: the codebook fills the LDS, 128 KiB at head_dim 128) stages its KV head's codebook once
 // and takes items in turn.  A prefix item is a group of 32 NR rows (NR 2: 64 rows per gathered operand, which the
@@ -29,12 +31,16 @@
 // (matrix cores).
 //
 // Measured, one MI355X, whole calls with the merge: 128 sequences of 64 query heads (8 KV heads of 128 dims, byte codes of
-// dim 4) on a prefix of 65,536 tokens with up to 1,024 own ones 412 us, 64 sequences of 32 on 32,768 76; attending every
-// sequence's copy of the prefix by itself, 64 on 8,192: 122 against 55.  A tile of 32 tokens and 64 rows takes a wave
+// dim 4) on a prefix of 65,536 tokens with up to 1,024 own ones 415-424 us, 64 sequences of 32 on 32,768 73-76; attending
+// every sequence's copy of the prefix by itself, 64 on 8,192: 122 against 55.  A tile of 32 tokens and 64 rows takes a wave
 // 1.35 us, where the rate of a large library product (1.39 PFLOP/s) would take 1.16 for its 48 MFMAs, and the MFMAs
 // alone, in this loop, 1.0: the matrix cores bound long prefixes, at 86 % of the rate that they reach.  Of a short one's
 // 50 us, 3 to 4 are the codebook's staging, 3 the queries', 2.5 the first loads, 4 the join, 9 the own
 // items, 8 the merge (a launch of its own).
+//
+// A row's maximum is its first tile's until the probabilities outgrow kPfOver; while a mask has hidden all its tokens
+// there is none, and the first visible score sets it.  An infinite or NaN value counts wherever its tile is, also at
+// probability 0 (0 times infinity is NaN), and a row of NaN scores is NaN, not one with nothing to attend.
 #pragma once
 
 #include "ssq_common.h"

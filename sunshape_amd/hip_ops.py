@@ -333,8 +333,8 @@ def decode_prefix(q: torch.Tensor, codes: torch.Tensor, v: torch.Tensor, perm: t
     and lengths of 0 are fine).  All lengths stay on the device.  mask: additive, broadcastable to
     [B, Hq, Lq, max_pages * page], over the own tokens (the prefix is seen by every row).
     Returns out [B, Hq, Lq, Dv] in v's dtype, and lse [B, Hq, Lq] (fp32) when requested; a row with
-    nothing to attend gives 0 and -inf.  kernel 1 takes the decode kernels that serve every codec,
-    for comparisons.  No counterpart in the reference.
+    nothing to attend gives 0 and -inf, one whose query holds a NaN gives NaN.  kernel 1 takes the decode
+    kernels that serve every codec, for comparisons.  No derivative; no counterpart in the reference.
     """
     if not (q.is_cuda and codes.is_cuda and v.is_cuda):
         for name, t in (("query", q), ("codes", codes), ("value", v)):
@@ -377,8 +377,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: Optional[torch
     None for all three: norm only.  q_weight / k_weight [D]: norm weights of any of the dtypes, shared
     by the heads; None: no norm.  Computed in fp32 (the norm's sum in 64 bits) and rounded once.
     Returns new tensors in the inputs' stride order, (q, k) or (q, None).  A position outside the
-    tables makes the row's rotated dims NaN.  No counterpart in the reference, whose model code
-    rotates before the cache sees the keys.
+    tables makes the row's rotated dims NaN.  No derivative: for serving, not for a training step (a backward
+    pass through the result gives none, with torch's warning).  No counterpart in the reference, whose
+    model code rotates before the cache sees the keys.
     """
     if not q.is_cuda:
         _on_gpu("query", q)
@@ -406,7 +407,8 @@ def append_kv(keys: torch.Tensor, values: Optional[torch.Tensor], perm: torch.Te
     does, into codes_out [P, Hkv, page, nb] and, for heavy blocks, pt_out [P, Hkv, page, slots, bd];
     values go to v_out [P, Hkv, Dv, page], converted to its dtype.  metric, grid, direct and rotation (the
     codec's rotated mode, after the position rotation) as in encode(); kernel: 0, or 1 for the exact
-    scan.  No counterpart in the reference.
+    scan.  A position outside the tables stores the codes of a NaN key.  No derivative; no counterpart in
+    the reference.
     """
     if not keys.is_cuda:
         _on_gpu("key_states", keys)

@@ -225,7 +225,8 @@ class PagedSunShapeCache:
                scale: Optional[float] = None) -> torch.Tensor:
         """One step over raw projections: query [B, Hq, S, D], keys and values [B, Hkv, S, ..] of the S next
         tokens of each sequence.  Norms and rotates them, appends keys and values, and attends causally;
-        returns [B, Hq, S, Dv].  A step that is refused leaves the sequences as they were."""
+        returns [B, Hq, S, Dv].  scale as in decode (None: the query as it is).  A step that is refused leaves the
+        sequences as they were.  With S > 1 the causal mask takes 4 B S times the longest own table's tokens in bytes."""
         B, _, S, _ = query.shape
         if len(set(seq_ids)) != len(seq_ids):
             raise RuntimeError("attend takes each sequence once")

@@ -204,8 +204,8 @@ class PagedSunShapeCache:
     def decode(self, seq_ids: list[int], query: torch.Tensor, *, scale: Optional[float] = None,
                return_lse: bool = False, mask: Optional[torch.Tensor] = None):
         """Fused decode of query [B, Hq, Lq, D] against the cached sequences; forked ones attend their shared
-        prefix's tokens first (the sequences of one call continue the same one, or none).  mask: additive, broadcastable to [B, Hq, Lq, T], T the sequences' own
-        table width times the page size."""
+        prefix's tokens first (the sequences of one call continue the same one, or none).  mask: additive,
+        broadcastable to [B, Hq, Lq, T], T the sequences' own table width times the page size."""
         prefix = self._shared_prefix(seq_ids)
         bt, lens = self.tables(seq_ids)
         if prefix is None:

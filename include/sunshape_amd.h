@@ -44,7 +44,8 @@ enum ssq_status {
     SSQ_ERR_UNSUPPORTED = 4 /* valid input outside what the kernels implement */
 };
 
-enum ssq_dtype { SSQ_F32 = 0, SSQ_BF16 = 1, SSQ_F16 = 2 };
+enum ssq_dtype { SSQ_F32 = 0, SSQ_BF16 = 1, SSQ_F16 = 2,
+                 SSQ_E4M3 = 3 /* 8-bit values (OCP e4m3fn) of ssq_append_values and ssq_decode_window only */ };
 
 /* Width of the stored codes, as the reference's _compact_index_dtype (sunshape/codec.py:78-83):
  * one byte for n_centroids <= 256, 16 bits (read unsigned) up to 65535, 32 bits beyond, at most
@@ -336,6 +337,79 @@ typedef struct ssq_prefix_args {
 
 size_t ssq_decode_prefix_workspace_size(const ssq_prefix_args* a);
 int ssq_decode_prefix(const ssq_prefix_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Values to 8-bit pages (no counterpart in the reference): v[b*v_sb + kv*v_sh + s*v_ss + d] (d < value_dim) goes to
+ * v_pages[page*vp_sb + kv*vp_sh + d*vp_sd + off] as e4m3(v / s), s = v_scale[page*vs_sb + kv*vs_sh], slot =
+ * slot_mapping[b*sm_sb + s] = page * page_size + off.  s is the smallest power of two >= 2^-100 with |v| <= 448 s for the
+ * finite values of the page's tokens, and no less than it was unless offset 0 is among the new ones; the page's earlier
+ * tokens (those before its first new one) are taken to a grown s.  NaN and infinities are stored as NaN.  A negative
+ * slot, or one past the pages, is padding.  The slots of a call are distinct, and those of one page stand in one row b
+ * with nothing but padding between them.  page_size: a multiple of 16; value rows 16-byte aligned.
+ */
+typedef struct ssq_values_args {
+    uint32_t struct_size;
+    const void* v; int32_t v_dtype; int64_t v_sb, v_sh, v_ss;
+    int32_t batch, num_kv_heads, seq_len, value_dim;
+    void* v_pages; int64_t vp_sb, vp_sh, vp_sd;
+    float* v_scale; int64_t vs_sb, vs_sh;
+    const int64_t* slot_mapping; int64_t sm_sb;
+    int32_t page_size;
+    int64_t num_pages;
+} ssq_values_args;
+
+int ssq_append_values(const ssq_values_args* a, void* stream);
+
+/* ssq_append with the values in 8 bits: app.v_pages holds e4m3 (app.vp_dtype SSQ_E4M3) and v_scale / vs_sb / vs_sh its
+ * scales, as for ssq_append_values. */
+typedef struct ssq_append8_args {
+    uint32_t struct_size;
+    ssq_append_args app;
+    float* v_scale; int64_t vs_sb, vs_sh;
+} ssq_append8_args;
+
+size_t ssq_append8_workspace_size(const ssq_append8_args* a);
+int ssq_append8(const ssq_append8_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Causal attention of the newest tokens over pages, with a sliding window and first tokens that stay visible (no
+ * counterpart in the reference).  dec: SSQ_PAGED with v, no mask, no scores; the q_len rows of sequence b are its newest
+ * tokens, appended already: row i stands at p = seq_lens[b] - q_len + i and sees token j iff j <= p and (window == 0 or
+ * j > p - window or j < sinks).  A row that sees nothing (p < 0) gives 0 and lse -inf; one whose query holds a
+ * NaN or an infinity gives NaN.  Pages that no row sees are not read, whatever the tables say of them, and a table's
+ * entry outside [0, num_pages) is taken into it.  dec.v_dtype SSQ_E4M3: 8-bit values times v_scale[page*vs_sb + kv*vs_sh]
+ * (positive); SSQ_BF16 or SSQ_F16: v_scale NULL.  out is of out_dtype.  Serves byte codes of dims 2, 4 or 8 (at most 256
+ * codewords, no passthrough blocks), head_dim 64 or 128, value_dim the same, page sizes of 16 to 256.
+ */
+typedef struct ssq_window_args {
+    uint32_t struct_size;
+    ssq_decode_args dec;
+    int32_t window, sinks;
+    int32_t out_dtype;
+    int64_t num_pages;
+    const float* v_scale; int64_t vs_sb, vs_sh;
+} ssq_window_args;
+
+size_t ssq_decode_window_workspace_size(const ssq_window_args* a);
+int ssq_decode_window(const ssq_window_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copies pages (no counterpart in the reference): for every pool, page to[i] of dst becomes page from[i] of src, i <
+ * n_pairs (device int64 arrays).  A page is `bytes` consecutive bytes, *_stride bytes from the next.  Pairs with an
+ * index outside the pools are left out.  No page is written twice, nor both read and written. */
+#define SSQ_COPY_POOLS 8
+typedef struct ssq_copy_pool {
+    const void* src; void* dst;
+    int64_t src_stride, dst_stride, src_pages, dst_pages, bytes;
+} ssq_copy_pool;
+typedef struct ssq_copy_args {
+    uint32_t struct_size;
+    int32_t n_pools;
+    ssq_copy_pool pool[SSQ_COPY_POOLS];
+    const int64_t* from; const int64_t* to;
+    int64_t n_pairs;
+} ssq_copy_args;
+
+int ssq_copy_pages(const ssq_copy_args* a, void* stream);
 
 const char* ssq_last_error(void);
 int ssq_abi_version(void);

@@ -145,3 +145,91 @@ class PrefixArgs(ctypes.Structure):
         self.dec.struct_size = ctypes.sizeof(DecodeArgs)
         for k, v in kw.items():
             setattr(self, k, v)
+
+
+class ValuesArgs(ctypes.Structure):
+    """Mirror of ``ssq_values_args``."""
+
+    _fields_ = [
+        ("struct_size", _u32),
+        ("v", _vp), ("v_dtype", _i32), ("v_sb", _i64), ("v_sh", _i64), ("v_ss", _i64),
+        ("batch", _i32), ("num_kv_heads", _i32), ("seq_len", _i32), ("value_dim", _i32),
+        ("v_pages", _vp), ("vp_sb", _i64), ("vp_sh", _i64), ("vp_sd", _i64),
+        ("v_scale", _vp), ("vs_sb", _i64), ("vs_sh", _i64),
+        ("slot_mapping", _vp), ("sm_sb", _i64),
+        ("page_size", _i32),
+        ("num_pages", _i64),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(ValuesArgs)
+        for k, v in kw.items():
+            setattr(self, k, v)
+
+
+class Append8Args(ctypes.Structure):
+    """Mirror of ``ssq_append8_args``."""
+
+    _fields_ = [
+        ("struct_size", _u32),
+        ("app", AppendArgs),
+        ("v_scale", _vp), ("vs_sb", _i64), ("vs_sh", _i64),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(Append8Args)
+        self.app.struct_size = ctypes.sizeof(AppendArgs)
+        self.app.enc.struct_size = ctypes.sizeof(EncodeArgs)
+        for k, v in kw.items():
+            setattr(self, k, v)
+
+
+class WindowArgs(ctypes.Structure):
+    """Mirror of ``ssq_window_args``."""
+
+    _fields_ = [
+        ("struct_size", _u32),
+        ("dec", DecodeArgs),
+        ("window", _i32), ("sinks", _i32),
+        ("out_dtype", _i32),
+        ("num_pages", _i64),
+        ("v_scale", _vp), ("vs_sb", _i64), ("vs_sh", _i64),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(WindowArgs)
+        self.dec.struct_size = ctypes.sizeof(DecodeArgs)
+        for k, v in kw.items():
+            setattr(self, k, v)
+
+
+COPY_POOLS = 8  # SSQ_COPY_POOLS
+
+
+class CopyPool(ctypes.Structure):
+    """Mirror of ``ssq_copy_pool``."""
+
+    _fields_ = [
+        ("src", _vp), ("dst", _vp),
+        ("src_stride", _i64), ("dst_stride", _i64), ("src_pages", _i64), ("dst_pages", _i64), ("bytes", _i64),
+    ]
+
+
+class CopyArgs(ctypes.Structure):
+    """Mirror of ``ssq_copy_args``."""
+
+    _fields_ = [
+        ("struct_size", _u32), ("n_pools", _i32),
+        ("pool", CopyPool * COPY_POOLS),
+        ("src_pages", _vp), ("dst_pages", _vp),
+        ("n_pairs", _i64),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(CopyArgs)
+        for k, v in kw.items():
+            setattr(self, k, v)

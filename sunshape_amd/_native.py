@@ -26,6 +26,7 @@ SSQ_ERR_ABI = 3
 SSQ_ERR_UNSUPPORTED = 4
 
 SSQ_F32, SSQ_BF16, SSQ_F16 = 0, 1, 2
+SSQ_E4M3 = 3  # 8-bit values
 SSQ_CONTIGUOUS, SSQ_PAGED = 0, 1
 
 DTYPE_CODE = {torch.float32: SSQ_F32, torch.bfloat16: SSQ_BF16, torch.float16: SSQ_F16}
@@ -52,11 +53,18 @@ EXPORTED_SYMBOLS = (
     "ssq_append",
     "ssq_decode_prefix_workspace_size",
     "ssq_decode_prefix",
+    "ssq_append_values",
+    "ssq_append8_workspace_size",
+    "ssq_append8",
+    "ssq_decode_window_workspace_size",
+    "ssq_decode_window",
+    "ssq_copy_pages",
     "ssq_last_error",
     "ssq_abi_version",
 )
 
-from ._abi import AppendArgs, DecodeArgs, EncodeArgs, PrefixArgs, Rope, RopeArgs  # noqa: E402  (the structs, torch-free)
+from ._abi import (Append8Args, AppendArgs, CopyArgs, DecodeArgs, EncodeArgs, PrefixArgs, Rope, RopeArgs,  # noqa: E402
+                   ValuesArgs, WindowArgs)  # the structs, torch-free
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -108,6 +116,18 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ssq_decode_prefix_workspace_size.restype = ctypes.c_size_t
     lib.ssq_decode_prefix.argtypes = [P(PrefixArgs), _vp, ctypes.c_size_t, _vp]
     lib.ssq_decode_prefix.restype = ctypes.c_int
+    lib.ssq_append_values.argtypes = [P(ValuesArgs), _vp]
+    lib.ssq_append_values.restype = ctypes.c_int
+    lib.ssq_append8_workspace_size.argtypes = [P(Append8Args)]
+    lib.ssq_append8_workspace_size.restype = ctypes.c_size_t
+    lib.ssq_append8.argtypes = [P(Append8Args), _vp, ctypes.c_size_t, _vp]
+    lib.ssq_append8.restype = ctypes.c_int
+    lib.ssq_decode_window_workspace_size.argtypes = [P(WindowArgs)]
+    lib.ssq_decode_window_workspace_size.restype = ctypes.c_size_t
+    lib.ssq_decode_window.argtypes = [P(WindowArgs), _vp, ctypes.c_size_t, _vp]
+    lib.ssq_decode_window.restype = ctypes.c_int
+    lib.ssq_copy_pages.argtypes = [P(CopyArgs), _vp]
+    lib.ssq_copy_pages.restype = ctypes.c_int
     lib.ssq_last_error.argtypes = []
     lib.ssq_last_error.restype = ctypes.c_char_p
     lib.ssq_abi_version.argtypes = []

@@ -739,3 +739,45 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
     if (rc) return rc;
     return ssq_encode(&enc, stream);
 }
+
+// The values of an 8-bit append are those of ssq_append_values, the rest those of ssq_append without values.
+int ssq_values_check(const ssq_values_args* a);
+
+namespace {
+
+int check8(const ssq_append8_args* a, ssq_append_args& keys, ssq_values_args& v) {
+    if (!a) return ssq_fail(SSQ_ERR_INVALID, "args is NULL");
+    if (a->struct_size != sizeof(ssq_append8_args))
+        return ssq_fail(SSQ_ERR_ABI, "ssq_append8_args size %u != library's %zu", a->struct_size, sizeof(ssq_append8_args));
+    keys = a->app;
+    keys.v = nullptr;
+    int rc = check(&keys);
+    if (rc) return rc;
+    SSQ_REQUIRE(a->app.vp_dtype == SSQ_E4M3, "append8 writes 8-bit values");
+    const ssq_encode_args& e = keys.enc;
+    v = ssq_values_args{};
+    v.struct_size = sizeof(v);
+    v.v = a->app.v; v.v_dtype = a->app.v_dtype; v.v_sb = a->app.v_sb; v.v_sh = a->app.v_sh; v.v_ss = a->app.v_ss;
+    v.batch = e.batch; v.num_kv_heads = e.num_kv_heads; v.seq_len = e.seq_len; v.value_dim = a->app.value_dim;
+    v.v_pages = a->app.v_pages; v.vp_sb = a->app.vp_sb; v.vp_sh = a->app.vp_sh; v.vp_sd = a->app.vp_sd;
+    v.v_scale = a->v_scale; v.vs_sb = a->vs_sb; v.vs_sh = a->vs_sh;
+    v.slot_mapping = e.slot_mapping; v.sm_sb = e.sm_sb;
+    v.page_size = e.page_size; v.num_pages = a->app.num_pages;
+    return ssq_values_check(&v);
+}
+
+}  // namespace
+
+extern "C" size_t ssq_append8_workspace_size(const ssq_append8_args* a) {
+    ssq_append_args keys;
+    ssq_values_args v;
+    return check8(a, keys, v) == SSQ_OK ? ssq_append_workspace_size(&keys) : 0;
+}
+
+extern "C" int ssq_append8(const ssq_append8_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    ssq_append_args keys;
+    ssq_values_args v;
+    int rc = check8(a, keys, v);
+    if (rc == SSQ_OK) rc = ssq_append(&keys, workspace, workspace_bytes, stream);
+    return rc == SSQ_OK ? ssq_append_values(&v, stream) : rc;
+}

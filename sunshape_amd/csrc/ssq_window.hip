@@ -1,0 +1,130 @@
+// Causal attention over pages with a sliding window, sinks and 8-bit values (ssq_decode_window): the checks and the plan
+// of a call.  The kernel is in ssq_window.h, its instantiations in ssq_window_*.hip.
+#include "ssq_window.h"
+
+#include <limits.h>
+
+int ssq_decode_validate(const ssq_decode_args* a);
+
+namespace {
+
+struct Plan {
+    SsqWindowParams p;
+    int nr;
+    size_t part_bytes, bytes;
+};
+
+int check(const ssq_window_args* a) {
+    if (!a) return ssq_fail(SSQ_ERR_INVALID, "args is NULL");
+    if (a->struct_size != sizeof(ssq_window_args))
+        return ssq_fail(SSQ_ERR_ABI, "ssq_window_args size %u != library's %zu", a->struct_size, sizeof(ssq_window_args));
+    ssq_decode_args d = a->dec;
+    const bool v8 = d.v_dtype == SSQ_E4M3;
+    SSQ_REQUIRE(d.layout == SSQ_PAGED, "decode_window takes pages");
+    SSQ_REQUIRE(d.v, "decode_window needs values");
+    SSQ_REQUIRE(!d.scores && !d.mask, "decode_window takes no mask and gives no scores");
+    SSQ_REQUIRE(a->window >= 0 && a->sinks >= 0, "window and sinks must not be negative");
+    SSQ_REQUIRE(a->out_dtype >= SSQ_F32 && a->out_dtype <= SSQ_F16, "bad out_dtype");
+    SSQ_REQUIRE(a->num_pages >= 1 && a->num_pages <= INT_MAX, "bad num_pages");
+    SSQ_REQUIRE(!v8 || a->v_scale, "8-bit values need v_scale");
+    SSQ_REQUIRE(v8 || !a->v_scale, "v_scale goes with 8-bit values");
+    SSQ_REQUIRE(d.batch >= 0 && d.num_q_heads >= 0 && d.q_len >= 0 && d.num_kv_heads >= 1, "bad batch/heads/q_len");
+    SSQ_REQUIRE((int64_t)d.batch * (d.num_q_heads > 0 ? d.num_q_heads : 1) <= (1 << 24) && d.q_len <= 1 << 20 &&
+                    (int64_t)d.batch * d.num_q_heads * d.q_len <= 1 << 30,
+                "too many query rows");
+    if (v8) d.v_dtype = SSQ_F16;  // the decode's checks know 16 bits
+    int rc = ssq_decode_validate(&d);
+    if (rc) return rc;
+    SSQ_UNSUPPORTED(!d.heavy_mask[0] && !d.heavy_mask[1], "decode_window serves codecs without passthrough blocks");
+    SSQ_UNSUPPORTED((d.head_dim == 64 || d.head_dim == 128) && d.value_dim == d.head_dim,
+                    "decode_window serves head_dim 64 or 128 with value_dim the same, not %d and %d", d.head_dim, d.value_dim);
+    SSQ_UNSUPPORTED(d.block_dim == 2 || d.block_dim == 4 || d.block_dim == 8, "decode_window serves block_dim 2, 4 or 8, not %d",
+                    d.block_dim);
+    SSQ_UNSUPPORTED(d.n_centroids <= 256 && d.code_bits == 0, "decode_window serves byte codes (at most 256 codewords)");
+    SSQ_UNSUPPORTED(v8 || d.v_dtype == SSQ_BF16 || d.v_dtype == SSQ_F16, "decode_window serves values of 8 or 16 bits");
+    SSQ_UNSUPPORTED(d.page_size >= 16 && (d.page_size & (d.page_size - 1)) == 0 && d.page_size <= 1 << 16,
+                    "decode_window serves page sizes that are powers of two from 16, not %d", d.page_size);
+    SSQ_REQUIRE((uintptr_t)d.cent % 16 == 0 && d.cent_sh % 4 == 0, "centroids must be 16-byte aligned");
+    const int64_t piece = d.n_blocks / 4;  // bytes of a token's codes that a lane loads at once
+    SSQ_REQUIRE((uintptr_t)d.codes % piece == 0 && d.c_sb % piece == 0 && d.c_sh % piece == 0 && d.c_st % piece == 0,
+                "code rows must be aligned to %lld bytes", (long long)piece);
+    const int64_t per = v8 ? 16 : 8;
+    SSQ_REQUIRE((uintptr_t)d.v % 16 == 0 && d.v_sb % per == 0 && d.v_sh % per == 0 && d.v_st % per == 0,
+                "value rows must be 16-byte aligned");
+    SSQ_REQUIRE(d.v_st >= 0 && d.v_st <= 1 << 22, "the values' dim stride must be at most 2^22");
+    SSQ_REQUIRE((int64_t)d.batch * d.num_q_heads * d.q_len == 0 || d.num_kv_heads <= 1 << 16, "too many KV heads");
+    return SSQ_OK;
+}
+
+// The most tiles of an item (any length that the tables hold).
+int most_tiles(const SsqWindowParams& p, int nr, bool v8) {
+    const int cap = p.a.seq_len;
+    int most = 0;
+    const int last = (p.rgroups - 1) * 16 * nr;
+    for (int row0 : {0, last})
+        for (int len : {cap, cap - 63 > 0 ? cap - 63 : cap}) {  // a window's tiles depend on where it ends
+            const int n = v8 ? win_tiles<64>(p, len, row0, 16 * nr).n : win_tiles<32>(p, len, row0, 16 * nr).n;
+            most = n > most ? n : most;
+        }
+    return p.window == INT_MAX ? most : most + 2;
+}
+
+void make_plan(const ssq_window_args& a, Plan& pl) {
+    const ssq_decode_args& d = a.dec;
+    SsqWindowParams& p = pl.p;
+    p = SsqWindowParams{};
+    p.a = d;
+    p.window = a.window > 0 ? a.window : INT_MAX;
+    p.sinks = a.sinks;
+    p.out_dtype = a.out_dtype;
+    p.n_pages = (int)a.num_pages;
+    p.v_scale = a.v_scale;
+    p.vs_sb = a.vs_sb;
+    p.vs_sh = a.vs_sh;
+    p.G = d.num_q_heads / d.num_kv_heads;
+    p.rows = p.G * d.q_len;
+    pl.nr = p.rows <= 16 ? 1 : 2;
+    const int rp = 16 * pl.nr;
+    p.rgroups = (p.rows + rp - 1) / rp;
+    p.items = d.batch * p.rgroups;
+    const int cus = ssq_device_cus();
+    p.n_wg = cus / d.num_kv_heads > 0 ? cus / d.num_kv_heads : 1;
+    const int waves = win_waves(pl.nr);
+    p.fixed = 2 * waves;
+    p.least = 2 * waves;
+    p.whole = most_tiles(p, pl.nr, d.v_dtype == SSQ_E4M3) <= 2 * waves;
+    if (p.whole && p.n_wg > p.items) p.n_wg = p.items;
+    while ((16 << p.psh) < d.page_size) ++p.psh;
+    pl.part_bytes = p.whole ? 0 : (size_t)d.num_kv_heads * p.n_wg * 2 * rp * (d.value_dim + 2) * 4;
+    pl.bytes = p.whole ? 0 : pl.part_bytes + (size_t)p.items * 8;
+}
+
+}  // namespace
+
+extern "C" size_t ssq_decode_window_workspace_size(const ssq_window_args* a) {
+    if (check(a) != SSQ_OK || a->dec.batch == 0 || a->dec.num_q_heads == 0 || a->dec.q_len == 0) return 0;
+    Plan pl;
+    make_plan(*a, pl);
+    return pl.bytes;
+}
+
+extern "C" int ssq_decode_window(const ssq_window_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check(a);
+    if (rc) return rc;
+    const ssq_decode_args& d = a->dec;
+    if (d.batch == 0 || d.num_q_heads == 0 || d.q_len == 0) return SSQ_OK;
+    Plan pl;
+    make_plan(*a, pl);
+    SSQ_REQUIRE(workspace_bytes >= pl.bytes && (workspace || pl.bytes == 0), "workspace too small: %zu < %zu bytes", workspace_bytes,
+                pl.bytes);
+    SSQ_REQUIRE((uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");
+    pl.p.part = reinterpret_cast<float*>(workspace);
+    pl.p.meta = reinterpret_cast<int*>(reinterpret_cast<char*>(workspace) + pl.part_bytes);
+    hipStream_t st = (hipStream_t)stream;
+    const bool small = d.head_dim == 64;
+    switch (d.v_dtype) {
+        case SSQ_E4M3: return small ? ssq_window_64_e4m3(pl.p, pl.nr, st) : ssq_window_128_e4m3(pl.p, pl.nr, st);
+        case SSQ_BF16: return small ? ssq_window_64_bf16(pl.p, pl.nr, st) : ssq_window_128_bf16(pl.p, pl.nr, st);
+        default: return small ? ssq_window_64_f16(pl.p, pl.nr, st) : ssq_window_128_f16(pl.p, pl.nr, st);
+    }
+}

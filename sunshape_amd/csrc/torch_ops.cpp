@@ -1,6 +1,6 @@
 // Torch operators over the sunshape_amd C ABI (host code only; the kernels live in
-// libsunshape_amd.so): torch.ops.sunshape.decode, .scores, .encode_into, .qk_norm_rope, .append_kv and
-// .decode_prefix.
+// libsunshape_amd.so): torch.ops.sunshape.decode, .scores, .encode_into, .qk_norm_rope, .append_kv,
+// .decode_prefix, .append_values, .decode_window and .copy_pages.
 //
 // Each operator validates its tensors (the checks and messages of the Python surface,
 // sunshape_amd/hip_ops.py), allocates outputs and workspace through torch's caching allocator
@@ -472,12 +472,22 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q_in, const std::optional<
     return {q_out, k_out};
 }
 
+// 8-bit value pages [P, Hkv, Dv, page] come with fp32 scales [P, Hkv], others without
+void check_scale(const Tensor& v_pages, const std::optional<Tensor>& v_scale, const Tensor& ref) {
+    const bool v8 = v_pages.scalar_type() == at::kFloat8_e4m3fn;
+    TORCH_CHECK(v8 == given(v_scale), v8 ? "8-bit values need v_scale" : "v_scale goes with 8-bit values (float8_e4m3fn)");
+    if (!v8) return;
+    same_device("v_scale", *v_scale, ref);
+    TORCH_CHECK(v_scale->scalar_type() == at::kFloat && v_scale->dim() == 2 && v_scale->size(0) == v_pages.size(0) &&
+                    v_scale->size(1) == v_pages.size(1), "v_scale must be float32 [", v_pages.size(0), ", ", v_pages.size(1), "]");
+}
+
 void append_kv(const Tensor& keys_in, const std::optional<Tensor>& v_in, const Tensor& perm_in, const Tensor& cent_in,
                int64_t hm0, int64_t hm1, bool pt_dense, const Tensor& codes, const std::optional<Tensor>& pt,
                const std::optional<Tensor>& v_pages, const Tensor& slot_mapping, const std::optional<Tensor>& metric_in,
                const std::optional<Tensor>& grid, int64_t kernel, bool direct, const std::optional<Tensor>& cos,
                const std::optional<Tensor>& sin, const std::optional<Tensor>& positions,
-               const std::optional<Tensor>& k_weight, double eps, bool interleaved) {
+               const std::optional<Tensor>& k_weight, double eps, bool interleaved, const std::optional<Tensor>& v_scale) {
     on_gpu("key_states", keys_in);
     TORCH_CHECK(keys_in.dim() == 4, "append_kv expects key_states with shape [batch, kv_heads, seq_len, head_dim].");
     const Tensor keys = keys_in.stride(-1) == 1 ? keys_in : keys_in.contiguous();
@@ -515,6 +525,9 @@ void append_kv(const Tensor& keys_in, const std::optional<Tensor>& v_in, const T
         TORCH_CHECK(v_pages->dim() == 4 && v_pages->size(0) == P && v_pages->size(1) == Hkv &&
                         v_pages->size(2) == v.size(3) && v_pages->size(3) == page && v_pages->stride(3) == 1,
                     "v_out must be [", P, ", ", Hkv, ", ", v.size(3), ", ", page, "], contiguous over tokens");
+        check_scale(*v_pages, v_scale, keys);
+    } else {
+        TORCH_CHECK(!given(v_scale), "v_scale goes with 8-bit values");
     }
     Tensor metric;
     int64_t metric_sh = 0;
@@ -528,7 +541,9 @@ void append_kv(const Tensor& keys_in, const std::optional<Tensor>& v_in, const T
             metric_sh = D * D;
         }
     }
-    ssq_append_args a{};
+    ssq_append8_args a8{};
+    a8.struct_size = sizeof(ssq_append8_args);
+    ssq_append_args& a = a8.app;
     a.struct_size = sizeof(ssq_append_args);
     a.rope = rope_of(cos, sin, positions, interleaved, eps, B, S, D, keys);
     const Tensor kw = weight_of("k_weight", k_weight, D, keys);
@@ -569,8 +584,15 @@ void append_kv(const Tensor& keys_in, const std::optional<Tensor>& v_in, const T
         a.v = v.data_ptr(); a.v_dtype = dtype_code(v);
         a.v_sb = v.stride(0); a.v_sh = v.stride(1); a.v_ss = v.stride(2);
         a.value_dim = (int32_t)v.size(3);
-        a.v_pages = v_pages->data_ptr(); a.vp_dtype = dtype_code(*v_pages);
+        a.v_pages = v_pages->data_ptr(); a.vp_dtype = given(v_scale) ? SSQ_E4M3 : dtype_code(*v_pages);
         a.vp_sb = v_pages->stride(0); a.vp_sh = v_pages->stride(1); a.vp_sd = v_pages->stride(2);
+    }
+    if (given(v_scale)) {
+        a8.v_scale = v_scale->data_ptr<float>(); a8.vs_sb = v_scale->stride(0); a8.vs_sh = v_scale->stride(1);
+        const size_t ws_bytes = ssq_append8_workspace_size(&a8);
+        Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, keys.options().dtype(at::kByte)) : Tensor();
+        check_status(ssq_append8(&a8, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, stream_of(keys)));
+        return;
     }
     const size_t ws_bytes = ssq_append_workspace_size(&a);
     Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, keys.options().dtype(at::kByte)) : Tensor();
@@ -672,6 +694,147 @@ std::tuple<Tensor, Tensor> decode_prefix(const Tensor& q_in, const Tensor& codes
     return {out, lse};
 }
 
+void append_values(const Tensor& v_in, const Tensor& v_pages, const Tensor& v_scale, const Tensor& slot_mapping) {
+    on_gpu("value_states", v_in);
+    TORCH_CHECK(v_in.dim() == 4, "append_values expects value_states with shape [batch, kv_heads, seq_len, value_dim].");
+    const Tensor v = v_in.stride(-1) == 1 ? v_in : v_in.contiguous();
+    const int64_t B = v.size(0), Hkv = v.size(1), S = v.size(2), Dv = v.size(3);
+    c10::hip::HIPGuard guard(v.device().index());
+    same_device("v_out", v_pages, v);
+    TORCH_CHECK(v_pages.scalar_type() == at::kFloat8_e4m3fn, "append_values writes float8_e4m3fn pages, got ", v_pages.scalar_type());
+    TORCH_CHECK(v_pages.dim() == 4 && v_pages.size(1) == Hkv && v_pages.size(2) == Dv && v_pages.stride(3) == 1 && v_pages.size(3) >= 1,
+                "v_out must be [P, ", Hkv, ", ", Dv, ", page], contiguous over tokens");
+    check_scale(v_pages, v_scale, v);
+    same_device("slot_mapping", slot_mapping, v);
+    TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.dim() == 2 && slot_mapping.size(0) == B &&
+                    slot_mapping.size(1) == S && (slot_mapping.stride(1) == 1 || S <= 1),
+                "slot_mapping must be int64 [", B, ", ", S, "] with unit last stride");
+    if (B * S * Hkv * Dv == 0 || v_pages.size(0) == 0) return;  // no row, or no slot to write
+    TORCH_CHECK(B <= 0x7fffffff && S <= 0x7fffffff && Dv <= 8192, "value_states are too large");
+    ssq_values_args a{};
+    a.struct_size = sizeof(ssq_values_args);
+    a.v = v.data_ptr(); a.v_dtype = dtype_code(v); a.v_sb = v.stride(0); a.v_sh = v.stride(1); a.v_ss = v.stride(2);
+    a.batch = (int32_t)B; a.num_kv_heads = (int32_t)Hkv; a.seq_len = (int32_t)S; a.value_dim = (int32_t)Dv;
+    a.v_pages = v_pages.data_ptr(); a.vp_sb = v_pages.stride(0); a.vp_sh = v_pages.stride(1); a.vp_sd = v_pages.stride(2);
+    a.v_scale = v_scale.data_ptr<float>(); a.vs_sb = v_scale.stride(0); a.vs_sh = v_scale.stride(1);
+    a.slot_mapping = slot_mapping.data_ptr<int64_t>(); a.sm_sb = slot_mapping.stride(0);
+    a.page_size = (int32_t)v_pages.size(3);
+    a.num_pages = v_pages.size(0);
+    check_status(ssq_append_values(&a, stream_of(v)));
+}
+
+std::tuple<Tensor, Tensor> decode_window(const Tensor& q_in, const Tensor& codes, const Tensor& v, const Tensor& perm_in,
+                                         const Tensor& cent_in, std::optional<double> scale, int64_t hm0, int64_t hm1,
+                                         const std::optional<Tensor>& v_scale, const Tensor& bt, const Tensor& seq_lens,
+                                         int64_t window, int64_t sinks, at::ScalarType out_dtype, bool return_lse) {
+    on_gpu("query", q_in);
+    TORCH_CHECK(q_in.dim() == 4, "Quantized attention expects query/value tensors with shape [batch, heads, seq, dim].");
+    const Tensor q = q_in.stride(-1) == 1 ? q_in : q_in.contiguous();
+    const int64_t B = q.size(0), Hq = q.size(1), Lq = q.size(2), D = q.size(3);
+    same_device("codes", codes, q);
+    same_device("value", v, q);
+    TORCH_CHECK(codes.dim() == 4 && codes.stride(-1) == 1, "codes must be [P, kv_heads, page, nb], contiguous in the last dim");
+    const int64_t P = codes.size(0), Hkv = codes.size(1), page = codes.size(2);
+    TORCH_CHECK(Hkv >= 1 && Hq % Hkv == 0, "Query head count must be divisible by kv-head count.");
+    c10::hip::HIPGuard guard(q.device().index());
+    same_device("permutation", perm_in, q);
+    same_device("centroids", cent_in, q);
+    Codec c = codec_arrays(perm_in, cent_in, D, Hkv);
+    if ((uintptr_t)c.cent.data_ptr() % 16) c.cent = c.cent.clone();  // a view's
+    check_codes(codes, c.nb, c.nc, 0);
+    TORCH_CHECK(v.dim() == 4 && v.size(0) == P && v.size(1) == Hkv && v.size(3) == page && v.stride(-1) == 1,
+                "paged V must be [P, Hkv, Dv, page], contiguous over tokens");
+    check_scale(v, v_scale, q);
+    same_device("block_table", bt, q);
+    same_device("seq_lens", seq_lens, q);
+    TORCH_CHECK(bt.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt, "block_table and seq_lens must be int32");
+    TORCH_CHECK(bt.dim() == 2 && bt.size(0) == B && (bt.stride(1) == 1 || bt.size(1) <= 1), "block_table must be [B, max_pages]");
+    TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == B && (B <= 1 || seq_lens.stride(0) == 1), "seq_lens must be [B]");
+    TORCH_CHECK(window >= 0 && sinks >= 0 && window <= 0x7fffffff && sinks <= 0x7fffffff, "window must be positive and sinks not negative");
+    const int64_t T = bt.size(1) * page, Dv = v.size(2);
+    TORCH_CHECK(T <= 0x7fffffff - 64, "the block table is too long");
+    Tensor out = at::empty({B, Hq, Lq, Dv}, q.options().dtype(out_dtype));
+    Tensor lse = at::empty({return_lse ? B : 0, Hq, Lq}, q.options().dtype(at::kFloat));
+    const int out_code = dtype_code(out);
+    if (B * Hq * Lq == 0) return {out, lse};
+    if (P == 0 || T == 0) {  // nothing to see
+        out.zero_();
+        lse.fill_(-std::numeric_limits<float>::infinity());
+        return {out, lse};
+    }
+    TORCH_CHECK(B <= 0x7fffffff && Hq <= 0x7fffffff && Lq <= 0x7fffffff && D <= 0x7fffffff && P <= 0x7fffffff && page <= 0x7fffffff,
+                "query is too large");
+    ssq_window_args wa{};
+    wa.struct_size = sizeof(ssq_window_args);
+    wa.window = (int32_t)window; wa.sinks = (int32_t)sinks; wa.out_dtype = out_code; wa.num_pages = P;
+    if (given(v_scale)) {
+        wa.v_scale = v_scale->data_ptr<float>(); wa.vs_sb = v_scale->stride(0); wa.vs_sh = v_scale->stride(1);
+    }
+    ssq_decode_args& a = wa.dec;
+    a.struct_size = sizeof(ssq_decode_args);
+    a.q = q.data_ptr(); a.q_dtype = dtype_code(q);
+    a.q_sb = q.stride(0); a.q_sh = q.stride(1); a.q_sl = q.stride(2);
+    a.batch = (int32_t)B; a.num_q_heads = (int32_t)Hq; a.q_len = (int32_t)Lq; a.head_dim = (int32_t)D;
+    a.num_kv_heads = (int32_t)Hkv;
+    a.has_scale = scale.has_value() ? 1 : 0;
+    a.scale = scale.has_value() ? (float)*scale : 0.f;
+    a.perm = c.perm.data_ptr<int64_t>(); a.perm_sh = c.perm_sh;
+    a.cent = c.cent.data_ptr<float>(); a.cent_sh = c.cent_sh;
+    a.block_dim = (int32_t)c.bd; a.n_blocks = (int32_t)c.nb; a.n_centroids = (int32_t)c.nc;
+    a.heavy_mask[0] = (uint64_t)hm0; a.heavy_mask[1] = (uint64_t)hm1;
+    a.pt = hm0 || hm1 ? codes.data_ptr() : nullptr;  // refused by the library, which names the reason
+    a.layout = SSQ_PAGED;
+    a.seq_len = (int32_t)T;
+    a.codes = reinterpret_cast<const uint8_t*>(codes.data_ptr());
+    a.c_sb = codes.stride(0); a.c_sh = codes.stride(1); a.c_st = codes.stride(2);
+    a.block_table = bt.data_ptr<int32_t>(); a.bt_sb = bt.stride(0);
+    a.seq_lens = seq_lens.data_ptr<int32_t>();
+    a.page_size = (int32_t)page;
+    a.v = v.data_ptr(); a.v_dtype = given(v_scale) ? SSQ_E4M3 : dtype_code(v); a.value_dim = (int32_t)Dv;
+    a.v_sb = v.stride(0); a.v_sh = v.stride(1); a.v_st = v.stride(2);
+    a.out = out.data_ptr(); a.o_sb = out.stride(0); a.o_sh = out.stride(1); a.o_sl = out.stride(2);
+    a.lse = return_lse ? lse.data_ptr<float>() : nullptr;
+    const size_t ws_bytes = ssq_decode_window_workspace_size(&wa);
+    Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte)) : Tensor();
+    check_status(ssq_decode_window(&wa, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, stream_of(q)));
+    return {out, lse};
+}
+
+void copy_pages(at::TensorList src, at::TensorList dst, const Tensor& from, const Tensor& to) {
+    TORCH_CHECK(!src.empty() && src.size() == dst.size() && src.size() <= SSQ_COPY_POOLS, "copy_pages takes 1 to ", SSQ_COPY_POOLS,
+                " pools, and as many to copy into");
+    const Tensor& ref = src[0];
+    on_gpu("pool", ref);
+    c10::hip::HIPGuard guard(ref.device().index());
+    for (const Tensor* t : {&from, &to}) {
+        same_device("src and dst", *t, ref);
+        TORCH_CHECK(t->scalar_type() == at::kLong && t->dim() == 1 && t->size(0) == from.size(0) && (t->stride(0) == 1 || t->size(0) <= 1),
+                    "src and dst must be int64 [pairs], alike");
+    }
+    ssq_copy_args a{};
+    a.struct_size = sizeof(ssq_copy_args);
+    a.n_pools = (int32_t)src.size();
+    a.from = from.data_ptr<int64_t>(); a.to = to.data_ptr<int64_t>(); a.n_pairs = from.size(0);
+    for (size_t k = 0; k < src.size(); ++k) {
+        const Tensor &s = src[k], &d = dst[k];
+        same_device("pool", s, ref);
+        same_device("pool", d, ref);
+        TORCH_CHECK(s.dim() >= 1 && s.dim() == d.dim() && s.scalar_type() == d.scalar_type() && s.sizes().slice(1) == d.sizes().slice(1),
+                    "pool ", k, " and the one it is copied into must hold pages of one shape and dtype");
+        int64_t n = 1;
+        for (int64_t i = s.dim() - 1; i >= 1; --i) {
+            TORCH_CHECK(s.size(i) <= 1 || n == 0 || (s.stride(i) == n && d.stride(i) == n), "the pages of pool ", k, " must be contiguous");
+            n *= s.size(i);
+        }
+        const int64_t e = (int64_t)s.element_size();
+        a.pool[k].src = s.data_ptr(); a.pool[k].dst = d.data_ptr();
+        a.pool[k].src_stride = s.stride(0) * e; a.pool[k].dst_stride = d.stride(0) * e;
+        a.pool[k].src_pages = s.size(0); a.pool[k].dst_pages = d.size(0); a.pool[k].bytes = n * e;
+    }
+    if (a.n_pairs == 0) return;
+    check_status(ssq_copy_pages(&a, stream_of(ref)));
+}
+
 }  // namespace
 
 TORCH_LIBRARY(sunshape, m) {
@@ -686,10 +849,16 @@ TORCH_LIBRARY(sunshape, m) {
           "Tensor? k_weight, float eps, bool interleaved) -> (Tensor, Tensor)");
     m.def("append_kv(Tensor keys, Tensor? v, Tensor perm, Tensor cent, int hm0, int hm1, bool pt_dense, Tensor(a!) codes, "
           "Tensor(b!)? pt, Tensor(c!)? v_pages, Tensor slot_mapping, Tensor? metric, Tensor? grid, int kernel, bool direct, "
-          "Tensor? cos, Tensor? sin, Tensor? positions, Tensor? k_weight, float eps, bool interleaved) -> ()");
+          "Tensor? cos, Tensor? sin, Tensor? positions, Tensor? k_weight, float eps, bool interleaved, "
+          "Tensor(d!)? v_scale=None) -> ()");
     m.def("decode_prefix(Tensor q, Tensor codes, Tensor v, Tensor perm, Tensor cent, float? scale, Tensor? mask, int hm0, "
           "int hm1, Tensor? pt, bool pt_dense, Tensor prefix_table, Tensor prefix_len, Tensor block_table, Tensor seq_lens, "
           "bool return_lse, int kernel, int code_bits) -> (Tensor, Tensor)");
+    m.def("append_values(Tensor v, Tensor(a!) v_pages, Tensor(b!) v_scale, Tensor slot_mapping) -> ()");
+    m.def("decode_window(Tensor q, Tensor codes, Tensor v, Tensor perm, Tensor cent, float? scale, int hm0, int hm1, "
+          "Tensor? v_scale, Tensor block_table, Tensor seq_lens, int window, int sinks, ScalarType out_dtype, "
+          "bool return_lse) -> (Tensor, Tensor)");
+    m.def("copy_pages(Tensor[] src, Tensor(a!)[] dst, Tensor src_pages, Tensor dst_pages) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(sunshape, CUDA, m) {
@@ -699,4 +868,7 @@ TORCH_LIBRARY_IMPL(sunshape, CUDA, m) {
     m.impl("qk_norm_rope", &qk_norm_rope);
     m.impl("append_kv", &append_kv);
     m.impl("decode_prefix", &decode_prefix);
+    m.impl("append_values", &append_values);
+    m.impl("decode_window", &decode_window);
+    m.impl("copy_pages", &copy_pages);
 }

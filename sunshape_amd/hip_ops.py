@@ -397,7 +397,8 @@ def append_kv(keys: torch.Tensor, values: Optional[torch.Tensor], perm: torch.Te
               positions: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
               interleaved: bool = False, heavy: Optional[Sequence[bool]] = None, pt_out: Optional[torch.Tensor] = None,
               pt_dense: bool = False, metric: Optional[torch.Tensor] = None, grid: Optional[torch.Tensor] = None,
-              direct: bool = False, kernel: int = 0, rotation: Optional[torch.Tensor] = None) -> None:
+              direct: bool = False, kernel: int = 0, rotation: Optional[torch.Tensor] = None,
+              v_scale: Optional[torch.Tensor] = None) -> None:
     """Append raw keys and values to a paged cache, the keys normed and rotated on the way.
 
     keys [B, Hkv, S, D] (before their norm and rotation), values [B, Hkv, S, Dv] or None; slot_mapping
@@ -405,7 +406,8 @@ def append_kv(keys: torch.Tensor, values: Optional[torch.Tensor], perm: torch.Te
     padding and writes nothing.  The keys are taken through qk_norm_rope's norm (k_weight) and rotation
     (cos, sin, positions), each left out when None, rounded to their dtype, and encoded as encode()
     does, into codes_out [P, Hkv, page, nb] and, for heavy blocks, pt_out [P, Hkv, page, slots, bd];
-    values go to v_out [P, Hkv, Dv, page], converted to its dtype.  metric, grid, direct and rotation (the
+    values go to v_out [P, Hkv, Dv, page], converted to its dtype; a float8_e4m3fn v_out takes v_scale [P, Hkv] and
+    holds them as append_values does.  metric, grid, direct and rotation (the
     codec's rotated mode, after the position rotation) as in encode(); kernel: 0, or 1 for the exact
     scan.  A position outside the tables stores the codes of a NaN key.  No derivative; no counterpart in
     the reference.
@@ -423,7 +425,83 @@ def append_kv(keys: torch.Tensor, values: Optional[torch.Tensor], perm: torch.Te
     try:
         N.torch_ops().append_kv(keys, values, perm, cent, hm0, hm1, bool(pt_dense), codes_out, pt_out, v_out, slot_mapping,
                                 metric, grid, int(kernel), bool(direct), cos, sin, positions, k_weight, float(eps),
-                                bool(interleaved))
+                                bool(interleaved), v_scale)
+    except RuntimeError as e:
+        raise N.kernel_error(e) from None
+
+
+def append_values(values: torch.Tensor, v_out: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Append values [B, Hkv, S, Dv] to 8-bit pages: v_out float8_e4m3fn [P, Hkv, Dv, page] with one fp32 scale
+    per page and KV head, v_scale [P, Hkv] (a stored value stands for v_out * v_scale).
+
+    slot_mapping int64 [B, S] as in append_kv (page * page_size + offset, distinct; a negative slot, or one past
+    the pages, is padding); the tokens of one page stand in one row with nothing but padding between them.
+    A page's scale is the smallest power of two (at least 2^-100) that holds its finite values within e4m3's 448:
+    it starts anew with offset 0 and grows with later tokens, where the page's earlier tokens (those before its
+    first new one) are taken to the new scale: exact but for what falls below e4m3's normal range.  NaN and infinities
+    are stored as NaN.  Bytes behind the new tokens stay.  page: a multiple of 16.  No derivative; no counterpart
+    in the reference.
+    """
+    if not values.is_cuda:
+        _on_gpu("value_states", values)
+    try:
+        N.torch_ops().append_values(values, v_out, v_scale, slot_mapping)
+    except RuntimeError as e:
+        raise N.kernel_error(e) from None
+
+
+def decode_window(q: torch.Tensor, codes: torch.Tensor, v: torch.Tensor, perm: torch.Tensor, cent: torch.Tensor, *,
+                  block_table: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
+                  window: Optional[int] = None, sinks: int = 0, v_scale: Optional[torch.Tensor] = None,
+                  heavy: Optional[Sequence[bool]] = None, return_lse: bool = False,
+                  out_dtype: Optional[torch.dtype] = None, rotation: Optional[torch.Tensor] = None):
+    """Causal attention of the newest tokens over pages, with 8- or 16-bit values, a sliding window and sinks.
+
+    q [B, Hq, Lq, D]: the queries of each sequence's Lq newest tokens, whose keys and values are in the pages
+    already: row i stands at p = seq_lens[b] - Lq + i and sees token j iff j <= p and (j > p - window or j <
+    sinks); window None: every j <= p.  codes uint8 [P, Hkv, page, nb], v [P, Hkv, Dv, page] in bfloat16, float16, or
+    float8_e4m3fn with v_scale fp32 [P, Hkv] (append_values); block_table int32 [B, max_pages], seq_lens int32
+    [B], both on the device.  Pages that no row sees may be anything: their table entries are not used.
+    Serves byte codes of dims 2, 4 or 8, head_dim 64 or 128 with Dv the same, pages of 16 to 256 tokens; others,
+    and passthrough blocks (heavy), are refused.  scale, rotation as in decode.  Returns out [B, Hq, Lq, Dv] in
+    out_dtype (v's dtype, or for 8-bit values the query's), and lse [B, Hq, Lq] (fp32) when requested; a row
+    that sees nothing gives 0 and -inf, one whose query holds a NaN or an infinity gives NaN.  No derivative; no
+    counterpart in the reference.
+    """
+    if not (q.is_cuda and codes.is_cuda and v.is_cuda):
+        for name, t in (("query", q), ("codes", codes), ("value", v)):
+            _on_gpu(name, t)
+    _require(window is None or window >= 1, "window must be at least 1 (None: no window)")
+    if out_dtype is None:
+        out_dtype = q.dtype if v.dtype == torch.float8_e4m3fn else v.dtype
+    if rotation is not None:
+        _require(q.ndim == 4, "Quantized attention expects query/value tensors with shape [batch, heads, seq, dim].")
+        q = transform_rows(q, rotation, scale=scale)
+        scale = None
+        perm = _identity_like(perm)
+    hm0, hm1 = N.mask_words_signed(heavy)
+    try:
+        out, lse = N.torch_ops().decode_window(q, codes, v, perm, cent, None if scale is None else float(scale), hm0, hm1,
+                                               v_scale, block_table, seq_lens, window or 0, int(sinks), out_dtype,
+                                               bool(return_lse))
+    except RuntimeError as e:
+        raise N.kernel_error(e) from None
+    return (out, lse) if return_lse else out
+
+
+def copy_pages(pools: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, *,
+               into: Optional[Sequence[torch.Tensor]] = None) -> None:
+    """Copy pages of every pool (codes, values, scales, passthrough: [P, ...], each page contiguous) in one launch:
+    page dst[i] becomes a copy of page src[i], in place, or in the pools `into` (pages of the same shapes and dtypes).
+
+    src, dst: int64 [pairs] on the device.  Pairs with an index outside the pools are left out.  No page may be
+    written twice, nor both read and written.  No counterpart in the reference.
+    """
+    pools = list(pools)
+    for t in pools:
+        _on_gpu("pool", t)
+    try:
+        N.torch_ops().copy_pages(pools, pools if into is None else list(into), src, dst)
     except RuntimeError as e:
         raise N.kernel_error(e) from None
 

@@ -54,17 +54,22 @@ SSQ_WINDOW_UNIT(ssq_window_128_f16);
 // the registers hold one
 __host__ __device__ constexpr int win_waves(int nr) { return nr == 1 ? 8 : 4; }
 
+// what the tiles of an item follow from, beside its length
+struct WinShape { int window, sinks, q_len, G, rows; };
+__host__ __device__ __forceinline__ WinShape win_shape(const SsqWindowParams& p) {
+    return {p.window, p.sinks, p.a.q_len, p.G, p.rows};
+}
 // tiles of an item that some row of it sees
 struct WinTiles {
     int p_lo, p_hi;      // the first and last row's positions
     int n, n_sink, from; // tile i: i < n_sink ? i : from + i - n_sink
 };
 template <int TT>
-__host__ __device__ __forceinline__ WinTiles win_tiles(const SsqWindowParams& p, int len, int row0, int rows_per) {
+__host__ __device__ __forceinline__ WinTiles win_tiles(const WinShape& p, int len, int row0, int rows_per) {
     WinTiles t;
     const int last = (row0 + rows_per < p.rows ? row0 + rows_per : p.rows) - 1;
-    t.p_lo = len - p.a.q_len + row0 / p.G;
-    t.p_hi = len - p.a.q_len + last / p.G;
+    t.p_lo = len - p.q_len + row0 / p.G;
+    t.p_hi = len - p.q_len + last / p.G;
     t.n = t.n_sink = t.from = 0;
     if (t.p_hi < 0) return t;
     const int lo = t.p_lo >= p.window ? t.p_lo - p.window + 1 : 0;
@@ -140,6 +145,15 @@ __device__ __forceinline__ float win_sum4(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// A kernel's arguments, to be loaded where they are used: taken from the parameter, all 60 words of them would stay in scalar
+// registers across the loops, and those that do not fit in lanes of vector registers, which the tiles need.
+typedef const __attribute__((address_space(4))) SsqWindowParams* WinArgs;
+__device__ __forceinline__ WinArgs win_args() {
+    WinArgs k = (WinArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(k));
+    return k;
+}
+
 // Equal shares of the items' tiles: the items of a KV head lie end to end on a cost axis, fixed + tiles each, and
 // workgroup w takes [w share, (w + 1) share).  An item inside one share is written out by its workgroup; one that spans
 // several leaves a partial in each: slot 0 of a workgroup for the item its share starts in, slot 1 for one that starts in
@@ -147,10 +161,11 @@ __device__ __forceinline__ float win_sum4(float v) {
 template <int TT, int RP>
 struct WinCut {
     int share, total;
-    __device__ __forceinline__ static int cost(const SsqWindowParams& p, int i) {
-        if (i >= p.items) return 0;
-        const int b = i / p.rgroups, g = i - b * p.rgroups;
-        return p.fixed + win_tiles<TT>(p, max(0, min(p.a.seq_lens[b], p.a.seq_len)), g * RP, RP).n;
+    __device__ __forceinline__ static int cost(WinArgs p, int i) {
+        if (i >= p->items) return 0;
+        const int b = i / p->rgroups, g = i - b * p->rgroups;
+        const WinShape s{p->window, p->sinks, p->a.q_len, p->G, p->rows};
+        return p->fixed + win_tiles<TT>(s, max(0, min(p->a.seq_lens[b], p->a.seq_len)), g * RP, RP).n;
     }
     __device__ __forceinline__ static int scan(int v) {  // inclusive, over the wave
         v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
@@ -162,15 +177,15 @@ struct WinCut {
         return v;
     }
     // (the whole wave calls these two)
-    __device__ __forceinline__ void init(const SsqWindowParams& p, int lane) {
+    __device__ __forceinline__ void init(WinArgs p, int lane) {
         total = 0;
-        for (int i = 0; i < p.items; i += SSQ_WAVE) total += __builtin_amdgcn_readlane(scan(cost(p, i + lane)), 63);
-        share = (max((total + p.n_wg - 1) / p.n_wg, p.least) + 7) & ~7;
+        for (int i = 0; i < p->items; i += SSQ_WAVE) total += __builtin_amdgcn_readlane(scan(cost(p, i + lane)), 63);
+        share = (max((total + p->n_wg - 1) / p->n_wg, p->least) + 7) & ~7;
     }
     // the item that holds cost position x < total, its start and cost
-    __device__ __forceinline__ void find(const SsqWindowParams& p, int lane, int x, int& item, int& s, int& c) const {
+    __device__ __forceinline__ void find(WinArgs p, int lane, int x, int& item, int& s, int& c) const {
         int base = 0;
-        for (int f = 0; f < p.items; f += SSQ_WAVE) {
+        for (int f = 0; f < p->items; f += SSQ_WAVE) {
             const int mine = cost(p, f + lane), v = scan(mine);
             const uint64_t hit = __builtin_amdgcn_ballot_w64(base + v > x);
             if (hit) {
@@ -182,7 +197,7 @@ struct WinCut {
             }
             base += __builtin_amdgcn_readlane(v, 63);
         }
-        item = p.items;
+        item = p->items;
         s = x;
         c = 0;
     }
@@ -231,8 +246,10 @@ struct WinRun {
         float scale;
     };
 
-    const SsqWindowParams& p;
-    int lane, col, grp, kv;
+    int lane, col, grp;
+    int window, sinks, n_pages, psh;
+    int64_t c_sb, c_st, v_sb, vs_sb;
+    const float* v_scale;           // of this KV head
     uint32_t book;                  // LDS address of the codebook, and this group's blocks in it
     uint4 q[QP][NR][NQ];
     float fac[NR];                  // scores to log2 units
@@ -250,8 +267,8 @@ struct WinRun {
     // the page table's entry of chunk g of tile i: its page (always one of the cache's) and place in it
     __device__ __forceinline__ void entry(int i, int g, int& page, int& at) const {
         const int tok = min(TT * tile_of(i) + CH * g, last_tok & ~(CH - 1));
-        page = min((uint32_t)table[(tok >> 4) >> p.psh], (uint32_t)(p.n_pages - 1));
-        at = tok & ((16 << p.psh) - 1);
+        page = min((uint32_t)table[(tok >> 4) >> psh], (uint32_t)(n_pages - 1));
+        at = tok & ((16 << psh) - 1);
     }
     struct Place { int page, at; };
     __device__ __forceinline__ Place place(int i, int g) const {
@@ -261,10 +278,10 @@ struct WinRun {
     }
     __device__ __forceinline__ int code_chunk() const { return (lane >> 2) & 3; }
     __device__ __forceinline__ void load_codes(const Place& e, Codes& r) const {
-        const uint8_t* row = cbase + (int64_t)e.page * p.a.c_sb + (int64_t)e.at * p.a.c_st;
+        const uint8_t* row = cbase + (int64_t)e.page * c_sb + (int64_t)e.at * c_st;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const uint8_t* src = row + (int64_t)(4 * s) * p.a.c_st;
+            const uint8_t* src = row + (int64_t)(4 * s) * c_st;
             if constexpr (NCL == 16) {
                 const w4u x = __builtin_nontemporal_load(reinterpret_cast<const w4u*>(src));
                 r.w[s][0] = x.x; r.w[s][1] = x.y; r.w[s][2] = x.z; r.w[s][3] = x.w;
@@ -279,13 +296,19 @@ struct WinRun {
         }
     }
     __device__ __forceinline__ const uint8_t* val_row(const Place& e) const {
-        return vbase + ((int64_t)e.page * p.a.v_sb + e.at) * (kV8 ? 1 : 2);
+        return vbase + ((int64_t)e.page * v_sb + e.at) * (kV8 ? 1 : 2);
     }
     __device__ __forceinline__ w4u load_val(const uint8_t* row, int dt) const {
         return __builtin_nontemporal_load(reinterpret_cast<const w4u*>(row + dt * vstep));
     }
+    __device__ __forceinline__ void load_vals(const Place& e, Vals& r) const {
+        r.scale = load_scale(e);
+        const uint8_t* row = val_row(e);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) r.v[dt] = load_val(row, dt);
+    }
     __device__ __forceinline__ float load_scale(const Place& e) const {
-        if constexpr (kV8) return p.v_scale[(int64_t)e.page * p.vs_sb + (int64_t)kv * p.vs_sh];
+        if constexpr (kV8) return v_scale[(int64_t)e.page * vs_sb];
         else return 1.f;
     }
 
@@ -310,14 +333,13 @@ struct WinRun {
             return make_uint4(x.x, x.y, y.x, y.y);
         }
     }
-    uint4 ring[kAhead];
-    __device__ __forceinline__ void prime(const Codes& c) {
+    // A tile's scores.  Gathers run kAhead steps before their products; the barriers keep the compiler from gathering a whole
+    // tile ahead, which does not fit the registers.
+    __device__ __forceinline__ void scores(const Codes& c, w4f (&s)[NS][NR]) const {
+        uint4 ring[kAhead];
 #pragma unroll
         for (int st = 0; st < kAhead; ++st) ring[st] = operand(c, st);
-    }
-    // A tile's scores.  Gathers run kAhead steps before their products, into the next tile's codes at the end; the
-    // barriers keep the compiler from gathering a whole tile ahead, which does not fit the registers.
-    __device__ __forceinline__ void scores(const Codes& c, const Codes& next, w4f (&s)[NS][NR]) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int st = 0; st < NST; ++st) {
             const uint4 x = ring[st % kAhead];
@@ -328,12 +350,15 @@ struct WinRun {
                     w4f& acc = s[st / NK][n];
                     acc = win_mfma(x, q[h][n][BD == 8 ? st % NK / 2 : st % NK], st % NK || h ? acc : w4f{});
                 }
-            ring[st % kAhead] = st + kAhead < NST ? operand(c, st + kAhead) : operand(next, st + kAhead - NST);
+            if (st + kAhead < NST) ring[st % kAhead] = operand(c, st + kAhead);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    __device__ __forceinline__ bool sees(int at, int tok) const {
-        return tok <= at && (tok > at - p.window || tok < p.sinks);
+    // bits [0, n) of a chunk's tokens
+    __device__ __forceinline__ static uint32_t below(int n) { return (1u << min(max(n, 0), CH)) - 1u; }
+    // the chunk's tokens that some row at a position from `first` to `last` sees; with the two swapped, that all do
+    __device__ __forceinline__ uint32_t sees(int first, int last, int tok) const {
+        return below(last + 1 - tok) & (~below(max(max(first, 0) - window, -1) + 1 - tok) | below(sinks - tok));
     }
     // the value operand of 8 tokens from 8 jj of this lane's chunk, those in `gone` (a bit a token of the chunk) as 0
     __device__ __forceinline__ uint4 vals(const w4u& v, int jj) const {
@@ -344,45 +369,38 @@ struct WinRun {
             return make_uint4(v.x, v.y, v.z, v.w);
         }
     }
-    __device__ __forceinline__ static w4u cleared(w4u v, uint32_t gone) {
+    // all bits of the values of the chunk's tokens whose bit is set
+    __device__ __forceinline__ static w4u spread(uint32_t bits) {
+        w4u r;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            uint32_t keep = 0xFFFFFFFFu;
             if constexpr (kV8) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (gone >> (4 * k + j) & 1) keep &= ~(0xFFu << (8 * j));
+                const uint32_t b = (bits >> (4 * k)) & 0xFu;
+                r[k] = ((b * 0x00204081u) & 0x01010101u) * 0xFFu;  // a bit to a byte each
             } else {
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (gone >> (2 * k + j) & 1) keep &= ~(0xFFFFu << (16 * j));
+                const uint32_t b = bits >> (2 * k);
+                r[k] = (b & 1u ? 0xFFFFu : 0u) | (b & 2u ? 0xFFFF0000u : 0u);
             }
-            v[k] &= keep;
         }
-        return v;
+        return r;
     }
-    // whether a value of the tokens in `which` is infinite or NaN
-    __device__ __forceinline__ static bool wild(const w4u& v, uint32_t which) {
-        bool is = false;
-#pragma unroll
-        for (int t = 0; t < CH; ++t) {
-            const uint32_t x = kV8 ? (v[t >> 2] >> (8 * (t & 3))) & 0x7Fu : (v[t >> 1] >> (16 * (t & 1))) & 0x7FFFu;
-            is |= (which >> t & 1) && (kV8 ? x == 0x7Fu : VT == SSQ_BF16 ? x >= 0x7F80u : x >= 0x7C00u);
-        }
-        return is;
+    // the top bit of each value that is infinite or NaN
+    __device__ __forceinline__ static uint32_t wild(uint32_t w) {
+        if constexpr (kV8) return (w & 0x7F7F7F7Fu) + 0x01010101u;
+        else return (w & 0x7FFF7FFFu) + (VT == SSQ_BF16 ? 0x00800080u : 0x04000400u);
     }
 };
 
 template <int D, int BD, int VT, int NR, int QP>
-__global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_waves_per_eu(NR == 1 ? 2 : 1, NR == 1 ? 2 : 1))) void k_window(const SsqWindowParams p) {
+__global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_waves_per_eu(NR == 1 ? 2 : 1, NR == 1 ? 2 : 1))) void k_window(const SsqWindowParams) {
     using W = WinRun<D, BD, VT, NR, QP>;
     using L = typename W::L;
     constexpr int RP = W::RP, TT = W::TT, CH = W::CH, NS = W::NS, DT = W::DT;
     constexpr int kWinWaves = win_waves(NR), kWinThreads = kWinWaves * SSQ_WAVE;
     extern __shared__ __align__(16) unsigned char smem[];
-    const ssq_decode_args& a = p.a;
+    WinArgs p = win_args();
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kv = blockIdx.x % a.num_kv_heads, wg = blockIdx.x / a.num_kv_heads;
+    const int kv = blockIdx.x % p->a.num_kv_heads, wg = blockIdx.x / p->a.num_kv_heads;
     float* red = reinterpret_cast<float*>(smem + L::kRed);
     uint16_t* perm = reinterpret_cast<uint16_t*>(smem + L::kPerm);
     float* mls = reinterpret_cast<float*>(smem + L::kMl);
@@ -392,13 +410,14 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
     constexpr int kPer = W::NB * 256 / kWinThreads;
     int book_exp;  // the codebook is staged times 2^book_exp
     {
-        const float* cent = a.cent + (int64_t)kv * a.cent_sh;
+        const float* cent = p->a.cent + (int64_t)kv * p->a.cent_sh;
+        const int n_centroids = p->a.n_centroids;
         float c[kPer][BD];
         float most = 0.f;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             const int e = tid + k * kWinThreads, blk = e >> 8, w = e & 255;
-            const float* src = cent + (int64_t)(blk * a.n_centroids + min(w, a.n_centroids - 1)) * BD;
+            const float* src = cent + (int64_t)(blk * n_centroids + min(w, n_centroids - 1)) * BD;
             if constexpr (BD >= 4) {
 #pragma unroll
                 for (int d = 0; d < BD; d += 4) {
@@ -411,7 +430,7 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
             }
         }
         if (tid < D) {
-            const uint64_t j = (uint64_t)a.perm[(int64_t)kv * a.perm_sh + tid];
+            const uint64_t j = (uint64_t)p->a.perm[(int64_t)kv * p->a.perm_sh + tid];
             perm[tid] = (uint16_t)(j < (uint64_t)D ? j : D - 1);
         }
 #pragma unroll
@@ -435,7 +454,7 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
             uint32_t hi[BD / 2], lo[BD / 2];
 #pragma unroll
             for (int d = 0; d < BD; d += 2) {
-                const bool in = (e & 255) < a.n_centroids;
+                const bool in = (e & 255) < n_centroids;
                 win_split(in ? c[k][d] * scale : 0.f, in ? c[k][d + 1] * scale : 0.f, hi[d / 2], lo[d / 2]);
             }
             unsigned char* at = smem + e * (4 * BD);
@@ -450,16 +469,21 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
         }
     }
 
-    W u{p};
-    u.lane = lane; u.col = lane & 15; u.grp = lane >> 4; u.kv = kv;
+    W u;
+    u.lane = lane; u.col = lane & 15; u.grp = lane >> 4;
+    u.window = p->window; u.sinks = p->sinks; u.n_pages = p->n_pages; u.psh = p->psh;
+    u.c_sb = p->a.c_sb; u.c_st = p->a.c_st; u.v_sb = p->a.v_sb; u.vs_sb = p->vs_sb;
+    u.v_scale = p->v_scale + (int64_t)kv * p->vs_sh;
+    const int q_len = p->a.q_len;
     u.book = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)smem + u.grp * (W::NCL * 1024 * BD);
-    u.cbase = a.codes + (int64_t)kv * a.c_sh + (int64_t)(u.col & 3) * a.c_st + u.grp * W::NCL;
-    u.vbase = reinterpret_cast<const uint8_t*>(a.v) + ((int64_t)kv * a.v_sh + (int64_t)u.col * a.v_st) * (W::kV8 ? 1 : 2);
-    u.vstep = 16 * (uint32_t)a.v_st * (W::kV8 ? 1 : 2);
+    u.cbase = p->a.codes + (int64_t)kv * p->a.c_sh + (int64_t)(u.col & 3) * u.c_st + u.grp * W::NCL;
+    u.vbase = reinterpret_cast<const uint8_t*>(p->a.v) + ((int64_t)kv * p->a.v_sh + (int64_t)u.col * p->a.v_st) * (W::kV8 ? 1 : 2);
+    u.vstep = 16 * (uint32_t)p->a.v_st * (W::kV8 ? 1 : 2);
 
     WinCut<TT, RP> cut;
     int x = wg, x_end = 0;
-    if (!p.whole) {
+    const int whole = p->whole;
+    if (!whole) {
         cut.init(p, lane);
         x = min((int64_t)wg * cut.share, (int64_t)cut.total);
         x_end = min((int64_t)(wg + 1) * cut.share, (int64_t)cut.total);
@@ -467,35 +491,36 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
     const int x_begin = x;
     for (;;) {
         // ---- the next item and this workgroup's tiles of it
+        p = win_args();
         int item, i0 = 0, i1, slot = -1, start = 0, c = 0;
-        if (p.whole) {
-            if (x >= p.items) break;
+        if (whole) {
+            if (x >= p->items) break;
             item = x;
-            x += p.n_wg;
+            x += p->n_wg;
         } else {
             if (x >= x_end) break;
             cut.find(p, lane, x, item, start, c);
-            if (item >= p.items) break;
+            if (item >= p->items) break;
             x = start + c;
         }
         item = __builtin_amdgcn_readfirstlane(item);
-        const int b = item / p.rgroups, row0 = (item - b * p.rgroups) * RP;
-        const int len = max(0, min(a.seq_lens[b], a.seq_len));
-        u.t = win_tiles<TT>(p, len, row0, RP);
+        const int b = item / p->rgroups, row0 = (item - b * p->rgroups) * RP;
+        const int len = max(0, min(p->a.seq_lens[b], p->a.seq_len)), rows = p->rows, G = p->G;
+        u.t = win_tiles<TT>(WinShape{u.window, u.sinks, q_len, G, rows}, len, row0, RP);
         i1 = u.t.n;
-        if (!p.whole) {
-            i0 = max(0, x_begin - start - p.fixed);
-            i1 = max(0, min(u.t.n, x_end - start - p.fixed));
+        if (!whole) {
+            i0 = max(0, x_begin - start - p->fixed);
+            i1 = max(0, min(u.t.n, x_end - start - p->fixed));
             if (u.t.n == 0 ? start < x_begin : i1 <= i0) continue;  // its part here is of the fixed cost
             const bool mine = i0 == 0 && i1 == u.t.n;
             if (!mine) slot = start < x_begin ? 0 : 1;
             if (i0 == 0 && kv == 0 && tid == 0) {  // pieces, for the merge
                 const int w_last = (start + c - 1) / cut.share;
-                p.meta[2 * item] = 2 * wg + (slot > 0 ? 1 : 0);
-                p.meta[2 * item + 1] = mine ? 1 : w_last - wg + 1;
+                p->meta[2 * item] = 2 * wg + (slot > 0 ? 1 : 0);
+                p->meta[2 * item + 1] = mine ? 1 : w_last - wg + 1;
             }
         }
-        const int nr = min(RP, p.rows - row0);
+        const int nr = min(RP, rows - row0);
 
         // ---- its query rows: scaled in their dtype, permuted, in f16 at a power of two of each row's
         __syncthreads();  // (the codebook is staged, the last join is read)
@@ -506,18 +531,18 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
             for (int r0 = 0; r0 < RP; r0 += kWinThreads / kLpr) {
                 const int r = r0 + tid / kLpr, j = 4 * (tid % kLpr);
                 if (RP < kWinThreads / kLpr && r >= RP) break;  // whole waves
-                const int row = row0 + r, qi = row / p.G, h = kv * p.G + row - qi * p.G;
+                const int row = row0 + r, qi = row / G, h = kv * G + row - qi * G;
                 float y[4] = {0.f, 0.f, 0.f, 0.f}, most = 0.f;
                 if (r < nr) {
-                    const int64_t at = (int64_t)b * a.q_sb + (int64_t)h * a.q_sh + (int64_t)qi * a.q_sl;
+                    const int64_t at = (int64_t)b * p->a.q_sb + (int64_t)h * p->a.q_sh + (int64_t)qi * p->a.q_sl;
                     int64_t idx[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) idx[k] = at + perm[j + k];
-                    ssq_load_elems(a.q, a.q_dtype, idx, y);
+                    ssq_load_elems(p->a.q, p->a.q_dtype, idx, y);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    if (a.has_scale) y[k] = ssq_round_to(y[k] * a.scale, a.q_dtype);
+                    if (p->a.has_scale) y[k] = ssq_round_to(y[k] * p->a.scale, p->a.q_dtype);
                     const float z = fabsf(y[k]);
                     most = fmaxf(most, z < INFINITY ? z : 0.f);
                 }
@@ -536,7 +561,7 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
         // this wave's first places
         const int n_mine = i1 > i0 + wave ? (i1 - i0 - wave + kWinWaves - 1) / kWinWaves : 0;
         const int last_i = i0 + wave + kWinWaves * (n_mine - 1);
-        u.table = a.block_table + (int64_t)b * a.bt_sb;
+        u.table = p->a.block_table + (int64_t)b * p->a.bt_sb;
         u.last_tok = u.t.p_hi;
         // the places of the next tile's values and of the codes after the next tile's; the codes of this and the next tile
         typename W::Place pv{}, pc{};
@@ -546,15 +571,13 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
             const int i = i0 + wave, in = min(i + kWinWaves, last_i);
             pc = u.place(i, u.code_chunk());
             pv = u.place(i, u.grp);
-            const typename W::Place pn = u.place(in, u.code_chunk());
+            const typename W::Place pcn = u.place(in, u.code_chunk()), pvn = u.place(in, u.grp);
+            const typename W::Place pc2 = u.place(min(i + 2 * kWinWaves, last_i), u.code_chunk());
             u.load_codes(pc, c0);
-            val.scale = u.load_scale(pv);
-            const uint8_t* row = u.val_row(pv);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) val.v[dt] = u.load_val(row, dt);
-            u.load_codes(pn, c1);
-            pv = u.place(in, u.grp);
-            pc = u.place(min(in + kWinWaves, last_i), u.code_chunk());
+            u.load_codes(pcn, c1);
+            u.load_vals(pv, val);
+            pc = pc2;
+            pv = pvn;
         }
         __syncthreads();
         {
@@ -562,7 +585,7 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 u.fac[n] = facs[16 * n + u.col];
-                u.pos[n] = len - a.q_len + min(row0 + 16 * n + u.col, p.rows - 1) / p.G;
+                u.pos[n] = len - q_len + min(row0 + 16 * n + u.col, rows - 1) / G;
 #pragma unroll
                 for (int h = 0; h < QP; ++h) {
                     const uint16_t* src = qs + (h * RP + 16 * n + u.col) * L::kQRow + u.grp * (D / 4);
@@ -590,38 +613,38 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[n][dt] = w4f{};
         }
-        if (n_mine > 0) u.prime(c0);
-        for (int k = 0, i = i0 + wave; k < n_mine; ++k, i += kWinWaves) {
+        // Loads return in order: a place is asked for a tile before it is used, and before that tile's values.
+        for (int i = i0 + wave; i < i1; i += kWinWaves) {
             w4f s[NS][NR];
-            u.scores(c0, c1, s);
+            u.scores(c0, s);
             c0 = c1;
             u.load_codes(pc, c1);
             pc = u.place(min(i + 3 * kWinWaves, last_i), u.code_chunk());
             const int t0 = TT * u.tile_of(i), tok = t0 + CH * u.grp;
             // tokens of the tile that some row does not see (uniform)
-            const bool edge = t0 + TT - 1 > u.t.p_lo || (t0 <= u.t.p_hi - p.window && t0 + TT > p.sinks);
+            const bool edge = (t0 + TT - 1 > u.t.p_lo) | ((t0 <= u.t.p_hi - u.window) & (t0 + TT > u.sinks));
             bool apart = false;
             if (edge) {
-                uint32_t none = 0, some = 0;  // tokens that no row sees, that some do not
+                const uint32_t any = u.sees(u.t.p_lo, u.t.p_hi, tok), all = u.sees(u.t.p_hi, u.t.p_lo, tok);
 #pragma unroll
-                for (int e = 0; e < CH; ++e) {
-                    const int w = tok + e;
-                    const bool all = w <= u.t.p_lo && (w > u.t.p_hi - p.window || w < p.sinks);
-                    const bool any = w <= u.t.p_hi && (w > max(u.t.p_lo, 0) - p.window || w < p.sinks);
-                    none |= any ? 0u : 1u << e;
-                    some |= all ? 0u : 1u << e;
+                for (int n = 0; n < NR; ++n) {
+                    const uint32_t mine = u.sees(u.pos[n], u.pos[n], tok);
 #pragma unroll
-                    for (int n = 0; n < NR; ++n)
-                        if (!u.sees(u.pos[n], w)) s[e >> 2][n][e & 3] = -INFINITY;
+                    for (int e = 0; e < CH; ++e) s[e >> 2][n][e & 3] = mine >> e & 1u ? s[e >> 2][n][e & 3] : -INFINITY;
                 }
-                if (none == (1u << CH) - 1u) val.scale = 0.f;  // no page of this tile's
-                bool wild = false;
+                if (any == 0) val.scale = 0.f;  // no page of this tile's
+                const w4u off = W::spread(~any);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    val.v[dt] = W::cleared(val.v[dt], none);
-                    wild |= W::wild(val.v[dt], some);
+                for (int dt = 0; dt < DT; ++dt) val.v[dt] &= ~off;
+                if (q_len > 1) {
+                    const w4u part = W::spread(~all) & (W::kV8 ? 0x80808080u : 0x80008000u);
+                    uint32_t found = 0;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) found |= W::wild(val.v[dt][k]) & part[k];
+                    apart = __builtin_amdgcn_ballot_w64(found != 0) != 0;
                 }
-                apart = a.q_len > 1 && __builtin_amdgcn_ballot_w64(wild) != 0;
             }
             float top[NR];
             bool over = false;
@@ -675,7 +698,9 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
                     pw[n][e / 2] = W::kV8 ? win_pack_p<VT>(x0 * by, x1 * by) : win_pack_p<VT>(x0, x1);
                 }
             const uint8_t* next_row = u.val_row(pv);
-            const float next_scale = u.load_scale(pv);
+            val.scale = u.load_scale(pv);
+            pv = u.place(min(i + 2 * kWinWaves, last_i), u.grp);
+            __builtin_amdgcn_sched_barrier(0);
             if (!apart) {  // a value operand's successor loads once it is used
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
@@ -693,12 +718,10 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
                 // An infinite or NaN value that some rows see and others do not: the rows of one position at a time, the
                 // values that they do not see as 0.
                 for (int at = u.t.p_lo; at <= u.t.p_hi; ++at) {
-                    uint32_t gone = 0;
-#pragma unroll
-                    for (int e = 0; e < CH; ++e) gone |= u.sees(at, tok + e) ? 0u : 1u << e;
+                    const w4u off = W::spread(~u.sees(at, at, tok));
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        const w4u kept = W::cleared(val.v[dt], gone);
+                        const w4u kept = val.v[dt] & ~off;
 #pragma unroll
                         for (int n = 0; n < NR; ++n) {
                             w4f y = o[n][dt];
@@ -713,11 +736,10 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) val.v[dt] = u.load_val(next_row, dt);
             }
-            val.scale = next_scale;
-            pv = u.place(min(i + 2 * kWinWaves, last_i), u.grp);
         }
 
         // ---- the waves' join, 4 rows at a time
+        p = win_args();
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             l[n] = win_sum4(l[n]);
@@ -761,13 +783,13 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
                     ot += join[(w * 4 + r - r0) * kRow + dv];
                 }
                 if (slot < 0) {
-                    const int row = row0 + r, qi = row / p.G, h = kv * p.G + row - qi * p.G;
-                    ssq_store_elem(a.out, p.out_dtype, (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)qi * a.o_sl + dv,
+                    const int row = row0 + r, qi = row / p->G, h = kv * p->G + row - qi * p->G;
+                    ssq_store_elem(p->a.out, p->out_dtype, (int64_t)b * p->a.o_sb + (int64_t)h * p->a.o_sh + (int64_t)qi * p->a.o_sl + dv,
                                    lt == 0.f ? 0.f : ot / lt);
-                    if (a.lse && dv == 0)
-                        a.lse[((int64_t)b * a.num_q_heads + h) * a.q_len + qi] = lt == 0.f ? -INFINITY : (mt + log2f(lt)) * kWinLn2;
+                    if (p->a.lse && dv == 0)
+                        p->a.lse[((int64_t)b * p->a.num_q_heads + h) * p->a.q_len + qi] = lt == 0.f ? -INFINITY : (mt + log2f(lt)) * kWinLn2;
                 } else {
-                    float* dst = p.part + ((int64_t)(kv * p.n_wg + wg) * 2 + slot) * (RP * (D + 2));
+                    float* dst = p->part + ((int64_t)(kv * p->n_wg + wg) * 2 + slot) * (RP * (D + 2));
                     dst[r * D + dv] = ot;
                     if (dv == 0) {
                         dst[RP * D + r] = mt;

@@ -63,7 +63,7 @@ int most_tiles(const SsqWindowParams& p, int nr, bool v8) {
     const int last = (p.rgroups - 1) * 16 * nr;
     for (int row0 : {0, last})
         for (int len : {cap, cap - 63 > 0 ? cap - 63 : cap}) {  // a window's tiles depend on where it ends
-            const int n = v8 ? win_tiles<64>(p, len, row0, 16 * nr).n : win_tiles<32>(p, len, row0, 16 * nr).n;
+            const int n = v8 ? win_tiles<64>(win_shape(p), len, row0, 16 * nr).n : win_tiles<32>(win_shape(p), len, row0, 16 * nr).n;
             most = n > most ? n : most;
         }
     return p.window == INT_MAX ? most : most + 2;

@@ -248,7 +248,7 @@ struct WinRun {
 
     int lane, col, grp;
     int window, sinks, n_pages, psh;
-    int64_t c_sb, c_st, v_sb, vs_sb;
+    uint32_t c_sb, c_st, v_sb, vs_sb;  // strides (v_sb in bytes)
     const float* v_scale;           // of this KV head
     uint32_t book;                  // LDS address of the codebook, and this group's blocks in it
     uint4 q[QP][NR][NQ];
@@ -278,10 +278,10 @@ struct WinRun {
     }
     __device__ __forceinline__ int code_chunk() const { return (lane >> 2) & 3; }
     __device__ __forceinline__ void load_codes(const Place& e, Codes& r) const {
-        const uint8_t* row = cbase + (int64_t)e.page * c_sb + (int64_t)e.at * c_st;
+        const uint8_t* row = cbase + (uint64_t)(uint32_t)e.page * c_sb + (uint32_t)e.at * c_st;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const uint8_t* src = row + (int64_t)(4 * s) * c_st;
+            const uint8_t* src = row + 4 * s * c_st;
             if constexpr (NCL == 16) {
                 const w4u x = __builtin_nontemporal_load(reinterpret_cast<const w4u*>(src));
                 r.w[s][0] = x.x; r.w[s][1] = x.y; r.w[s][2] = x.z; r.w[s][3] = x.w;
@@ -296,7 +296,7 @@ struct WinRun {
         }
     }
     __device__ __forceinline__ const uint8_t* val_row(const Place& e) const {
-        return vbase + ((int64_t)e.page * v_sb + e.at) * (kV8 ? 1 : 2);
+        return vbase + (uint64_t)(uint32_t)e.page * v_sb + (uint32_t)e.at * (kV8 ? 1u : 2u);
     }
     __device__ __forceinline__ w4u load_val(const uint8_t* row, int dt) const {
         return __builtin_nontemporal_load(reinterpret_cast<const w4u*>(row + dt * vstep));
@@ -308,7 +308,7 @@ struct WinRun {
         for (int dt = 0; dt < DT; ++dt) r.v[dt] = load_val(row, dt);
     }
     __device__ __forceinline__ float load_scale(const Place& e) const {
-        if constexpr (kV8) return v_scale[(int64_t)e.page * vs_sb];
+        if constexpr (kV8) return v_scale[(uint64_t)(uint32_t)e.page * vs_sb];
         else return 1.f;
     }
 
@@ -472,10 +472,11 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
     W u;
     u.lane = lane; u.col = lane & 15; u.grp = lane >> 4;
     u.window = p->window; u.sinks = p->sinks; u.n_pages = p->n_pages; u.psh = p->psh;
-    u.c_sb = p->a.c_sb; u.c_st = p->a.c_st; u.v_sb = p->a.v_sb; u.vs_sb = p->vs_sb;
+    u.c_sb = (uint32_t)p->a.c_sb; u.c_st = (uint32_t)p->a.c_st; u.v_sb = (uint32_t)p->a.v_sb * (W::kV8 ? 1 : 2); u.vs_sb = (uint32_t)p->vs_sb;
     u.v_scale = p->v_scale + (int64_t)kv * p->vs_sh;
     const int q_len = p->a.q_len;
     u.book = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)smem + u.grp * (W::NCL * 1024 * BD);
+    asm("" : "+v"(u.book));  // opaque, or every block's address takes a register instead of the gather's offset field
     u.cbase = p->a.codes + (int64_t)kv * p->a.c_sh + (int64_t)(u.col & 3) * u.c_st + u.grp * W::NCL;
     u.vbase = reinterpret_cast<const uint8_t*>(p->a.v) + ((int64_t)kv * p->a.v_sh + (int64_t)u.col * p->a.v_st) * (W::kV8 ? 1 : 2);
     u.vstep = 16 * (uint32_t)p->a.v_st * (W::kV8 ? 1 : 2);
@@ -623,7 +624,7 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
             const int t0 = TT * u.tile_of(i), tok = t0 + CH * u.grp;
             // tokens of the tile that some row does not see (uniform)
             const bool edge = (t0 + TT - 1 > u.t.p_lo) | ((t0 <= u.t.p_hi - u.window) & (t0 + TT > u.sinks));
-            bool apart = false;
+            bool apart = false;  // an infinite or NaN value that some rows see and others do not
             if (edge) {
                 const uint32_t any = u.sees(u.t.p_lo, u.t.p_hi, tok), all = u.sees(u.t.p_hi, u.t.p_lo, tok);
 #pragma unroll
@@ -697,44 +698,40 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
                     l[n] += x0 + x1;
                     pw[n][e / 2] = W::kV8 ? win_pack_p<VT>(x0 * by, x1 * by) : win_pack_p<VT>(x0, x1);
                 }
-            const uint8_t* next_row = u.val_row(pv);
-            val.scale = u.load_scale(pv);
-            pv = u.place(min(i + 2 * kWinWaves, last_i), u.grp);
-            __builtin_amdgcn_sched_barrier(0);
-            if (!apart) {  // a value operand's successor loads once it is used
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-                    for (int jj = 0; jj < CH / 8; ++jj) {
-                        const uint4 v = u.vals(val.v[dt], jj);
-#pragma unroll
-                        for (int n = 0; n < NR; ++n)
-                            o[n][dt] = win_mfma_v<VT>(v, make_uint4(pw[n][4 * jj], pw[n][4 * jj + 1], pw[n][4 * jj + 2], pw[n][4 * jj + 3]), o[n][dt]);
-                    }
-                    val.v[dt] = u.load_val(next_row, dt);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            } else {
-                // An infinite or NaN value that some rows see and others do not: the rows of one position at a time, the
-                // values that they do not see as 0.
+            if (apart) {
+                // The rows of one position at a time, the values that they do not see as 0; the products below then add nothing.
                 for (int at = u.t.p_lo; at <= u.t.p_hi; ++at) {
-                    const w4u off = W::spread(~u.sees(at, at, tok));
+                    const w4u on = W::spread(u.sees(at, at, tok));
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const w4u kept = val.v[dt] & ~off;
+                    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                         for (int n = 0; n < NR; ++n) {
                             w4f y = o[n][dt];
 #pragma unroll
                             for (int jj = 0; jj < CH / 8; ++jj)
-                                y = win_mfma_v<VT>(u.vals(kept, jj), make_uint4(pw[n][4 * jj], pw[n][4 * jj + 1], pw[n][4 * jj + 2], pw[n][4 * jj + 3]), y);
+                                y = win_mfma_v<VT>(u.vals(val.v[dt] & on, jj), make_uint4(pw[n][4 * jj], pw[n][4 * jj + 1], pw[n][4 * jj + 2], pw[n][4 * jj + 3]), y);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) o[n][dt][e] = u.pos[n] == at ? y[e] : o[n][dt][e];
                         }
-                    }
                 }
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) val.v[dt] = u.load_val(next_row, dt);
+                for (int dt = 0; dt < DT; ++dt) val.v[dt] = w4u{};
+            }
+            const uint8_t* next_row = u.val_row(pv);
+            val.scale = u.load_scale(pv);
+            pv = u.place(min(i + 2 * kWinWaves, last_i), u.grp);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {  // a value operand's successor loads once it is used
+#pragma unroll
+                for (int jj = 0; jj < CH / 8; ++jj) {
+                    const uint4 v = u.vals(val.v[dt], jj);
+#pragma unroll
+                    for (int n = 0; n < NR; ++n)
+                        o[n][dt] = win_mfma_v<VT>(v, make_uint4(pw[n][4 * jj], pw[n][4 * jj + 1], pw[n][4 * jj + 2], pw[n][4 * jj + 3]), o[n][dt]);
+                }
+                val.v[dt] = u.load_val(next_row, dt);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
 

@@ -52,6 +52,9 @@ int check(const ssq_window_args* a) {
     SSQ_REQUIRE((uintptr_t)d.v % 16 == 0 && d.v_sb % per == 0 && d.v_sh % per == 0 && d.v_st % per == 0,
                 "value rows must be 16-byte aligned");
     SSQ_REQUIRE(d.v_st >= 0 && d.v_st <= 1 << 22, "the values' dim stride must be at most 2^22");
+    SSQ_REQUIRE(d.c_sb >= 0 && d.c_sb < 1ll << 31 && d.c_st >= 0 && d.c_st <= 1 << 22 && d.v_sb >= 0 && d.v_sb < 1ll << 30 &&
+                    a->vs_sb >= 0 && a->vs_sb < 1ll << 30,
+                "page strides must be below 2^30 elements");
     SSQ_REQUIRE((int64_t)d.batch * d.num_q_heads * d.q_len == 0 || d.num_kv_heads <= 1 << 16, "too many KV heads");
     return SSQ_OK;
 }

@@ -25,6 +25,8 @@
 
 #include "ssq_common.h"
 
+#include <type_traits>
+
 struct SsqWindowParams {
     ssq_decode_args a;
     int window, sinks;       // window: INT_MAX where everything is seen
@@ -32,17 +34,18 @@ struct SsqWindowParams {
     int n_pages;
     const float* v_scale;
     int64_t vs_sb, vs_sh;
-    int G, rows, rgroups;    // query rows of a (sequence, KV head): (qi, g), g fastest; groups of 16 NR rows
+    int G, rows, rgroups;    // query rows of a (sequence, KV head): (qi, g), g fastest; groups of 16 rows
     int items;               // batch * rgroups
     int n_wg;                // workgroups per KV head
-    int whole;               // a workgroup takes whole items; else equal shares of all their tiles (WinCut)
+    int team;                // a workgroup's waves share whole items; else each wave has an equal share of all tiles (WinCut)
     int fixed, least;        // an item's cost beside its tiles, and the smallest share, both in tiles
     int psh;                 // log2(page_size / 16)
-    float* part;             // [Hkv][n_wg][2] slots of 16 NR rows x (Dv + 2): o, then m (log2 units), l
-    int* meta;               // [items][2]: first workgroup * 2 + its slot, and pieces
+    int q_vec, out_vec;      // query rows load in 16-byte pieces; four values of the output store as one
+    float* part;             // [Hkv][n_wg * 8 waves][2] slots of 16 rows x (Dv + 2): o, then m (log2 units), l
+    int* meta;               // [items][2]: first worker * 2 + its slot, and pieces
 };
 
-#define SSQ_WINDOW_UNIT(name) int name(const SsqWindowParams& p, int nr, hipStream_t st)
+#define SSQ_WINDOW_UNIT(name) int name(const SsqWindowParams& p, hipStream_t st)
 SSQ_WINDOW_UNIT(ssq_window_64_e4m3);
 SSQ_WINDOW_UNIT(ssq_window_64_bf16);
 SSQ_WINDOW_UNIT(ssq_window_64_f16);
@@ -50,9 +53,9 @@ SSQ_WINDOW_UNIT(ssq_window_128_e4m3);
 SSQ_WINDOW_UNIT(ssq_window_128_bf16);
 SSQ_WINDOW_UNIT(ssq_window_128_f16);
 
-// waves of a workgroup: two a SIMD, so that one's matrix products run beside the other's vector work; with 32 query rows
-// the registers hold one
-__host__ __device__ constexpr int win_waves(int nr) { return nr == 1 ? 8 : 4; }
+// waves of a workgroup: two a SIMD, so that one's matrix products run beside the other's vector work.  (32 rows a wave, half as
+// many gathers for a row, leave registers for one: 20 rows a sequence 43 us for 36, a chunk of 512 tokens 162 for 119.)
+constexpr int kWinWaves = 8, kWinThreads = kWinWaves * 64, kWinRows = 16;
 
 // what the tiles of an item follow from, beside its length
 struct WinShape { int window, sinks, q_len, G, rows; };
@@ -65,9 +68,9 @@ struct WinTiles {
     int n, n_sink, from; // tile i: i < n_sink ? i : from + i - n_sink
 };
 template <int TT>
-__host__ __device__ __forceinline__ WinTiles win_tiles(const WinShape& p, int len, int row0, int rows_per) {
+__host__ __device__ __forceinline__ WinTiles win_tiles(const WinShape& p, int len, int row0) {
     WinTiles t;
-    const int last = (row0 + rows_per < p.rows ? row0 + rows_per : p.rows) - 1;
+    const int last = (row0 + kWinRows < p.rows ? row0 + kWinRows : p.rows) - 1;
     t.p_lo = len - p.q_len + row0 / p.G;
     t.p_hi = len - p.q_len + last / p.G;
     t.n = t.n_sink = t.from = 0;
@@ -119,11 +122,12 @@ __device__ __forceinline__ uint32_t win_pack_p(float a, float b) {
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, w2h));
 }
 __device__ __forceinline__ float win_h(uint32_t w, int i) { return ssq_f16_to_f32(i ? w >> 16 : w & 0xFFFFu); }
-// x rounded to f16, and the rounding of what that left (0 beside an infinity or NaN)
+// x rounded to f16, and the rounding of what that left (CHECKED: 0 beside an infinity)
+template <bool CHECKED>
 __device__ __forceinline__ void win_split(float x, float y, uint32_t& hi, uint32_t& lo) {
     hi = win_pack_h(x, y);
     const float u = x - win_h(hi, 0), v = y - win_h(hi, 1);
-    lo = win_pack_h(__builtin_isfinite(u) ? u : 0.f, __builtin_isfinite(v) ? v : 0.f);
+    lo = CHECKED ? win_pack_h(__builtin_isfinite(u) ? u : 0.f, __builtin_isfinite(v) ? v : 0.f) : win_pack_h(u, v);
 }
 // four e4m3 values as two packed pairs of f16 (exact)
 __device__ __forceinline__ w2u win_e4m3(uint32_t w) {
@@ -134,6 +138,24 @@ __device__ __forceinline__ w2u win_e4m3(uint32_t w) {
 }
 // exponent e with x < 2^e, of a positive finite x (0: 0)
 __device__ __forceinline__ int win_exp(float x) { return x > 0.f ? __builtin_amdgcn_frexp_expf(x) : 0; }
+
+// four values to the output's dtype, as one piece
+__device__ __forceinline__ void win_store4(void* out, int dtype, int64_t i, w4f z) {
+    if (dtype == SSQ_F32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + i) = make_float4(z[0], z[1], z[2], z[3]);
+    } else {
+        const uint2 w = dtype == SSQ_BF16 ? make_uint2(win_pack_p<SSQ_BF16>(z[0], z[1]), win_pack_p<SSQ_BF16>(z[2], z[3]))
+                                          : make_uint2(win_pack_h(z[0], z[1]), win_pack_h(z[2], z[3]));
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + i) = w;
+    }
+}
+
+// a wave's LDS writes before this point are seen by its reads after it (one wave's LDS operations execute in order)
+__device__ __forceinline__ void win_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // a group's value over the four lane groups of a column
 __device__ __forceinline__ float win_max4(float v) {
@@ -154,18 +176,20 @@ __device__ __forceinline__ WinArgs win_args() {
     return k;
 }
 
-// Equal shares of the items' tiles: the items of a KV head lie end to end on a cost axis, fixed + tiles each, and
-// workgroup w takes [w share, (w + 1) share).  An item inside one share is written out by its workgroup; one that spans
-// several leaves a partial in each: slot 0 of a workgroup for the item its share starts in, slot 1 for one that starts in
-// it.  Everything follows from the lengths, which the host does not see.
-template <int TT, int RP>
+// Equal shares of the items' tiles: the items of a KV head lie end to end on a cost axis, fixed + tiles each, and worker w (a
+// wave; the waves of a workgroup are n_wg apart) takes [w share, (w + 1) share).  An item inside one share is written out by its
+// wave; one that spans several leaves a partial in each: slot 0 of a worker for the item its share starts in, slot 1 for one that
+// starts in it.  Everything follows from the lengths, which the host does not see.  Waves that wait for nobody keep the memory
+// busy through one another's beginnings and ends.
+template <int TT>
 struct WinCut {
     int share, total;
-    __device__ __forceinline__ static int cost(WinArgs p, int i) {
+    int c0, v0;  // this lane's cost and inclusive sum over the first 64 items
+    __device__ __forceinline__ static int length(WinArgs p, int i) { return p->a.seq_lens[min(i, p->items - 1) / p->rgroups]; }
+    __device__ __forceinline__ static int cost(WinArgs p, int i, int len) {
         if (i >= p->items) return 0;
-        const int b = i / p->rgroups, g = i - b * p->rgroups;
         const WinShape s{p->window, p->sinks, p->a.q_len, p->G, p->rows};
-        return p->fixed + win_tiles<TT>(s, max(0, min(p->a.seq_lens[b], p->a.seq_len)), g * RP, RP).n;
+        return p->fixed + win_tiles<TT>(s, max(0, min(len, p->a.seq_len)), i % p->rgroups * kWinRows).n;
     }
     __device__ __forceinline__ static int scan(int v) {  // inclusive, over the wave
         v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
@@ -176,17 +200,20 @@ struct WinCut {
         v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
         return v;
     }
-    // (the whole wave calls these two)
-    __device__ __forceinline__ void init(WinArgs p, int lane) {
-        total = 0;
-        for (int i = 0; i < p->items; i += SSQ_WAVE) total += __builtin_amdgcn_readlane(scan(cost(p, i + lane)), 63);
-        share = (max((total + p->n_wg - 1) / p->n_wg, p->least) + 7) & ~7;
+    // (the whole wave calls these two; len: length(lane), asked for before)
+    __device__ __forceinline__ void init(WinArgs p, int lane, int len) {
+        c0 = cost(p, lane, len);
+        v0 = scan(c0);
+        total = __builtin_amdgcn_readlane(v0, 63);
+        for (int i = SSQ_WAVE; i < p->items; i += SSQ_WAVE)
+            total += __builtin_amdgcn_readlane(scan(cost(p, i + lane, length(p, i + lane))), 63);
+        const int workers = p->n_wg * kWinWaves;
+        share = max((total + workers - 1) / workers, p->least);
     }
     // the item that holds cost position x < total, its start and cost
     __device__ __forceinline__ void find(WinArgs p, int lane, int x, int& item, int& s, int& c) const {
-        int base = 0;
-        for (int f = 0; f < p->items; f += SSQ_WAVE) {
-            const int mine = cost(p, f + lane), v = scan(mine);
+        int base = 0, mine = c0, v = v0;
+        for (int f = 0;;) {
             const uint64_t hit = __builtin_amdgcn_ballot_w64(base + v > x);
             if (hit) {
                 const int l = __builtin_ctzll(hit);
@@ -196,6 +223,10 @@ struct WinCut {
                 return;
             }
             base += __builtin_amdgcn_readlane(v, 63);
+            f += SSQ_WAVE;
+            if (f >= p->items) break;  // not reached for x < total
+            mine = cost(p, f + lane, length(p, f + lane));
+            v = scan(mine);
         }
         item = p->items;
         s = x;
@@ -203,26 +234,22 @@ struct WinCut {
     }
 };
 
-// LDS: codebook | scratch: query parts, then the waves' join | m, l [waves][RP] | rows' factors [RP] | reduction [waves] | permutation [D]
-template <int D, int NR, int QP>
+// LDS: codebook | the waves' query rows, and their join | m, l [waves][16] | reduction [waves] | permutation [D]
+template <int D>
 struct WinLds {
-    static constexpr int RP = 16 * NR, kWaves = win_waves(NR);
     static constexpr int kBook = D * 256 * 4;
     static constexpr int kJoinRows = 4;
     static constexpr int kJoinRow = D + 4;  // floats
-    static constexpr int kQRow = D + 8;      // f16 elements
-    static constexpr int kQ = RP * kQRow * 2 * QP;
-    static constexpr int kJoin = kWaves * kJoinRows * kJoinRow * 4;
-    static constexpr int kScratch = kQ > kJoin ? kQ : kJoin;
-    static constexpr int kMl = kBook + kScratch;
-    static constexpr int kFac = kMl + 2 * kWaves * RP * 4;
-    static constexpr int kRed = kFac + RP * 4;
-    static constexpr int kPerm = kRed + kWaves * 4;
+    static constexpr int kQRow = 2 * D + 16;  // bytes of a 16-bit query row; 8 of them a wave at a time, or 4 of 32 bits
+    static constexpr int kQ = kWinWaves * 8 * kQRow, kJoin = kWinWaves * kJoinRows * kJoinRow * 4;
+    static constexpr int kMl = kBook + (kQ > kJoin ? kQ : kJoin);
+    static constexpr int kRed = kMl + 2 * kWinWaves * kWinRows * 4;
+    static constexpr int kPerm = kRed + kWinWaves * 4;
     static constexpr int kTotal = kPerm + 2 * D;
 };
 
-// D: head_dim and value_dim, BD: block_dim, VT: value dtype, NR: columns of 16 query rows, QP: query parts
-template <int D, int BD, int VT, int NR, int QP>
+// D: head_dim and value_dim, BD: block_dim, VT: value dtype, QP: query parts
+template <int D, int BD, int VT, int QP>
 struct WinRun {
     static constexpr bool kV8 = VT == SSQ_E4M3;
     static constexpr int CH = kV8 ? 16 : 8;        // tokens of a lane group
@@ -232,10 +259,10 @@ struct WinRun {
     static constexpr int NCL = NB / 4;             // codes of a token that a lane gathers
     static constexpr int NW = (NCL + 3) / 4;       // in words
     static constexpr int DT = D / 16;
-    static constexpr int RP = 16 * NR;
     static constexpr int NK = D / 16;              // score MFMAs of 16 tokens (a lane's four dims, hi and lo, each)
     static constexpr int NQ = BD == 8 ? NK / 2 : NK;  // query operands
-    using L = WinLds<D, NR, QP>;
+    static constexpr int NE = D / 4;               // query dims of a lane
+    using L = WinLds<D>;
 
     static constexpr int NST = NS * NK;            // score steps of a tile
     static constexpr int kAhead = 4;               // operands gathered ahead
@@ -251,11 +278,11 @@ struct WinRun {
     uint32_t c_sb, c_st, v_sb, vs_sb;  // strides (v_sb in bytes)
     const float* v_scale;           // of this KV head
     uint32_t book;                  // LDS address of the codebook, and this group's blocks in it
-    uint4 q[QP][NR][NQ];
-    float fac[NR];                  // scores to log2 units
+    uint4 q[QP][NQ];
+    float fac;                      // scores to log2 units
     // the item
-    int pos[NR];                    // this column's positions
-    WinTiles t;
+    int pos;                        // this column's position
+    WinTiles t{};
     const int32_t* table;
     int last_tok;
     // addresses
@@ -335,7 +362,7 @@ struct WinRun {
     }
     // A tile's scores.  Gathers run kAhead steps before their products; the barriers keep the compiler from gathering a whole
     // tile ahead, which does not fit the registers.
-    __device__ __forceinline__ void scores(const Codes& c, w4f (&s)[NS][NR]) const {
+    __device__ __forceinline__ void scores(const Codes& c, w4f (&s)[NS]) const {
         uint4 ring[kAhead];
 #pragma unroll
         for (int st = 0; st < kAhead; ++st) ring[st] = operand(c, st);
@@ -343,13 +370,9 @@ struct WinRun {
 #pragma unroll
         for (int st = 0; st < NST; ++st) {
             const uint4 x = ring[st % kAhead];
+            w4f& acc = s[st / NK];
 #pragma unroll
-            for (int h = 0; h < QP; ++h)
-#pragma unroll
-                for (int n = 0; n < NR; ++n) {
-                    w4f& acc = s[st / NK][n];
-                    acc = win_mfma(x, q[h][n][BD == 8 ? st % NK / 2 : st % NK], st % NK || h ? acc : w4f{});
-                }
+            for (int h = 0; h < QP; ++h) acc = win_mfma(x, q[h][BD == 8 ? st % NK / 2 : st % NK], st % NK || h ? acc : w4f{});
             if (st + kAhead < NST) ring[st % kAhead] = operand(c, st + kAhead);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -391,12 +414,12 @@ struct WinRun {
     }
 };
 
-template <int D, int BD, int VT, int NR, int QP>
-__global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_waves_per_eu(NR == 1 ? 2 : 1, NR == 1 ? 2 : 1))) void k_window(const SsqWindowParams) {
-    using W = WinRun<D, BD, VT, NR, QP>;
+template <int D, int BD, int VT, int QP, bool TEAM>
+__global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_window(const SsqWindowParams) {
+    using W = WinRun<D, BD, VT, QP>;
     using L = typename W::L;
-    constexpr int RP = W::RP, TT = W::TT, CH = W::CH, NS = W::NS, DT = W::DT;
-    constexpr int kWinWaves = win_waves(NR), kWinThreads = kWinWaves * SSQ_WAVE;
+    constexpr int TT = W::TT, CH = W::CH, NS = W::NS, DT = W::DT, NE = W::NE;
+    constexpr int kStep = TEAM ? kWinWaves : 1;  // from a wave's tile to its next
     extern __shared__ __align__(16) unsigned char smem[];
     WinArgs p = win_args();
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -404,20 +427,16 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
     float* red = reinterpret_cast<float*>(smem + L::kRed);
     uint16_t* perm = reinterpret_cast<uint16_t*>(smem + L::kPerm);
     float* mls = reinterpret_cast<float*>(smem + L::kMl);
-    float* facs = reinterpret_cast<float*>(smem + L::kFac);
 
-    // ---- the codebook, 64 (32) floats a thread, all asked for at once
+    // ---- the codebook, 64 (32) floats a thread, all asked for at once behind the permutation
     constexpr int kPer = W::NB * 256 / kWinThreads;
-    int book_exp;  // the codebook is staged times 2^book_exp
+    // (No branches around these loads or the first tiles': they return in order, and a wait behind a branch is for all of them.)
+    const int64_t at_perm = p->a.perm[(int64_t)kv * p->a.perm_sh + min(tid, D - 1)];
+    const int first_len = TEAM ? 0 : WinCut<TT>::length(p, lane);
+    float c[kPer][BD];
     {
         const float* cent = p->a.cent + (int64_t)kv * p->a.cent_sh;
-        const int n_centroids = p->a.n_centroids;
-        float c[kPer][BD];
-        float most = 0.f;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int e = tid + k * kWinThreads, blk = e >> 8, w = e & 255;
-            const float* src = cent + (int64_t)(blk * n_centroids + min(w, n_centroids - 1)) * BD;
+        auto entry = [&](int k, const float* src) {
             if constexpr (BD >= 4) {
 #pragma unroll
                 for (int d = 0; d < BD; d += 4) {
@@ -428,46 +447,13 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
                 const float2 x = *reinterpret_cast<const float2*>(src);
                 c[k][0] = x.x; c[k][1] = x.y;
             }
-        }
-        if (tid < D) {
-            const uint64_t j = (uint64_t)p->a.perm[(int64_t)kv * p->a.perm_sh + tid];
-            perm[tid] = (uint16_t)(j < (uint64_t)D ? j : D - 1);
-        }
+        };
+        const int n = p->a.n_centroids;  // entry e = tid + k * kWinThreads: block e / 256, codeword e % 256
+        const float* src = cent + ((tid >> 8) * n + min(tid & 255, n - 1)) * BD;
 #pragma unroll
-        for (int k = 0; k < kPer; ++k)
-#pragma unroll
-            for (int d = 0; d < BD; ++d) {
-                const float x = fabsf(c[k][d]);
-                most = fmaxf(most, x < INFINITY ? x : 0.f);
-            }
-        most = ssq_wave_max(most);
-        if (lane == 0) red[wave] = most;
-        __syncthreads();
-        most = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWinWaves; ++w) most = fmaxf(most, red[w]);
-        book_exp = min(15 - win_exp(most), 126);
-        const float scale = ldexpf(1.f, book_exp);
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int e = tid + k * kWinThreads;
-            uint32_t hi[BD / 2], lo[BD / 2];
-#pragma unroll
-            for (int d = 0; d < BD; d += 2) {
-                const bool in = (e & 255) < n_centroids;
-                win_split(in ? c[k][d] * scale : 0.f, in ? c[k][d + 1] * scale : 0.f, hi[d / 2], lo[d / 2]);
-            }
-            unsigned char* at = smem + e * (4 * BD);
-            if constexpr (BD == 8) {
-                *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(at + 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            } else if constexpr (BD == 4) {
-                *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
-            } else {
-                *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], lo[0]);
-            }
-        }
+        for (int k = 0; k < kPer; ++k) entry(k, src + k * (kWinThreads / 256 * BD) * n);
     }
+    if (tid < D) perm[tid] = (uint16_t)((uint64_t)at_perm < (uint64_t)D ? at_perm : D - 1);
 
     W u;
     u.lane = lane; u.col = lane & 15; u.grp = lane >> 4;
@@ -481,158 +467,248 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
     u.vbase = reinterpret_cast<const uint8_t*>(p->a.v) + ((int64_t)kv * p->a.v_sh + (int64_t)u.col * p->a.v_st) * (W::kV8 ? 1 : 2);
     u.vstep = 16 * (uint32_t)p->a.v_st * (W::kV8 ? 1 : 2);
 
-    WinCut<TT, RP> cut;
-    int x = wg, x_end = 0;
-    const int whole = p->whole;
-    if (!whole) {
-        cut.init(p, lane);
-        x = min((int64_t)wg * cut.share, (int64_t)cut.total);
-        x_end = min((int64_t)(wg + 1) * cut.share, (int64_t)cut.total);
+    // ---- what is to be done: an item's tiles [i0, i1), and where they go (slot -1: the output)
+    WinCut<TT> cut;
+    const int worker = TEAM ? wg : wave * p->n_wg + wg;
+    int x = worker, x_begin = 0, x_end = 0;
+    if constexpr (!TEAM) {
+        cut.init(p, lane, first_len);
+        x = x_begin = (int)min((int64_t)worker * cut.share, (int64_t)cut.total);
+        x_end = (int)min((int64_t)(worker + 1) * cut.share, (int64_t)cut.total);
     }
-    const int x_begin = x;
-    for (;;) {
-        // ---- the next item and this workgroup's tiles of it
+    int b = 0, row0 = 0, nr = 0, len = 0, i0 = 0, i1 = 0, slot = -1;
+    auto next = [&]() {
         p = win_args();
-        int item, i0 = 0, i1, slot = -1, start = 0, c = 0;
-        if (whole) {
-            if (x >= p->items) break;
-            item = x;
-            x += p->n_wg;
-        } else {
-            if (x >= x_end) break;
-            cut.find(p, lane, x, item, start, c);
-            if (item >= p->items) break;
-            x = start + c;
-        }
-        item = __builtin_amdgcn_readfirstlane(item);
-        const int b = item / p->rgroups, row0 = (item - b * p->rgroups) * RP;
-        const int len = max(0, min(p->a.seq_lens[b], p->a.seq_len)), rows = p->rows, G = p->G;
-        u.t = win_tiles<TT>(WinShape{u.window, u.sinks, q_len, G, rows}, len, row0, RP);
-        i1 = u.t.n;
-        if (!whole) {
-            i0 = max(0, x_begin - start - p->fixed);
-            i1 = max(0, min(u.t.n, x_end - start - p->fixed));
-            if (u.t.n == 0 ? start < x_begin : i1 <= i0) continue;  // its part here is of the fixed cost
-            const bool mine = i0 == 0 && i1 == u.t.n;
-            if (!mine) slot = start < x_begin ? 0 : 1;
-            if (i0 == 0 && kv == 0 && tid == 0) {  // pieces, for the merge
-                const int w_last = (start + c - 1) / cut.share;
-                p->meta[2 * item] = 2 * wg + (slot > 0 ? 1 : 0);
-                p->meta[2 * item + 1] = mine ? 1 : w_last - wg + 1;
+        for (;;) {
+            int item, start = 0, cost = 0;
+            if constexpr (TEAM) {
+                if (x >= p->items) return false;
+                item = x;
+                x += p->n_wg;
+            } else {
+                if (x >= x_end) return false;
+                cut.find(p, lane, x, item, start, cost);
+                if (item >= p->items) return false;
+                x = start + cost;
             }
-        }
-        const int nr = min(RP, rows - row0);
-
-        // ---- its query rows: scaled in their dtype, permuted, in f16 at a power of two of each row's
-        __syncthreads();  // (the codebook is staged, the last join is read)
-        {
-            constexpr int kLpr = D / 4;  // lanes of a row, 4 dims each
-            uint16_t* qs = reinterpret_cast<uint16_t*>(smem + L::kBook);
-#pragma unroll
-            for (int r0 = 0; r0 < RP; r0 += kWinThreads / kLpr) {
-                const int r = r0 + tid / kLpr, j = 4 * (tid % kLpr);
-                if (RP < kWinThreads / kLpr && r >= RP) break;  // whole waves
-                const int row = row0 + r, qi = row / G, h = kv * G + row - qi * G;
-                float y[4] = {0.f, 0.f, 0.f, 0.f}, most = 0.f;
-                if (r < nr) {
-                    const int64_t at = (int64_t)b * p->a.q_sb + (int64_t)h * p->a.q_sh + (int64_t)qi * p->a.q_sl;
-                    int64_t idx[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) idx[k] = at + perm[j + k];
-                    ssq_load_elems(p->a.q, p->a.q_dtype, idx, y);
+            item = __builtin_amdgcn_readfirstlane(item);
+            b = item / p->rgroups;
+            row0 = (item - b * p->rgroups) * kWinRows;
+            len = max(0, min(p->a.seq_lens[b], p->a.seq_len));
+            nr = min(kWinRows, p->rows - row0);
+            u.t = win_tiles<TT>(WinShape{u.window, u.sinks, q_len, p->G, p->rows}, len, row0);
+            slot = -1;
+            i0 = TEAM ? wave : 0;
+            i1 = u.t.n;
+            if constexpr (!TEAM) {
+                i0 = max(0, x_begin - start - p->fixed);
+                i1 = max(0, min(u.t.n, x_end - start - p->fixed));
+                if (u.t.n == 0 ? start < x_begin : i1 <= i0) continue;  // its part here is of the fixed cost
+                const bool mine = i0 == 0 && i1 == u.t.n;
+                if (!mine) slot = start < x_begin ? 0 : 1;
+                if (i0 == 0 && kv == 0 && lane == 0) {  // pieces, for the merge
+                    p->meta[2 * item] = 2 * worker + (slot > 0 ? 1 : 0);
+                    p->meta[2 * item + 1] = mine ? 1 : (start + cost - 1) / cut.share - worker + 1;
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (p->a.has_scale) y[k] = ssq_round_to(y[k] * p->a.scale, p->a.q_dtype);
-                    const float z = fabsf(y[k]);
-                    most = fmaxf(most, z < INFINITY ? z : 0.f);
-                }
-#pragma unroll
-                for (int o = 1; o < kLpr; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
-                const int up = min(15 - win_exp(most), 126);
-                const float s = ldexpf(1.f, up);
-                uint32_t hi[2], lo[2];
-                win_split(y[0] * s, y[1] * s, hi[0], lo[0]);
-                win_split(y[2] * s, y[3] * s, hi[1], lo[1]);
-                *reinterpret_cast<uint2*>(qs + r * L::kQRow + j) = make_uint2(hi[0], hi[1]);
-                if constexpr (QP == 2) *reinterpret_cast<uint2*>(qs + (RP + r) * L::kQRow + j) = make_uint2(lo[0], lo[1]);
-                if (tid % kLpr == 0) facs[r] = ldexpf(kWinLog2e, max(-book_exp - up, -126));  // above 0
             }
+            return true;
         }
-        // this wave's first places
-        const int n_mine = i1 > i0 + wave ? (i1 - i0 - wave + kWinWaves - 1) / kWinWaves : 0;
-        const int last_i = i0 + wave + kWinWaves * (n_mine - 1);
+    };
+    // ---- its first loads: the tiles', then the query rows'
+    // the places of the next tile's values and of the codes after the next tile's; the codes of this and the next tile
+    typename W::Place pv{}, pc{};
+    typename W::Codes c0, c1;
+    typename W::Vals val;
+    // Query rows come in 16-byte pieces, 1 KiB a wave at once, kPieces times: 16 rows of 16 bits, or 8 of 32 (those behind are
+    // loaded when their turn comes).
+    constexpr int kPieces = D / 32;
+    uint4 qraw[kPieces];
+    int last_i = 0;
+    // piece k of a batch from row r0 on: its row and byte in it
+    auto q_at = [&](int k, int r0, int& r, int& byte) {
+        constexpr int row_bytes = QP == 2 ? 4 * D : 2 * D;
+        const int o = (k * SSQ_WAVE + lane) * 16;
+        r = r0 + o / row_bytes;
+        byte = o % row_bytes;
+    };
+    auto q_load = [&](int k, int r0) {
+        int r, byte;
+        q_at(k, r0, r, byte);
+        const int row = row0 + max(0, min(r, nr - 1)), qi = row / p->G, h = kv * p->G + row - qi * p->G;
+        constexpr int size = QP == 2 ? 4 : 2;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(p->a.q) + ((int64_t)b * p->a.q_sb + (int64_t)h * p->a.q_sh + (int64_t)qi * p->a.q_sl) * size + byte;
+        if (p->q_vec) return *reinterpret_cast<const uint4*>(src);
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = size == 4 ? reinterpret_cast<const uint32_t*>(src)[e]
+                             : (uint32_t)reinterpret_cast<const uint16_t*>(src)[2 * e] | (uint32_t)reinterpret_cast<const uint16_t*>(src)[2 * e + 1] << 16;
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    auto load = [&]() {
         u.table = p->a.block_table + (int64_t)b * p->a.bt_sb;
-        u.last_tok = u.t.p_hi;
-        // the places of the next tile's values and of the codes after the next tile's; the codes of this and the next tile
-        typename W::Place pv{}, pc{};
-        typename W::Codes c0, c1;
-        typename W::Vals val;
-        if (n_mine > 0) {
-            const int i = i0 + wave, in = min(i + kWinWaves, last_i);
-            pc = u.place(i, u.code_chunk());
-            pv = u.place(i, u.grp);
-            const typename W::Place pcn = u.place(in, u.code_chunk()), pvn = u.place(in, u.grp);
-            const typename W::Place pc2 = u.place(min(i + 2 * kWinWaves, last_i), u.code_chunk());
-            u.load_codes(pc, c0);
-            u.load_codes(pcn, c1);
-            u.load_vals(pv, val);
-            pc = pc2;
-            pv = pvn;
+        u.last_tok = max(u.t.p_hi, 0);
+        u.pos = len - q_len + min(row0 + u.col, p->rows - 1) / p->G;
+        // (a wave without tiles loads the last one's)
+        const int i = max(0, min(i0, i1 - 1));
+        last_i = i0 < i1 ? i1 - 1 - (i1 - 1 - i0) % kStep : i;
+        const int in = min(i + kStep, last_i);
+        pc = u.place(i, u.code_chunk());
+        pv = u.place(i, u.grp);
+        const typename W::Place pcn = u.place(in, u.code_chunk()), pvn = u.place(in, u.grp);
+        const typename W::Place pc2 = u.place(min(i + 2 * kStep, last_i), u.code_chunk());
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) qraw[k] = q_load(k, 0);
+        u.load_codes(pc, c0);
+        u.load_codes(pcn, c1);
+        u.load_vals(pv, val);
+        pc = pc2;
+        pv = pvn;
+    };
+    int book_exp;  // the codebook is staged times 2^book_exp
+    // ---- the query rows as operands: f16, at a power of two of each row's
+    auto query_of = [&](auto type) {
+        constexpr int dtype = decltype(type)::value, wide = dtype == SSQ_F32 ? 1 : 0;
+        const bool in = u.col < nr;
+        const float scale = p->a.has_scale ? p->a.scale : 1.f;  // (a factor of 1 is exact)
+        // through the wave's LDS rows, 8 (4) at a time, permuted on the way back
+        unsigned char* rows = smem + L::kBook + wave * 8 * L::kQRow;
+        const int row_bytes = L::kQRow << wide, per = 8 >> wide;
+        uint32_t idx[NE / 2];
+#pragma unroll
+        for (int k = 0; k < NE / 8; ++k) {
+            const uint4 w = reinterpret_cast<const uint4*>(perm + u.grp * NE)[k];
+            idx[4 * k] = w.x; idx[4 * k + 1] = w.y; idx[4 * k + 2] = w.z; idx[4 * k + 3] = w.w;
         }
-        __syncthreads();
-        {
-            const uint16_t* qs = reinterpret_cast<const uint16_t*>(smem + L::kBook);
+        float y[NE];
 #pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                u.fac[n] = facs[16 * n + u.col];
-                u.pos[n] = len - q_len + min(row0 + 16 * n + u.col, rows - 1) / G;
+        for (int k = 0; k < NE; ++k) y[k] = 0.f;
+        for (int r0 = 0; r0 < nr; r0 += per) {
+            if (wide && r0 == 8)  // the second batch of 32-bit rows
 #pragma unroll
-                for (int h = 0; h < QP; ++h) {
-                    const uint16_t* src = qs + (h * RP + 16 * n + u.col) * L::kQRow + u.grp * (D / 4);
+                for (int k = 0; k < kPieces; ++k) qraw[k] = q_load(k, 8);
 #pragma unroll
-                    for (int k = 0; k < W::NQ; ++k) {
-                        if constexpr (BD == 8) {
-                            u.q[h][n][k] = *reinterpret_cast<const uint4*>(src + 8 * k);
-                        } else {
-                            const uint2 w = *reinterpret_cast<const uint2*>(src + 4 * k);
-                            if constexpr (BD == 4) u.q[h][n][k] = make_uint4(w.x, w.y, w.x, w.y);
-                            else u.q[h][n][k] = make_uint4(w.x, w.x, w.y, w.y);
-                        }
-                    }
+            for (int k = 0; k < kPieces; ++k) {
+                int r, byte;
+                q_at(k, wide ? r0 & 8 : 0, r, byte);
+                if (r >= r0 && r < r0 + per) *reinterpret_cast<uint4*>(rows + (r - r0) * row_bytes + byte) = qraw[k];
+            }
+            win_lds_sync();
+            if (u.col >= r0 && u.col < r0 + per) {
+                const unsigned char* mine = rows + (u.col - r0) * row_bytes;
+#pragma unroll
+                for (int k = 0; k < NE; ++k) {
+                    const uint32_t j = k & 1 ? idx[k / 2] >> 16 : idx[k / 2] & 0xFFFFu;
+                    y[k] = ssq_bits_to_f32(wide ? reinterpret_cast<const uint32_t*>(mine)[j] : reinterpret_cast<const uint16_t*>(mine)[j], dtype);
                 }
             }
+            win_lds_sync();
         }
+        float most = 0.f;
+#pragma unroll
+        for (int k = 0; k < NE; ++k) {
+            y[k] = in ? ssq_round_to(y[k] * scale, dtype) : 0.f;
+            const float z = fabsf(y[k]);
+            most = fmaxf(most, z < INFINITY ? z : 0.f);
+        }
+        const int up = min(15 - win_exp(win_max4(most)), 126);
+        const float s = ldexpf(1.f, up);
+        u.fac = ldexpf(kWinLog2e, max(-book_exp - up, -126));  // above 0
+        uint32_t hi[NE / 2], lo[NE / 2];
+#pragma unroll
+        for (int k = 0; k < NE; k += 2) win_split<true>(y[k] * s, y[k + 1] * s, hi[k / 2], lo[k / 2]);
+#pragma unroll
+        for (int h = 0; h < QP; ++h) {
+            const uint32_t* w = h ? lo : hi;
+#pragma unroll
+            for (int k = 0; k < W::NQ; ++k) {
+                if constexpr (BD == 8) u.q[h][k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                else if constexpr (BD == 4) u.q[h][k] = make_uint4(w[2 * k], w[2 * k + 1], w[2 * k], w[2 * k + 1]);
+                else u.q[h][k] = make_uint4(w[2 * k], w[2 * k], w[2 * k + 1], w[2 * k + 1]);
+            }
+        }
+    };
+    auto query = [&]() {
+        if constexpr (QP == 2) query_of(std::integral_constant<int, SSQ_F32>{});
+        else if (p->a.q_dtype == SSQ_BF16) query_of(std::integral_constant<int, SSQ_BF16>{});
+        else query_of(std::integral_constant<int, SSQ_F16>{});
+    };
 
-        // ---- this wave's tiles
-        float m[NR], l[NR], unit = W::kV8 ? kWinScale : 1.f, inv_unit = 1.f / unit;
-        w4f o[NR][DT];
+    __syncthreads();  // the permutation
+    bool more = next();
+    load();
+    {
+        // the largest finite codeword; infinite ones (rare) cost a second look and checks on the way
+        auto largest = [&](auto checked) {
+            float most = 0.f;
 #pragma unroll
-        for (int n = 0; n < NR; ++n) {
-            m[n] = kWinNone;
-            l[n] = 0.f;
+            for (int k = 0; k < kPer; ++k)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[n][dt] = w4f{};
-        }
-        // Loads return in order: a place is asked for a tile before it is used, and before that tile's values.
-        for (int i = i0 + wave; i < i1; i += kWinWaves) {
-            w4f s[NS][NR];
+                for (int d = 0; d < BD; ++d) {
+                    const float z = fabsf(c[k][d]);
+                    most = fmaxf(most, !checked || z < INFINITY ? z : 0.f);
+                }
+            most = ssq_wave_max(most);
+            __syncthreads();
+            if (lane == 0) red[wave] = most;
+            __syncthreads();
+            most = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWinWaves; ++w) most = fmaxf(most, red[w]);
+            return most;
+        };
+        const int n_centroids = win_args()->a.n_centroids;
+        auto stage = [&](auto checked) {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const int e = tid + k * kWinThreads;
+                const float scale = (e & 255) < n_centroids ? ldexpf(1.f, book_exp) : 0.f;
+                uint32_t hi[BD / 2], lo[BD / 2];
+#pragma unroll
+                for (int d = 0; d < BD; d += 2) win_split<checked>(c[k][d] * scale, c[k][d + 1] * scale, hi[d / 2], lo[d / 2]);
+                unsigned char* at = smem + e * (4 * BD);
+                if constexpr (BD == 8) {
+                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(at + 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                } else if constexpr (BD == 4) {
+                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+                } else {
+                    *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], lo[0]);
+                }
+            }
+        };
+        float most = largest(std::false_type{});
+        const bool infinite = most == INFINITY;  // uniform
+        if (infinite) most = largest(std::true_type{});
+        book_exp = min(15 - win_exp(most), 126);
+        if (infinite) stage(std::true_type{});
+        else stage(std::false_type{});
+        __syncthreads();
+    }
+    while (more) {
+        query();
+
+        // ---- this wave's tiles.  Loads return in order: a place is asked for a tile before it is used, and before that
+        // tile's values.
+        float m = kWinNone, l = 0.f, unit = W::kV8 ? kWinScale : 1.f, inv_unit = 1.f / unit;
+        w4f o[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = w4f{};
+        for (int i = i0; i < i1; i += kStep) {
+            w4f s[NS];
             u.scores(c0, s);
             c0 = c1;
             u.load_codes(pc, c1);
-            pc = u.place(min(i + 3 * kWinWaves, last_i), u.code_chunk());
+            pc = u.place(min(i + 3 * kStep, last_i), u.code_chunk());
             const int t0 = TT * u.tile_of(i), tok = t0 + CH * u.grp;
             // tokens of the tile that some row does not see (uniform)
             const bool edge = (t0 + TT - 1 > u.t.p_lo) | ((t0 <= u.t.p_hi - u.window) & (t0 + TT > u.sinks));
             bool apart = false;  // an infinite or NaN value that some rows see and others do not
             if (edge) {
                 const uint32_t any = u.sees(u.t.p_lo, u.t.p_hi, tok), all = u.sees(u.t.p_hi, u.t.p_lo, tok);
+                const uint32_t mine = u.sees(u.pos, u.pos, tok);
 #pragma unroll
-                for (int n = 0; n < NR; ++n) {
-                    const uint32_t mine = u.sees(u.pos[n], u.pos[n], tok);
-#pragma unroll
-                    for (int e = 0; e < CH; ++e) s[e >> 2][n][e & 3] = mine >> e & 1u ? s[e >> 2][n][e & 3] : -INFINITY;
-                }
+                for (int e = 0; e < CH; ++e) s[e >> 2][e & 3] = mine >> e & 1u ? s[e >> 2][e & 3] : -INFINITY;
                 if (any == 0) val.scale = 0.f;  // no page of this tile's
                 const w4u off = W::spread(~any);
 #pragma unroll
@@ -647,28 +723,17 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
                     apart = __builtin_amdgcn_ballot_w64(found != 0) != 0;
                 }
             }
-            float top[NR];
-            bool over = false;
+            float top = s[0][0];
 #pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                top[n] = s[0][n][0];
+            for (int e = 1; e < CH; ++e) top = fmaxf(top, s[e >> 2][e & 3]);
+            top *= u.fac;
+            if (__builtin_amdgcn_ballot_w64(top > m + kWinOver) != 0) {
+                const float mn = fmaxf(m, win_max4(top) - kWinTop);
+                const float f = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= f;
 #pragma unroll
-                for (int e = 1; e < CH; ++e) top[n] = fmaxf(top[n], s[e >> 2][n][e & 3]);
-                top[n] *= u.fac[n];
-                over |= top[n] > m[n] + kWinOver;
-            }
-            if (__builtin_amdgcn_ballot_w64(over) != 0) {
-#pragma unroll
-                for (int n = 0; n < NR; ++n) {
-                    const float mn = fmaxf(m[n], win_max4(top[n]) - kWinTop);
-                    const float f = __builtin_amdgcn_exp2f(m[n] - mn);
-                    m[n] = mn;
-                    l[n] *= f;
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[n][dt][e] *= f;
-                }
+                for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
             }
             float by = 1.f;  // this group's page scale, in units of O
             if constexpr (W::kV8) {
@@ -680,163 +745,196 @@ __global__ __launch_bounds__(win_waves(NR) * SSQ_WAVE) __attribute__((amdgpu_wav
                     unit = __uint_as_float(big);
                     inv_unit = 1.f / unit;
 #pragma unroll
-                    for (int n = 0; n < NR; ++n)
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[n][dt][e] *= f;
+                    for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
                 }
                 by = val.scale * inv_unit;
             }
-            uint32_t pw[NR][CH / 2];
+            uint32_t pw[CH / 2];
 #pragma unroll
-            for (int n = 0; n < NR; ++n)
-#pragma unroll
-                for (int e = 0; e < CH; e += 2) {
-                    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][n][e & 3], u.fac[n], -m[n]));
-                    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][n][(e & 3) + 1], u.fac[n], -m[n]));
-                    l[n] += x0 + x1;
-                    pw[n][e / 2] = W::kV8 ? win_pack_p<VT>(x0 * by, x1 * by) : win_pack_p<VT>(x0, x1);
-                }
+            for (int e = 0; e < CH; e += 2) {
+                const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3], u.fac, -m));
+                const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][(e & 3) + 1], u.fac, -m));
+                l += x0 + x1;
+                pw[e / 2] = W::kV8 ? win_pack_p<VT>(x0 * by, x1 * by) : win_pack_p<VT>(x0, x1);
+            }
             if (apart) {
                 // The rows of one position at a time, the values that they do not see as 0; the products below then add nothing.
                 for (int at = u.t.p_lo; at <= u.t.p_hi; ++at) {
                     const w4u on = W::spread(u.sees(at, at, tok));
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
+                    for (int dt = 0; dt < DT; ++dt) {
+                        w4f z = o[dt];
 #pragma unroll
-                        for (int n = 0; n < NR; ++n) {
-                            w4f y = o[n][dt];
+                        for (int jj = 0; jj < CH / 8; ++jj)
+                            z = win_mfma_v<VT>(u.vals(val.v[dt] & on, jj), make_uint4(pw[4 * jj], pw[4 * jj + 1], pw[4 * jj + 2], pw[4 * jj + 3]), z);
 #pragma unroll
-                            for (int jj = 0; jj < CH / 8; ++jj)
-                                y = win_mfma_v<VT>(u.vals(val.v[dt] & on, jj), make_uint4(pw[n][4 * jj], pw[n][4 * jj + 1], pw[n][4 * jj + 2], pw[n][4 * jj + 3]), y);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[n][dt][e] = u.pos[n] == at ? y[e] : o[n][dt][e];
-                        }
+                        for (int e = 0; e < 4; ++e) o[dt][e] = u.pos == at ? z[e] : o[dt][e];
+                    }
                 }
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) val.v[dt] = w4u{};
             }
             const uint8_t* next_row = u.val_row(pv);
             val.scale = u.load_scale(pv);
-            pv = u.place(min(i + 2 * kWinWaves, last_i), u.grp);
+            pv = u.place(min(i + 2 * kStep, last_i), u.grp);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {  // a value operand's successor loads once it is used
 #pragma unroll
-                for (int jj = 0; jj < CH / 8; ++jj) {
-                    const uint4 v = u.vals(val.v[dt], jj);
-#pragma unroll
-                    for (int n = 0; n < NR; ++n)
-                        o[n][dt] = win_mfma_v<VT>(v, make_uint4(pw[n][4 * jj], pw[n][4 * jj + 1], pw[n][4 * jj + 2], pw[n][4 * jj + 3]), o[n][dt]);
-                }
+                for (int jj = 0; jj < CH / 8; ++jj)
+                    o[dt] = win_mfma_v<VT>(u.vals(val.v[dt], jj), make_uint4(pw[4 * jj], pw[4 * jj + 1], pw[4 * jj + 2], pw[4 * jj + 3]), o[dt]);
                 val.v[dt] = u.load_val(next_row, dt);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        l = win_sum4(l);
 
-        // ---- the waves' join, 4 rows at a time
         p = win_args();
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-            l[n] = win_sum4(l[n]);
-            if (lane < 16) {
-                mls[wave * RP + 16 * n + lane] = m[n];
-                mls[(kWinWaves + wave) * RP + 16 * n + lane] = l[n];
+        if constexpr (TEAM) {
+            // ---- the waves' join, 4 rows at a time
+            if (lane < kWinRows) {
+                mls[wave * kWinRows + lane] = m;
+                mls[(kWinWaves + wave) * kWinRows + lane] = l;
             }
-        }
-        __syncthreads();
-        float f[NR];
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
+            __syncthreads();
             float mt = kWinNone;
 #pragma unroll
-            for (int w = 0; w < kWinWaves; ++w) mt = fmaxf(mt, mls[w * RP + 16 * n + u.col]);
-            f[n] = __builtin_amdgcn_exp2f(m[n] - mt) * unit;
-        }
-        float* join = reinterpret_cast<float*>(smem + L::kBook);
-        constexpr int kRow = L::kJoinRow;
+            for (int w = 0; w < kWinWaves; ++w) mt = fmaxf(mt, mls[w * kWinRows + u.col]);
+            const float f = __builtin_amdgcn_exp2f(m - mt) * unit;
+            float* join = reinterpret_cast<float*>(smem + L::kBook);
+            constexpr int kRow = L::kJoinRow;
 #pragma unroll 1
-        for (int r0 = 0; r0 < nr; r0 += L::kJoinRows) {
+            for (int r0 = 0; r0 < nr; r0 += L::kJoinRows) {
+                if ((u.col & ~3) == r0) {
 #pragma unroll
-            for (int n = 0; n < NR; ++n)
-                if (r0 / 16 == n && (u.col & ~3) == (r0 & 15)) {
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-                        *reinterpret_cast<float4*>(join + (wave * 4 + (u.col & 3)) * kRow + 16 * dt + 4 * u.grp) =
-                            make_float4(o[n][dt][0] * f[n], o[n][dt][1] * f[n], o[n][dt][2] * f[n], o[n][dt][3] * f[n]);
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const w4f z = o[dt] * f;
+                        *reinterpret_cast<float4*>(join + (wave * 4 + (u.col & 3)) * kRow + 16 * dt + 4 * u.grp) = make_float4(z[0], z[1], z[2], z[3]);
+                    }
                 }
-            __syncthreads();
-            for (int e = tid; e < 4 * D; e += kWinThreads) {
-                const int r = r0 + e / D, dv = e % D;
-                if (r >= nr) continue;
-                float mt = kWinNone;
+                __syncthreads();
+                const int r = r0 + tid / D, dv = tid % D;
+                if (tid < 4 * D && r < nr) {
+                    float mr = kWinNone, lt = 0.f, ot = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWinWaves; ++w) mt = fmaxf(mt, mls[w * RP + r]);
-                float lt = 0.f, ot = 0.f;
+                    for (int w = 0; w < kWinWaves; ++w) mr = fmaxf(mr, mls[w * kWinRows + r]);
 #pragma unroll
-                for (int w = 0; w < kWinWaves; ++w) {
-                    lt += mls[(kWinWaves + w) * RP + r] * __builtin_amdgcn_exp2f(mls[w * RP + r] - mt);
-                    ot += join[(w * 4 + r - r0) * kRow + dv];
-                }
-                if (slot < 0) {
+                    for (int w = 0; w < kWinWaves; ++w) {
+                        lt += mls[(kWinWaves + w) * kWinRows + r] * __builtin_amdgcn_exp2f(mls[w * kWinRows + r] - mr);
+                        ot += join[(w * 4 + r - r0) * kRow + dv];
+                    }
                     const int row = row0 + r, qi = row / p->G, h = kv * p->G + row - qi * p->G;
                     ssq_store_elem(p->a.out, p->out_dtype, (int64_t)b * p->a.o_sb + (int64_t)h * p->a.o_sh + (int64_t)qi * p->a.o_sl + dv,
                                    lt == 0.f ? 0.f : ot / lt);
                     if (p->a.lse && dv == 0)
-                        p->a.lse[((int64_t)b * p->a.num_q_heads + h) * p->a.q_len + qi] = lt == 0.f ? -INFINITY : (mt + log2f(lt)) * kWinLn2;
-                } else {
-                    float* dst = p->part + ((int64_t)(kv * p->n_wg + wg) * 2 + slot) * (RP * (D + 2));
-                    dst[r * D + dv] = ot;
-                    if (dv == 0) {
-                        dst[RP * D + r] = mt;
-                        dst[RP * D + RP + r] = lt;
-                    }
+                        p->a.lse[((int64_t)b * p->a.num_q_heads + h) * p->a.q_len + qi] = lt == 0.f ? -INFINITY : (mr + log2f(lt)) * kWinLn2;
+                }
+                __syncthreads();
+            }
+        } else if (u.col < nr) {
+            if (slot < 0) {
+                const int row = row0 + u.col, qi = row / p->G, h = kv * p->G + row - qi * p->G;
+                const float f = l == 0.f ? 0.f : unit / l;
+                const int64_t at = (int64_t)b * p->a.o_sb + (int64_t)h * p->a.o_sh + (int64_t)qi * p->a.o_sl + 4 * u.grp;
+                const int dtype = p->out_dtype;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const w4f z = l == 0.f ? w4f{} : o[dt] * f;
+                    if (p->out_vec) win_store4(p->a.out, dtype, at + 16 * dt, z);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) ssq_store_elem(p->a.out, dtype, at + 16 * dt + e, z[e]);
+                }
+                if (p->a.lse && u.grp == 0)
+                    p->a.lse[((int64_t)b * p->a.num_q_heads + h) * p->a.q_len + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * kWinLn2;
+            } else {
+                float* dst = p->part + ((int64_t)(kv * p->n_wg * kWinWaves + worker) * 2 + slot) * (kWinRows * (D + 2));
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const w4f z = o[dt] * unit;
+                    *reinterpret_cast<float4*>(dst + u.col * D + 16 * dt + 4 * u.grp) = make_float4(z[0], z[1], z[2], z[3]);
+                }
+                if (u.grp == 0) {
+                    dst[kWinRows * D + u.col] = m;
+                    dst[kWinRows * D + kWinRows + u.col] = l;
                 }
             }
-            __syncthreads();
         }
+        more = next();
+        if (more) load();
     }
 }
 
-// Joins the pieces of the items that workgroups shared.  One wave a query row, lanes over the value dims.
-template <int RP, int D>
-__global__ __launch_bounds__(256) void k_window_merge(const SsqWindowParams p) {
-    constexpr int E = D / SSQ_WAVE;
+// Joins the pieces of the items that waves shared: a query row by one wave of four, or by all W waves of a workgroup where pieces
+// may be many; lanes over the value dims, 8 pieces in flight a wave.
+template <int D, int W>
+__global__ __launch_bounds__((W > 1 ? W : 4) * SSQ_WAVE) void k_window_merge(const SsqWindowParams p) {
+    constexpr bool WIDE = W > 1;
+    constexpr int E = D / SSQ_WAVE, kAhead = 8, kSlot = kWinRows * (D + 2);
+    __shared__ float mo[W][D], ml[W][2];
     const ssq_decode_args& a = p.a;
-    const int lane = threadIdx.x & 63;
-    const int id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (sequence, KV head, row)
-    const int bk = id / p.rows, row = id - bk * p.rows, b = bk / a.num_kv_heads, kv = bk - b * a.num_kv_heads;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t id = WIDE ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;  // (sequence, KV head, row)
+    const int64_t bk = id / p.rows;
+    const int row = (int)(id - bk * p.rows), b = (int)(bk / a.num_kv_heads), kv = (int)(bk - (int64_t)b * a.num_kv_heads);
     if (b >= a.batch) return;
-    const int item = b * p.rgroups + row / RP, r = row % RP;
+    const int item = b * p.rgroups + row / kWinRows, r = row % kWinRows;
     const int first = p.meta[2 * item], pieces = p.meta[2 * item + 1];
     if (pieces <= 1) return;
-    const float* base = p.part + (int64_t)kv * p.n_wg * 2 * (RP * (D + 2));
-    auto at = [&](int i) { return base + (int64_t)(i ? 2 * ((first >> 1) + i) : first) * (RP * (D + 2)); };
-    float M = kWinNone;
-    for (int i = lane; i < pieces; i += SSQ_WAVE) M = fmaxf(M, at(i)[RP * D + r]);
-    M = ssq_wave_max(M);
-    float l = 0.f, o[E];
+    const float* base = p.part + (int64_t)kv * p.n_wg * kWinWaves * 2 * kSlot;
+    auto at = [&](int i) { return base + (int64_t)(i ? 2 * ((first >> 1) + i) : first) * kSlot; };
+    float M = kWinNone, l = 0.f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
-    constexpr int kAhead = 8;
-    for (int i0 = 0; i0 < pieces; i0 += kAhead) {
-        float w[kAhead], lp[kAhead], op[kAhead][E];
+    for (int i0 = WIDE ? wave * kAhead : 0; i0 < pieces; i0 += W * kAhead) {
+        float m[kAhead], lp[kAhead], op[kAhead][E];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const float* src = at(min(i0 + j, pieces - 1));
-            w[j] = src[RP * D + r];
-            lp[j] = src[RP * D + RP + r];
+            m[j] = src[kWinRows * D + r];
+            lp[j] = src[kWinRows * D + kWinRows + r];
 #pragma unroll
             for (int e = 0; e < E; ++e) op[j][e] = src[r * D + lane * E + e];
         }
+        float mt = M;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) mt = fmaxf(mt, m[j]);  // (those past the last are it)
+        const float f0 = __builtin_amdgcn_exp2f(M - mt);
+        M = mt;
+        l *= f0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= f0;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             if (i0 + j >= pieces) continue;
-            const float f = __builtin_amdgcn_exp2f(w[j] - M);
+            const float f = __builtin_amdgcn_exp2f(m[j] - M);
             l += lp[j] * f;
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] += op[j][e] * f;
+        }
+    }
+    if constexpr (WIDE) {
+        if (lane == 0) {
+            ml[wave][0] = M;
+            ml[wave][1] = l;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) mo[wave][lane * E + e] = o[e];
+        __syncthreads();
+        if (wave) return;
+        M = kWinNone;
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, ml[w][0]);
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w * kAhead >= pieces) continue;  // had none
+            const float f = __builtin_amdgcn_exp2f(ml[w][0] - M);
+            l += ml[w][1] * f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += mo[w][lane * E + e] * f;
         }
     }
     const int qi = row / p.G, h = kv * p.G + row - qi * p.G;
@@ -847,33 +945,35 @@ __global__ __launch_bounds__(256) void k_window_merge(const SsqWindowParams p) {
     if (a.lse && lane == 0) a.lse[((int64_t)b * a.num_q_heads + h) * a.q_len + qi] = l == 0.f ? -INFINITY : (M + log2f(l)) * kWinLn2;
 }
 
-template <int D, int BD, int VT, int NR, int QP>
+template <int D, int BD, int VT, int QP, bool TEAM>
 int win_launch(const SsqWindowParams& p, hipStream_t st) {
-    using L = WinLds<D, NR, QP>;
+    using L = WinLds<D>;
     static_assert(L::kTotal <= 160 * 1024, "a workgroup's LDS");
-    auto kern = k_window<D, BD, VT, NR, QP>;
-    constexpr int kWinThreads = win_waves(NR) * SSQ_WAVE;
+    auto kern = k_window<D, BD, VT, QP, TEAM>;
     int rc = ssq_allow_lds((const void*)kern, L::kTotal, "hipFuncSetAttribute(k_window)");
     if (rc) return rc;
     hipLaunchKernelGGL(kern, dim3(p.n_wg * p.a.num_kv_heads), dim3(kWinThreads), L::kTotal, st, p);
     rc = ssq_check_hip(hipGetLastError(), "k_window launch");
-    if (rc || p.whole) return rc;
+    if (rc || TEAM) return rc;
+    // An item of few may have as many pieces as there are waves; of many, each has few.
     const int64_t rows = (int64_t)p.a.batch * p.a.num_kv_heads * p.rows;
-    hipLaunchKernelGGL((k_window_merge<16 * NR, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
+    if (p.items <= 8) hipLaunchKernelGGL((k_window_merge<D, 16>), dim3((unsigned)rows), dim3(1024), 0, st, p);
+    else if (rows <= 4096) hipLaunchKernelGGL((k_window_merge<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((k_window_merge<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
     return ssq_check_hip(hipGetLastError(), "k_window_merge launch");
 }
 template <int D, int BD, int VT>
-int win_rows(const SsqWindowParams& p, int nr, hipStream_t st) {
+int win_form(const SsqWindowParams& p, hipStream_t st) {
     const bool split = p.a.q_dtype == SSQ_F32;
-    if (nr == 1) return split ? win_launch<D, BD, VT, 1, 2>(p, st) : win_launch<D, BD, VT, 1, 1>(p, st);
-    return split ? win_launch<D, BD, VT, 2, 2>(p, st) : win_launch<D, BD, VT, 2, 1>(p, st);
+    if (p.team) return split ? win_launch<D, BD, VT, 2, true>(p, st) : win_launch<D, BD, VT, 1, true>(p, st);
+    return split ? win_launch<D, BD, VT, 2, false>(p, st) : win_launch<D, BD, VT, 1, false>(p, st);
 }
 template <int D, int VT>
-int win_blocks(const SsqWindowParams& p, int nr, hipStream_t st) {
+int win_blocks(const SsqWindowParams& p, hipStream_t st) {
     switch (p.a.block_dim) {
-        case 2: return win_rows<D, 2, VT>(p, nr, st);
-        case 4: return win_rows<D, 4, VT>(p, nr, st);
-        default: return win_rows<D, 8, VT>(p, nr, st);
+        case 2: return win_form<D, 2, VT>(p, st);
+        case 4: return win_form<D, 4, VT>(p, st);
+        default: return win_form<D, 8, VT>(p, st);
     }
 }
 

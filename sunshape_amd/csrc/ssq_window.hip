@@ -10,7 +10,6 @@ namespace {
 
 struct Plan {
     SsqWindowParams p;
-    int nr;
     size_t part_bytes, bytes;
 };
 
@@ -23,6 +22,7 @@ int check(const ssq_window_args* a) {
     SSQ_REQUIRE(d.layout == SSQ_PAGED, "decode_window takes pages");
     SSQ_REQUIRE(d.v, "decode_window needs values");
     SSQ_REQUIRE(!d.scores && !d.mask, "decode_window takes no mask and gives no scores");
+    SSQ_REQUIRE(d.seq_len >= d.page_size, "decode_window needs a block table of at least one page");
     SSQ_REQUIRE(a->window >= 0 && a->sinks >= 0, "window and sinks must not be negative");
     SSQ_REQUIRE(a->out_dtype >= SSQ_F32 && a->out_dtype <= SSQ_F16, "bad out_dtype");
     SSQ_REQUIRE(a->num_pages >= 1 && a->num_pages <= INT_MAX, "bad num_pages");
@@ -55,21 +55,18 @@ int check(const ssq_window_args* a) {
     SSQ_REQUIRE(d.c_sb >= 0 && d.c_sb < 1ll << 31 && d.c_st >= 0 && d.c_st <= 1 << 22 && d.v_sb >= 0 && d.v_sb < 1ll << 30 &&
                     a->vs_sb >= 0 && a->vs_sb < 1ll << 30,
                 "page strides must be below 2^30 elements");
-    SSQ_REQUIRE((int64_t)d.batch * d.num_q_heads * d.q_len == 0 || d.num_kv_heads <= 1 << 16, "too many KV heads");
+    const int64_t items = d.batch * (((int64_t)d.num_q_heads / d.num_kv_heads * d.q_len + kWinRows - 1) / kWinRows);
+    SSQ_UNSUPPORTED(d.num_kv_heads <= 1 << 16 && items * (d.seq_len / 32 + 8) < 1ll << 31, "too many query rows for so long a context");
     return SSQ_OK;
 }
 
-// The most tiles of an item (any length that the tables hold).
-int most_tiles(const SsqWindowParams& p, int nr, bool v8) {
-    const int cap = p.a.seq_len;
-    int most = 0;
-    const int last = (p.rgroups - 1) * 16 * nr;
-    for (int row0 : {0, last})
-        for (int len : {cap, cap - 63 > 0 ? cap - 63 : cap}) {  // a window's tiles depend on where it ends
-            const int n = v8 ? win_tiles<64>(win_shape(p), len, row0, 16 * nr).n : win_tiles<32>(win_shape(p), len, row0, 16 * nr).n;
-            most = n > most ? n : most;
-        }
-    return p.window == INT_MAX ? most : most + 2;
+// The most tiles of an item (any length that the tables hold; a window's tiles depend on where it ends).
+int64_t most_tiles(const SsqWindowParams& p, bool v8) {
+    const int tt = v8 ? 64 : 32;
+    const int64_t all = (p.a.seq_len + tt - 1) / tt;
+    if (p.window == INT_MAX) return all;
+    const int64_t seen = ((int64_t)p.window + kWinRows + tt - 1) / tt + 1 + ((int64_t)p.sinks + tt - 1) / tt;
+    return seen < all ? seen : all;
 }
 
 void make_plan(const ssq_window_args& a, Plan& pl) {
@@ -86,20 +83,21 @@ void make_plan(const ssq_window_args& a, Plan& pl) {
     p.vs_sh = a.vs_sh;
     p.G = d.num_q_heads / d.num_kv_heads;
     p.rows = p.G * d.q_len;
-    pl.nr = p.rows <= 16 ? 1 : 2;
-    const int rp = 16 * pl.nr;
-    p.rgroups = (p.rows + rp - 1) / rp;
+    p.rgroups = (p.rows + kWinRows - 1) / kWinRows;
     p.items = d.batch * p.rgroups;
     const int cus = ssq_device_cus();
     p.n_wg = cus / d.num_kv_heads > 0 ? cus / d.num_kv_heads : 1;
-    const int waves = win_waves(pl.nr);
-    p.fixed = 2 * waves;
-    p.least = 2 * waves;
-    p.whole = most_tiles(p, pl.nr, d.v_dtype == SSQ_E4M3) <= 2 * waves;
-    if (p.whole && p.n_wg > p.items) p.n_wg = p.items;
+    p.fixed = 2;
+    p.least = 2;
+    p.team = most_tiles(p, d.v_dtype == SSQ_E4M3) <= 2 * kWinWaves;
+    if (p.team && p.n_wg > p.items) p.n_wg = p.items;
     while ((16 << p.psh) < d.page_size) ++p.psh;
-    pl.part_bytes = p.whole ? 0 : (size_t)d.num_kv_heads * p.n_wg * 2 * rp * (d.value_dim + 2) * 4;
-    pl.bytes = p.whole ? 0 : pl.part_bytes + (size_t)p.items * 8;
+    const int per = d.q_dtype == SSQ_F32 ? 4 : 8;
+    p.q_vec = (uintptr_t)d.q % 16 == 0 && d.q_sb % per == 0 && d.q_sh % per == 0 && d.q_sl % per == 0;
+    const int size = p.out_dtype == SSQ_F32 ? 16 : 8;
+    p.out_vec = (uintptr_t)d.out % size == 0 && d.o_sb % 4 == 0 && d.o_sh % 4 == 0 && d.o_sl % 4 == 0;
+    pl.part_bytes = p.team ? 0 : (size_t)d.num_kv_heads * p.n_wg * kWinWaves * 2 * kWinRows * (d.value_dim + 2) * 4;
+    pl.bytes = p.team ? 0 : pl.part_bytes + (size_t)p.items * 8;
 }
 
 }  // namespace
@@ -126,8 +124,8 @@ extern "C" int ssq_decode_window(const ssq_window_args* a, void* workspace, size
     hipStream_t st = (hipStream_t)stream;
     const bool small = d.head_dim == 64;
     switch (d.v_dtype) {
-        case SSQ_E4M3: return small ? ssq_window_64_e4m3(pl.p, pl.nr, st) : ssq_window_128_e4m3(pl.p, pl.nr, st);
-        case SSQ_BF16: return small ? ssq_window_64_bf16(pl.p, pl.nr, st) : ssq_window_128_bf16(pl.p, pl.nr, st);
-        default: return small ? ssq_window_64_f16(pl.p, pl.nr, st) : ssq_window_128_f16(pl.p, pl.nr, st);
+        case SSQ_E4M3: return small ? ssq_window_64_e4m3(pl.p, st) : ssq_window_128_e4m3(pl.p, st);
+        case SSQ_BF16: return small ? ssq_window_64_bf16(pl.p, st) : ssq_window_128_bf16(pl.p, st);
+        default: return small ? ssq_window_64_f16(pl.p, st) : ssq_window_128_f16(pl.p, st);
     }
 }

@@ -211,7 +211,7 @@ struct WinCut {
         share = max((total + workers - 1) / workers, p->least);
     }
     // the item that holds cost position x < total, its start and cost
-    __device__ __forceinline__ void find(WinArgs p, int lane, int x, int& item, int& s, int& c) const {
+    __device__ __forceinline__ void find(WinArgs p, int lane, int x, int& item, int& s, int& c) const {  // (uniform results)
         int base = 0, mine = c0, v = v0;
         for (int f = 0;;) {
             const uint64_t hit = __builtin_amdgcn_ballot_w64(base + v > x);
@@ -955,10 +955,11 @@ int win_launch(const SsqWindowParams& p, hipStream_t st) {
     hipLaunchKernelGGL(kern, dim3(p.n_wg * p.a.num_kv_heads), dim3(kWinThreads), L::kTotal, st, p);
     rc = ssq_check_hip(hipGetLastError(), "k_window launch");
     if (rc || TEAM) return rc;
-    // An item of few may have as many pieces as there are waves; of many, each has few.
+    // An item of few may have as many pieces as there are waves; of many, each has few.  (One of 131,071 tokens: 16 waves a row 9.4
+    // us, 4 waves 20; 64 of 66 tiles: one 4, four 5.)
     const int64_t rows = (int64_t)p.a.batch * p.a.num_kv_heads * p.rows;
     if (p.items <= 8) hipLaunchKernelGGL((k_window_merge<D, 16>), dim3((unsigned)rows), dim3(1024), 0, st, p);
-    else if (rows <= 4096) hipLaunchKernelGGL((k_window_merge<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p);
+    else if (p.items < p.n_wg) hipLaunchKernelGGL((k_window_merge<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p);
     else hipLaunchKernelGGL((k_window_merge<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
     return ssq_check_hip(hipGetLastError(), "k_window_merge launch");
 }

@@ -69,6 +69,24 @@ int64_t most_tiles(const SsqWindowParams& p, bool v8) {
     return seen < all ? seen : all;
 }
 
+// A workgroup's waves on one item at a time, joined in LDS and written out, or every wave an equal share of all tiles and a
+// second launch that joins them?  Together an item takes as many rounds as it has tiles / 8, and items wait for the longest
+// one's; shares cost the join, about 9 us.  By what calls took, tenths of a microsecond: a round of 8 tiles 26 where all CUs
+// have one to load, 19 where less than three quarters have, 23 where groups of rows share the tokens; 50 an item, 80 a call; a tile
+// of a share 32 (24), 170 a call.  Measured us together and in shares, 32 / 8 heads of 128: 1 sequence of 1,100 tokens 15.6 and
+// 18.1, of 4,100 26.8 and 18.3; 16 of 2,100 20.7 and 25.5; 48 of 4,100 59.7 and 57.8, of 600 23.9 and 24.7; 128 of 600 43.7 and
+// 37.9; 16 times 5 rows under a window of 1,001 22.2 and 33.9; 64 under one of 4,096 70.4 and 73.5; 14 / 2 heads of 64: 128 of
+// 4,100 26.9 and 36.0.  Past 80 tiles lengths may differ by more than a round is worth (48 ragged ones of up to 8,192 92.0 and 82.3).
+bool team(const SsqWindowParams& p, int64_t most) {
+    if (most > 80) return false;
+    const int64_t turns = (p.items + p.n_wg - 1) / p.n_wg;
+    const bool shared = p.rgroups > 1;
+    const int64_t round = shared ? 23 : 4 * (int64_t)p.items >= 3 * (int64_t)p.n_wg ? 26 : 19;
+    const int64_t together = turns * ((most > 8 ? most : 8) * round / 8 + 50) + 80;
+    const int64_t shares = 170 + (shared ? 24 : 32) * (int64_t)p.items * (most + p.fixed) / (p.n_wg * kWinWaves);
+    return together <= shares;
+}
+
 void make_plan(const ssq_window_args& a, Plan& pl) {
     const ssq_decode_args& d = a.dec;
     SsqWindowParams& p = pl.p;
@@ -89,7 +107,7 @@ void make_plan(const ssq_window_args& a, Plan& pl) {
     p.n_wg = cus / d.num_kv_heads > 0 ? cus / d.num_kv_heads : 1;
     p.fixed = 2;
     p.least = 2;
-    p.team = most_tiles(p, d.v_dtype == SSQ_E4M3) <= 2 * kWinWaves;
+    p.team = team(p, most_tiles(p, d.v_dtype == SSQ_E4M3));
     if (p.team && p.n_wg > p.items) p.n_wg = p.items;
     while ((16 << p.psh) < d.page_size) ++p.psh;
     const int per = d.q_dtype == SSQ_F32 ? 4 : 8;

@@ -14,8 +14,12 @@
 // where the time goes, takes those.  8,192 tokens of the same layer: 19.8 us for 67 MB (3.4 TB/s) and 61.5 us.
 #include "ssq_encode_math.h"
 #include "ssq_rope.h"
+#include "ssq_values.h"
 
 #include <math.h>
+
+int ssq_values_check(const ssq_values_args* a);
+SsqValues ssq_values_params(const ssq_values_args& a);
 
 namespace {
 
@@ -329,22 +333,29 @@ __device__ __forceinline__ void block_dims(const unsigned char* row, const int (
 }
 
 // BD: the block dim at compile time (1, 2, 4 or 8), or 0 for any other up to 16; S: lanes of a key.  x: value
-// tiles, then blocks and their tiles of keys; y: KV heads.
-template <int BD, int S>
-__global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
+// tiles, then blocks and their tiles of keys; y: KV heads.  V8: the values go to 8-bit pages (p8), p8_blocks workgroups a head.
+template <int BD, int S, bool V8>
+__device__ __forceinline__ void append_few(const AppendParams& p, const SsqValues* p8, int p8_blocks) {
     constexpr int kX = BD ? BD : 16, kPer = kThreads / S;
     extern __shared__ __align__(16) unsigned char few_lds[];
     const ssq_encode_args& a = p.e;
     const int kv = blockIdx.y, n = a.batch * a.seq_len;
     int kt = blockIdx.x;
-    if (kt < p.vtiles * p.dchunks) {
+    if constexpr (V8) {
+        if (kt < p8_blocks) {
+            const int64_t w = (int64_t)kt * (kThreads / SSQ_WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / SSQ_WAVE);
+            if (kv < p8->hgroups) val_wave(*p8, w * p8->hgroups + kv, threadIdx.x & (SSQ_WAVE - 1));
+            return;
+        }
+        kt -= p8_blocks;
+    } else if (kt < p.vtiles * p.dchunks) {
         __shared__ ValSlots vs;
         const int dc = kt / p.vtiles, tile = kt - dc * p.vtiles;
         if (p.vone) value_rows(p, tile, kv, dc);
         else value_tile(p, few_lds, vs, tile, kv, dc);
         return;
     }
-    kt -= p.vtiles * p.dchunks;
+    if constexpr (!V8) kt -= p.vtiles * p.dchunks;
     const int blk = kt / p.ktiles;
     kt -= blk * p.ktiles;
     const int sl = threadIdx.x & (S - 1), local = (int)threadIdx.x / S, i = kt * kPer + local;
@@ -516,6 +527,13 @@ __global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) {
     }
     if (put) store_code(a.codes, cw, crow + blk, j_best);
 }
+template <int BD, int S>
+__global__ __launch_bounds__(kThreads) void k_append_few(const AppendParams p) { append_few<BD, S, false>(p, nullptr, 0); }
+// (a kernel of its own: the values' registers would cost the 16-bit one waves)
+template <int BD, int S>
+__global__ __launch_bounds__(kThreads) void k_append_few8(const AppendParams p, const SsqValues p8, int p8_blocks) {
+    append_few<BD, S, true>(p, &p8, p8_blocks);
+}
 
 bool uses_grid(const ssq_encode_args& e) {  // as ssq_encode chooses
     return e.kernel == 0 && e.grid && !e.direct_dist && ssq_encode_grid_supported(&e);
@@ -657,14 +675,19 @@ int run_prep(const AppendParams& p, const SsqRopeRows& r, bool turn, hipStream_t
     return ssq_check_hip(hipGetLastError(), "k_append_prep launch");
 }
 
+template <int BD, int S>
+void launch_few(const AppendParams& p, const SsqValues* p8, int p8_blocks, dim3 grid, size_t lds, hipStream_t st) {
+    if (p8) hipLaunchKernelGGL((k_append_few8<BD, S>), grid, dim3(kThreads), lds, st, p, *p8, p8_blocks);
+    else hipLaunchKernelGGL((k_append_few<BD, S>), grid, dim3(kThreads), lds, st, p);
+}
 template <int S>
-int launch_few(const AppendParams& p, dim3 grid, size_t lds, hipStream_t st) {
+int launch_few(const AppendParams& p, const SsqValues* p8, int p8_blocks, dim3 grid, size_t lds, hipStream_t st) {
     switch (p.e.block_dim) {
-        case 1: hipLaunchKernelGGL((k_append_few<1, S>), grid, dim3(kThreads), lds, st, p); break;
-        case 2: hipLaunchKernelGGL((k_append_few<2, S>), grid, dim3(kThreads), lds, st, p); break;
-        case 4: hipLaunchKernelGGL((k_append_few<4, S>), grid, dim3(kThreads), lds, st, p); break;
-        case 8: hipLaunchKernelGGL((k_append_few<8, S>), grid, dim3(kThreads), lds, st, p); break;
-        default: hipLaunchKernelGGL((k_append_few<0, S>), grid, dim3(kThreads), lds, st, p); break;
+        case 1: launch_few<1, S>(p, p8, p8_blocks, grid, lds, st); break;
+        case 2: launch_few<2, S>(p, p8, p8_blocks, grid, lds, st); break;
+        case 4: launch_few<4, S>(p, p8, p8_blocks, grid, lds, st); break;
+        case 8: launch_few<8, S>(p, p8, p8_blocks, grid, lds, st); break;
+        default: launch_few<0, S>(p, p8, p8_blocks, grid, lds, st); break;
     }
     return ssq_check_hip(hipGetLastError(), "k_append_few launch");
 }
@@ -676,7 +699,8 @@ extern "C" size_t ssq_append_workspace_size(const ssq_append_args* a) {
     return (size_t)(rows_bytes(*a) + (int64_t)a->enc.batch * a->enc.seq_len * 8);
 }
 
-extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+// v8: the values' 8-bit append, beside the keys' (a->v NULL) in the one launch of few rows, else in one of its own
+static int append_run(const ssq_append_args* a, const ssq_values_args* v8, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check(a);
     if (rc) return rc;
     const ssq_encode_args& e = a->enc;
@@ -701,17 +725,24 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
         p.chunk = e.n_centroids < stage ? e.n_centroids : stage;
         const int per = kThreads / S;
         p.ktiles = (int)((n + per - 1) / per);
-        const int64_t xs = (int64_t)p.vtiles * p.dchunks + (int64_t)p.ktiles * e.n_blocks;
+        SsqValues p8{};
+        int64_t p8_blocks = 0;
+        if (v8 && a->num_pages > 0) {
+            p8 = ssq_values_params(*v8);
+            p8_blocks = ((int64_t)p8.batch * p8.chunks + kThreads / SSQ_WAVE - 1) / (kThreads / SSQ_WAVE);
+        }
+        const SsqValues* vp = v8 ? &p8 : nullptr;
+        const int64_t xs = p8_blocks + (int64_t)p.vtiles * p.dchunks + (int64_t)p.ktiles * e.n_blocks;
         SSQ_UNSUPPORTED(xs <= 0x7fffffff, "too many rows");
         dim3 grid((unsigned)xs, e.num_kv_heads);
         size_t lds = (((size_t)p.chunk * (e.block_dim + 1) * 4 + 15) & ~(size_t)15) + (size_t)per * p.krow;
         const size_t vlds = a->v && !p.vone ? (size_t)kValTok * val_row(a->vp_dtype == SSQ_F32 ? 4 : 2) : 0;
         if (vlds > lds) lds = vlds;
         switch (S) {
-            case 4: return launch_few<4>(p, grid, lds, st);
-            case 8: return launch_few<8>(p, grid, lds, st);
-            case 16: return launch_few<16>(p, grid, lds, st);
-            default: return launch_few<SSQ_WAVE>(p, grid, lds, st);
+            case 4: return launch_few<4>(p, vp, (int)p8_blocks, grid, lds, st);
+            case 8: return launch_few<8>(p, vp, (int)p8_blocks, grid, lds, st);
+            case 16: return launch_few<16>(p, vp, (int)p8_blocks, grid, lds, st);
+            default: return launch_few<SSQ_WAVE>(p, vp, (int)p8_blocks, grid, lds, st);
         }
     }
     const int64_t rows = rows_bytes(*a);
@@ -736,12 +767,16 @@ extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t work
         enc.k_sb = r.y_sb[0]; enc.k_sh = r.y_sh[0]; enc.k_ss = r.y_ss[0];
     }
     rc = run_prep(p, r, turns(*a), st);
+    if (rc == SSQ_OK && v8) rc = ssq_append_values(v8, stream);
     if (rc) return rc;
     return ssq_encode(&enc, stream);
 }
 
+extern "C" int ssq_append(const ssq_append_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    return append_run(a, nullptr, workspace, workspace_bytes, stream);
+}
+
 // The values of an 8-bit append are those of ssq_append_values, the rest those of ssq_append without values.
-int ssq_values_check(const ssq_values_args* a);
 
 namespace {
 
@@ -778,6 +813,5 @@ extern "C" int ssq_append8(const ssq_append8_args* a, void* workspace, size_t wo
     ssq_append_args keys;
     ssq_values_args v;
     int rc = check8(a, keys, v);
-    if (rc == SSQ_OK) rc = ssq_append(&keys, workspace, workspace_bytes, stream);
-    return rc == SSQ_OK ? ssq_append_values(&v, stream) : rc;
+    return rc == SSQ_OK ? append_run(&keys, &v, workspace, workspace_bytes, stream) : rc;
 }

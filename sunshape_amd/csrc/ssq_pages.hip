@@ -37,7 +37,7 @@ __device__ __forceinline__ void move(const uint8_t* src, uint8_t* dst, int lane,
             if (i + SSQ_WAVE * k < n) x[k] = __builtin_nontemporal_load(s + i + SSQ_WAVE * k);
 #pragma unroll
         for (int k = 0; k < kInFlight; ++k)
-            if (i + SSQ_WAVE * k < n) d[i + SSQ_WAVE * k] = x[k];
+            if (i + SSQ_WAVE * k < n) __builtin_nontemporal_store(x[k], d + i + SSQ_WAVE * k);
     }
 }
 

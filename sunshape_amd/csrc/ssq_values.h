@@ -10,8 +10,8 @@
 // A run is the tokens of a row (b, .) that go to one page; it starts at its first one, whose wave takes the run whole, so
 // a page's scale needs no atomic and nothing depends on an order.  A wave looks at kRunChunk positions of a row for starts,
 // for one head of up to 128 dims or two of up to 64 at a time: a lane holds two dims of up to 16 tokens, which become two
-// 16-byte rows of the dim-major page in registers.  Bound by bytes for prompts; for a step by its chain of loads
-// (slots, then values, scale and page together).
+// 16-byte rows of the dim-major page in registers (ValWave::small; ValWave::run serves any run).  Bound by bytes for prompts;
+// for a step by its chain of loads (slots, then values, scale and page together).
 #pragma once
 
 #include "ssq_common.h"
@@ -118,13 +118,13 @@ struct ValWave {
     }
 
     // One run: it starts at position s0; the 64 positions from there are this wave's lanes (r: theirs).
-    __device__ void run(int s0, At r) const {
+    __device__ __forceinline__ void run(int s0, At r) const {
         const int page = __builtin_amdgcn_readfirstlane(r.page);
         const float held = on ? p.scale[(int64_t)page * p.vs_sb + (int64_t)head * p.vs_sh] : kValLeast;
         const int D = p.value_dim, step = 2 * L;
         // ---- the run's tokens: the largest value, the first offset
-        float top = 0.f, x[16][2];
-        int n = 0, in_x = 0, first = p.page_size, lead = 0;
+        float top = 0.f;
+        int n = 0, first = p.page_size, lead = 0;
         bool in_order = true, in_row = true;  // offsets ascend by one; positions do
         uint64_t bits = 0;                    // the run's positions from s0 (the first 64)
         for (int base = 0;; base += SSQ_WAVE) {
@@ -156,11 +156,7 @@ struct ValWave {
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    top = most(top, y[j]);
-                    if (n == 0) { x[j][0] = y[j][0]; x[j][1] = y[j][1]; }
-                }
-                if (n == 0) in_x = k;
+                for (int j = 0; j < 16; ++j) top = most(top, y[j]);
                 n += k;
             }
             for (int d = dim + step; d < (D + step - 1) / step * step; d += step)  // dims past the first 2 L
@@ -176,46 +172,7 @@ struct ValWave {
         const float now = first > 0 ? fmaxf(held, need) : need, inv = 1.f / now, again = held * inv;
         const bool grown = first > 0 && now != held;
         if (on && dim == 0) p.scale[(int64_t)page * p.vs_sb + (int64_t)head * p.vs_sh] = now;
-        if (p.page_size == 16 && in_order && n == in_x && D <= step) {
-            // ---- one 16-byte row a dim: the held bytes, the new ones from `first`
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (!on || dim + e >= D) continue;
-                uint8_t* dst = row(page, dim + e);
-                uint32_t w[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    w[k] = val_pack(val_in(x[4 * k][e], inv), val_in(x[4 * k + 1][e], inv), val_in(x[4 * k + 2][e], inv),
-                                    val_in(x[4 * k + 3][e], inv));
-                if (n == 16) {
-                    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-                    continue;
-                }
-                uint4 old = *reinterpret_cast<const uint4*>(dst);
-                if (grown) old = val_rescale(old, first, again);
-                uint32_t ow[4] = {old.x, old.y, old.z, old.w}, nw[4];
-                // w moved up by `first` bytes (uniform)
-                const int ws = first >> 2, bs = 8 * (first & 3);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint32_t hi = 0, lo = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j == k - ws) hi = w[j];
-                        if (j == k - ws - 1) lo = w[j];
-                    }
-                    nw[k] = bs ? (hi << bs) | (lo >> (32 - bs)) : hi;
-                    uint32_t take = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (4 * k + j >= first && 4 * k + j < first + n) take |= 0xFFu << (8 * j);
-                    ow[k] = (ow[k] & ~take) | (nw[k] & take);
-                }
-                *reinterpret_cast<uint4*>(dst) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
-            }
-            return;
-        }
-        // ---- any run: the held bytes, then the new ones, whole 16-byte rows where offsets and positions ascend together
+        // ---- the held bytes, then the new ones, whole 16-byte rows where offsets and positions ascend together
         for (int d0 = dim; d0 < (D + step - 1) / step * step; d0 += step) {
             for (int e = 0; e < 2; ++e) {
                 const int d = d0 + e;
@@ -273,17 +230,105 @@ struct ValWave {
         if (on && d < p.value_dim) row(page, d)[off] = (uint8_t)w;
         if (on && d + 1 < p.value_dim) row(page, d + 1)[off] = (uint8_t)(w >> 8);
     }
-    __device__ void chunk(int c) const {
+    // A run of n <= 16 tokens at ascending offsets from `first` in a page of 16, at the positions s0 + (the bits of `mine`): one
+    // 16-byte row a dim, the held bytes and the new ones.  Everything is asked for at once.
+    __device__ __forceinline__ void small(int s0, uint64_t mine, int n, int page, int first) const {
+        float x[16][2];
+        const int64_t at0 = (int64_t)b * p.v_sb + (int64_t)head * p.v_sh + (dim < p.value_dim ? dim : 0);
+        const bool pair = p.vec != 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {  // (those behind the last repeat it)
+            const int64_t i = at0 + (int64_t)(s0 + __builtin_ctzll(mine)) * p.v_ss;
+            const uint64_t rest = mine & (mine - 1);
+            mine = rest ? rest : mine;
+            if (pair) {  // uniform
+                if (p.v_dtype == SSQ_F32) {
+                    const float2 w = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.v) + i);
+                    x[j][0] = w.x; x[j][1] = w.y;
+                } else {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(p.v) + i);
+                    x[j][0] = __uint_as_float(w);  // both, unpacked below
+                }
+            } else {
+                x[j][0] = ssq_load_elem(p.v, p.v_dtype, i);
+                x[j][1] = dim + 1 < p.value_dim ? ssq_load_elem(p.v, p.v_dtype, i + 1) : 0.f;
+            }
+        }
+        float* at_scale = p.scale + (int64_t)page * p.vs_sb + (int64_t)head * p.vs_sh;
+        const float held = *at_scale;
+        const bool two = on && dim + 1 < p.value_dim, one = on && dim < p.value_dim;
+        uint8_t* dst = row(page, one ? dim : 0);
+        uint4 old[2];
+        old[0] = old[1] = make_uint4(0, 0, 0, 0);
+        if (n < 16) {  // uniform
+            old[0] = *reinterpret_cast<const uint4*>(dst);
+            old[1] = *reinterpret_cast<const uint4*>(two ? dst + p.vp_sd : dst);
+        }
+        if (pair && p.v_dtype != SSQ_F32) {
+            const bool bf = p.v_dtype == SSQ_BF16;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const uint32_t w = __float_as_uint(x[j][0]);
+                x[j][0] = bf ? ssq_bf16_to_f32(w & 0xFFFFu) : ssq_f16_to_f32(w & 0xFFFFu);
+                x[j][1] = bf ? __uint_as_float(w & 0xFFFF0000u) : ssq_f16_to_f32(w >> 16);
+            }
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = most(top, x[j]);
+        if (!one) top = 0.f;
+        for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float need = val_scale(top);
+        const float now = first > 0 ? fmaxf(held, need) : need, inv = 1.f / now, again = held * inv;
+        const bool grown = first > 0 && now != held;
+        if (on && dim == 0) *at_scale = now;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (!(e ? two : one)) continue;
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                w[k] = val_pack(val_in(x[4 * k][e], inv), val_in(x[4 * k + 1][e], inv), val_in(x[4 * k + 2][e], inv),
+                                val_in(x[4 * k + 3][e], inv));
+            if (n < 16) {  // uniform
+                if (grown) old[e] = val_rescale(old[e], first, again);
+                const uint32_t ow[4] = {old[e].x, old[e].y, old[e].z, old[e].w};
+                // w moved up by `first` bytes (uniform)
+                const int ws = first >> 2, bs = 8 * (first & 3);
+                uint32_t nw[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t hi = 0, lo = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j == k - ws) hi = w[j];
+                        if (j == k - ws - 1) lo = w[j];
+                    }
+                    nw[k] = bs ? (hi << bs) | (lo >> (32 - bs)) : hi;
+                    uint32_t take = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (4 * k + j >= first && 4 * k + j < first + n) take |= 0xFFu << (8 * j);
+                    nw[k] = (ow[k] & ~take) | (nw[k] & take);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = nw[k];
+            }
+            *reinterpret_cast<uint4*>(dst + e * p.vp_sd) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    __device__ __forceinline__ void chunk(int c) const {
         const int s0 = kRunChunk * c;
-        // lanes 48 ..: the chunk; the lanes before them: the positions before it
-        const At r = at(s0 - 48 + lane);
-        const uint64_t live = __builtin_amdgcn_ballot_w64(r.page >= 0);
-        const uint64_t before = live & ((1ull << 48) - 1ull);
+        // the chunk's positions and those after them, and the 64 before
+        const At r = at(s0 + lane), back = at(s0 - 64 + lane);
+        const uint64_t live = __builtin_amdgcn_ballot_w64(r.page >= 0), before = __builtin_amdgcn_ballot_w64(back.page >= 0);
+        uint64_t own = live & ((1ull << kRunChunk) - 1ull);
+        if (!own) return;
         int prev = -1;
         if (before) {
-            prev = __builtin_amdgcn_readlane(r.page, 63 - __builtin_clzll(before));
+            prev = __builtin_amdgcn_readlane(back.page, 63 - __builtin_clzll(before));
         } else {
-            for (int s = s0 - 48; s > 0; s -= SSQ_WAVE) {
+            for (int s = s0 - 64; s > 0; s -= SSQ_WAVE) {
                 const At q = at(s - 1 - lane);
                 const uint64_t any = __builtin_amdgcn_ballot_w64(q.page >= 0);
                 if (any) {
@@ -292,10 +337,20 @@ struct ValWave {
                 }
             }
         }
-        for (uint64_t own = live >> 48; own; own &= own - 1) {
-            const int l = __builtin_ctzll(own), page = __builtin_amdgcn_readlane(r.page, 48 + l);
-            if (page != prev) run(s0 + l, at(s0 + l + lane));
+        while (own) {
+            const int l = __builtin_ctzll(own), page = __builtin_amdgcn_readlane(r.page, l);
+            own &= own - 1;
+            if (page == prev) continue;
             prev = page;
+            // the run's positions among the 64: up to the next one of another page
+            const uint64_t from = ~0ull << l, same = __builtin_amdgcn_ballot_w64(r.page == page) & from, other = live & ~same & from;
+            const uint64_t mine = other ? same & ((1ull << __builtin_ctzll(other)) - 1ull) : same;
+            const int n = __builtin_popcountll(mine), first = __builtin_amdgcn_readlane(r.off, l);
+            const bool is = mine >> lane & 1ull;
+            const int rank = __builtin_popcountll(mine & ((1ull << lane) - 1ull));
+            const bool whole = (other || s0 + SSQ_WAVE >= p.seq_len) && __builtin_amdgcn_ballot_w64(is && r.off != first + rank) == 0;
+            if (whole && p.page_size == 16 && p.value_dim <= 2 * L) small(s0, mine, n, page, first);
+            else run(s0 + l, at(s0 + l + lane));
         }
     }
 };

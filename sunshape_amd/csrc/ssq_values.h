@@ -16,6 +16,8 @@
 
 #include "ssq_common.h"
 
+#include <type_traits>
+
 struct SsqValues {
     const void* v;
     int v_dtype;
@@ -136,13 +138,13 @@ struct ValWave {
                 bits = mine;
                 lead = __builtin_amdgcn_readfirstlane(r.off);
             }
-            // rows 16 at a time
+            // rows 8 at a time
             uint64_t left = mine;
             while (left) {
-                float y[16][2];
+                float y[8][2];
                 int k = 0;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
+                for (int j = 0; j < 8; ++j) {
                     y[j][0] = y[j][1] = 0.f;
                     if (left) {  // uniform
                         const int l = __builtin_ctzll(left);
@@ -156,7 +158,7 @@ struct ValWave {
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 16; ++j) top = most(top, y[j]);
+                for (int j = 0; j < 8; ++j) top = most(top, y[j]);
                 n += k;
             }
             for (int d = dim + step; d < (D + step - 1) / step * step; d += step)  // dims past the first 2 L
@@ -232,64 +234,65 @@ struct ValWave {
     }
     // A run of n <= 16 tokens at ascending offsets from `first` in a page of 16, at the positions s0 + (the bits of `mine`): one
     // 16-byte row a dim, the held bytes and the new ones.  Everything is asked for at once.
+    template <int DT>
     __device__ __forceinline__ void small(int s0, uint64_t mine, int n, int page, int first) const {
-        float x[16][2];
-        const int64_t at0 = (int64_t)b * p.v_sb + (int64_t)head * p.v_sh + (dim < p.value_dim ? dim : 0);
-        const bool pair = p.vec != 0;
+        using Raw = std::conditional_t<DT == SSQ_F32, uint2, uint32_t>;  // a token's two values
+        constexpr int kSize = DT == SSQ_F32 ? 4 : 2;
+        Raw raw[16];
+        const bool one = on && dim < p.value_dim;  // (pairs load whole: value_dim is even)
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(p.v) + ((int64_t)b * p.v_sb + (int64_t)head * p.v_sh + (one ? dim : 0)) * kSize;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {  // (those behind the last repeat it)
-            const int64_t i = at0 + (int64_t)(s0 + __builtin_ctzll(mine)) * p.v_ss;
+            raw[j] = *reinterpret_cast<const Raw*>(src + (int64_t)(s0 + __builtin_ctzll(mine)) * p.v_ss * kSize);
             const uint64_t rest = mine & (mine - 1);
             mine = rest ? rest : mine;
-            if (pair) {  // uniform
-                if (p.v_dtype == SSQ_F32) {
-                    const float2 w = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.v) + i);
-                    x[j][0] = w.x; x[j][1] = w.y;
-                } else {
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(p.v) + i);
-                    x[j][0] = __uint_as_float(w);  // both, unpacked below
-                }
-            } else {
-                x[j][0] = ssq_load_elem(p.v, p.v_dtype, i);
-                x[j][1] = dim + 1 < p.value_dim ? ssq_load_elem(p.v, p.v_dtype, i + 1) : 0.f;
-            }
         }
         float* at_scale = p.scale + (int64_t)page * p.vs_sb + (int64_t)head * p.vs_sh;
         const float held = *at_scale;
-        const bool two = on && dim + 1 < p.value_dim, one = on && dim < p.value_dim;
         uint8_t* dst = row(page, one ? dim : 0);
         uint4 old[2];
         old[0] = old[1] = make_uint4(0, 0, 0, 0);
         if (n < 16) {  // uniform
             old[0] = *reinterpret_cast<const uint4*>(dst);
-            old[1] = *reinterpret_cast<const uint4*>(two ? dst + p.vp_sd : dst);
+            old[1] = *reinterpret_cast<const uint4*>(dst + (one ? p.vp_sd : 0));
         }
-        if (pair && p.v_dtype != SSQ_F32) {
-            const bool bf = p.v_dtype == SSQ_BF16;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const uint32_t w = __float_as_uint(x[j][0]);
-                x[j][0] = bf ? ssq_bf16_to_f32(w & 0xFFFFu) : ssq_f16_to_f32(w & 0xFFFFu);
-                x[j][1] = bf ? __uint_as_float(w & 0xFFFF0000u) : ssq_f16_to_f32(w >> 16);
-            }
-        }
+        auto value = [&](int j, int e) {
+            if constexpr (DT == SSQ_F32) return __uint_as_float(e ? raw[j].y : raw[j].x);
+            else return ssq_bits_to_f32(e ? raw[j] >> 16 : raw[j] & 0xFFFFu, DT);
+        };
+        // (NaN leaves a maximum as it is; infinite ones are rare, and take a second look)
         float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) top = most(top, x[j]);
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, fmaxf(fabsf(value(j, 0)), fabsf(value(j, 1))));
+        const bool wild = __builtin_amdgcn_ballot_w64(top == INFINITY) != 0;
+        if (wild) {
+            top = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float x[2] = {value(j, 0), value(j, 1)};
+                top = most(top, x);
+            }
+        }
         if (!one) top = 0.f;
         for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
         const float need = val_scale(top);
         const float now = first > 0 ? fmaxf(held, need) : need, inv = 1.f / now, again = held * inv;
         const bool grown = first > 0 && now != held;
         if (on && dim == 0) *at_scale = now;
+        if (!one) return;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            if (!(e ? two : one)) continue;
             uint32_t w[4];
+            if (wild) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                w[k] = val_pack(val_in(x[4 * k][e], inv), val_in(x[4 * k + 1][e], inv), val_in(x[4 * k + 2][e], inv),
-                                val_in(x[4 * k + 3][e], inv));
+                for (int k = 0; k < 4; ++k)
+                    w[k] = val_pack(val_in(value(4 * k, e), inv), val_in(value(4 * k + 1, e), inv), val_in(value(4 * k + 2, e), inv),
+                                    val_in(value(4 * k + 3, e), inv));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    w[k] = val_pack(value(4 * k, e) * inv, value(4 * k + 1, e) * inv, value(4 * k + 2, e) * inv, value(4 * k + 3, e) * inv);
+            }
             if (n < 16) {  // uniform
                 if (grown) old[e] = val_rescale(old[e], first, again);
                 const uint32_t ow[4] = {old[e].x, old[e].y, old[e].z, old[e].w};
@@ -349,8 +352,10 @@ struct ValWave {
             const bool is = mine >> lane & 1ull;
             const int rank = __builtin_popcountll(mine & ((1ull << lane) - 1ull));
             const bool whole = (other || s0 + SSQ_WAVE >= p.seq_len) && __builtin_amdgcn_ballot_w64(is && r.off != first + rank) == 0;
-            if (whole && p.page_size == 16 && p.value_dim <= 2 * L) small(s0, mine, n, page, first);
-            else run(s0 + l, at(s0 + l + lane));
+            if (!whole || p.page_size != 16 || p.value_dim > 2 * L || !p.vec) run(s0 + l, at(s0 + l + lane));
+            else if (p.v_dtype == SSQ_BF16) small<SSQ_BF16>(s0, mine, n, page, first);
+            else if (p.v_dtype == SSQ_F16) small<SSQ_F16>(s0, mine, n, page, first);
+            else small<SSQ_F32>(s0, mine, n, page, first);
         }
     }
 };

@@ -8,7 +8,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__global__ __launch_bounds__(kThreads) void k_append_values(const SsqValues p) {
+__global__ __launch_bounds__(kThreads, 6) void k_append_values(const SsqValues p) {
     val_wave(p, (int64_t)blockIdx.x * (kThreads / SSQ_WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / SSQ_WAVE),
              threadIdx.x & (SSQ_WAVE - 1));
 }

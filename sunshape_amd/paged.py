@@ -8,10 +8,13 @@ layout.  This is the caller on the write side of the decode kernel:
   a slot mapping (token slot = page * page_size + offset), no dense key tensor;
 * passthrough [P, Hkv, page, n_heavy, bd] for SunShape-Mixed heavy blocks;
 * value pages [P, Hkv, Dv, page] -- vLLM's dim-major value layout, which the
-  MFMA decode kernel reads as B-operand fragments directly;
+  MFMA decode kernel reads as B-operand fragments directly; 16 bits, or 8 (float8_e4m3fn) with a scale per
+  page and KV head [P, Hkv];
 * per-sequence block tables and lengths, with a simple free-page allocator;
 * sequences that continue a shared one (``fork``): its pages are held once, and decode reads them once
-  for the whole batch.
+  for the whole batch; or, with 8-bit values or a window, sequences that share whole pages and go on by themselves;
+* a sliding window with first tokens that stay visible, whose dead pages ``release`` gives back;
+* ``compact`` and ``resize``, which move pages.
 
 ``attend`` is one layer's step of a serving loop: norm and rotation of the queries, the append of raw keys
 and values with the same for the keys, and the attention.
@@ -30,10 +33,21 @@ from . import hip_ops
 class PagedSunShapeCache:
     def __init__(self, codec, *, num_pages: int, num_kv_heads: int, value_dim: int, page_size: int = 16,
                  value_dtype: torch.dtype = torch.bfloat16, passthrough_dtype: torch.dtype = torch.bfloat16,
-                 device: Optional[torch.device] = None):
+                 device: Optional[torch.device] = None, window: Optional[int] = None, sinks: int = 0):
+        """value_dtype float8_e4m3fn: values in 8 bits (hip_ops.append_values).  window, sinks: every token sees the
+        window's newest tokens up to itself and the first `sinks` ones.  Either takes hip_ops.decode_window,
+        which is causal and serves fewer codecs: others are refused here."""
         reason = codec.unsupported_reason()
         if reason is not None:
             raise RuntimeError(reason)
+        self.window, self.sinks = window, int(sinks)
+        self.causal = window is not None or value_dtype == torch.float8_e4m3fn  # decode_window serves decode
+        if self.causal:
+            reason = self._causal_unsupported(codec, value_dim, page_size, value_dtype, window, sinks)
+            if reason is not None:
+                raise RuntimeError(reason)
+        elif sinks:
+            raise RuntimeError("sinks go with a window")
         self.codec = codec
         self.device = torch.device(device) if device is not None else codec.device
         self.page_size = int(page_size)
@@ -44,6 +58,9 @@ class PagedSunShapeCache:
         self.code_pages = torch.zeros(num_pages, num_kv_heads, page_size, nb, device=self.device,
                                       dtype=hip_ops.index_dtype(self.codec.n_centroids))
         self.v_pages = torch.zeros(num_pages, num_kv_heads, value_dim, page_size, dtype=value_dtype, device=self.device)
+        self.v_scale = None
+        if value_dtype == torch.float8_e4m3fn:
+            self.v_scale = torch.zeros(num_pages, num_kv_heads, device=self.device)
         heavy = codec.heavy_blocks()
         self.heavy = heavy
         self.pt_pages = None
@@ -54,6 +71,28 @@ class PagedSunShapeCache:
         self.block_tables: dict[int, list[int]] = {}
         self.seq_lens: dict[int, int] = {}
         self.prefix_of: dict[int, int] = {}  # forked sequence -> the sequence it continues
+        self._refs: dict[int, int] = {}      # page -> the sequences that hold it, where several do
+        self._released: dict[int, int] = {}  # sequence -> the token that pages given back end at
+
+    @staticmethod
+    def _causal_unsupported(codec, value_dim, page_size, value_dtype, window, sinks) -> Optional[str]:
+        """Why decode_window does not serve a cache (None: it does)."""
+        D, bd = codec.n_blocks * codec.block_dim, codec.block_dim
+        if window is not None and window < 1:
+            return "window must be at least 1 (None: no window)"
+        if sinks < 0 or (sinks and window is None):
+            return "sinks go with a window, and are not negative"
+        if codec.heavy_blocks() is not None:
+            return "8-bit values and windows take codecs without passthrough blocks"
+        if D not in (64, 128) or value_dim != D:
+            return f"8-bit values and windows take head_dim 64 or 128 with value_dim the same, not {D} and {value_dim}"
+        if bd not in (2, 4, 8) or codec.n_centroids > 256:
+            return "8-bit values and windows take byte codes of block_dim 2, 4 or 8"
+        if page_size not in (16, 32, 64, 128, 256):
+            return f"8-bit values and windows take pages of 16, 32, 64, 128 or 256 tokens, not {page_size}"
+        if value_dtype not in (torch.bfloat16, torch.float16, torch.float8_e4m3fn):
+            return f"a window takes values of 8 or 16 bits, not {value_dtype}"
+        return None
 
     # ------------------------------------------------------------------ pages
     def _pages(self, length: int) -> int:
@@ -84,12 +123,28 @@ class PagedSunShapeCache:
             raise RuntimeError(f"sequence {seq_id} is the prefix of others; free them first")
         self.prefix_of.pop(seq_id, None)
         for pg in self.block_tables.pop(seq_id, []):
-            self._free.append(pg)
+            self._drop(pg)
         self.seq_lens.pop(seq_id, None)
+        self._released.pop(seq_id, None)
+
+    def _drop(self, page: int) -> None:
+        """One holder less of a page (-1: released before)."""
+        if page < 0:
+            return
+        left = self._refs.get(page, 1) - 1
+        if left == 0:
+            self._free.append(page)
+        elif left == 1:
+            del self._refs[page]
+        else:
+            self._refs[page] = left
 
     def fork(self, prefix_id: int, seq_ids: list[int]) -> None:
-        """Start empty sequences that continue prefix_id's tokens.  The prefix takes no more tokens while
-        any of them lives."""
+        """Start sequences that continue prefix_id's tokens.  They start empty, and the prefix takes no more tokens while
+        any of them lives; in a cache with 8-bit values or a window they start as copies of it, which share its
+        whole pages and copy its last one if that is not full, and all of them go on by themselves."""
+        if self.causal:
+            return self._fork_copies(prefix_id, seq_ids)
         if not self.seq_lens.get(prefix_id) or prefix_id in self.prefix_of:
             raise RuntimeError(f"sequence {prefix_id} cannot be a prefix: it holds no tokens or continues another")
         if len(set(seq_ids)) != len(seq_ids) or any(s == prefix_id or s in self.seq_lens or s in self.prefix_of
@@ -97,6 +152,92 @@ class PagedSunShapeCache:
             raise RuntimeError("fork starts new, distinct sequences")
         for s in seq_ids:
             self.prefix_of[s] = prefix_id
+
+    def _fork_copies(self, prefix_id: int, seq_ids: list[int]) -> None:
+        length = self.seq_lens.get(prefix_id)
+        if not length:
+            raise RuntimeError(f"sequence {prefix_id} cannot be a prefix: it holds no tokens")
+        if len(set(seq_ids)) != len(seq_ids) or any(s in self.seq_lens or s in self.block_tables for s in seq_ids):
+            raise RuntimeError("fork starts new, distinct sequences")
+        table = self.block_tables[prefix_id]
+        whole = length // self.page_size
+        part = length % self.page_size != 0
+        if part and len(seq_ids) > len(self._free):
+            raise RuntimeError("PagedSunShapeCache is out of pages")
+        if part and seq_ids:
+            own = self._free[-len(seq_ids):][::-1]
+            hip_ops.copy_pages(self._pools(), self._index([table[whole]] * len(own)), self._index(own))
+            del self._free[-len(own):]
+        for i, s in enumerate(seq_ids):
+            for pg in table[:whole]:
+                if pg >= 0:
+                    self._refs[pg] = self._refs.get(pg, 1) + 1
+            self.block_tables[s] = table[:whole] + ([own[i]] if part else [])
+            self.seq_lens[s] = length
+            if prefix_id in self._released:
+                self._released[s] = self._released[prefix_id]
+
+    def _pools(self) -> list[torch.Tensor]:
+        return [p for p in (self.code_pages, self.v_pages, self.v_scale, self.pt_pages) if p is not None]
+
+    def _index(self, pages: list[int]) -> torch.Tensor:
+        return torch.tensor(pages, dtype=torch.int64, device=self.device)
+
+    def release(self, seq_ids: list[int]) -> int:
+        """Give back the pages whose tokens have left the window (and are no sinks) of each sequence's newest token;
+        returns how many are free again.  decode refuses queries older than that token, where they would see one."""
+        if self.window is None:
+            return 0
+        before = len(self._free)
+        for s in seq_ids:
+            first = (self.sinks + self.page_size - 1) // self.page_size
+            end = (self.seq_lens.get(s, 0) - self.window) // self.page_size  # pages [first, end) are dead
+            table = self.block_tables.get(s, [])
+            for i in range(max(first, self._released.get(s, 0) // self.page_size), end):
+                self._drop(table[i])
+                table[i] = -1
+            if end > first:
+                self._released[s] = max(self._released.get(s, 0), end * self.page_size)
+        return len(self._free) - before
+
+    def _held(self) -> list[int]:
+        return sorted({pg for t in self.block_tables.values() for pg in t if pg >= 0})
+
+    def _renumber(self, to: dict[int, int], num_pages: int) -> None:
+        for table in self.block_tables.values():
+            table[:] = [to.get(pg, pg) for pg in table]
+        self._refs = {to.get(pg, pg): n for pg, n in self._refs.items()}
+        used = set(self._held())
+        self._free = [pg for pg in range(num_pages - 1, -1, -1) if pg not in used]
+
+    def compact(self) -> int:
+        """Move the pages that sequences hold to the front of the pools, in place; returns how many there are.  Tables made
+        before are out of date."""
+        held = self._held()
+        n = len(held)
+        behind = [pg for pg in held if pg >= n]
+        room = sorted(set(range(n)) - set(held))
+        if behind:
+            hip_ops.copy_pages(self._pools(), self._index(behind), self._index(room))
+        self._renumber(dict(zip(behind, room)), self.num_pages)
+        return n
+
+    def resize(self, num_pages: int) -> None:
+        """New pools of num_pages pages with what the sequences hold at the front.  Tables and pools taken before are
+        out of date."""
+        held = self._held()
+        if num_pages < len(held):
+            raise RuntimeError(f"{len(held)} pages are held, more than {num_pages}")
+        old = self._pools()
+        new = [torch.zeros(num_pages, *p.shape[1:], dtype=p.dtype, device=p.device) for p in old]
+        if held:
+            hip_ops.copy_pages(old, self._index(held), self._index(list(range(len(held)))), into=new)
+        pools = iter(new)
+        self.code_pages, self.v_pages = next(pools), next(pools)
+        self.v_scale = None if self.v_scale is None else next(pools)
+        self.pt_pages = None if self.pt_pages is None else next(pools)
+        self.num_pages = int(num_pages)
+        self._renumber({pg: i for i, pg in enumerate(held)}, self.num_pages)
 
     def _shared_prefix(self, seq_ids: list[int]) -> Optional[int]:
         found = {self.prefix_of.get(s) for s in seq_ids}
@@ -155,6 +296,8 @@ class PagedSunShapeCache:
             raise RuntimeError("key/value shapes do not match the cache")
         if (cos is None) != (sin is None):
             raise RuntimeError("cos and sin come together")
+        if self.v_scale is not None and len(set(seq_ids)) != len(seq_ids):
+            raise RuntimeError("an append of 8-bit values takes each sequence once")
         if cos is not None or k_weight is not None:
             if len(seq_ids) != B:
                 raise RuntimeError(f"{B} rows of keys for {len(seq_ids)} sequences")
@@ -173,11 +316,17 @@ class PagedSunShapeCache:
                            metric=self.codec.encode_metric(), grid=self.codec.encode_search_grid(self.codec.centroids),
                            direct=hip_ops.cdist_direct(S, self.codec.n_centroids),
                            rotation=self.codec.rotation_matrix())
+            if self.v_scale is not None:
+                hip_ops.append_values(value_states.to(self.device), self.v_pages, self.v_scale, slots)
+                return slots
             flat = slots.reshape(-1)
             page, off = flat // self.page_size, flat % self.page_size
             vals = value_states.to(self.device, self.v_pages.dtype).permute(0, 2, 1, 3).reshape(B * S, Hkv, self.value_dim)
             self.v_pages[page, :, :, off] = vals
         return slots
+
+    def _scales(self) -> dict:
+        return {} if self.v_scale is None else {"v_scale": self.v_scale}
 
     def _append_raw(self, seq_ids, key_states, value_states, positions, **turn) -> torch.Tensor:
         S = key_states.shape[2]
@@ -188,7 +337,7 @@ class PagedSunShapeCache:
                               positions=positions, heavy=self.heavy, pt_out=self.pt_pages, metric=self.codec.encode_metric(),
                               grid=self.codec.encode_search_grid(self.codec.centroids),
                               direct=hip_ops.cdist_direct(S, self.codec.n_centroids),
-                              rotation=self.codec.rotation_matrix(), **turn)
+                              rotation=self.codec.rotation_matrix(), **turn, **self._scales())
         return slots
 
     def tables(self, seq_ids: list[int]) -> tuple[torch.Tensor, torch.Tensor]:
@@ -205,7 +354,18 @@ class PagedSunShapeCache:
                return_lse: bool = False, mask: Optional[torch.Tensor] = None):
         """Fused decode of query [B, Hq, Lq, D] against the cached sequences; forked ones attend their shared
         prefix's tokens first (the sequences of one call continue the same one, or none).  mask: additive,
-        broadcastable to [B, Hq, Lq, T], T the sequences' own table width times the page size."""
+        broadcastable to [B, Hq, Lq, T], T the sequences' own table width times the page size.  In a cache with 8-bit
+        values or a window the queries are those of each sequence's Lq newest tokens, each of which sees the tokens up
+        to itself (in its window); no mask."""
+        if self.causal:
+            if mask is not None:
+                raise RuntimeError("a cache with 8-bit values or a window takes no mask")
+            self._still_seen(seq_ids, query.shape[2])
+            bt, lens = self.tables(seq_ids)
+            return hip_ops.decode_window(query, self.code_pages, self.v_pages, self.codec.effective_permutation(),
+                                         self.codec.centroids, block_table=bt, seq_lens=lens, scale=scale,
+                                         window=self.window, sinks=self.sinks, return_lse=return_lse,
+                                         rotation=self.codec.rotation_matrix(), **self._scales())
         prefix = self._shared_prefix(seq_ids)
         bt, lens = self.tables(seq_ids)
         if prefix is None:
@@ -219,6 +379,12 @@ class PagedSunShapeCache:
                                      seq_lens=lens, scale=scale, mask=mask, heavy=self.heavy, pt=self.pt_pages,
                                      return_lse=return_lse, rotation=self.codec.rotation_matrix())
 
+    def _still_seen(self, seq_ids: list[int], num_rows: int) -> None:
+        """No token that the oldest of num_rows queries sees is in a released page."""
+        for s, end in self._released.items():
+            if s in seq_ids and self.seq_lens[s] - num_rows - self.window + 1 < end:
+                raise RuntimeError(f"pages that the oldest query of sequence {s} sees are released")
+
     def attend(self, seq_ids: list[int], query: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor, *,
                cos: torch.Tensor, sin: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
                k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
@@ -226,7 +392,8 @@ class PagedSunShapeCache:
         """One step over raw projections: query [B, Hq, S, D], keys and values [B, Hkv, S, ..] of the S next
         tokens of each sequence.  Norms and rotates them, appends keys and values, and attends causally;
         returns [B, Hq, S, Dv].  scale as in decode (None: the query as it is).  A step that is refused leaves the
-        sequences as they were.  With S > 1 the causal mask takes 4 B S times the longest own table's tokens in bytes."""
+        sequences as they were (8-bit values of a last page may have been rounded to a larger scale).  With S > 1 the causal mask takes 4 B S times the longest own table's tokens in bytes (none
+        in a cache with 8-bit values or a window, whose pages that left the window are given back after the step)."""
         B, _, S, _ = query.shape
         if len(set(seq_ids)) != len(seq_ids):
             raise RuntimeError("attend takes each sequence once")
@@ -242,10 +409,12 @@ class PagedSunShapeCache:
             self._append_raw(seq_ids, key_states, value_states, positions, cos=cos, sin=sin, k_weight=k_weight, eps=eps,
                              interleaved=interleaved)
             mask = None
-            if S > 1:  # new token i sees its sequence up to itself
+            if S > 1 and not self.causal:  # new token i sees its sequence up to itself
                 width = max(len(self.block_tables[s]) for s in seq_ids) * self.page_size
                 last = torch.tensor([self.seq_lens[s] - S for s in seq_ids], device=self.device)[:, None] + \
                     torch.arange(S, device=self.device)[None]
                 mask = torch.zeros(B, 1, S, width, device=self.device)
                 mask.masked_fill_(torch.arange(width, device=self.device) > last[:, None, :, None], float("-inf"))
-            return self.decode(seq_ids, q, scale=scale, mask=mask)
+            out = self.decode(seq_ids, q, scale=scale, mask=mask)
+        self.release(seq_ids)
+        return out

@@ -80,6 +80,7 @@ extern "C" int ssq_copy_pages(const ssq_copy_args* a, void* stream) {
     for (int k = 0; k < a->n_pools; ++k) {
         const ssq_copy_pool& c = a->pool[k];
         SSQ_REQUIRE(c.bytes >= 0 && c.src_pages >= 0 && c.dst_pages >= 0, "bad pool %d", k);
+        SSQ_UNSUPPORTED(c.bytes <= 1ll << 32, "pages are too large");
         SSQ_REQUIRE((c.src && c.dst) || c.bytes == 0 || c.src_pages == 0 || c.dst_pages == 0, "pool %d is NULL", k);
         const uint64_t at = (uint64_t)(uintptr_t)c.src | (uint64_t)(uintptr_t)c.dst | (uint64_t)c.src_stride | (uint64_t)c.dst_stride | (uint64_t)c.bytes;
         p.pool[k] = {reinterpret_cast<const uint8_t*>(c.src), reinterpret_cast<uint8_t*>(c.dst), c.src_stride, c.dst_stride,

@@ -32,7 +32,10 @@ int check(const ssq_window_args* a) {
     SSQ_REQUIRE((int64_t)d.batch * (d.num_q_heads > 0 ? d.num_q_heads : 1) <= (1 << 24) && d.q_len <= 1 << 20 &&
                     (int64_t)d.batch * d.num_q_heads * d.q_len <= 1 << 30,
                 "too many query rows");
-    if (v8) d.v_dtype = SSQ_F16;  // the decode's checks know 16 bits
+    if (v8) d.v_dtype = SSQ_F16;  // the decode's checks know 16 bits, and calls with something to do
+    if (d.batch == 0) d.batch = 1;
+    if (d.num_q_heads == 0) d.num_q_heads = d.num_kv_heads;
+    if (d.q_len == 0) d.q_len = 1;
     int rc = ssq_decode_validate(&d);
     if (rc) return rc;
     SSQ_UNSUPPORTED(!d.heavy_mask[0] && !d.heavy_mask[1], "decode_window serves codecs without passthrough blocks");
@@ -42,8 +45,8 @@ int check(const ssq_window_args* a) {
                     d.block_dim);
     SSQ_UNSUPPORTED(d.n_centroids <= 256 && d.code_bits == 0, "decode_window serves byte codes (at most 256 codewords)");
     SSQ_UNSUPPORTED(v8 || d.v_dtype == SSQ_BF16 || d.v_dtype == SSQ_F16, "decode_window serves values of 8 or 16 bits");
-    SSQ_UNSUPPORTED(d.page_size >= 16 && (d.page_size & (d.page_size - 1)) == 0 && d.page_size <= 1 << 16,
-                    "decode_window serves page sizes that are powers of two from 16, not %d", d.page_size);
+    SSQ_UNSUPPORTED(d.page_size >= 16, "decode_window serves page sizes from 16, not %d", d.page_size);  // and they divide 256
+    SSQ_UNSUPPORTED(d.seq_len <= 1 << 30, "the block table is too long");
     SSQ_REQUIRE((uintptr_t)d.cent % 16 == 0 && d.cent_sh % 4 == 0, "centroids must be 16-byte aligned");
     const int64_t piece = d.n_blocks / 4;  // bytes of a token's codes that a lane loads at once
     SSQ_REQUIRE((uintptr_t)d.codes % piece == 0 && d.c_sb % piece == 0 && d.c_sh % piece == 0 && d.c_st % piece == 0,

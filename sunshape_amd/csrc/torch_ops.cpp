@@ -473,13 +473,16 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q_in, const std::optional<
 }
 
 // 8-bit value pages [P, Hkv, Dv, page] come with fp32 scales [P, Hkv], others without
-void check_scale(const Tensor& v_pages, const std::optional<Tensor>& v_scale, const Tensor& ref) {
+void check_scale(const Tensor& v_pages, const std::optional<Tensor>& v_scale, const Tensor& ref, bool written) {
     const bool v8 = v_pages.scalar_type() == at::kFloat8_e4m3fn;
     TORCH_CHECK(v8 == given(v_scale), v8 ? "8-bit values need v_scale" : "v_scale goes with 8-bit values (float8_e4m3fn)");
     if (!v8) return;
     same_device("v_scale", *v_scale, ref);
     TORCH_CHECK(v_scale->scalar_type() == at::kFloat && v_scale->dim() == 2 && v_scale->size(0) == v_pages.size(0) &&
                     v_scale->size(1) == v_pages.size(1), "v_scale must be float32 [", v_pages.size(0), ", ", v_pages.size(1), "]");
+    for (int64_t i = 0; written && i < 2; ++i)
+        TORCH_CHECK((v_scale->size(i) <= 1 || v_scale->stride(i) != 0) && (v_pages.size(i) <= 1 || v_pages.stride(i) != 0),
+                    "pages and heads that are written have memory of their own");
 }
 
 void append_kv(const Tensor& keys_in, const std::optional<Tensor>& v_in, const Tensor& perm_in, const Tensor& cent_in,
@@ -525,7 +528,7 @@ void append_kv(const Tensor& keys_in, const std::optional<Tensor>& v_in, const T
         TORCH_CHECK(v_pages->dim() == 4 && v_pages->size(0) == P && v_pages->size(1) == Hkv &&
                         v_pages->size(2) == v.size(3) && v_pages->size(3) == page && v_pages->stride(3) == 1,
                     "v_out must be [", P, ", ", Hkv, ", ", v.size(3), ", ", page, "], contiguous over tokens");
-        check_scale(*v_pages, v_scale, keys);
+        check_scale(*v_pages, v_scale, keys, true);
     } else {
         TORCH_CHECK(!given(v_scale), "v_scale goes with 8-bit values");
     }
@@ -704,7 +707,7 @@ void append_values(const Tensor& v_in, const Tensor& v_pages, const Tensor& v_sc
     TORCH_CHECK(v_pages.scalar_type() == at::kFloat8_e4m3fn, "append_values writes float8_e4m3fn pages, got ", v_pages.scalar_type());
     TORCH_CHECK(v_pages.dim() == 4 && v_pages.size(1) == Hkv && v_pages.size(2) == Dv && v_pages.stride(3) == 1 && v_pages.size(3) >= 1,
                 "v_out must be [P, ", Hkv, ", ", Dv, ", page], contiguous over tokens");
-    check_scale(v_pages, v_scale, v);
+    check_scale(v_pages, v_scale, v, true);
     same_device("slot_mapping", slot_mapping, v);
     TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.dim() == 2 && slot_mapping.size(0) == B &&
                     slot_mapping.size(1) == S && (slot_mapping.stride(1) == 1 || S <= 1),
@@ -744,7 +747,7 @@ std::tuple<Tensor, Tensor> decode_window(const Tensor& q_in, const Tensor& codes
     check_codes(codes, c.nb, c.nc, 0);
     TORCH_CHECK(v.dim() == 4 && v.size(0) == P && v.size(1) == Hkv && v.size(3) == page && v.stride(-1) == 1,
                 "paged V must be [P, Hkv, Dv, page], contiguous over tokens");
-    check_scale(v, v_scale, q);
+    check_scale(v, v_scale, q, false);
     same_device("block_table", bt, q);
     same_device("seq_lens", seq_lens, q);
     TORCH_CHECK(bt.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt, "block_table and seq_lens must be int32");
@@ -826,6 +829,7 @@ void copy_pages(at::TensorList src, at::TensorList dst, const Tensor& from, cons
             TORCH_CHECK(s.size(i) <= 1 || n == 0 || (s.stride(i) == n && d.stride(i) == n), "the pages of pool ", k, " must be contiguous");
             n *= s.size(i);
         }
+        TORCH_CHECK(d.size(0) <= 1 || n == 0 || d.stride(0) >= n, "the pages of pool ", k, " that are written overlap");
         const int64_t e = (int64_t)s.element_size();
         a.pool[k].src = s.data_ptr(); a.pool[k].dst = d.data_ptr();
         a.pool[k].src_stride = s.stride(0) * e; a.pool[k].dst_stride = d.stride(0) * e;

@@ -709,7 +709,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                 const uint32_t mine = u.sees(u.pos, u.pos, tok);
 #pragma unroll
                 for (int e = 0; e < CH; ++e) s[e >> 2][e & 3] = mine >> e & 1u ? s[e >> 2][e & 3] : -INFINITY;
-                if (any == 0) val.scale = 0.f;  // no page of this tile's
+                if (mine == 0) val.scale = 0.f;  // not this row's page, or none of this tile's
                 const w4u off = W::spread(~any);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) val.v[dt] &= ~off;
@@ -737,12 +737,12 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
             }
             float by = 1.f;  // this group's page scale, in units of O
             if constexpr (W::kV8) {
+                // (positive floats compare as their bits; rows have units of their own where they do not see the same pages)
                 const uint32_t bits = __float_as_uint(val.scale);
-                uint32_t big = max(max((uint32_t)__builtin_amdgcn_readlane((int)bits, 0), (uint32_t)__builtin_amdgcn_readlane((int)bits, 16)),
-                                   max((uint32_t)__builtin_amdgcn_readlane((int)bits, 32), (uint32_t)__builtin_amdgcn_readlane((int)bits, 48)));
-                if (big > __float_as_uint(unit)) {  // uniform: positive floats compare as their bits
-                    const float f = unit / __uint_as_float(big);
-                    unit = __uint_as_float(big);
+                if (__builtin_amdgcn_ballot_w64(bits > __float_as_uint(unit)) != 0) {
+                    const float big = fmaxf(unit, win_max4(val.scale));
+                    const float f = unit / big;
+                    unit = big;
                     inv_unit = 1.f / unit;
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) o[dt] *= f;

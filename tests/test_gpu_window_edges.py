@@ -123,3 +123,22 @@ def test_written_pages_that_overlap_are_refused():
                  (pages[:, :1].expand(4, 2, 64, 16), scale)):
         with pytest.raises(RuntimeError, match="memory of their own"):
             hip_ops.append_values(v, p, s, slots)
+
+
+@pytest.mark.parametrize("window, sinks", [(None, 0), (40, 0), (40, 9)])
+@pytest.mark.parametrize("T", [90, 5000])
+def test_a_rows_scales_are_those_of_the_pages_it_sees(T, window, sinks):
+    """Pages that some of the rows that share a tile do not see (yet, or any longer) have scales 2^80 times the others'."""
+    log(f"scales that some rows see: {T} tokens, window {window}, sinks {sinks}")
+    pr = problem(35, B=2, Hq=4, Hkv=2, D=64, Lq=24, T=T, lens=[T, T - 5], spread=0)
+    for b in range(2):
+        n = int(pr["seq_lens"][b])
+        pr["v_scale"][pr["block_table"][b, (n - 1) // 16].long()] = 2.0 ** 80
+        if window:  # the page that the first rows' windows begin in
+            pr["v_scale"][pr["block_table"][b, (n - 24 - window + 1) // 16].long()] = 2.0 ** 80
+    out, lse = run(pr, window=window, sinks=sinks)
+    ref, rl, mag, pv = window64(pr, window, sinks)
+    ob, lb = window_bounds(pr, ref, rl, mag, pv, out.dtype)
+    assert ((out.cpu().double() - ref).abs() <= ob).all()
+    assert ((lse.cpu().double() - rl).abs() <= lb).all()
+    assert ref.abs().amax() > 1e20 and ref.abs().amin() < 1e6

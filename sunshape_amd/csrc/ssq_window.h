@@ -34,14 +34,16 @@ struct SsqWindowParams {
     int n_pages;
     const float* v_scale;
     int64_t vs_sb, vs_sh;
-    int G, rows, rgroups;    // query rows of a (sequence, KV head): (qi, g), g fastest; groups of 16 rows
+    int G, rows, rgroups;    // query rows of a (sequence, KV head): (qi, g), g fastest; groups of item_rows
     int items;               // batch * rgroups
     int n_wg;                // workgroups per KV head
-    int team;                // a workgroup's waves share whole items; else each wave has an equal share of all tiles (WinCut)
+    int form;                // kWinTeam: a workgroup's waves share whole items; kWinShares: each wave has an equal share of all
+                             // tiles (WinCut); kWinWide: each workgroup has, over items of 256 rows
+    int item_rows, workers;  // rows of an item; those that share the tiles of a KV head
     int fixed, least;        // an item's cost beside its tiles, and the smallest share, both in tiles
     int psh;                 // log2(page_size / 16)
     int q_vec, out_vec;      // query rows load in 16-byte pieces; four values of the output store as one
-    float* part;             // [Hkv][n_wg * 8 waves][2] slots of 16 rows x (Dv + 2): o, then m (log2 units), l
+    float* part;             // [Hkv][workers][2] slots of item_rows x (Dv + 2): o, then m (log2 units), l
     int* meta;               // [items][2]: first worker * 2 + its slot, and pieces
 };
 
@@ -55,7 +57,8 @@ SSQ_WINDOW_UNIT(ssq_window_128_f16);
 
 // waves of a workgroup: two a SIMD, so that one's matrix products run beside the other's vector work.  (32 rows a wave, half as
 // many gathers for a row, leave registers for one: 20 rows a sequence 43 us for 36, a chunk of 512 tokens 162 for 119.)
-constexpr int kWinWaves = 8, kWinThreads = kWinWaves * 64, kWinRows = 16;
+constexpr int kWinWaves = 8, kWinThreads = kWinWaves * 64, kWinRows = 16, kWinWideRows = 256;
+enum { kWinTeam, kWinShares, kWinWide };
 
 // what the tiles of an item follow from, beside its length
 struct WinShape { int window, sinks, q_len, G, rows; };
@@ -67,10 +70,10 @@ struct WinTiles {
     int p_lo, p_hi;      // the first and last row's positions
     int n, n_sink, from; // tile i: i < n_sink ? i : from + i - n_sink
 };
-template <int TT>
+template <int TT, int ROWS>
 __host__ __device__ __forceinline__ WinTiles win_tiles(const WinShape& p, int len, int row0) {
     WinTiles t;
-    const int last = (row0 + kWinRows < p.rows ? row0 + kWinRows : p.rows) - 1;
+    const int last = (row0 + ROWS < p.rows ? row0 + ROWS : p.rows) - 1;
     t.p_lo = len - p.q_len + row0 / p.G;
     t.p_hi = len - p.q_len + last / p.G;
     t.n = t.n_sink = t.from = 0;
@@ -177,11 +180,11 @@ __device__ __forceinline__ WinArgs win_args() {
 }
 
 // Equal shares of the items' tiles: the items of a KV head lie end to end on a cost axis, fixed + tiles each, and worker w (a
-// wave; the waves of a workgroup are n_wg apart) takes [w share, (w + 1) share).  An item inside one share is written out by its
+// wave, those of a workgroup n_wg apart; or a workgroup) takes [w share, (w + 1) share).  An item inside one share is written out by its
 // wave; one that spans several leaves a partial in each: slot 0 of a worker for the item its share starts in, slot 1 for one that
 // starts in it.  Everything follows from the lengths, which the host does not see.  Waves that wait for nobody keep the memory
 // busy through one another's beginnings and ends.
-template <int TT>
+template <int TT, int ROWS>
 struct WinCut {
     int share, total;
     int c0, v0;  // this lane's cost and inclusive sum over the first 64 items
@@ -189,7 +192,7 @@ struct WinCut {
     __device__ __forceinline__ static int cost(WinArgs p, int i, int len) {
         if (i >= p->items) return 0;
         const WinShape s{p->window, p->sinks, p->a.q_len, p->G, p->rows};
-        return p->fixed + win_tiles<TT>(s, max(0, min(len, p->a.seq_len)), i % p->rgroups * kWinRows).n;
+        return p->fixed + win_tiles<TT, ROWS>(s, max(0, min(len, p->a.seq_len)), i % p->rgroups * ROWS).n;
     }
     __device__ __forceinline__ static int scan(int v) {  // inclusive, over the wave
         v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
@@ -207,8 +210,7 @@ struct WinCut {
         total = __builtin_amdgcn_readlane(v0, 63);
         for (int i = SSQ_WAVE; i < p->items; i += SSQ_WAVE)
             total += __builtin_amdgcn_readlane(scan(cost(p, i + lane, length(p, i + lane))), 63);
-        const int workers = p->n_wg * kWinWaves;
-        share = max((total + workers - 1) / workers, p->least);
+        share = max((total + p->workers - 1) / p->workers, p->least);
     }
     // the item that holds cost position x < total, its start and cost
     __device__ __forceinline__ void find(WinArgs p, int lane, int x, int& item, int& s, int& c) const {  // (uniform results)
@@ -235,6 +237,81 @@ struct WinCut {
 };
 
 // LDS: codebook | the waves' query rows, and their join | m, l [waves][16] | reduction [waves] | permutation [D]
+// A KV head's codebook: 64 (32) floats a thread, all asked for at once, staged in LDS as two f16 parts times 2^k.
+template <int D, int BD>
+struct WinBook {
+    static constexpr int kPer = D / BD * 256 / kWinThreads;
+    float c[kPer][BD];
+    __device__ __forceinline__ void load(WinArgs p, int kv, int tid) {
+        const float* cent = p->a.cent + (int64_t)kv * p->a.cent_sh;
+        auto entry = [&](int k, const float* src) {
+            if constexpr (BD >= 4) {
+#pragma unroll
+                for (int d = 0; d < BD; d += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(src + d);
+                    c[k][d] = x.x; c[k][d + 1] = x.y; c[k][d + 2] = x.z; c[k][d + 3] = x.w;
+                }
+            } else {
+                const float2 x = *reinterpret_cast<const float2*>(src);
+                c[k][0] = x.x; c[k][1] = x.y;
+            }
+        };
+        const int n = p->a.n_centroids;  // entry e = tid + k * kWinThreads: block e / 256, codeword e % 256
+        const float* src = cent + ((tid >> 8) * n + min(tid & 255, n - 1)) * BD;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) entry(k, src + k * (kWinThreads / 256 * BD) * n);
+    }
+    // The whole workgroup; returns k.  Entry e is at 4 BD e: BD 2 hi, lo; 4 hi, hi, lo, lo; 8 four words hi, four lo.
+    __device__ __forceinline__ int stage(unsigned char* smem, float* red, int tid, int lane, int wave) const {
+        // the largest finite codeword; infinite ones (rare) cost a second look and checks on the way
+        auto largest = [&](auto checked) {
+            float most = 0.f;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k)
+#pragma unroll
+                for (int d = 0; d < BD; ++d) {
+                    const float z = fabsf(c[k][d]);
+                    most = fmaxf(most, !checked || z < INFINITY ? z : 0.f);
+                }
+            most = ssq_wave_max(most);
+            __syncthreads();
+            if (lane == 0) red[wave] = most;
+            __syncthreads();
+            most = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWinWaves; ++w) most = fmaxf(most, red[w]);
+            return most;
+        };
+        float most = largest(std::false_type{});
+        const bool infinite = most == INFINITY;  // uniform
+        if (infinite) most = largest(std::true_type{});
+        const int book_exp = min(15 - win_exp(most), 126), n_centroids = win_args()->a.n_centroids;
+        auto put = [&](auto checked) {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const int e = tid + k * kWinThreads;
+                const float scale = (e & 255) < n_centroids ? ldexpf(1.f, book_exp) : 0.f;
+                uint32_t hi[BD / 2], lo[BD / 2];
+#pragma unroll
+                for (int d = 0; d < BD; d += 2) win_split<checked>(c[k][d] * scale, c[k][d + 1] * scale, hi[d / 2], lo[d / 2]);
+                unsigned char* at = smem + e * (4 * BD);
+                if constexpr (BD == 8) {
+                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(at + 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                } else if constexpr (BD == 4) {
+                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+                } else {
+                    *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], lo[0]);
+                }
+            }
+        };
+        if (infinite) put(std::true_type{});
+        else put(std::false_type{});
+        __syncthreads();
+        return book_exp;
+    }
+};
+
 template <int D>
 struct WinLds {
     static constexpr int kBook = D * 256 * 4;
@@ -428,31 +505,12 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
     uint16_t* perm = reinterpret_cast<uint16_t*>(smem + L::kPerm);
     float* mls = reinterpret_cast<float*>(smem + L::kMl);
 
-    // ---- the codebook, 64 (32) floats a thread, all asked for at once behind the permutation
-    constexpr int kPer = W::NB * 256 / kWinThreads;
+    // ---- the codebook, behind the permutation
     // (No branches around these loads or the first tiles': they return in order, and a wait behind a branch is for all of them.)
     const int64_t at_perm = p->a.perm[(int64_t)kv * p->a.perm_sh + min(tid, D - 1)];
-    const int first_len = TEAM ? 0 : WinCut<TT>::length(p, lane);
-    float c[kPer][BD];
-    {
-        const float* cent = p->a.cent + (int64_t)kv * p->a.cent_sh;
-        auto entry = [&](int k, const float* src) {
-            if constexpr (BD >= 4) {
-#pragma unroll
-                for (int d = 0; d < BD; d += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(src + d);
-                    c[k][d] = x.x; c[k][d + 1] = x.y; c[k][d + 2] = x.z; c[k][d + 3] = x.w;
-                }
-            } else {
-                const float2 x = *reinterpret_cast<const float2*>(src);
-                c[k][0] = x.x; c[k][1] = x.y;
-            }
-        };
-        const int n = p->a.n_centroids;  // entry e = tid + k * kWinThreads: block e / 256, codeword e % 256
-        const float* src = cent + ((tid >> 8) * n + min(tid & 255, n - 1)) * BD;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) entry(k, src + k * (kWinThreads / 256 * BD) * n);
-    }
+    const int first_len = TEAM ? 0 : WinCut<TT, kWinRows>::length(p, lane);
+    WinBook<D, BD> book;
+    book.load(p, kv, tid);
     if (tid < D) perm[tid] = (uint16_t)((uint64_t)at_perm < (uint64_t)D ? at_perm : D - 1);
 
     W u;
@@ -468,7 +526,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
     u.vstep = 16 * (uint32_t)p->a.v_st * (W::kV8 ? 1 : 2);
 
     // ---- what is to be done: an item's tiles [i0, i1), and where they go (slot -1: the output)
-    WinCut<TT> cut;
+    WinCut<TT, kWinRows> cut;
     const int worker = TEAM ? wg : wave * p->n_wg + wg;
     int x = worker, x_begin = 0, x_end = 0;
     if constexpr (!TEAM) {
@@ -496,7 +554,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
             row0 = (item - b * p->rgroups) * kWinRows;
             len = max(0, min(p->a.seq_lens[b], p->a.seq_len));
             nr = min(kWinRows, p->rows - row0);
-            u.t = win_tiles<TT>(WinShape{u.window, u.sinks, q_len, p->G, p->rows}, len, row0);
+            u.t = win_tiles<TT, kWinRows>(WinShape{u.window, u.sinks, q_len, p->G, p->rows}, len, row0);
             slot = -1;
             i0 = TEAM ? wave : 0;
             i1 = u.t.n;
@@ -637,54 +695,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
     __syncthreads();  // the permutation
     bool more = next();
     load();
-    {
-        // the largest finite codeword; infinite ones (rare) cost a second look and checks on the way
-        auto largest = [&](auto checked) {
-            float most = 0.f;
-#pragma unroll
-            for (int k = 0; k < kPer; ++k)
-#pragma unroll
-                for (int d = 0; d < BD; ++d) {
-                    const float z = fabsf(c[k][d]);
-                    most = fmaxf(most, !checked || z < INFINITY ? z : 0.f);
-                }
-            most = ssq_wave_max(most);
-            __syncthreads();
-            if (lane == 0) red[wave] = most;
-            __syncthreads();
-            most = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWinWaves; ++w) most = fmaxf(most, red[w]);
-            return most;
-        };
-        const int n_centroids = win_args()->a.n_centroids;
-        auto stage = [&](auto checked) {
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                const int e = tid + k * kWinThreads;
-                const float scale = (e & 255) < n_centroids ? ldexpf(1.f, book_exp) : 0.f;
-                uint32_t hi[BD / 2], lo[BD / 2];
-#pragma unroll
-                for (int d = 0; d < BD; d += 2) win_split<checked>(c[k][d] * scale, c[k][d + 1] * scale, hi[d / 2], lo[d / 2]);
-                unsigned char* at = smem + e * (4 * BD);
-                if constexpr (BD == 8) {
-                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(at + 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                } else if constexpr (BD == 4) {
-                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
-                } else {
-                    *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], lo[0]);
-                }
-            }
-        };
-        float most = largest(std::false_type{});
-        const bool infinite = most == INFINITY;  // uniform
-        if (infinite) most = largest(std::true_type{});
-        book_exp = min(15 - win_exp(most), 126);
-        if (infinite) stage(std::true_type{});
-        else stage(std::false_type{});
-        __syncthreads();
-    }
+    book_exp = book.stage(smem, red, tid, lane, wave);
     while (more) {
         query();
 
@@ -848,7 +859,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                 if (p->a.lse && u.grp == 0)
                     p->a.lse[((int64_t)b * p->a.num_q_heads + h) * p->a.q_len + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * kWinLn2;
             } else {
-                float* dst = p->part + ((int64_t)(kv * p->n_wg * kWinWaves + worker) * 2 + slot) * (kWinRows * (D + 2));
+                float* dst = p->part + ((int64_t)(kv * p->workers + worker) * 2 + slot) * (kWinRows * (D + 2));
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     const w4f z = o[dt] * unit;
@@ -865,12 +876,18 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
     }
 }
 
+}  // namespace
+
+#include "ssq_window_wide.h"
+
+namespace {
+
 // Joins the pieces of the items that waves shared: a query row by one wave of four, or by all W waves of a workgroup where pieces
 // may be many; lanes over the value dims, 8 pieces in flight a wave.
 template <int D, int W>
 __global__ __launch_bounds__((W > 1 ? W : 4) * SSQ_WAVE) void k_window_merge(const SsqWindowParams p) {
     constexpr bool WIDE = W > 1;
-    constexpr int E = D / SSQ_WAVE, kAhead = 8, kSlot = kWinRows * (D + 2);
+    constexpr int E = D / SSQ_WAVE, kAhead = 8;
     __shared__ float mo[W][D], ml[W][2];
     const ssq_decode_args& a = p.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -879,10 +896,11 @@ __global__ __launch_bounds__((W > 1 ? W : 4) * SSQ_WAVE) void k_window_merge(con
     const int row = (int)(id - bk * p.rows), b = (int)(bk / a.num_kv_heads), kv = (int)(bk - (int64_t)b * a.num_kv_heads);
     if (b >= a.batch) return;
     const int item = b * p.rgroups + row / kWinRows, r = row % kWinRows;
+    constexpr int n = kWinRows, slot = n * (D + 2);
     const int first = p.meta[2 * item], pieces = p.meta[2 * item + 1];
     if (pieces <= 1) return;
-    const float* base = p.part + (int64_t)kv * p.n_wg * kWinWaves * 2 * kSlot;
-    auto at = [&](int i) { return base + (int64_t)(i ? 2 * ((first >> 1) + i) : first) * kSlot; };
+    const float* base = p.part + (int64_t)kv * p.workers * 2 * slot;
+    auto at = [&](int i) { return base + (int64_t)(i ? 2 * ((first >> 1) + i) : first) * slot; };
     float M = kWinNone, l = 0.f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
@@ -890,15 +908,17 @@ __global__ __launch_bounds__((W > 1 ? W : 4) * SSQ_WAVE) void k_window_merge(con
         float m[kAhead], lp[kAhead], op[kAhead][E];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            const float* src = at(min(i0 + j, pieces - 1));
-            m[j] = src[kWinRows * D + r];
-            lp[j] = src[kWinRows * D + kWinRows + r];
+            m[j] = kWinNone;
+            if (i0 + j >= pieces) continue;
+            const float* src = at(i0 + j);
+            m[j] = src[n * D + r];
+            lp[j] = src[n * D + n + r];
 #pragma unroll
             for (int e = 0; e < E; ++e) op[j][e] = src[r * D + lane * E + e];
         }
         float mt = M;
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) mt = fmaxf(mt, m[j]);  // (those past the last are it)
+        for (int j = 0; j < kAhead; ++j) mt = fmaxf(mt, m[j]);
         const float f0 = __builtin_amdgcn_exp2f(M - mt);
         M = mt;
         l *= f0;
@@ -945,29 +965,35 @@ __global__ __launch_bounds__((W > 1 ? W : 4) * SSQ_WAVE) void k_window_merge(con
     if (a.lse && lane == 0) a.lse[((int64_t)b * a.num_q_heads + h) * a.q_len + qi] = l == 0.f ? -INFINITY : (M + log2f(l)) * kWinLn2;
 }
 
-template <int D, int BD, int VT, int QP, bool TEAM>
-int win_launch(const SsqWindowParams& p, hipStream_t st) {
-    using L = WinLds<D>;
-    static_assert(L::kTotal <= 160 * 1024, "a workgroup's LDS");
-    auto kern = k_window<D, BD, VT, QP, TEAM>;
-    int rc = ssq_allow_lds((const void*)kern, L::kTotal, "hipFuncSetAttribute(k_window)");
-    if (rc) return rc;
-    hipLaunchKernelGGL(kern, dim3(p.n_wg * p.a.num_kv_heads), dim3(kWinThreads), L::kTotal, st, p);
-    rc = ssq_check_hip(hipGetLastError(), "k_window launch");
-    if (rc || TEAM) return rc;
-    // An item of few may have as many pieces as there are waves; of many, each has few.  (One of 131,071 tokens: 16 waves a row 9.4
-    // us, 4 waves 20; 64 of 66 tiles: one 4, four 5.)
+// An item of few may have as many pieces as there are workers; of many, each has few.  (One of 131,071 tokens: 16 waves a row 9.4
+// us, 4 waves 20; 64 of 66 tiles: one 4, four 5.)
+template <int D>
+int win_merge(const SsqWindowParams& p, hipStream_t st) {
+    if (p.form == kWinWide) {
+        hipLaunchKernelGGL(k_window_wide_merge<D>, dim3((unsigned)(p.items * p.a.num_kv_heads * kWinWaves)), dim3(D / 32 * SSQ_WAVE), 0, st, p);
+        return ssq_check_hip(hipGetLastError(), "k_window_wide_merge launch");
+    }
     const int64_t rows = (int64_t)p.a.batch * p.a.num_kv_heads * p.rows;
-    if (p.items <= 8) hipLaunchKernelGGL((k_window_merge<D, 16>), dim3((unsigned)rows), dim3(1024), 0, st, p);
-    else if (p.items < p.n_wg) hipLaunchKernelGGL((k_window_merge<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p);
+    const int pieces = p.workers / p.items;
+    if (pieces >= 32) hipLaunchKernelGGL((k_window_merge<D, 16>), dim3((unsigned)rows), dim3(1024), 0, st, p);
+    else if (pieces > 8) hipLaunchKernelGGL((k_window_merge<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p);
     else hipLaunchKernelGGL((k_window_merge<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
     return ssq_check_hip(hipGetLastError(), "k_window_merge launch");
 }
+template <int D, int BD, int VT, int QP>
+int win_launch(const SsqWindowParams& p, hipStream_t st) {
+    static_assert(WinLds<D>::kTotal <= 160 * 1024 && WideLds<D>::kTotal <= 160 * 1024, "a workgroup's LDS");
+    auto kern = p.form == kWinTeam ? k_window<D, BD, VT, QP, true> : p.form == kWinShares ? k_window<D, BD, VT, QP, false> : k_window_wide<D, BD, VT, QP>;
+    const int lds = p.form == kWinWide ? WideLds<D>::kTotal : WinLds<D>::kTotal;
+    int rc = ssq_allow_lds((const void*)kern, lds, "hipFuncSetAttribute(k_window)");
+    if (rc) return rc;
+    hipLaunchKernelGGL(kern, dim3(p.n_wg * p.a.num_kv_heads), dim3(kWinThreads), lds, st, p);
+    rc = ssq_check_hip(hipGetLastError(), "k_window launch");
+    return rc || p.form == kWinTeam ? rc : win_merge<D>(p, st);
+}
 template <int D, int BD, int VT>
 int win_form(const SsqWindowParams& p, hipStream_t st) {
-    const bool split = p.a.q_dtype == SSQ_F32;
-    if (p.team) return split ? win_launch<D, BD, VT, 2, true>(p, st) : win_launch<D, BD, VT, 1, true>(p, st);
-    return split ? win_launch<D, BD, VT, 2, false>(p, st) : win_launch<D, BD, VT, 1, false>(p, st);
+    return p.a.q_dtype == SSQ_F32 ? win_launch<D, BD, VT, 2>(p, st) : win_launch<D, BD, VT, 1>(p, st);
 }
 template <int D, int VT>
 int win_blocks(const SsqWindowParams& p, hipStream_t st) {

@@ -90,6 +90,28 @@ bool team(const SsqWindowParams& p, int64_t most) {
     return together <= shares;
 }
 
+// Items of 256 rows, whose workgroups decode a tile once for all of them?  They take longer to start and to join, and leave
+// waves idle where rows end.  By what calls took, tenths of a microsecond: head_dim 128 a tile of 64 tokens 24 a wave of 16 rows
+// and 240 a call, a tile of 32 tokens 15 a workgroup of 256 and 370 a call; head_dim 64 16 and 180, a tile of 64 18 and 270.  Measured
+// us by 16 rows and by 256, 32 / 8 heads of 128: 1 sequence of 16,384 and 33 new tokens 50 and 57, 64 69 and 60, 512 338 and 230;
+// 64 of 2,048 29 and 42; 32 times 64 of 8,192 697 and 480; 512 under a window of 1,024 49 and 48, of 4,096 97 and 89, 8 times 229
+// and 149; 16 prompts of 512 468 and 137; 14 / 2 heads of 64: 300 of 4,096 33.1 and 32.7, of 16,384 76 and 62.
+bool wide(const SsqWindowParams& p) {
+    if (p.rows <= kWinWideRows / 2) return false;
+    const bool small = p.a.head_dim == 64;
+    auto tiles = [&](int rows, int tt) {  // of all items of a KV head
+        int64_t seen = p.a.seq_len;
+        if (p.window != INT_MAX) {
+            const int64_t most = (int64_t)p.window + p.sinks + rows / p.G + tt;
+            if (most < seen) seen = most;
+        }
+        return (int64_t)p.a.batch * ((p.rows + rows - 1) / rows) * ((seen + tt - 1) / tt);
+    };
+    const int64_t few = (small ? 180 : 240) + (small ? 16 : 24) * tiles(kWinRows, 64) / (p.n_wg * kWinWaves);
+    const int64_t many = (small ? 270 : 370) + (small ? 18 : 15) * tiles(kWinWideRows, small ? 64 : 32) / p.n_wg;
+    return many <= few;
+}
+
 void make_plan(const ssq_window_args& a, Plan& pl) {
     const ssq_decode_args& d = a.dec;
     SsqWindowParams& p = pl.p;
@@ -104,21 +126,24 @@ void make_plan(const ssq_window_args& a, Plan& pl) {
     p.vs_sh = a.vs_sh;
     p.G = d.num_q_heads / d.num_kv_heads;
     p.rows = p.G * d.q_len;
-    p.rgroups = (p.rows + kWinRows - 1) / kWinRows;
-    p.items = d.batch * p.rgroups;
     const int cus = ssq_device_cus();
     p.n_wg = cus / d.num_kv_heads > 0 ? cus / d.num_kv_heads : 1;
     p.fixed = 2;
     p.least = 2;
-    p.team = team(p, most_tiles(p, d.v_dtype == SSQ_E4M3));
-    if (p.team && p.n_wg > p.items) p.n_wg = p.items;
+    const bool many = wide(p);
+    p.item_rows = many ? kWinWideRows : kWinRows;
+    p.rgroups = (p.rows + p.item_rows - 1) / p.item_rows;
+    p.items = d.batch * p.rgroups;
+    p.form = many ? kWinWide : team(p, most_tiles(p, d.v_dtype == SSQ_E4M3)) ? kWinTeam : kWinShares;
+    if (p.form == kWinTeam && p.n_wg > p.items) p.n_wg = p.items;
+    p.workers = p.form == kWinShares ? p.n_wg * kWinWaves : p.n_wg;
     while ((16 << p.psh) < d.page_size) ++p.psh;
     const int per = d.q_dtype == SSQ_F32 ? 4 : 8;
     p.q_vec = (uintptr_t)d.q % 16 == 0 && d.q_sb % per == 0 && d.q_sh % per == 0 && d.q_sl % per == 0;
     const int size = p.out_dtype == SSQ_F32 ? 16 : 8;
     p.out_vec = (uintptr_t)d.out % size == 0 && d.o_sb % 4 == 0 && d.o_sh % 4 == 0 && d.o_sl % 4 == 0;
-    pl.part_bytes = p.team ? 0 : (size_t)d.num_kv_heads * p.n_wg * kWinWaves * 2 * kWinRows * (d.value_dim + 2) * 4;
-    pl.bytes = p.team ? 0 : pl.part_bytes + (size_t)p.items * 8;
+    pl.part_bytes = p.form == kWinTeam ? 0 : (size_t)d.num_kv_heads * p.workers * 2 * p.item_rows * (d.value_dim + 2) * 4;
+    pl.bytes = p.form == kWinTeam ? 0 : pl.part_bytes + (size_t)p.items * 8;
 }
 
 }  // namespace

@@ -8,7 +8,8 @@
 // rows (which the norm needs anyhow), the codebook, the permutation, slots and positions are all asked for at once,
 // and only the table's and weights' entries after them.  64 sequences' step (8 heads of 128 dims, 256 codewords of dim
 // 4, norm and rotation, values): 9.3 us in a trace (8.2 a call among others, whose launches overlap), of which 1.0 the
-// values, 1.1 the norm, 0.9 the rotation, 2 the scan's vector instructions and about 4 the launch and the first loads.
+// values, 1.1 the norm, 0.9 the rotation, 2 the scan's vector instructions and about 4 the launch and the first loads.  With
+// 8-bit values (k_append_few8, the first workgroups as in ssq_values.h) 7.0 a call; 11.6 as two launches.
 //
 // Many rows: k_append_prep writes the pages' values and the rotated keys side by side, and ssq_encode, which is
 // where the time goes, takes those.  8,192 tokens of the same layer: 19.8 us for 67 MB (3.4 TB/s) and 61.5 us.

@@ -1,7 +1,9 @@
 // Copies of pages (ssq_copy_pages): every pool of a cache (codes, values, scales, passthrough rows) in one launch.
 //
 // A page of a pool is a run of bytes; the work is (pair, pool, piece of 4 KiB), one piece a wave at a time, 16 bytes a
-// lane, four loads in flight.  Bound by bytes for many pages, by the launch for few.
+// lane, four loads in flight.  Bound by bytes for many pages, by the launch for few: 16,384 pages
+// (336 MB read and as many written) 139 us, 4.8 TB/s, where a large copy reaches 5.1 (147 us with stores that stay in the
+// caches); 64 pages 6.4 us a call, 4.0 in the kernel.
 #include "ssq_common.h"
 
 namespace {

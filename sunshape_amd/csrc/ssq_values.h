@@ -11,7 +11,9 @@
 // a page's scale needs no atomic and nothing depends on an order.  A wave looks at kRunChunk positions of a row for starts,
 // for one head of up to 128 dims or two of up to 64 at a time: a lane holds two dims of up to 16 tokens, which become two
 // 16-byte rows of the dim-major page in registers (ValWave::small; ValWave::run serves any run).  Bound by bytes for prompts;
-// for a step by its chain of loads (slots, then values, scale and page together).
+// for a step by its chain of loads (slots, then values, scale and page together).  32,768 tokens of 8 heads of 128 dims, bf16
+// (101 MB): 38 us, 2.7 TB/s (65 with runs through LDS, 61 with runs in registers and value types at run time), a wave's one load, wait and
+// store; 37 times 5 rows of 2 heads of 64, a third of them padding: 8.3 us.
 #pragma once
 
 #include "ssq_common.h"

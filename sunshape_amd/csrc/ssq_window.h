@@ -20,7 +20,11 @@
 // in two parts.
 // Probabilities are 2^(x - m), m kept 14 below the row's running maximum, so that f16 holds them with 11 bits down to 2^-28 of
 // the largest (8-bit and f16 values; with bf16 values they are rounded to bf16, as in the other decode kernels).  A page's scale
-// joins them before the rounding, relative to the largest scale met, which O is kept in units of.
+// joins them before the rounding, relative to the largest scale that the row has met, which its O is kept in units of.
+//
+// Bound by memory for long contexts: 64 sequences of 32,768 tokens (32 / 8 heads of 128, 8-bit values, 2.69 GB) take 424 us,
+// 6.3 TB/s, where a probe that only reads reaches 6.85; by about 10 us before the first tile (loads, lengths, codebook, queries) and 5
+// of the join for short ones: one sequence of 517 tokens 11.5 us.  What k_window_wide takes from many rows is in ssq_window_wide.h.
 #pragma once
 
 #include "ssq_common.h"
@@ -965,8 +969,8 @@ __global__ __launch_bounds__((W > 1 ? W : 4) * SSQ_WAVE) void k_window_merge(con
     if (a.lse && lane == 0) a.lse[((int64_t)b * a.num_q_heads + h) * a.q_len + qi] = l == 0.f ? -INFINITY : (M + log2f(l)) * kWinLn2;
 }
 
-// An item of few may have as many pieces as there are workers; of many, each has few.  (One of 131,071 tokens: 16 waves a row 9.4
-// us, 4 waves 20; 64 of 66 tiles: one 4, four 5.)
+// An item of few may have as many pieces as there are workers; of many, each has few.  (One of 131,071 tokens: 16 waves a row 5.9
+// us; when pieces were read eight at a time, some twice, 9.4, and 4 waves 20; 64 of 66 tiles: one 4, four 5.)
 template <int D>
 int win_merge(const SsqWindowParams& p, hipStream_t st) {
     if (p.form == kWinWide) {

@@ -93,9 +93,9 @@ bool team(const SsqWindowParams& p, int64_t most) {
 // Items of 256 rows, whose workgroups decode a tile once for all of them?  They take longer to start and to join, and leave
 // waves idle where rows end.  By what calls took, tenths of a microsecond: head_dim 128 a tile of 64 tokens 24 a wave of 16 rows
 // and 240 a call, a tile of 32 tokens 15 a workgroup of 256 and 370 a call; head_dim 64 16 and 180, a tile of 64 18 and 270.  Measured
-// us by 16 rows and by 256, 32 / 8 heads of 128: 1 sequence of 16,384 and 33 new tokens 50 and 57, 64 69 and 60, 512 338 and 230;
+// us by 16 rows and by 256, 32 / 8 heads of 128: 1 sequence of 16,384 and 33 new tokens 50 and 57, 64 69 and 60, 512 338 and 235;
 // 64 of 2,048 29 and 42; 32 times 64 of 8,192 697 and 480; 512 under a window of 1,024 49 and 48, of 4,096 97 and 89, 8 times 229
-// and 149; 16 prompts of 512 468 and 137; 14 / 2 heads of 64: 300 of 4,096 33.1 and 32.7, of 16,384 76 and 62.
+// and 149; 16 prompts of 512 468 and 130; 14 / 2 heads of 64: 300 of 4,096 33.1 and 32.7, of 16,384 76 and 62.
 bool wide(const SsqWindowParams& p) {
     if (p.rows <= kWinWideRows / 2) return false;
     const bool small = p.a.head_dim == 64;
@@ -128,9 +128,11 @@ void make_plan(const ssq_window_args& a, Plan& pl) {
     p.rows = p.G * d.q_len;
     const int cus = ssq_device_cus();
     p.n_wg = cus / d.num_kv_heads > 0 ? cus / d.num_kv_heads : 1;
-    p.fixed = 2;
     p.least = 2;
     const bool many = wide(p);
+    // (An item of 256 rows costs 5 to 8 tiles of its own.  With 5 and 8, in turn: 16 prompts of 512 tokens 130 and 146 us, one of 8,192
+    // 900 and 860, 4 of 2,048 287 and 275, 512 tokens of 16,384 235 both.)
+    p.fixed = many ? 5 : 2;
     p.item_rows = many ? kWinWideRows : kWinRows;
     p.rgroups = (p.rows + p.item_rows - 1) / p.item_rows;
     p.items = d.batch * p.rgroups;

@@ -19,7 +19,8 @@
 // a power of two of the row's own: exact for 16-bit ones (elements below 2^-29 of the row's largest apart), fp32 ones
 // in two parts.
 // Probabilities are 2^(x - m), m kept 14 below the row's running maximum, so that f16 holds them with 11 bits down to 2^-28 of
-// the largest (8-bit and f16 values; with bf16 values they are rounded to bf16, as in the other decode kernels).  A page's scale
+// the largest (8-bit and f16 values; with bf16 values they are rounded to bf16, as in the other decode kernels, and kept small
+// enough that their sums of such values are finite: kWinTop).  What is joined is averages with their sums, not sums.  A page's scale
 // joins them before the rounding, relative to the largest scale that the row has met, which its O is kept in units of.
 //
 // Bound by memory for long contexts: 64 sequences of 32,768 tokens (32 / 8 heads of 128, 8-bit values, 2.69 GB) take 424 us,
@@ -105,7 +106,15 @@ typedef unsigned int w2u __attribute__((ext_vector_type(2)));
 
 constexpr float kWinLog2e = 1.4426950408889634f, kWinLn2 = 0.6931471805599453f;
 constexpr float kWinNone = -3.0e38f;  // m of a row that has met nothing
-constexpr float kWinTop = 14.f, kWinOver = 15.5f;  // log2 of the largest probability when m moves, and of what moves it
+// log2 of the largest probability when m moves, and of what moves it.  f16 holds the most below 2^15.5.  bf16 holds as many bits of any
+// size, but its values reach 2^128: what a row's probabilities sum to stays below 1 there, so that O, which is divided by the sum
+// at the end, never passes its values (a lane's sum is at most kWinMass when a tile begins, a row's four lanes' 2^-2, and a tile adds 64 * 2^-6.5 at most;
+// past kWinMass m moves 4 up).
+template <int VT>
+constexpr float kWinTop = VT == SSQ_BF16 ? -8.f : 14.f;
+template <int VT>
+constexpr float kWinOver = VT == SSQ_BF16 ? -6.5f : 15.5f;
+constexpr float kWinMass = 0.0625f;
 constexpr float kWinScale = 7.888609052210118e-31f;  // 2^-100, the smallest unit of O
 
 __device__ __forceinline__ w4f win_mfma(const uint4& a, const uint4& b, w4f c) {
@@ -164,6 +173,12 @@ __device__ __forceinline__ void win_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// whether a lane's largest score, or its sum, takes m up
+template <int VT>
+__device__ __forceinline__ bool win_over(float top, float m, float l) {
+    if constexpr (VT == SSQ_BF16) return (top > m + kWinOver<VT>) | (l > kWinMass);
+    else return top > m + kWinOver<VT>;
+}
 // a group's value over the four lane groups of a column
 __device__ __forceinline__ float win_max4(float v) {
     v = fmaxf(v, __shfl_xor(v, 16));
@@ -742,8 +757,9 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
             for (int e = 1; e < CH; ++e) top = fmaxf(top, s[e >> 2][e & 3]);
             top *= u.fac;
-            if (__builtin_amdgcn_ballot_w64(top > m + kWinOver) != 0) {
-                const float mn = fmaxf(m, win_max4(top) - kWinTop);
+            if (__builtin_amdgcn_ballot_w64(win_over<VT>(top, m, l)) != 0) {
+                float mn = fmaxf(m, win_max4(top) - kWinTop<VT>);
+                if (VT == SSQ_BF16 && win_max4(l) > kWinMass) mn = fmaxf(mn, m + 4.f);
                 const float f = __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
                 l *= f;
@@ -803,6 +819,11 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
             }
         }
         l = win_sum4(l);
+        // What the row's values average to here: everything that is joined or stored is a finite average of finite values, whatever
+        // their size (O in its units times the unit need not be).
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = l == 0.f ? w4f{} : W::kV8 ? o[dt] * inv * unit : o[dt] * inv;
 
         p = win_args();
         if constexpr (TEAM) {
@@ -812,10 +833,6 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                 mls[(kWinWaves + wave) * kWinRows + lane] = l;
             }
             __syncthreads();
-            float mt = kWinNone;
-#pragma unroll
-            for (int w = 0; w < kWinWaves; ++w) mt = fmaxf(mt, mls[w * kWinRows + u.col]);
-            const float f = __builtin_amdgcn_exp2f(m - mt) * unit;
             float* join = reinterpret_cast<float*>(smem + L::kBook);
             constexpr int kRow = L::kJoinRow;
 #pragma unroll 1
@@ -823,24 +840,27 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                 if ((u.col & ~3) == r0) {
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        const w4f z = o[dt] * f;
+                        const w4f z = o[dt];
                         *reinterpret_cast<float4*>(join + (wave * 4 + (u.col & 3)) * kRow + 16 * dt + 4 * u.grp) = make_float4(z[0], z[1], z[2], z[3]);
                     }
                 }
                 __syncthreads();
                 const int r = r0 + tid / D, dv = tid % D;
                 if (tid < 4 * D && r < nr) {
-                    float mr = kWinNone, lt = 0.f, ot = 0.f;
+                    float mr = kWinNone, lt = 0.f, ot = 0.f, lw[kWinWaves];
 #pragma unroll
                     for (int w = 0; w < kWinWaves; ++w) mr = fmaxf(mr, mls[w * kWinRows + r]);
 #pragma unroll
                     for (int w = 0; w < kWinWaves; ++w) {
-                        lt += mls[(kWinWaves + w) * kWinRows + r] * __builtin_amdgcn_exp2f(mls[w * kWinRows + r] - mr);
-                        ot += join[(w * 4 + r - r0) * kRow + dv];
+                        lw[w] = mls[(kWinWaves + w) * kWinRows + r] * __builtin_amdgcn_exp2f(mls[w * kWinRows + r] - mr);
+                        lt += lw[w];
                     }
+                    const float part = lt == 0.f ? 0.f : 1.f / lt;
+#pragma unroll
+                    for (int w = 0; w < kWinWaves; ++w) ot += join[(w * 4 + r - r0) * kRow + dv] * (lw[w] * part);
                     const int row = row0 + r, qi = row / p->G, h = kv * p->G + row - qi * p->G;
                     ssq_store_elem(p->a.out, p->out_dtype, (int64_t)b * p->a.o_sb + (int64_t)h * p->a.o_sh + (int64_t)qi * p->a.o_sl + dv,
-                                   lt == 0.f ? 0.f : ot / lt);
+                                   ot);
                     if (p->a.lse && dv == 0)
                         p->a.lse[((int64_t)b * p->a.num_q_heads + h) * p->a.q_len + qi] = lt == 0.f ? -INFINITY : (mr + log2f(lt)) * kWinLn2;
                 }
@@ -849,12 +869,11 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
         } else if (u.col < nr) {
             if (slot < 0) {
                 const int row = row0 + u.col, qi = row / p->G, h = kv * p->G + row - qi * p->G;
-                const float f = l == 0.f ? 0.f : unit / l;
                 const int64_t at = (int64_t)b * p->a.o_sb + (int64_t)h * p->a.o_sh + (int64_t)qi * p->a.o_sl + 4 * u.grp;
                 const int dtype = p->out_dtype;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    const w4f z = l == 0.f ? w4f{} : o[dt] * f;
+                    const w4f z = o[dt];
                     if (p->out_vec) win_store4(p->a.out, dtype, at + 16 * dt, z);
                     else
 #pragma unroll
@@ -866,7 +885,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                 float* dst = p->part + ((int64_t)(kv * p->workers + worker) * 2 + slot) * (kWinRows * (D + 2));
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    const w4f z = o[dt] * unit;
+                    const w4f z = o[dt];
                     *reinterpret_cast<float4*>(dst + u.col * D + 16 * dt + 4 * u.grp) = make_float4(z[0], z[1], z[2], z[3]);
                 }
                 if (u.grp == 0) {
@@ -877,6 +896,33 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
         }
         more = next();
         if (more) load();
+    }
+}
+
+// n of N pieces (m, l, average) joined to (M, L, average o): averages weighted by their share of the sum, which no size of values
+// takes past them.
+template <int N, int E, class T>
+__device__ __forceinline__ void win_join(float& M, float& L, T (&o)[E], const float (&m)[N], const float (&l)[N], const T (&op)[N][E], int n) {
+    float mt = M, w[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) mt = j < n ? fmaxf(mt, m[j]) : mt;
+    const float w0 = L * __builtin_amdgcn_exp2f(M - mt);
+    float sum = w0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        w[j] = j < n ? l[j] * __builtin_amdgcn_exp2f(m[j] - mt) : 0.f;
+        sum += w[j];
+    }
+    M = mt;
+    L = sum;
+    const float part = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = o[e] * (w0 * part);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        if (j >= n) continue;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += op[j][e] * (w[j] * part);
     }
 }
 
@@ -920,22 +966,7 @@ __global__ __launch_bounds__((W > 1 ? W : 4) * SSQ_WAVE) void k_window_merge(con
 #pragma unroll
             for (int e = 0; e < E; ++e) op[j][e] = src[r * D + lane * E + e];
         }
-        float mt = M;
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) mt = fmaxf(mt, m[j]);
-        const float f0 = __builtin_amdgcn_exp2f(M - mt);
-        M = mt;
-        l *= f0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] *= f0;
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            if (i0 + j >= pieces) continue;
-            const float f = __builtin_amdgcn_exp2f(m[j] - M);
-            l += lp[j] * f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += op[j][e] * f;
-        }
+        win_join<kAhead, E>(M, l, o, m, lp, op, pieces - i0);
     }
     if constexpr (WIDE) {
         if (lane == 0) {
@@ -946,26 +977,25 @@ __global__ __launch_bounds__((W > 1 ? W : 4) * SSQ_WAVE) void k_window_merge(con
         for (int e = 0; e < E; ++e) mo[wave][lane * E + e] = o[e];
         __syncthreads();
         if (wave) return;
-        M = kWinNone;
+        float m[W], lp[W], op[W][E];
 #pragma unroll
-        for (int w = 0; w < W; ++w) M = fmaxf(M, ml[w][0]);
+        for (int w = 0; w < W; ++w) {
+            m[w] = ml[w][0];
+            lp[w] = ml[w][1];
+#pragma unroll
+            for (int e = 0; e < E; ++e) op[w][e] = mo[w][lane * E + e];
+        }
+        M = kWinNone;
         l = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w * kAhead >= pieces) continue;  // had none
-            const float f = __builtin_amdgcn_exp2f(ml[w][0] - M);
-            l += ml[w][1] * f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += mo[w][lane * E + e] * f;
-        }
+        win_join<W, E>(M, l, o, m, lp, op, (pieces + kAhead - 1) / kAhead);  // (the waves behind had none)
     }
     const int qi = row / p.G, h = kv * p.G + row - qi * p.G;
 #pragma unroll
     for (int e = 0; e < E; ++e)
         ssq_store_elem(a.out, p.out_dtype, (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)qi * a.o_sl + lane * E + e,
-                       l == 0.f ? 0.f : o[e] / l);
+                       o[e]);
     if (a.lse && lane == 0) a.lse[((int64_t)b * a.num_q_heads + h) * a.q_len + qi] = l == 0.f ? -INFINITY : (M + log2f(l)) * kWinLn2;
 }
 

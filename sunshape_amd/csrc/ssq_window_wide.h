@@ -1,7 +1,7 @@
 // ssq_decode_window for many query rows of a sequence and KV head (a prompt's chunk): k_window_wide.  Included by ssq_window.h.
 //
-// The formulas and the numbers' forms are k_window's: S^T = K Q^T and O^T = V^T P^T, K in two f16 parts, probabilities below
-// 2^15.5 with the page's scale in them.  What differs is who decodes.  Sixteen rows at a time, a token's codewords are gathered
+// The formulas and the numbers' forms are k_window's: S^T = K Q^T and O^T = V^T P^T, K in two f16 parts, probabilities in 16 bits
+// with the page's scale in them.  What differs is who decodes.  Sixteen rows at a time, a token's codewords are gathered
 // from the codebook once per 16 rows: a chunk of 512 tokens (4 heads a KV head) spent 44 us of 87 in the LDS, two thirds of
 // it bank conflicts, and 46 in VALU instructions, with 21 us of matrix products.  Here eight waves of 32 rows share a tile of
 // 4096 / D tokens: each thread gathers 8 dims of a token and takes 8 tokens of a value dim, converted, to LDS rows that
@@ -464,8 +464,9 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
                     for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
                 top *= fac;
-                if (__builtin_amdgcn_ballot_w64(top > m + kWinOver) != 0) {
-                    const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)) - kWinTop);
+                if (__builtin_amdgcn_ballot_w64(win_over<VT>(top, m, l)) != 0) {
+                    float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)) - kWinTop<VT>);
+                    if (VT == SSQ_BF16 && fmaxf(l, __shfl_xor(l, 32)) > kWinMass) mn = fmaxf(mn, m + 4.f);
                     const float f = __builtin_amdgcn_exp2f(m - mn);
                     m = mn;
                     l *= f;
@@ -501,12 +502,15 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
             }
         }
         l += __shfl_xor(l, 32);
+        // what the row's values average to here, as in k_window
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = l == 0.f ? w16f{} : kV8 ? o[dt] * inv * unit : o[dt] * inv;
 
         p = win_args();
         if (WR * wave + col < nr) {
             if (slot < 0) {
                 const int qi = row / p->G, h = kv * p->G + row - qi * p->G;
-                const float f = l == 0.f ? 0.f : unit / l;
                 const int64_t at = (int64_t)b * p->a.o_sb + (int64_t)h * p->a.o_sh + (int64_t)qi * p->a.o_sl + 4 * grp;
                 const int dtype = p->out_dtype;
 #pragma unroll
@@ -515,7 +519,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                     for (int a = 0; a < 4; ++a) {
                         w4f z;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) z[e] = l == 0.f ? 0.f : o[dt][4 * a + e] * f;
+                        for (int e = 0; e < 4; ++e) z[e] = o[dt][4 * a + e];
                         if (p->out_vec) win_store4(p->a.out, dtype, at + 32 * dt + 8 * a, z);
                         else
 #pragma unroll
@@ -531,7 +535,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
                     for (int a = 0; a < 4; ++a)  // as the registers lie: a store is 1 KiB
                         *reinterpret_cast<float4*>(dst + ((wave * DT + dt) * 4 + a) * 256 + lane * 4) =
-                            make_float4(o[dt][4 * a] * unit, o[dt][4 * a + 1] * unit, o[dt][4 * a + 2] * unit, o[dt][4 * a + 3] * unit);
+                            make_float4(o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]);
                 if (grp == 0) {
                     dst[ROWS * D + r] = m;
                     dst[ROWS * D + ROWS + r] = l;
@@ -572,31 +576,14 @@ __global__ __launch_bounds__(D / 32 * SSQ_WAVE) void k_window_wide_merge(const S
 #pragma unroll
             for (int k = 0; k < 4; ++k) op[j][k] = *reinterpret_cast<const w4f*>(src + ((w * DT + dt) * 4 + k) * 256 + lane * 4);
         }
-        float mt = M;
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) mt = fmaxf(mt, m[j]);
-        const float f0 = __builtin_amdgcn_exp2f(M - mt);
-        M = mt;
-        l *= f0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] *= f0;
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            if (i0 + j >= pieces) continue;
-            const float f = __builtin_amdgcn_exp2f(m[j] - M);
-            l += lp[j] * f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] += op[j][k] * f;
-        }
+        win_join<kAhead, 4>(M, l, o, m, lp, op, pieces - i0);
     }
     if (row >= p.rows) return;
     const int qi = row / p.G, h = kv * p.G + row - qi * p.G;
     const int64_t at = (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)qi * a.o_sl + 32 * dt + 4 * grp;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        w4f z;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] = l == 0.f ? 0.f : o[k][e] / l;
+        const w4f z = o[k];
         if (p.out_vec) win_store4(a.out, p.out_dtype, at + 8 * k, z);
         else
 #pragma unroll

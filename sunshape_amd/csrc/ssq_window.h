@@ -21,7 +21,9 @@
 // Probabilities are 2^(x - m), m kept 14 below the row's running maximum, so that f16 holds them with 11 bits down to 2^-28 of
 // the largest (8-bit and f16 values; with bf16 values they are rounded to bf16, as in the other decode kernels, and kept small
 // enough that their sums of such values are finite: kWinTop).  What is joined is averages with their sums, not sums.  A page's scale
-// joins them before the rounding, relative to the largest scale that the row has met, which its O is kept in units of.
+// joins them before the rounding, relative to the largest scale that the row has met, which its O is kept in units of: f16 then has
+// 11 bits down to 2^-20 of the row's largest probability at the least (and nothing below 2^-31), as a tile with a page whose scale is less than
+// 2^-8 of that takes its products in 32 bits (kWinFar).
 //
 // Bound by memory for long contexts: 64 sequences of 32,768 tokens (32 / 8 heads of 128, 8-bit values, 2.69 GB) take 424 us,
 // 6.3 TB/s, where a probe that only reads reaches 6.85; by about 10 us before the first tile (loads, lengths, codebook, queries) and 5
@@ -116,6 +118,7 @@ template <int VT>
 constexpr float kWinOver = VT == SSQ_BF16 ? -6.5f : 15.5f;
 constexpr float kWinMass = 0.0625f;
 constexpr float kWinScale = 7.888609052210118e-31f;  // 2^-100, the smallest unit of O
+constexpr float kWinFar = 0.00390625f;  // 2^-8: of the unit, what a page's scale has to be for its probabilities to go to f16 with it
 
 __device__ __forceinline__ w4f win_mfma(const uint4& a, const uint4& b, w4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(w8h, a), __builtin_bit_cast(w8h, b), c, 0, 0, 0);
@@ -173,6 +176,14 @@ __device__ __forceinline__ void win_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// 32-bit products, a lane's value of its dim and its row's probability each, of a token a lane group: what a page far below the
+// unit takes, whose f16 would have bits to lose (16 of these for one of 16 bits, and rare)
+__device__ __forceinline__ w4f win_mfma_32(float a, float b, w4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// four e4m3 values
+__device__ __forceinline__ w4f win_e4m3_32(uint32_t w) {
+    return w4f{__builtin_amdgcn_cvt_f32_fp8((int)w, 0), __builtin_amdgcn_cvt_f32_fp8((int)w, 1), __builtin_amdgcn_cvt_f32_fp8((int)w, 2),
+               __builtin_amdgcn_cvt_f32_fp8((int)w, 3)};
+}
 // whether a lane's largest score, or its sum, takes m up
 template <int VT>
 __device__ __forceinline__ bool win_over(float top, float m, float l) {
@@ -492,16 +503,17 @@ struct WinRun {
     __device__ __forceinline__ static w4u spread(uint32_t bits) {
         w4u r;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if constexpr (kV8) {
-                const uint32_t b = (bits >> (4 * k)) & 0xFu;
-                r[k] = ((b * 0x00204081u) & 0x01010101u) * 0xFFu;  // a bit to a byte each
-            } else {
-                const uint32_t b = bits >> (2 * k);
-                r[k] = (b & 1u ? 0xFFFFu : 0u) | (b & 2u ? 0xFFFF0000u : 0u);
-            }
-        }
+        for (int k = 0; k < 4; ++k) r[k] = spread_word(bits, k);
         return r;
+    }
+    __device__ __forceinline__ static uint32_t spread_word(uint32_t bits, int k) {  // its word k
+        if constexpr (kV8) {
+            const uint32_t b = (bits >> (4 * k)) & 0xFu;
+            return ((b * 0x00204081u) & 0x01010101u) * 0xFFu;  // a bit to a byte each
+        } else {
+            const uint32_t b = bits >> (2 * k);
+            return (b & 1u ? 0xFFFFu : 0u) | (b & 2u ? 0xFFFF0000u : 0u);
+        }
     }
     // the top bit of each value that is infinite or NaN
     __device__ __forceinline__ static uint32_t wild(uint32_t w) {
@@ -766,7 +778,8 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
             }
-            float by = 1.f;  // this group's page scale, in units of O
+            float by = 1.f;    // this group's page scale, in units of O
+            bool far = false;  // a page's is too far below them
             if constexpr (W::kV8) {
                 // (positive floats compare as their bits; rows have units of their own where they do not see the same pages)
                 const uint32_t bits = __float_as_uint(val.scale);
@@ -779,15 +792,42 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                     for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
                 }
                 by = val.scale * inv_unit;
+                far = __builtin_amdgcn_ballot_w64((by < kWinFar) & (val.scale > 0.f)) != 0;
             }
-            uint32_t pw[CH / 2];
 #pragma unroll
             for (int e = 0; e < CH; e += 2) {
                 const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3], u.fac, -m));
                 const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][(e & 3) + 1], u.fac, -m));
                 l += x0 + x1;
-                pw[e / 2] = W::kV8 ? win_pack_p<VT>(x0 * by, x1 * by) : win_pack_p<VT>(x0, x1);
+                s[e >> 2][e & 3] = W::kV8 ? x0 * by : x0;
+                s[e >> 2][(e & 3) + 1] = W::kV8 ? x1 * by : x1;
             }
+            if constexpr (W::kV8) {
+                if (far) {  // in 32 bits; rows of one position at a time if `apart`, as below, else all
+                    for (int at = apart ? u.t.p_lo : u.t.p_hi; at <= u.t.p_hi; ++at) {
+                        const uint32_t on = apart ? u.sees(at, at, tok) : ~0u;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            w4f z = o[dt];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const w4f y = win_e4m3_32(val.v[dt][k] & W::spread_word(on, k));
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) z = win_mfma_32(y[e], s[k][e], z);
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[dt][e] = !apart || u.pos == at ? z[e] : o[dt][e];
+                        }
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) val.v[dt] = w4u{};
+                    apart = false;
+                }
+            }
+            uint32_t pw[CH / 2];
+#pragma unroll
+            for (int e = 0; e < CH; e += 2) pw[e / 2] = win_pack_p<VT>(s[e >> 2][e & 3], s[e >> 2][(e & 3) + 1]);
             if (apart) {
                 // The rows of one position at a time, the values that they do not see as 0; the products below then add nothing.
                 for (int at = u.t.p_lo; at <= u.t.p_hi; ++at) {

@@ -29,6 +29,7 @@ __device__ __forceinline__ w16f wide_mfma(const uint4& a, const uint4& b, w16f c
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(w8h, a), __builtin_bit_cast(w8h, b), c, 0, 0, 0);
 }
+__device__ __forceinline__ w16f wide_mfma_32(float a, float b, w16f c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 // a barrier for LDS alone: global loads stay in flight
 __device__ __forceinline__ void wide_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -386,8 +387,23 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
         uint4 pw[NT];
 #pragma unroll
         for (int c = 0; c < NT; ++c) pw[c] = uint4{};
+        bool far = false;  // 8-bit values: tile i - 1 has a page far below the unit; its probabilities are in s, in 32 bits, and 0 in pw
         for (int i = i0; i <= i1; ++i) {
             if (!late && i > i0) step(i);
+            if constexpr (kV8) {
+                if (far) {
+#pragma unroll
+                    for (int c = 0; c < NT; ++c)
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(vget + 32 * dt * L::kVRow + 32 * c);
+                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) o[dt] = wide_mfma_32(win_h(w[j / 2], j & 1), s[c / 2][8 * (c % 2) + j], o[dt]);
+                        }
+                }
+                far = false;
+            }
             gather();  // the next tile's (past the last: some tile's)
             const bool none = hidden(i);
             if (!none) {
@@ -490,14 +506,23 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                 for (int c = 0; c < NT; ++c) {
                     uint32_t w[4];
                     const float by = kV8 ? sc[c] * inv_unit : 1.f;
+                    if constexpr (kV8) far |= __builtin_amdgcn_ballot_w64((by < kWinFar) & (sc[c] > 0.f)) != 0;
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
-                        const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j], fac, -m));
-                        const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j + 1], fac, -m));
+                        float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j], fac, -m));
+                        float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c / 2][8 * (c % 2) + j + 1], fac, -m));
                         l += x0 + x1;
-                        w[j / 2] = kV8 ? win_pack_p<VT>(x0 * by, x1 * by) : win_pack_p<VT>(x0, x1);
+                        if constexpr (kV8) {
+                            s[c / 2][8 * (c % 2) + j] = x0 *= by;
+                            s[c / 2][8 * (c % 2) + j + 1] = x1 *= by;
+                        }
+                        w[j / 2] = win_pack_p<VT>(x0, x1);
                     }
                     pw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                if (far) {
+#pragma unroll
+                    for (int c = 0; c < NT; ++c) pw[c] = uint4{};
                 }
             }
         }

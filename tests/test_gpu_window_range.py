@@ -75,3 +75,85 @@ def test_small_values(form, vt):
     # (bf16 values: the largest weight is kept at 2^-8 until the sum is 2^-1, then taken 2^4 down)
     floor = pr["block_table"].shape[1] * 16 * 2.0 ** -149 * 2.0 ** 12 * up
     within(pr, out.double() * up, lse, big, window_bounds(pr, *big, F32), floor)
+
+
+def quiet(pr, seen_by_weight, nats=100.0):
+    """Codeword 255 of block 0 gives a token `nats` less than others': the codes of tokens in `seen_by_weight` (page, place) pairs, and
+    of no others.  Returns the problem with that codeword at 0 too, which the bounds' logits are of."""
+    bd, D = pr["cent"].shape[-1], pr["q"].shape[-1]
+    at = 0.5  # queries of block 0's dims
+    pr["q"][..., pr["perm"][:bd]] = at
+    pr["cent"][0, 255] = -nats / (pr["scale"] * bd * at)
+    c0 = pr["codes"][..., 0]
+    c0[c0 == 255] = 254
+    for page, place in seen_by_weight:
+        pr["codes"][page, :, place, 0] = 255
+    calm = dict(pr, cent=pr["cent"].clone())
+    calm["cent"][0, 255] = 0.0
+    return calm
+
+
+def last_page(pr, b, back=0):
+    return int(pr["block_table"][b, (int(pr["seq_lens"][b]) - 1) // 16 - back])
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("r", [6, 10, 20, 28, 60])
+@pytest.mark.parametrize("how", ["weightless", "zero"])
+def test_a_page_of_a_large_scale_that_counts_for_nothing(form, r, how):
+    """A page 2^r above the others whose tokens have a weight of e^-100, or values of 0: the others are what comes out, to their own
+    bits.  The rounding of weights to f16 counts from the row's largest weight: half of f16's smallest step, in units in which that weight is at
+    least 2^14 times 2^-8, is 2^-31 of it, times 448 and the scale, a token."""
+    log(f"range: a page 2^{r} up, {how}, {form}")
+    pr = of_form(form, 63, spread=0)
+    B = pr["q"].shape[0]
+    far = sorted({last_page(pr, b, back) for b in range(B) if int(pr["seq_lens"][b]) > 200 for back in (0, 5)})
+    pr["v_scale"][far] = 2.0 ** r
+    if how == "zero":
+        pr["v"].view(torch.uint8)[far] = 0
+    calm = quiet(pr, [(pg, t) for pg in far for t in range(16)] if how == "weightless" else [])
+    ref, mag = window64(pr), window64(calm)[2]
+    floor = pr["block_table"].shape[1] * 16 * 2.0 ** -31 * 448
+    for out_dtype in (BF, F32):
+        out, lse = call(on_gpu(pr), out_dtype=out_dtype)
+        within(pr, out, lse, ref, window_bounds(pr, ref[0], ref[1], mag, ref[3], out_dtype), floor)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_scales_that_lie_anywhere(form):
+    """Page scales of 2^-90 to 2^90, positive ones that are no powers of two: a row of them is held to the bits of its largest terms."""
+    log(f"range: scales of 2^-90 to 2^90, {form}")
+    pr = of_form(form, 64, spread=90)
+    pr["v_scale"] = pr["v_scale"] * (1 + torch.rand(pr["v_scale"].shape, generator=torch.Generator().manual_seed(1)))
+    ref = window64(pr)
+    out, lse = call(on_gpu(pr), out_dtype=F32)
+    within(pr, out, lse, ref, window_bounds(pr, *ref, F32))
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_scales_far_apart_beside_windows_and_nan(form):
+    """The newest pages, which the older rows of a tile do not see, 2^40 above the others, and NaN values that some rows see."""
+    log(f"range: scales, windows and NaN, {form}")
+    pr = of_form(form, 65, spread=0, **({} if form == "wide" else {"lens": [385, 369, 193] if form == "together" else [19985, 7777]}))
+    window = {"together": 100, "shares": 9000, "wide": 1750}[form]
+    B, Lq = pr["q"].shape[0], pr["q"].shape[2]
+    for b in range(B):
+        pr["v_scale"][last_page(pr, b)] = 2.0 ** 40
+    pr["v_scale"][last_page(pr, 0, 3)] = 2.0 ** 20
+    bad = dict(pr, v=pr["v"].clone())
+    n = int(pr["seq_lens"][0])
+    toks = {0: n - 1, 1: n - 2, 5: n - Lq - window + 1, 7: n - 60}  # by dim; the third is seen by the first row alone
+    for dim, tok in toks.items():
+        bad["v"].view(torch.uint8)[int(pr["block_table"][0, tok // 16]), :, dim, tok % 16] = 0x7F
+    ref = window64(pr, window, 3)
+    ob, lb = window_bounds(pr, *ref, F32)
+    out, lse = (t.cpu().double() for t in call(on_gpu(bad), window, 3, out_dtype=F32))
+    for i in range(Lq):
+        p = n - Lq + i
+        for dim, tok in toks.items():
+            if p - window < tok <= p:
+                assert torch.isnan(out[0, :, i, dim]).all(), (i, dim)
+                out[0, :, i, dim] = ref[0][0, :, i, dim]
+    assert torch.isfinite(out).all()
+    seen = ref[1] != -torch.inf
+    assert (((out - ref[0]).abs() / ob)[seen] <= 1).all() and (((lse - ref[1]).abs() / lb)[seen] <= 1).all()

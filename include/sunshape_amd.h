@@ -376,11 +376,13 @@ int ssq_append8(const ssq_append8_args* a, void* workspace, size_t workspace_byt
  * counterpart in the reference).  dec: SSQ_PAGED with v, no mask, no scores; the q_len rows of sequence b are its newest
  * tokens, appended already: row i stands at p = seq_lens[b] - q_len + i and sees token j iff j <= p and (window == 0 or
  * j > p - window or j < sinks).  A row that sees nothing (p < 0) gives 0 and lse -inf; one whose query holds a
- * NaN or an infinity gives NaN.  Pages that no row sees may be anything, and a table's entry outside [0, num_pages)
- * is taken into it.  dec.v_dtype SSQ_E4M3: 8-bit values times v_scale[page*vs_sb + kv*vs_sh] (positive; of the pages that a row
- * sees within 2^120 of each other); SSQ_BF16 or SSQ_F16: v_scale NULL.  Probabilities are rounded to 11 bits down to 2^-20 (8-bit
- * values, whatever their scales) or 2^-28 (f16) of the row's largest, and to fewer below; to 8 bits with bf16 values.  out is of out_dtype.  Serves byte codes of dims 2, 4 or 8 (at most 256
- * codewords, no passthrough blocks), head_dim 64 or 128, value_dim the same, page sizes of 16 to 256.
+ * NaN or an infinity gives NaN; an infinite or NaN value that it sees makes that dim infinite or NaN, whatever it weighs.  Pages
+ * that no row sees may be anything, and a table's entry outside [0, num_pages) is taken into it.  dec.v_dtype SSQ_E4M3:
+ * 8-bit values times v_scale[page*vs_sb + kv*vs_sh], positive (a row loses those of scales below 2^-120 of the largest that it
+ * sees); SSQ_BF16 or SSQ_F16: v_scale NULL.  Probabilities are rounded to 11 bits down to 2^-20 (8-bit values, whatever their
+ * scales) or 2^-28 (f16) of the row's largest, and to fewer below; to 8 bits with bf16 values.  out is of out_dtype.  Serves
+ * byte codes of dims 2, 4 or 8 (at most 256 codewords, no passthrough blocks), head_dim 64 or 128, value_dim the same, page
+ * sizes of 16 to 256.
  */
 typedef struct ssq_window_args {
     uint32_t struct_size;

@@ -184,6 +184,9 @@ __device__ __forceinline__ w4f win_e4m3_32(uint32_t w) {
     return w4f{__builtin_amdgcn_cvt_f32_fp8((int)w, 0), __builtin_amdgcn_cvt_f32_fp8((int)w, 1), __builtin_amdgcn_cvt_f32_fp8((int)w, 2),
                __builtin_amdgcn_cvt_f32_fp8((int)w, 3)};
 }
+// a part w of an average, or infinite as it is (its weight is above 0, whatever 32 bits make of it)
+__device__ __forceinline__ float win_part(float z, float w) { return fabsf(z) == INFINITY ? z : z * w; }
+__device__ __forceinline__ w4f win_part(w4f z, float w) { return w4f{win_part(z[0], w), win_part(z[1], w), win_part(z[2], w), win_part(z[3], w)}; }
 // whether a lane's largest score, or its sum, takes m up
 template <int VT>
 __device__ __forceinline__ bool win_over(float top, float m, float l) {
@@ -519,6 +522,55 @@ struct WinRun {
     __device__ __forceinline__ static uint32_t wild(uint32_t w) {
         if constexpr (kV8) return (w & 0x7F7F7F7Fu) + 0x01010101u;
         else return (w & 0x7FFF7FFFu) + (VT == SSQ_BF16 ? 0x00800080u : 0x04000400u);
+    }
+    // Infinite and NaN values (16 bits) that this column's row sees in tiles i0, i0 + step, .. below i1, put into its O: a dim is
+    // infinite, or NaN, whatever the probabilities.  Whether a row sees one of a kind is a product of ones.
+    __device__ __forceinline__ void put_wild(int i0, int i1, int step, w4f (&o)[DT]) const {
+        constexpr uint32_t one = VT == SSQ_BF16 ? 0x3F80u : 0x3C00u, infinity = VT == SSQ_BF16 ? 0x7F80u : 0x7C00u;
+        uint32_t nan = 0, inf = 0, neg = 0;  // a bit a (dt, e)
+        for (int i = i0; i < i1; i += step) {
+            const uint8_t* row = val_row(place(i, grp));
+            const w4u on = spread(sees(pos, pos, TT * tile_of(i) + CH * grp)) & (one * 0x10001u);
+            const uint4 seen = make_uint4(on.x, on.y, on.z, on.w);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const w4u v = load_val(row, dt);
+                uint32_t kind[3][4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t a = v[k] & 0xFFFFu, b = v[k] >> 16;
+                    kind[0][k] = ((a & 0x7FFFu) > infinity ? one : 0u) | ((b & 0x7FFFu) > infinity ? one << 16 : 0u);
+                    kind[1][k] = (a == infinity ? one : 0u) | (b == infinity ? one << 16 : 0u);
+                    kind[2][k] = (a == (infinity | 0x8000u) ? one : 0u) | (b == (infinity | 0x8000u) ? one << 16 : 0u);
+                }
+                auto any = [&](const uint32_t (&x)[4]) {
+                    const w4f z = win_mfma_v<VT>(make_uint4(x[0], x[1], x[2], x[3]), seen, w4f{});
+                    uint32_t r = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) r |= (__float_as_uint(fminf(z[e], 1.f)) >> 29 & 1u) << e;  // a count: 0, or 1 and more
+                    return r;
+                };
+                nan |= any(kind[0]) << (4 * dt);
+                inf |= any(kind[1]) << (4 * dt);
+                neg |= any(kind[2]) << (4 * dt);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        nan |= inf & neg;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t x = __float_as_uint(o[dt][e]);
+                auto put = [&](uint32_t bits, uint32_t y) {
+                    const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)bits, 4 * dt + e, 1);
+                    x = (x & ~on) | (y & on);
+                };
+                put(inf, 0x7F800000u);
+                put(neg, 0xFF800000u);
+                put(nan, 0x7FC00000u);
+                o[dt][e] = __uint_as_float(x);
+            }
     }
 };
 
@@ -859,6 +911,16 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
             }
         }
         l = win_sum4(l);
+        if constexpr (!W::kV8) {
+            // A probability that 16 bits hold as 0, or a rescale by one that 32 do, makes NaN of an infinity: what is not finite is looked at
+            // again (scores of NaN leave l NaN).
+            float odd = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd = __builtin_fmaf(o[dt][e], 0.f, odd);
+            if (__builtin_amdgcn_ballot_w64(odd != 0.f) != 0) u.put_wild(i0, i1, kStep, o);
+        }
         // What the row's values average to here: everything that is joined or stored is a finite average of finite values, whatever
         // their size (O in its units times the unit need not be).
         const float inv = 1.f / l;
@@ -897,7 +959,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                     }
                     const float part = lt == 0.f ? 0.f : 1.f / lt;
 #pragma unroll
-                    for (int w = 0; w < kWinWaves; ++w) ot += join[(w * 4 + r - r0) * kRow + dv] * (lw[w] * part);
+                    for (int w = 0; w < kWinWaves; ++w) ot += win_part(join[(w * 4 + r - r0) * kRow + dv], lw[w] * part);
                     const int row = row0 + r, qi = row / p->G, h = kv * p->G + row - qi * p->G;
                     ssq_store_elem(p->a.out, p->out_dtype, (int64_t)b * p->a.o_sb + (int64_t)h * p->a.o_sh + (int64_t)qi * p->a.o_sl + dv,
                                    ot);
@@ -957,12 +1019,12 @@ __device__ __forceinline__ void win_join(float& M, float& L, T (&o)[E], const fl
     L = sum;
     const float part = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * (w0 * part);
+    for (int e = 0; e < E; ++e) o[e] = win_part(o[e], w0 * part);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         if (j >= n) continue;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += op[j][e] * (w[j] * part);
+        for (int e = 0; e < E; ++e) o[e] += win_part(op[j][e], w[j] * part);
     }
 }
 

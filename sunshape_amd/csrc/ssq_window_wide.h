@@ -487,7 +487,12 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
                     m = mn;
                     l *= f;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+                    for (int dt = 0; dt < DT; ++dt) {
+                        if constexpr (kV8) o[dt] *= f;
+                        else
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[dt][e] = win_part(o[dt][e], f);  // (f may be 0)
+                    }
                 }
                 if constexpr (kV8) {  // a row's units: the largest scale of a page that it sees
                     float big = sc[0];

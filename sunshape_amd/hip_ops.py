@@ -465,10 +465,10 @@ def decode_window(q: torch.Tensor, codes: torch.Tensor, v: torch.Tensor, perm: t
     Serves byte codes of dims 2, 4 or 8, head_dim 64 or 128 with Dv the same, pages of 16 to 256 tokens; others,
     and passthrough blocks (heavy), are refused.  scale, rotation as in decode.  Returns out [B, Hq, Lq, Dv] in
     out_dtype (v's dtype, or for 8-bit values the query's), and lse [B, Hq, Lq] (fp32) when requested; a row
-    that sees nothing gives 0 and -inf, one whose query holds a NaN or an infinity gives NaN.  Probabilities are
-    rounded to 11 bits down to 2^-20 (8-bit values, whatever their scales, which of the pages that a row sees lie within 2^120 of each
-    other) or 2^-28 (float16) of the row's largest, and to fewer below; to 8 bits with bfloat16 values.  No derivative; no
-    counterpart in the reference.
+    that sees nothing gives 0 and -inf, one whose query holds a NaN or an infinity gives NaN; an infinite or NaN value that it
+    sees makes that dim infinite or NaN, whatever it weighs.  Probabilities are rounded to 11 bits down to 2^-20 (8-bit values,
+    whatever their scales; values of scales below 2^-120 of the largest that a row sees are lost to it) or 2^-28 (float16) of the
+    row's largest, and to fewer below; to 8 bits with bfloat16 values.  No derivative; no counterpart in the reference.
     """
     if not (q.is_cuda and codes.is_cuda and v.is_cuda):
         for name, t in (("query", q), ("codes", codes), ("value", v)):

@@ -157,3 +157,58 @@ def test_scales_far_apart_beside_windows_and_nan(form):
     assert torch.isfinite(out).all()
     seen = ref[1] != -torch.inf
     assert (((out - ref[0]).abs() / ob)[seen] <= 1).all() and (((lse - ref[1]).abs() / lb)[seen] <= 1).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("vt", [BF, F16])
+@pytest.mark.parametrize("nats", [30.0, 100.0])
+def test_infinite_values_of_little_weight(form, vt, nats):
+    """Infinite values of tokens whose weight is e^-30 or e^-100, the first tokens among them (what is summed before the weights
+    that count): a row's dims are infinite where it sees one, NaN where it sees both or a NaN, and to the bit as without them elsewhere."""
+    log(f"range: infinite values e^-{nats}, {form}, {vt}")
+    inf, nan = torch.inf, torch.nan
+    pr = of_form(form, 66, vt=vt, **({} if form == "wide" else {"lens": [400, 399, 250] if form == "together" else [20000, 19999]}))
+    window = {"together": 300, "shares": 19000, "wide": 1800}[form]
+    B, Hq, Lq, D = pr["q"].shape
+    n0 = int(pr["seq_lens"][0])
+    old = n0 - Lq - window + 1  # the oldest token that the first row sees, which the next does not
+    # (token, dim, value) of sequence 0; the first quarter of what is seen and some of the newest tokens weigh little
+    put = [(old, 0, inf), (old + 1, 1, -inf), (old + 40, 2, inf), (n0 - 1, 3, -inf), (n0 - 2, 4, inf), (old + 41, 5, inf),
+           (n0 - 40, 5, -inf), (old + 70, 6, nan), (n0 - 33, 7, inf), (n0 - 33, 40, -inf), (old + 80, 41, inf), (old + 80, 42, nan),
+           (n0 - 70, 42, inf)]
+    few = sorted({t for t, _, _ in put} | set(range(old, old + window // 4)))
+    quiet(pr, [(int(pr["block_table"][0, t // 16]), t % 16) for t in few], nats)
+    bad = dict(pr, v=pr["v"].clone())
+    zero = dict(pr, v=pr["v"].clone())
+    for tok, dim, x in put:
+        page = int(pr["block_table"][0, tok // 16])
+        bad["v"][page, :, dim, tok % 16] = x
+        zero["v"][page, :, dim, tok % 16] = 0
+    out, lse = (t.cpu() for t in call(on_gpu(bad), window, 0, out_dtype=F32))
+    want, wl = (t.cpu() for t in call(on_gpu(zero), window, 0, out_dtype=F32))
+    assert torch.equal(lse, wl) and torch.isfinite(want).all()
+    p = n0 - Lq + torch.arange(Lq)
+    for dim in {d for _, d, _ in put}:
+        total = torch.zeros(Lq)
+        for tok, d, x in put:
+            if d == dim:
+                total = total + torch.where((p - window < tok) & (tok <= p), x, 0.0)
+        hit = total != 0  # (NaN too)
+        assert hit.any()
+        want[0, :, hit, dim] = total[hit]
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(out.nan_to_num(nan=7.0, posinf=inf, neginf=-inf), want.nan_to_num(nan=7.0, posinf=inf, neginf=-inf))
+
+
+def test_infinite_values_in_pieces_that_weigh_nothing():
+    """Parts of a long context whose weight in the join is 0 in 32 bits keep their infinities."""
+    for vt in (BF, F16):
+        log(f"range: infinite values, pieces without weight, {vt}")
+        pr = problem(67, B=1, Hq=4, Hkv=1, D=64, T=60000, per_head=False, vt=vt)
+        quiet(pr, [(int(pr["block_table"][0, t // 16]), t % 16) for t in range(30000)])
+        pr["v"][int(pr["block_table"][0, 1000 // 16]), 0, 3, 5] = torch.inf
+        pr["v"][int(pr["block_table"][0, 29000 // 16]), 0, 4, 5] = -torch.inf
+        pr["v"][int(pr["block_table"][0, 50000 // 16]), 0, 5, 5] = torch.inf
+        out = call(on_gpu(pr))[0].cpu()
+        assert (out[..., 3] == torch.inf).all() and (out[..., 4] == -torch.inf).all() and (out[..., 5] == torch.inf).all()
+        assert torch.isfinite(out[..., 6:]).all() and torch.isfinite(out[..., :3]).all()

@@ -245,16 +245,15 @@ struct WinCut {
             total += __builtin_amdgcn_readlane(scan(cost(p, i + lane, length(p, i + lane))), 63);
         share = max((total + p->workers - 1) / p->workers, p->least);
     }
-    // the item that holds cost position x < total, its start and cost
-    __device__ __forceinline__ void find(WinArgs p, int lane, int x, int& item, int& s, int& c) const {  // (uniform results)
+    // the item that holds cost position x < total, and its start.  Once a worker: the items behind it follow one by one.
+    __device__ __forceinline__ void find(WinArgs p, int lane, int x, int& item, int& s) const {  // (uniform results)
         int base = 0, mine = c0, v = v0;
         for (int f = 0;;) {
             const uint64_t hit = __builtin_amdgcn_ballot_w64(base + v > x);
             if (hit) {
                 const int l = __builtin_ctzll(hit);
                 item = f + l;
-                c = __builtin_amdgcn_readlane(mine, l);
-                s = base + __builtin_amdgcn_readlane(v, l) - c;
+                s = base + __builtin_amdgcn_readlane(v, l) - __builtin_amdgcn_readlane(mine, l);
                 return;
             }
             base += __builtin_amdgcn_readlane(v, 63);
@@ -265,7 +264,6 @@ struct WinCut {
         }
         item = p->items;
         s = x;
-        c = 0;
     }
 };
 
@@ -611,28 +609,20 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
     // ---- what is to be done: an item's tiles [i0, i1), and where they go (slot -1: the output)
     WinCut<TT, kWinRows> cut;
     const int worker = TEAM ? wg : wave * p->n_wg + wg;
-    int x = worker, x_begin = 0, x_end = 0;
+    int x = 0, x_begin = 0, x_end = 0, ahead = worker;  // the next item, and its cost position
     if constexpr (!TEAM) {
         cut.init(p, lane, first_len);
         x = x_begin = (int)min((int64_t)worker * cut.share, (int64_t)cut.total);
         x_end = (int)min((int64_t)(worker + 1) * cut.share, (int64_t)cut.total);
+        if (x_begin < x_end) cut.find(p, lane, x_begin, ahead, x);
     }
     int b = 0, row0 = 0, nr = 0, len = 0, i0 = 0, i1 = 0, slot = -1;
     auto next = [&]() {
         p = win_args();
         for (;;) {
-            int item, start = 0, cost = 0;
-            if constexpr (TEAM) {
-                if (x >= p->items) return false;
-                item = x;
-                x += p->n_wg;
-            } else {
-                if (x >= x_end) return false;
-                cut.find(p, lane, x, item, start, cost);
-                if (item >= p->items) return false;
-                x = start + cost;
-            }
-            item = __builtin_amdgcn_readfirstlane(item);
+            const int item = __builtin_amdgcn_readfirstlane(ahead), start = x;
+            if ((!TEAM && x >= x_end) || item >= p->items) return false;
+            ahead = item + (TEAM ? p->n_wg : 1);
             b = item / p->rgroups;
             row0 = (item - b * p->rgroups) * kWinRows;
             len = max(0, min(p->a.seq_lens[b], p->a.seq_len));
@@ -642,6 +632,8 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
             i0 = TEAM ? wave : 0;
             i1 = u.t.n;
             if constexpr (!TEAM) {
+                const int cost = p->fixed + u.t.n;
+                x = start + cost;
                 i0 = max(0, x_begin - start - p->fixed);
                 i1 = max(0, min(u.t.n, x_end - start - p->fixed));
                 if (u.t.n == 0 ? start < x_begin : i1 <= i0) continue;  // its part here is of the fixed cost

@@ -75,7 +75,8 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
     if (tid < D) perm[tid] = (uint16_t)((uint64_t)at_perm < (uint64_t)D ? at_perm : D - 1);
     cut.init(p, lane, first_len);
     const int x_begin = (int)min((int64_t)wg * cut.share, (int64_t)cut.total), x_end = (int)min((int64_t)(wg + 1) * cut.share, (int64_t)cut.total);
-    int x = x_begin;
+    int x = x_begin, ahead = 0;  // the next item, and its cost position
+    if (x_begin < x_end) cut.find(p, lane, x_begin, ahead, x);
 
     // ---- this thread's piece of a tile: 8 dims of a token, and 8 tokens of a value dim
     const int window = p->window, sinks = p->sinks, q_len = p->a.q_len, n_pages = p->n_pages, psh = p->psh;
@@ -95,17 +96,16 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
     auto next = [&]() {
         p = win_args();
         for (;;) {
-            if (x >= x_end) return false;
-            int item, start, cost;
-            cut.find(p, lane, x, item, start, cost);
-            if (item >= p->items) return false;
-            x = start + cost;
-            item = __builtin_amdgcn_readfirstlane(item);
+            const int item = __builtin_amdgcn_readfirstlane(ahead), start = x;
+            if (x >= x_end || item >= p->items) return false;
+            ahead = item + 1;
             b = item / p->rgroups;
             row0 = (item - b * p->rgroups) * ROWS;
             len = max(0, min(p->a.seq_lens[b], p->a.seq_len));
             nr = min(ROWS, p->rows - row0);
             t = win_tiles<TT, ROWS>(WinShape{window, sinks, q_len, p->G, p->rows}, len, row0);
+            const int cost = p->fixed + t.n;
+            x = start + cost;
             i0 = max(0, x_begin - start - p->fixed);
             i1 = max(0, min(t.n, x_end - start - p->fixed));
             if (t.n == 0 ? start < x_begin : i1 <= i0) continue;  // its part here is of the fixed cost

@@ -58,17 +58,15 @@ int check(const ssq_window_args* a) {
     SSQ_REQUIRE(d.c_sb >= 0 && d.c_sb < 1ll << 31 && d.c_st >= 0 && d.c_st <= 1 << 22 && d.v_sb >= 0 && d.v_sb < 1ll << 30 &&
                     a->vs_sb >= 0 && a->vs_sb < 1ll << 30,
                 "page strides must be below 2^30 elements");
-    const int64_t items = d.batch * (((int64_t)d.num_q_heads / d.num_kv_heads * d.q_len + kWinRows - 1) / kWinRows);
-    SSQ_UNSUPPORTED(d.num_kv_heads <= 1 << 16 && items * (d.seq_len / 32 + 8) < 1ll << 31, "too many query rows for so long a context");
+    SSQ_UNSUPPORTED(d.num_kv_heads <= 1 << 16, "too many KV heads");
     return SSQ_OK;
 }
 
-// The most tiles of an item (any length that the tables hold; a window's tiles depend on where it ends).
-int64_t most_tiles(const SsqWindowParams& p, bool v8) {
-    const int tt = v8 ? 64 : 32;
-    const int64_t all = (p.a.seq_len + tt - 1) / tt;
+// The most tiles of tt tokens of an item of `rows` rows (any length that the tables hold; a window's tiles depend on where it ends).
+int64_t most_tiles(const SsqWindowParams& p, int tt, int rows) {
+    const int64_t all = ((int64_t)p.a.seq_len + tt - 1) / tt;
     if (p.window == INT_MAX) return all;
-    const int64_t seen = ((int64_t)p.window + kWinRows + tt - 1) / tt + 1 + ((int64_t)p.sinks + tt - 1) / tt;
+    const int64_t seen = ((int64_t)p.window + rows + tt - 1) / tt + 1 + ((int64_t)p.sinks + tt - 1) / tt;
     return seen < all ? seen : all;
 }
 
@@ -112,7 +110,7 @@ bool wide(const SsqWindowParams& p) {
     return many <= few;
 }
 
-void make_plan(const ssq_window_args& a, Plan& pl) {
+int make_plan(const ssq_window_args& a, Plan& pl) {
     const ssq_decode_args& d = a.dec;
     SsqWindowParams& p = pl.p;
     p = SsqWindowParams{};
@@ -136,7 +134,11 @@ void make_plan(const ssq_window_args& a, Plan& pl) {
     p.item_rows = many ? kWinWideRows : kWinRows;
     p.rgroups = (p.rows + p.item_rows - 1) / p.item_rows;
     p.items = d.batch * p.rgroups;
-    p.form = many ? kWinWide : team(p, most_tiles(p, d.v_dtype == SSQ_E4M3)) ? kWinTeam : kWinShares;
+    const int tt = many ? 4096 / d.head_dim : d.v_dtype == SSQ_E4M3 ? 64 : 32;
+    const int64_t most = most_tiles(p, tt, p.item_rows);
+    p.form = many ? kWinWide : team(p, most) ? kWinTeam : kWinShares;
+    // the cost axis that shares are cut from has 32 bits
+    SSQ_UNSUPPORTED(p.form == kWinTeam || p.items * (most + p.fixed) < 1ll << 31, "too many query rows for so long a context");
     if (p.form == kWinTeam && p.n_wg > p.items) p.n_wg = p.items;
     p.workers = p.form == kWinShares ? p.n_wg * kWinWaves : p.n_wg;
     while ((16 << p.psh) < d.page_size) ++p.psh;
@@ -146,6 +148,7 @@ void make_plan(const ssq_window_args& a, Plan& pl) {
     p.out_vec = (uintptr_t)d.out % size == 0 && d.o_sb % 4 == 0 && d.o_sh % 4 == 0 && d.o_sl % 4 == 0;
     pl.part_bytes = p.form == kWinTeam ? 0 : (size_t)d.num_kv_heads * p.workers * 2 * p.item_rows * (d.value_dim + 2) * 4;
     pl.bytes = p.form == kWinTeam ? 0 : pl.part_bytes + (size_t)p.items * 8;
+    return SSQ_OK;
 }
 
 }  // namespace
@@ -153,8 +156,7 @@ void make_plan(const ssq_window_args& a, Plan& pl) {
 extern "C" size_t ssq_decode_window_workspace_size(const ssq_window_args* a) {
     if (check(a) != SSQ_OK || a->dec.batch == 0 || a->dec.num_q_heads == 0 || a->dec.q_len == 0) return 0;
     Plan pl;
-    make_plan(*a, pl);
-    return pl.bytes;
+    return make_plan(*a, pl) == SSQ_OK ? pl.bytes : 0;
 }
 
 extern "C" int ssq_decode_window(const ssq_window_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -163,7 +165,8 @@ extern "C" int ssq_decode_window(const ssq_window_args* a, void* workspace, size
     const ssq_decode_args& d = a->dec;
     if (d.batch == 0 || d.num_q_heads == 0 || d.q_len == 0) return SSQ_OK;
     Plan pl;
-    make_plan(*a, pl);
+    rc = make_plan(*a, pl);
+    if (rc) return rc;
     SSQ_REQUIRE(workspace_bytes >= pl.bytes && (workspace || pl.bytes == 0), "workspace too small: %zu < %zu bytes", workspace_bytes,
                 pl.bytes);
     SSQ_REQUIRE((uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");

@@ -194,3 +194,25 @@ def test_operators_without_a_gpu_say_so():
                               block_table=z(1, 4, dt=torch.int32), seq_lens=z(1, dt=torch.int32))
     with pytest.raises(RuntimeError, match="pool"):
         hip_ops.copy_pages([z(4, 2)], z(1, dt=torch.int64), z(1, dt=torch.int64))
+
+
+def test_window_takes_every_prompt_whose_shares_can_be_counted():
+    """What is refused is a cost axis past 32 bits: items of the form that the call takes, with the tiles that they can see."""
+    lib = N.lib()
+    size = lambda **kw: lib.ssq_decode_window_workspace_size(ctypes.byref(_window_args(**kw)))  # noqa: E731
+    prompt = dict(num_q_heads=32, num_kv_heads=8, head_dim=128, n_blocks=32, c_st=32, c_sh=512, value_dim=128)
+    for kw in (dict(batch=1, q_len=1 << 19, seq_len=1 << 19, window=4096, sinks=4), dict(batch=1, q_len=1 << 19, seq_len=1 << 19),
+               dict(batch=16, q_len=1 << 17, seq_len=1 << 17), dict(batch=1, q_len=1 << 20, seq_len=1 << 20, window=4096)):
+        assert size(**prompt, **kw) > 0, lib.ssq_last_error()
+    # 2^22 items of 256 rows, which cost 5 tiles each beside those of 64 tokens: 506 of them fit, 507 do not
+    most = dict(batch=1, num_q_heads=1024, num_kv_heads=1, q_len=1 << 20)
+    assert size(**most, seq_len=506 * 64) > 0
+    assert size(**most, seq_len=507 * 64) == 0 and b"too many query rows" in lib.ssq_last_error()
+    a = _window_args(**most, seq_len=507 * 64)
+    assert lib.ssq_decode_window(ctypes.byref(a), ALIGNED, 1 << 40, None) == N.SSQ_ERR_UNSUPPORTED
+    # under a window they are those that it holds: 256 + 17 tokens' and one sink's
+    assert size(**most, seq_len=1 << 22, window=17, sinks=1) > 0
+    # 2^24 sequences of one row: shares of single waves, 2 tiles beside those of 64 tokens
+    many = dict(batch=1 << 24, num_q_heads=1, num_kv_heads=1, q_len=1)
+    assert size(**many, seq_len=125 * 64) > 0
+    assert size(**many, seq_len=126 * 64) == 0 and b"too many query rows" in lib.ssq_last_error()

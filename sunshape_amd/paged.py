@@ -401,6 +401,8 @@ class PagedSunShapeCache:
             raise RuntimeError("query, keys and values must hold the same new tokens of each sequence")
         if key_states.shape[1] != self.num_kv_heads or value_states.shape[:3] != key_states.shape[:3]:
             raise RuntimeError("key/value shapes do not match the cache")
+        if query.shape[1] % self.num_kv_heads:  # (decode would find it behind the append)
+            raise RuntimeError("Query head count must be divisible by kv-head count.")
         self._shared_prefix(seq_ids)
         self._within(seq_ids, S, cos)
         positions = self.positions(seq_ids, S)

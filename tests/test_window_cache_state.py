@@ -284,3 +284,15 @@ def test_masks_and_repeated_sequences_are_refused(ops):
             cache.append([0, 0], _rows(2, 1), _rows(2, 1), **turn)
     assert _state(cache) == before
     assert math.isfinite(cache.v_scale.sum())
+
+
+def test_heads_that_do_not_divide_are_refused_before_anything_is_appended(ops):
+    """8-bit values of a page are rounded to a scale that grows with the new ones: a step that decode would refuse must not get there."""
+    for cache in (_cache(), _cache(value_dtype=BF, window=20)):
+        _attend(cache, [0], 4)
+        before = _state(cache)
+        ops.calls.clear()
+        cos, sin = hip_ops.rope_table(64, 64)
+        with pytest.raises(RuntimeError, match="divisible"):
+            cache.attend([0], _rows(1, 1, 3), _rows(1, 1), _rows(1, 1), cos=cos, sin=sin)
+        assert _state(cache) == before and not [c for c in ops.calls if c[0] == "append_kv"]

@@ -212,3 +212,18 @@ def test_infinite_values_in_pieces_that_weigh_nothing():
         out = call(on_gpu(pr))[0].cpu()
         assert (out[..., 3] == torch.inf).all() and (out[..., 4] == -torch.inf).all() and (out[..., 5] == torch.inf).all()
         assert torch.isfinite(out[..., 6:]).all() and torch.isfinite(out[..., :3]).all()
+
+
+@pytest.mark.parametrize("vt", [E4M3, BF])
+def test_the_largest_values_over_many_tiles_a_wave(vt):
+    """Alike values of 3e38 under alike weights, dozens of tiles a wave, so that its sum passes every threshold."""
+    log(f"range: 3e38 over many tiles, {vt}")
+    pr = problem(68, B=6, Hq=8, Hkv=8, D=64, T=30000, lens=[30000, 29999, 30000, 30000, 17000, 5], per_head=False, vt=vt, gain=1e-6, spread=0)
+    if vt == E4M3:
+        pr["v_scale"].fill_(2.0 ** 119)
+        pr["v"] = torch.full(pr["v"].shape, 448.0).to(E4M3)
+    else:
+        pr["v"] = torch.full(pr["v"].shape, 3e38).to(BF)
+    ref = window64(pr)
+    out, lse = call(on_gpu(pr))
+    within(pr, out, lse, ref, window_bounds(pr, *ref, BF))

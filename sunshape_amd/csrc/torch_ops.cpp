@@ -483,6 +483,7 @@ void check_scale(const Tensor& v_pages, const std::optional<Tensor>& v_scale, co
     for (int64_t i = 0; written && i < 2; ++i)
         TORCH_CHECK((v_scale->size(i) <= 1 || v_scale->stride(i) != 0) && (v_pages.size(i) <= 1 || v_pages.stride(i) != 0),
                     "pages and heads that are written have memory of their own");
+    TORCH_CHECK(!written || v_pages.size(2) <= 1 || v_pages.stride(2) != 0, "value dims that are written have memory of their own");
 }
 
 void append_kv(const Tensor& keys_in, const std::optional<Tensor>& v_in, const Tensor& perm_in, const Tensor& cent_in,

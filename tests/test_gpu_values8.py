@@ -313,3 +313,11 @@ def test_copy_refusals():
                            (([a], i, i), dict(into=[a[:, :1]]), "shape")):
         with pytest.raises(RuntimeError, match=word):
             hip_ops.copy_pages(*args, **kw)
+
+
+def test_dims_that_share_memory_are_refused():
+    """Written value dims have memory of their own, as written pages and heads do."""
+    v, slots = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(1, 1, dtype=torch.int64, device=DEV)
+    pages = torch.zeros(4, 2, 1, 16, dtype=torch.uint8, device=DEV).view(E4M3).expand(4, 2, 64, 16)
+    with pytest.raises(RuntimeError, match="memory of their own"):
+        hip_ops.append_values(v, pages, torch.zeros(4, 2, device=DEV), slots)

@@ -98,7 +98,7 @@ def last_page(pr, b, back=0):
 
 
 @pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("r", [6, 10, 20, 28, 60])
+@pytest.mark.parametrize("r", [6, 10, 20, 28, 60, 118])
 @pytest.mark.parametrize("how", ["weightless", "zero"])
 def test_a_page_of_a_large_scale_that_counts_for_nothing(form, r, how):
     """A page 2^r above the others whose tokens have a weight of e^-100, or values of 0: the others are what comes out, to their own

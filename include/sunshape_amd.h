@@ -382,7 +382,7 @@ int ssq_append8(const ssq_append8_args* a, void* workspace, size_t workspace_byt
  * sees); SSQ_BF16 or SSQ_F16: v_scale NULL.  Probabilities are rounded to 11 bits down to 2^-20 (8-bit values, whatever their
  * scales) or 2^-28 (f16) of the row's largest, and to fewer below; to 8 bits with bf16 values.  out is of out_dtype.  Serves
  * byte codes of dims 2, 4 or 8 (at most 256 codewords, no passthrough blocks), head_dim 64 or 128, value_dim the same, page
- * sizes of 16 to 256.
+ * sizes of 16 to 256.  The form that a call takes, and its workspace, follow from dec.seq_len (the table's width), not from the lengths.
  */
 typedef struct ssq_window_args {
     uint32_t struct_size;

@@ -27,7 +27,7 @@
 //
 // Bound by memory for long contexts: 64 sequences of 32,768 tokens (32 / 8 heads of 128, 8-bit values, 2.69 GB) take 424 us,
 // 6.3 TB/s, where a probe that only reads reaches 6.85; by about 10 us before the first tile (loads, lengths, codebook, queries) and 5
-// of the join for short ones: one sequence of 517 tokens 11.5 us.  What k_window_wide takes from many rows is in ssq_window_wide.h.
+// of the join for short ones: one sequence of 517 tokens 11.7 us.  What k_window_wide takes from many rows is in ssq_window_wide.h.
 #pragma once
 
 #include "ssq_common.h"
@@ -177,7 +177,8 @@ __device__ __forceinline__ void win_lds_sync() {
 }
 
 // 32-bit products, a lane's value of its dim and its row's probability each, of a token a lane group: what a page far below the
-// unit takes, whose f16 would have bits to lose (16 of these for one of 16 bits, and rare)
+// unit takes, whose f16 would have bits to lose (16 of these for one of 16 bits, and rare: with such a page in every tile 64 sequences
+// of 32,768 take 886 us for 424)
 __device__ __forceinline__ w4f win_mfma_32(float a, float b, w4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // four e4m3 values
 __device__ __forceinline__ w4f win_e4m3_32(uint32_t w) {
@@ -245,7 +246,8 @@ struct WinCut {
             total += __builtin_amdgcn_readlane(scan(cost(p, i + lane, length(p, i + lane))), 63);
         share = max((total + p->workers - 1) / p->workers, p->least);
     }
-    // the item that holds cost position x < total, and its start.  Once a worker: the items behind it follow one by one.
+    // the item that holds cost position x < total, and its start.  Once a worker: the items behind it follow one by one (131,072 short
+    // sequences 2.2 ms, 61 with a search for each).
     __device__ __forceinline__ void find(WinArgs p, int lane, int x, int& item, int& s) const {  // (uniform results)
         int base = 0, mine = c0, v = v0;
         for (int f = 0;;) {

@@ -10,8 +10,8 @@
 //
 // What bounds it: an operand of 1 KiB from LDS feeds one product of 32 cycles, so four SIMDs' products take what the LDS
 // can give; a step of 32 tokens (head_dim 128) takes 1.5 us, its products 0.7, its LDS reads 0.8, the probabilities 0.4.  Beside that about
-// 37 us of start, partials and join.  Measured us by 16 rows and here: 512 new tokens of 16,384 seeing 4,096 97 and 89, seeing
-// all 338 and 235; 16 prompts of 512 468 and 130 (what is chosen: wide() in ssq_window.hip).  Eight operands ahead in place of four: no
+// 37 us of start, partials and join.  Measured us by 16 rows and here: 512 new tokens of 16,384 seeing 4,096 97 and 88, seeing
+// all 338 and 234; 16 prompts of 512 468 and 134 (what is chosen: wide() in ssq_window.hip).  Eight operands ahead in place of four: no
 // gain.  Partials in the registers' order (a store is 1 KiB, the join reads what it wrote) 95 -> 89; by rows: 16 bytes each.
 //
 // Matrix row m = 8 a + 4 g + i (a lane's register 4 a + i in group g = lane / 32) of a score block of 32 is token

@@ -461,7 +461,8 @@ def decode_window(q: torch.Tensor, codes: torch.Tensor, v: torch.Tensor, perm: t
     already: row i stands at p = seq_lens[b] - Lq + i and sees token j iff j <= p and (j > p - window or j <
     sinks); window None: every j <= p.  codes uint8 [P, Hkv, page, nb], v [P, Hkv, Dv, page] in bfloat16, float16, or
     float8_e4m3fn with v_scale fp32 [P, Hkv] (append_values); block_table int32 [B, max_pages], seq_lens int32
-    [B], both on the device.  Pages that no row sees may be anything: their table entries are not used.
+    [B], both on the device.  Pages that no row sees may be anything: their table entries are not used.  The kernel's form
+    follows the table's width, as the lengths are not known here: a table as wide as the longest sequence is the fastest.
     Serves byte codes of dims 2, 4 or 8, head_dim 64 or 128 with Dv the same, pages of 16 to 256 tokens; others,
     and passthrough blocks (heavy), are refused.  scale, rotation as in decode.  Returns out [B, Hq, Lq, Dv] in
     out_dtype (v's dtype, or for 8-bit values the query's), and lse [B, Hq, Lq] (fp32) when requested; a row

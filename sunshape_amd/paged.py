@@ -141,8 +141,9 @@ class PagedSunShapeCache:
 
     def fork(self, prefix_id: int, seq_ids: list[int]) -> None:
         """Start sequences that continue prefix_id's tokens.  They start empty, and the prefix takes no more tokens while
-        any of them lives; in a cache with 8-bit values or a window they start as copies of it, which share its
-        whole pages and copy its last one if that is not full, and all of them go on by themselves."""
+        any of them lives, and decode reads them once for all; in a cache with 8-bit values or a window they start as copies
+        of it, which share its whole pages, copy its last one if that is not full and go on by themselves, and decode reads
+        the shared pages once for each."""
         if self.causal:
             return self._fork_copies(prefix_id, seq_ids)
         if not self.seq_lens.get(prefix_id) or prefix_id in self.prefix_of:
@@ -392,8 +393,9 @@ class PagedSunShapeCache:
         """One step over raw projections: query [B, Hq, S, D], keys and values [B, Hkv, S, ..] of the S next
         tokens of each sequence.  Norms and rotates them, appends keys and values, and attends causally;
         returns [B, Hq, S, Dv].  scale as in decode (None: the query as it is).  A step that is refused leaves the
-        sequences as they were (8-bit values of a last page may have been rounded to a larger scale).  With S > 1 the causal mask takes 4 B S times the longest own table's tokens in bytes (none
-        in a cache with 8-bit values or a window, whose pages that left the window are given back after the step)."""
+        sequences as they were (8-bit values of a last page may have been rounded to a larger scale).  With S > 1 the causal
+        mask takes 4 B S times the longest own table's tokens in bytes (none in a cache with 8-bit values or a window, whose
+        pages that left the window are given back after the step)."""
         B, _, S, _ = query.shape
         if len(set(seq_ids)) != len(seq_ids):
             raise RuntimeError("attend takes each sequence once")
